@@ -126,6 +126,21 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "bioemu_trunk_uncond_fwd_f32": (_c_int, [_c_void_p] * 10 + [_c_size_t] + [_c_int64] * 3 + [_c_void_p]),
     "bioemu_distogram_f32_workspace_bytes": (_c_size_t, [_c_int64] * 3),
     "bioemu_distogram_fwd_f32": (_c_int, [_c_void_p] * 5 + [_c_size_t] + [_c_int64] * 4 + [_c_void_p]),
+    "bioemu_layer_norm_fwd": (
+        _c_int,
+        [_c_void_p] * 5 + [_c_int64] * 3 + [ctypes.c_float, _c_int, _c_int, _c_void_p],
+    ),
+    "bioemu_layer_norm_bwd_workspace_bytes": (_c_size_t, [_c_int64] * 2),
+    "bioemu_layer_norm_bwd": (
+        _c_int,
+        [_c_void_p] * 8 + [_c_size_t] + [_c_int64] * 4 + [_c_int, _c_int, _c_void_p],
+    ),
+    "bioemu_relpos_fwd": (_c_int, [_c_void_p] * 6 + [_c_int64] * 5 + [_c_int, _c_int, _c_void_p]),
+    "bioemu_relpos_bwd_workspace_bytes": (_c_size_t, [_c_int64] * 4),
+    "bioemu_relpos_bwd": (
+        _c_int,
+        [_c_void_p] * 6 + [_c_size_t] + [_c_int64] * 5 + [_c_int, _c_int, _c_void_p],
+    ),
 }
 
 _lock = threading.Lock()

@@ -1,0 +1,297 @@
+"""Trainable torch ops over the C ABI: LayerNorm, relative positions.
+
+As ``_ops``: ``launch_*`` functions validate tensors and call the C ABI on the
+current HIP stream of the tensors' device with caller-provided outputs, and
+``torch.ops.bioemu_mi355x.*`` are ``torch.library`` custom ops (HIP only) with a
+registered gradient.  A plain call does not pass the dispatcher: without
+gradients it reaches the body, with them one ``autograd.Function``.  Gradients
+are first order.
+"""
+
+from __future__ import annotations
+
+import contextlib
+import ctypes
+
+import torch
+from torch import Tensor
+
+from ._lib import check, lib
+from ._ops import BF16, F32, _check_tensor, _Op, _ptr, _stream, _unobserved, require_gpu, workspace
+
+_TYPES = (BF16, F32)
+
+
+def _on(t: Tensor):
+    """A launch reaches the device of its tensors, current or not."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == t.get_device() else torch.cuda.device(t.device)
+
+
+class _TrainOp(_Op):
+    """An ``_Op`` with a gradient.  ``save`` takes (ctx, args, outputs), ``grad`` (ctx, gradients of the outputs);
+    ``for_grad`` and ``no_grad`` give the body's arguments of a call with and without gradients, where those differ
+    (what the backward pass reads is not written by a serving call).  The op's first output is what callers get."""
+
+    def __init__(self, name: str, body, save, grad):
+        super().__init__(name, body)
+        self.op.register_autograd(grad, setup_context=lambda ctx, inputs, output: save(ctx, inputs, output))
+
+        def forward(ctx, *args):
+            out = body(*args)
+            save(ctx, args, out)
+            return out[0]
+
+        def backward(ctx, g):
+            return grad(ctx, g, None)
+
+        self.fn = type(name, (torch.autograd.Function,),
+                       {"forward": staticmethod(forward),
+                        "backward": staticmethod(torch.autograd.function.once_differentiable(backward))})
+
+    def __call__(self, *args):
+        """args[-1] of the op says whether a gradient is wanted, and is filled in here."""
+        train = torch.is_grad_enabled() and any(isinstance(a, Tensor) and a.requires_grad for a in args)
+        if _unobserved(args) and self._own():
+            return self.fn.apply(*args, True) if train else self.body(*args, False)[0]
+        return self.op(*args, train)[0]
+
+
+def _param_type(t: Tensor | None, what: str, shape: tuple[int, ...], device) -> int:
+    """1 for bf16 and 0 for fp32 parameters."""
+    if t is None:
+        return 0
+    if t.dtype not in _TYPES:
+        raise ValueError(f"{what}: expected fp32 or bf16, got {t.dtype}")
+    _check_tensor(t, what, t.dtype, shape, device)
+    return int(t.dtype == BF16)
+
+
+def _activation(t: Tensor, what: str) -> int:
+    """1 for fp32 and 0 for bf16 activations."""
+    require_gpu(t, what)
+    if t.dtype not in _TYPES:
+        raise ValueError(f"{what}: expected fp32 or bf16, got {t.dtype}")
+    return int(t.dtype == F32)
+
+
+# ----------------------------------------------------------------------------
+# LayerNorm
+# ----------------------------------------------------------------------------
+def _as_rows(x: Tensor) -> Tensor:
+    """``x`` as [rows, c] with neighbouring values adjacent: a view where its strides allow, a copy else."""
+    c = x.shape[-1]
+    if x.is_contiguous():
+        return x.view(-1, c)
+    if x.stride(-1) == 1 or c == 1:
+        try:
+            rows = x.view(-1, c)
+            return rows if rows.stride(1) == 1 else rows.contiguous()
+        except RuntimeError:
+            pass
+    return x.contiguous().view(-1, c)
+
+
+def layer_norm_bwd_workspace_bytes(rows: int, c: int) -> int:
+    return int(lib().bioemu_layer_norm_bwd_workspace_bytes(rows, c))
+
+
+def launch_layer_norm(x: Tensor, weight: Tensor | None, bias: Tensor | None, y: Tensor, eps: float,
+                      stats: Tensor | None = None) -> Tensor:
+    """LayerNorm of the rows ``x`` [rows, c] (any row stride) into contiguous ``y``; ``stats`` [rows, 2] fp32."""
+    f32 = _activation(x, "layer_norm")
+    if x.ndim != 2 or x.stride(1) != 1:
+        raise ValueError("layer_norm: x must be [rows, c] with adjacent values")
+    rows, c = x.shape
+    _check_tensor(y, "layer_norm y", x.dtype, (rows, c), x.device)
+    w16 = _param_type(weight, "layer_norm weight", (c,), x.device)
+    if bias is not None and weight is not None and bias.dtype != weight.dtype:
+        raise ValueError(f"layer_norm: weight is {weight.dtype}, bias {bias.dtype}")
+    w16 |= _param_type(bias, "layer_norm bias", (c,), x.device)
+    if stats is not None:
+        _check_tensor(stats, "layer_norm stats", F32, (rows, 2), x.device)
+    with _on(x):
+        rc = lib().bioemu_layer_norm_fwd(_ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _ptr(stats), rows, c, x.stride(0),
+                                         eps, f32, w16, _stream(x))
+    check(rc, "bioemu_layer_norm_fwd")
+    return y
+
+
+def launch_layer_norm_bwd(x: Tensor, dy: Tensor, stats: Tensor, weight: Tensor | None, dx: Tensor | None,
+                          dweight: Tensor | None, dbias: Tensor | None, ws: Tensor | None = None) -> None:
+    """Gradients of ``launch_layer_norm`` into ``dx`` [rows, c], ``dweight``, ``dbias`` (each may be None)."""
+    f32 = _activation(x, "layer_norm_bwd")
+    if x.ndim != 2 or x.stride(1) != 1 or dy.shape != x.shape or dy.dtype != x.dtype or dy.stride(1) != 1:
+        raise ValueError("layer_norm_bwd: x and dy must be [rows, c] of one type with adjacent values")
+    rows, c = x.shape
+    dev = x.device
+    _check_tensor(stats, "layer_norm stats", F32, (rows, 2), dev)
+    if dx is not None:
+        _check_tensor(dx, "layer_norm dx", x.dtype, (rows, c), dev)
+    w16 = _param_type(weight, "layer_norm weight", (c,), dev)
+    for t in (dweight, dbias):
+        if t is not None and weight is not None and t.dtype != weight.dtype:
+            raise ValueError("layer_norm_bwd: weight gradients take the weight's type")
+        w16 |= _param_type(t, "layer_norm weight gradient", (c,), dev)
+    need = layer_norm_bwd_workspace_bytes(rows, c) if dweight is not None or dbias is not None else 0
+    if need and (ws is None or ws.numel() < need):
+        ws = workspace(need, dev)
+    with _on(x):
+        rc = lib().bioemu_layer_norm_bwd(
+            _ptr(x), _ptr(dy), _ptr(stats), _ptr(weight), _ptr(dx), _ptr(dweight), _ptr(dbias), _ptr(ws),
+            ctypes.c_size_t(0 if ws is None else ws.numel()), rows, c, x.stride(0), dy.stride(0), f32, w16, _stream(x))
+    check(rc, "bioemu_layer_norm_bwd")
+
+
+def _layer_norm(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float, train: bool) -> tuple[Tensor, Tensor]:
+    rows = _as_rows(x)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty((rows.shape[0] if train else 0, 2), dtype=F32, device=x.device)
+    launch_layer_norm(rows, weight, bias, y.view(rows.shape), eps, stats if train else None)
+    return y, stats
+
+
+def _layer_norm_backward(x: Tensor, dy: Tensor, stats: Tensor, weight: Tensor | None, want_x: bool, want_w: bool,
+                         want_b: bool, bias_bf16: bool) -> tuple[Tensor, Tensor, Tensor]:
+    rows = _as_rows(x)
+    c = x.shape[-1]
+    wt = weight.dtype if weight is not None else (BF16 if bias_bf16 else F32)
+    dx = torch.empty(x.shape if want_x else (0,), dtype=x.dtype, device=x.device)
+    dw = torch.empty((c if want_w else 0,), dtype=wt, device=x.device)
+    db = torch.empty((c if want_b else 0,), dtype=wt, device=x.device)
+    if x.numel() == 0:
+        return dx, dw.zero_(), db.zero_()
+    launch_layer_norm_bwd(rows, _as_rows(dy), stats, weight, dx.view(rows.shape) if want_x else None,
+                          dw if want_w else None, db if want_b else None)
+    return dx, dw, db
+
+
+layer_norm_backward = _Op("layer_norm_backward", _layer_norm_backward)
+
+
+@layer_norm_backward.register_fake
+def _(x, dy, stats, weight, want_x, want_w, want_b, bias_bf16):
+    wt = weight.dtype if weight is not None else (BF16 if bias_bf16 else F32)
+    return (x.new_empty(x.shape if want_x else (0,)), x.new_empty((x.shape[-1] if want_w else 0,), dtype=wt),
+            x.new_empty((x.shape[-1] if want_b else 0,), dtype=wt))
+
+
+def _layer_norm_save(ctx, inputs, output) -> None:
+    x, weight, bias, _, _ = inputs
+    ctx.save_for_backward(x, weight, output[1])
+    ctx.bias_bf16 = bias is not None and bias.dtype == BF16
+
+
+def _layer_norm_grad(ctx, dy, _):
+    x, weight, stats = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    dx, dw, db = layer_norm_backward(x, dy, stats, weight, need[0], need[1], need[2], ctx.bias_bf16)
+    return (dx if need[0] else None, dw if need[1] else None, db if need[2] else None, None, None)
+
+
+layer_norm = _TrainOp("layer_norm", _layer_norm, _layer_norm_save, _layer_norm_grad)
+
+
+@layer_norm.register_fake
+def _(x, weight, bias, eps, train):
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device), x.new_empty(
+        (x.numel() // x.shape[-1] if train else 0, 2), dtype=F32)
+
+
+# ----------------------------------------------------------------------------
+# Relative positions
+# ----------------------------------------------------------------------------
+def relpos_bwd_workspace_bytes(B: int, N: int, C: int, num_buckets: int) -> int:
+    return int(lib().bioemu_relpos_bwd_workspace_bytes(B, N, C, num_buckets))
+
+
+def _check_relpos(what: str, buckets: Tensor, positions: Tensor, chains: Tensor | None, dev) -> int:
+    if positions.ndim != 2:
+        raise ValueError(f"{what}: positions must be [B, N], got {tuple(positions.shape)}")
+    _check_tensor(positions, f"{what} positions", torch.int32, tuple(positions.shape), dev)
+    if chains is not None:
+        _check_tensor(chains, f"{what} chains", torch.int32, tuple(positions.shape), dev)
+    if buckets.ndim != 1 or buckets.numel() % 2 == 0:
+        raise ValueError(f"{what}: buckets must be [2 * radius + 1], got {tuple(buckets.shape)}")
+    _check_tensor(buckets, f"{what} buckets", torch.uint8, tuple(buckets.shape), dev)
+    return buckets.numel() // 2
+
+
+def launch_relpos(table: Tensor, buckets: Tensor, positions: Tensor, chains: Tensor | None, z: Tensor | None,
+                  out: Tensor) -> Tensor:
+    """``out`` [B, N, N, C] = ``z`` + ``table`` [num_buckets, C] at the buckets of the pairs' offsets."""
+    f32 = _activation(out, "relpos")
+    radius = _check_relpos("relpos", buckets, positions, chains, out.device)
+    (B, N), (NB, C) = positions.shape, table.shape
+    t16 = _param_type(table, "relpos table", (NB, C), out.device)
+    _check_tensor(out, "relpos out", out.dtype, (B, N, N, C), out.device)
+    if z is not None:
+        _check_tensor(z, "relpos z", out.dtype, (B, N, N, C), out.device)
+    with _on(out):
+        rc = lib().bioemu_relpos_fwd(_ptr(table), _ptr(buckets), _ptr(positions), _ptr(chains), _ptr(z), _ptr(out), B, N,
+                                     C, radius, NB, f32, t16, _stream(out))
+    check(rc, "bioemu_relpos_fwd")
+    return out
+
+
+def launch_relpos_bwd(dout: Tensor, buckets: Tensor, positions: Tensor, chains: Tensor | None, dtable: Tensor,
+                      ws: Tensor | None = None) -> Tensor:
+    """``dtable`` [num_buckets, C]: the sums of ``dout`` [B, N, N, C] by bucket."""
+    f32 = _activation(dout, "relpos_bwd")
+    radius = _check_relpos("relpos_bwd", buckets, positions, chains, dout.device)
+    (B, N), (NB, C) = positions.shape, dtable.shape
+    _check_tensor(dout, "relpos_bwd dout", dout.dtype, (B, N, N, C), dout.device)
+    t16 = _param_type(dtable, "relpos_bwd dtable", (NB, C), dout.device)
+    need = relpos_bwd_workspace_bytes(B, N, C, NB)
+    if ws is None or ws.numel() < need:
+        ws = workspace(need, dout.device)
+    with _on(dout):
+        rc = lib().bioemu_relpos_bwd(_ptr(dout), _ptr(buckets), _ptr(positions), _ptr(chains), _ptr(dtable), _ptr(ws),
+                                     ctypes.c_size_t(ws.numel()), B, N, C, radius, NB, f32, t16, _stream(dout))
+    check(rc, "bioemu_relpos_bwd")
+    return dtable
+
+
+def _relative_position(table: Tensor, z: Tensor | None, buckets: Tensor, positions: Tensor, chains: Tensor | None,
+                       dtype: torch.dtype, train: bool) -> tuple[Tensor, Tensor]:
+    B, N = positions.shape
+    out = torch.empty((B, N, N, table.shape[1]), dtype=dtype, device=table.device)
+    launch_relpos(table.contiguous(), buckets, positions, chains, None if z is None else z.contiguous(), out)
+    return out, table.new_empty((0,))   # a gradient reads no result
+
+
+def _relative_position_backward(dout: Tensor, buckets: Tensor, positions: Tensor, chains: Tensor | None,
+                                num_buckets: int, dtype: torch.dtype) -> Tensor:
+    dtable = torch.empty((num_buckets, dout.shape[-1]), dtype=dtype, device=dout.device)
+    if dout.numel() == 0:
+        return dtable.zero_()
+    return launch_relpos_bwd(dout.contiguous(), buckets, positions, chains, dtable)
+
+
+relative_position_backward = _Op("relative_position_backward", _relative_position_backward)
+
+
+@relative_position_backward.register_fake
+def _(dout, buckets, positions, chains, num_buckets, dtype):
+    return dout.new_empty((num_buckets, dout.shape[-1]), dtype=dtype)
+
+
+def _relative_position_save(ctx, inputs, output) -> None:
+    table, _, buckets, positions, chains, _, _ = inputs
+    ctx.save_for_backward(buckets, positions, chains)
+    ctx.table = table.shape[0], table.dtype
+
+
+def _relative_position_grad(ctx, dout, _):
+    buckets, positions, chains = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    dtable = relative_position_backward(dout, buckets, positions, chains, *ctx.table) if need[0] else None
+    return (dtable, dout if need[1] else None, None, None, None, None, None)
+
+
+relative_position = _TrainOp("relative_position", _relative_position, _relative_position_save, _relative_position_grad)
+
+
+@relative_position.register_fake
+def _(table, z, buckets, positions, chains, dtype, train):
+    B, N = positions.shape
+    return table.new_empty((B, N, N, table.shape[1]), dtype=dtype), table.new_empty((0,))

@@ -452,6 +452,48 @@ int bioemu_triatt_fwd_f32(const float* z, const uint8_t* mask, const float* norm
                           const float* w_proj, const float* w_o, float* out, void* workspace, size_t workspace_bytes,
                           int64_t B, int64_t N, int64_t D, int64_t H, int starting, int residual, hipStream_t stream);
 
+/*
+ * Trainable operators.  Unlike the entry points above they have a backward
+ * pass.  `f32` chooses the type of the activations (0: bf16, 1: fp32); sums and
+ * statistics are fp32 in both.  Results do not depend on the order in which
+ * workgroups run.
+ *
+ * LayerNorm over the last dimension: y = (x - mean) / sqrt(var + eps) * weight
+ * + bias.  x: rows of c values, x_stride elements apart; y: contiguous rows of
+ * x's type.  weight and bias: c values of fp32 or bf16 (weight_bf16), or NULL
+ * (1 and 0).  stats: NULL, or [rows][2] fp32 (mean, 1 / deviation) for the
+ * backward pass.  c is at most 16384 where rows are whole 16-byte vectors at
+ * 16-byte addresses, 4096 else.
+ * Backward: dx (contiguous rows, or NULL), dweight and dbias (of weight's type,
+ * or NULL; without both the workspace may be NULL); rows >= 1.
+ */
+int bioemu_layer_norm_fwd(const void* x, const void* weight, const void* bias, void* y, float* stats, int64_t rows,
+                          int64_t c, int64_t x_stride, float eps, int f32, int weight_bf16, hipStream_t stream);
+size_t bioemu_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t c);
+int bioemu_layer_norm_bwd(const void* x, const void* dy, const float* stats, const void* weight, void* dx,
+                          void* dweight, void* dbias, void* workspace, size_t workspace_bytes, int64_t rows, int64_t c,
+                          int64_t x_stride, int64_t dy_stride, int f32, int weight_bf16, hipStream_t stream);
+
+/*
+ * Relative-position embedding of the pair representation (what the reference's
+ * token_rel_pos_feats and relative_position_encoder hold), and its table's gradient:
+ *   t(b,i,j) = chain_i == chain_j ? buckets[clamp(pos_j - pos_i, -radius, radius) + radius] : num_buckets - 1
+ *   out[b,i,j] = z[b,i,j] + table[t(b,i,j)];   dtable[t] = sum over the pairs of bucket t of dout
+ * table: [num_buckets, C] fp32 or bf16 (table_bf16); buckets: [2 radius + 1]
+ * uint8, values past num_buckets - 1 count as that; positions, chains: [B, N]
+ * int32 (chains may be NULL: one chain); z (may be NULL), out, dout:
+ * [B, N, N, C] of the type f32 names; dtable: of table's type.
+ * num_buckets is at most 256; C at most 4096, or 256 where rows are not whole
+ * 16-byte vectors.
+ */
+int bioemu_relpos_fwd(const void* table, const uint8_t* buckets, const int32_t* positions, const int32_t* chains,
+                      const void* z, void* out, int64_t B, int64_t N, int64_t C, int64_t radius, int64_t num_buckets,
+                      int f32, int table_bf16, hipStream_t stream);
+size_t bioemu_relpos_bwd_workspace_bytes(int64_t B, int64_t N, int64_t C, int64_t num_buckets);
+int bioemu_relpos_bwd(const void* dout, const uint8_t* buckets, const int32_t* positions, const int32_t* chains,
+                      void* dtable, void* workspace, size_t workspace_bytes, int64_t B, int64_t N, int64_t C,
+                      int64_t radius, int64_t num_buckets, int f32, int table_bf16, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

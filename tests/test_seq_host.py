@@ -1,0 +1,81 @@
+"""Host side of the trainable operators (CPU only): bucket maps, refusals, state dicts, C ABI checks."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from bioemu2_amd import _lib
+from bioemu2_amd.layer_norm import LayerNorm, layer_norm
+from bioemu2_amd.relative_position import RelativePosition, distance_buckets, relative_position
+
+
+def test_distance_buckets_own_bucket_each():
+    assert distance_buckets(3).tolist() == [0, 1, 2, 3, 4, 5, 6]
+    assert distance_buckets(0).tolist() == [0]
+
+
+@pytest.mark.parametrize("radius,nb", [(128, 32), (128, 64), (64, 64), (1000, 128), (16, 64), (200, 4), (512, 256)])
+def test_distance_buckets_log_borders_are_exact(radius, nb):
+    """Bucket k of the far distances starts at the least d with (d / exact)^steps >= (radius / exact)^k, in whole
+    numbers; both directions alike; offset 0 among the positive ones."""
+    m = distance_buckets(radius, nb).tolist()
+    half, exact = nb // 2, nb // 4
+    steps = half - exact
+    assert len(m) == 2 * radius + 1 and m[radius] == 0
+    for d in range(1, radius + 1):
+        if d < exact:
+            want = d
+        else:
+            k = max(k for k in range(steps + 1) if d ** steps * exact ** k >= radius ** k * exact ** steps)
+            want = min(half - 1, exact + k)
+        assert m[radius + d] == want and m[radius - d] == half + want, d
+
+
+def test_distance_buckets_refusals():
+    for args in ((-1,), (128,), (128, 6), (128, 260), (5, 64)):
+        with pytest.raises(ValueError):
+            distance_buckets(*args)
+
+
+def test_cpu_tensors_are_rejected():
+    x = torch.randn(2, 8)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        layer_norm(x)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        LayerNorm(8)(x)
+    pos = torch.arange(4)[None]
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        relative_position(x, distance_buckets(0), pos)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        RelativePosition(8)(pos)
+    with pytest.raises(ValueError, match="last dimension"):
+        LayerNorm(9)(x)
+    with pytest.raises(ValueError, match="at most 256"):
+        RelativePosition(8, radius=127, num_buckets=None) and RelativePosition(8, radius=200)
+
+
+def test_layer_norm_c_abi_refusals():
+    lib = _lib.lib()
+    assert lib.bioemu_layer_norm_fwd(None, None, None, None, None, 4, 64, 64, 1e-5, 1, 0, None) == -1
+    assert b"null" in lib.bioemu_last_error()
+    assert lib.bioemu_layer_norm_fwd(None, None, None, None, None, 4, 0, 0, 1e-5, 1, 0, None) == -1
+    assert lib.bioemu_layer_norm_fwd(16, None, None, 16, None, 4, 16388, 16388, 1e-5, 1, 0, None) == -2
+    assert lib.bioemu_layer_norm_fwd(None, None, None, None, None, 0, 64, 64, 1e-5, 1, 0, None) == 0
+    assert lib.bioemu_layer_norm_bwd(16, 16, 16, None, 16, 16, None, None, 0, 4, 64, 64, 64, 1, 0, None) == -3
+    assert lib.bioemu_layer_norm_bwd(16, 16, 16, None, 16, None, None, None, 0, 0, 64, 64, 64, 1, 0, None) == -1
+    assert lib.bioemu_layer_norm_bwd_workspace_bytes(1 << 20, 128) == 1024 * 2 * 128 * 4
+    assert lib.bioemu_layer_norm_bwd_workspace_bytes(0, 128) == 0
+
+
+def test_relpos_c_abi_refusals():
+    lib = _lib.lib()
+    assert lib.bioemu_relpos_fwd(None, None, None, None, None, None, 1, 8, 16, 2, 5, 1, 0, None) == -1
+    assert lib.bioemu_relpos_fwd(16, 16, 16, None, None, 16, 1, 8, 16, 2, 257, 1, 0, None) == -2
+    assert lib.bioemu_relpos_fwd(16, 16, 16, None, None, 16, 1, 8, 16, 2, 0, 1, 0, None) == -1
+    assert lib.bioemu_relpos_fwd(16, 16, 16, None, None, 16, 0, 8, 16, 2, 5, 1, 0, None) == 0
+    assert lib.bioemu_relpos_bwd(16, 16, 16, None, 16, None, 0, 1, 8, 16, 2, 5, 1, 0, None) == -3
+    assert lib.bioemu_relpos_bwd_workspace_bytes(0, 8, 16, 5) == 0
+    assert math.prod((1, 5, 16, 4)) == lib.bioemu_relpos_bwd_workspace_bytes(1, 8, 16, 5)
