@@ -17,6 +17,23 @@ _c_size_t = ctypes.c_size_t
 _c_int64 = ctypes.c_int64
 _c_int = ctypes.c_int
 
+
+
+class AttentionArgs(ctypes.Structure):
+    """``bioemu_attention_args`` (strides one by one)."""
+
+    _fields_ = (
+        [(n, _c_void_p) for n in ("q", "k", "v")]
+        + [(f"{t}_{n}", _c_int64) for t in ("q", "k", "v") for n in ("batch", "row", "head")]
+        + [(n, _c_void_p) for n in ("q_segments", "k_segments", "prefix", "lengths", "bias_table", "bias_buckets")]
+        + [(n, _c_int64) for n in ("B", "Nq", "Nk", "H", "Hk", "D", "radius", "num_buckets")]
+        + [("scale", ctypes.c_float), ("cap", ctypes.c_float)]
+        + [(n, _c_int) for n in ("causal", "f32", "table_bf16")]
+    )
+
+
+_attn_p = ctypes.POINTER(AttentionArgs)
+
 # name -> (restype, argtypes).  Keep in the order of include/bioemu2_mi355x.h.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "bioemu_version": (ctypes.c_char_p, []),
@@ -140,6 +157,13 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "bioemu_relpos_bwd": (
         _c_int,
         [_c_void_p] * 6 + [_c_size_t] + [_c_int64] * 5 + [_c_int, _c_int, _c_void_p],
+    ),
+    "bioemu_attention_workspace_bytes": (_c_size_t, [_attn_p]),
+    "bioemu_attention_fwd": (_c_int, [_attn_p] + [_c_void_p] * 3 + [_c_size_t, _c_void_p]),
+    "bioemu_attention_bwd_workspace_bytes": (_c_size_t, [_attn_p, _c_int]),
+    "bioemu_attention_bwd": (
+        _c_int,
+        [_attn_p] + [_c_void_p] * 3 + [ctypes.POINTER(_c_int64 * 3)] + [_c_void_p] * 5 + [_c_size_t, _c_void_p],
     ),
 }
 

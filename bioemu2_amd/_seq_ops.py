@@ -1,4 +1,4 @@
-"""Trainable torch ops over the C ABI: LayerNorm, relative positions.
+"""Trainable torch ops over the C ABI: LayerNorm, relative positions, attention.
 
 As ``_ops``: ``launch_*`` functions validate tensors and call the C ABI on the
 current HIP stream of the tensors' device with caller-provided outputs, and
@@ -16,7 +16,7 @@ import ctypes
 import torch
 from torch import Tensor
 
-from ._lib import check, lib
+from ._lib import AttentionArgs, check, lib
 from ._ops import BF16, F32, _check_tensor, _Op, _ptr, _stream, _unobserved, require_gpu, workspace
 
 _TYPES = (BF16, F32)
@@ -295,3 +295,165 @@ relative_position = _TrainOp("relative_position", _relative_position, _relative_
 def _(table, z, buckets, positions, chains, dtype, train):
     B, N = positions.shape
     return table.new_empty((B, N, N, table.shape[1]), dtype=dtype), table.new_empty((0,))
+
+
+# ----------------------------------------------------------------------------
+# Attention
+# ----------------------------------------------------------------------------
+_MAX_ROW_STRIDE = 1 << 23
+
+
+def _heads(t: Tensor) -> Tensor:
+    """[B, N, H, D] with adjacent values of a head and rows at 16-byte addresses: ``t`` where it is so, a copy else."""
+    per = 16 // t.element_size()
+    b, n, h, d = t.stride()
+    rows, width = t.shape[1], t.shape[3]
+    if (d == 1 and (n >= width or rows <= 1) and n <= _MAX_ROW_STRIDE and not (b % per or n % per or h % per)
+            and t.data_ptr() % 16 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _attention_args(q, k, v, table, buckets, q_segments, k_segments, prefix, lengths, scale: float, cap: float,
+                    causal: bool) -> AttentionArgs:
+    f32 = _activation(q, "attention")
+    dev = q.device
+    if q.ndim != 4 or k.ndim != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError(f"attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"attention: q is {q.dtype}, k {k.dtype}, v {v.dtype}")
+    if k.device != dev or v.device != dev:
+        raise ValueError(f"attention: q on {dev}, k on {k.device}, v on {v.device}")
+    B, Nq, H, D = q.shape
+    Nk, Hk = k.shape[1], k.shape[2]
+    if (q_segments is None) != (k_segments is None):
+        raise ValueError("attention: segments of queries and of keys come together")
+    for t, name, shape in ((q_segments, "segments", (B, Nq)), (k_segments, "key segments", (B, Nk)),
+                           (prefix, "prefix", (B,)), (lengths, "cache_lengths", (B,))):
+        if t is not None:
+            _check_tensor(t, f"attention {name}", torch.int32, shape, dev)
+    radius = nb = t16 = 0
+    if table is not None:
+        if buckets is None or table.ndim != 2:
+            raise ValueError("attention: a bias table [num_buckets, H] comes with its buckets")
+        if buckets.ndim != 1 or buckets.numel() % 2 == 0:
+            raise ValueError(f"attention: buckets must be [2 * radius + 1], got {tuple(buckets.shape)}")
+        _check_tensor(buckets, "attention buckets", torch.uint8, tuple(buckets.shape), dev)
+        radius, nb = buckets.numel() // 2, table.shape[0]
+        t16 = _param_type(table, "attention bias table", (nb, H), dev)
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    return AttentionArgs(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+        _ptr(q_segments), _ptr(k_segments), _ptr(prefix), _ptr(lengths), _ptr(table),
+        None if table is None else buckets.data_ptr(), B, Nq, Nk, H, Hk, D, radius, nb, scale, cap, int(causal), f32,
+        t16)
+
+
+def launch_attention(q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor | None = None, *,
+                     bias_table: Tensor | None = None, bias_buckets: Tensor | None = None,
+                     q_segments: Tensor | None = None, k_segments: Tensor | None = None, prefix: Tensor | None = None,
+                     lengths: Tensor | None = None, scale: float, cap: float = 0.0, causal: bool = False,
+                     ws: Tensor | None = None) -> Tensor:
+    """``out`` [B, Nq, H, D] (contiguous); ``lse`` [B, H, Nq] fp32 is what the backward pass needs."""
+    args = _attention_args(q, k, v, bias_table, bias_buckets, q_segments, k_segments, prefix, lengths, scale, cap, causal)
+    _check_tensor(out, "attention out", q.dtype, tuple(q.shape), q.device)
+    if lse is not None:
+        _check_tensor(lse, "attention lse", F32, (q.shape[0], q.shape[2], q.shape[1]), q.device)
+    with _on(q):
+        need = int(lib().bioemu_attention_workspace_bytes(args))
+        if need and (ws is None or ws.numel() < need):
+            ws = workspace(need, q.device)
+        rc = lib().bioemu_attention_fwd(args, out.data_ptr(), _ptr(lse), _ptr(ws),
+                                        ctypes.c_size_t(0 if ws is None else ws.numel()), _stream(q))
+    check(rc, "bioemu_attention_fwd")
+    return out
+
+
+def launch_attention_bwd(q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, dout: Tensor, dq: Tensor,
+                         dk: Tensor, dv: Tensor, dtable: Tensor | None = None, *, bias_table: Tensor | None = None,
+                         bias_buckets: Tensor | None = None, q_segments: Tensor | None = None,
+                         k_segments: Tensor | None = None, prefix: Tensor | None = None,
+                         lengths: Tensor | None = None, scale: float, cap: float = 0.0, causal: bool = False,
+                         ws: Tensor | None = None) -> None:
+    """Gradients of ``launch_attention`` (contiguous ``dq``, ``dk``, ``dv``; ``dtable`` may be None)."""
+    args = _attention_args(q, k, v, bias_table, bias_buckets, q_segments, k_segments, prefix, lengths, scale, cap, causal)
+    dev = q.device
+    _check_tensor(out, "attention out", q.dtype, tuple(q.shape), dev)
+    _check_tensor(lse, "attention lse", F32, (q.shape[0], q.shape[2], q.shape[1]), dev)
+    if dout.shape != q.shape or dout.dtype != q.dtype or dout.device != dev or dout.stride(3) != 1:
+        raise ValueError(f"attention_bwd: dout {dout.dtype} {tuple(dout.shape)} of q {q.dtype} {tuple(q.shape)}")
+    for t, like, name in ((dq, q, "dq"), (dk, k, "dk"), (dv, v, "dv")):
+        _check_tensor(t, f"attention {name}", q.dtype, tuple(like.shape), dev)
+    if dtable is not None:
+        if bias_table is None:
+            raise ValueError("attention_bwd: dtable without a bias table")
+        _check_tensor(dtable, "attention dtable", bias_table.dtype, tuple(bias_table.shape), dev)
+    st = dout.stride()
+    with _on(q):
+        need = int(lib().bioemu_attention_bwd_workspace_bytes(args, int(dtable is not None)))
+        if ws is None or ws.numel() < need:
+            ws = workspace(need, dev)
+        rc = lib().bioemu_attention_bwd(args, out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+                                        (ctypes.c_int64 * 3)(st[0], st[1], st[2]), dq.data_ptr(), dk.data_ptr(),
+                                        dv.data_ptr(), _ptr(dtable), ws.data_ptr(), ctypes.c_size_t(ws.numel()),
+                                        _stream(q))
+    check(rc, "bioemu_attention_bwd")
+
+
+def _attention(q: Tensor, k: Tensor, v: Tensor, table: Tensor | None, buckets: Tensor | None,
+               q_segments: Tensor | None, k_segments: Tensor | None, prefix: Tensor | None, lengths: Tensor | None,
+               scale: float, cap: float, causal: bool, train: bool) -> tuple[Tensor, Tensor]:
+    require_gpu(q, "attention")
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]) if train else (0,), dtype=F32, device=q.device)
+    launch_attention(_heads(q), _heads(k), _heads(v), out, lse if train else None, bias_table=table,
+                     bias_buckets=buckets, q_segments=q_segments, k_segments=k_segments, prefix=prefix,
+                     lengths=lengths, scale=scale, cap=cap, causal=causal)
+    return out, lse
+
+
+def _attention_backward(q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, dout: Tensor, table: Tensor | None,
+                        buckets: Tensor | None, q_segments: Tensor | None, k_segments: Tensor | None,
+                        prefix: Tensor | None, lengths: Tensor | None, scale: float, cap: float, causal: bool,
+                        want_table: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    dtable = torch.empty(table.shape if want_table else (0,), dtype=q.dtype if table is None else table.dtype,
+                         device=q.device)
+    if q.shape[0] == 0 or q.shape[1] == 0:
+        return dq, dk.zero_(), dv.zero_(), dtable.zero_()
+    launch_attention_bwd(_heads(q), _heads(k), _heads(v), out, lse, _heads(dout), dq, dk, dv,
+                         dtable if want_table else None, bias_table=table, bias_buckets=buckets,
+                         q_segments=q_segments, k_segments=k_segments, prefix=prefix, lengths=lengths, scale=scale,
+                         cap=cap, causal=causal)
+    return dq, dk, dv, dtable
+
+
+attention_backward = _Op("attention_backward", _attention_backward)
+
+
+@attention_backward.register_fake
+def _(q, k, v, out, lse, dout, table, buckets, q_segments, k_segments, prefix, lengths, scale, cap, causal, want_table):
+    return (q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape),
+            table.new_empty(table.shape) if want_table else q.new_empty((0,)))
+
+
+def _attention_save(ctx, inputs, output) -> None:
+    q, k, v, table, buckets, q_segments, k_segments, prefix, lengths, scale, cap, causal, _ = inputs
+    ctx.save_for_backward(q, k, v, output[0], output[1], table, buckets, q_segments, k_segments, prefix, lengths)
+    ctx.plain = scale, cap, causal
+
+
+def _attention_grad(ctx, dout, _):
+    q, k, v, out, lse, *rest = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    dq, dk, dv, dtable = attention_backward(q, k, v, out, lse, dout, *rest, *ctx.plain, need[3])
+    return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None,
+            dtable if need[3] else None) + (None,) * 9
+
+
+attention = _TrainOp("attention", _attention, _attention_save, _attention_grad)
+
+
+@attention.register_fake
+def _(q, k, v, table, buckets, q_segments, k_segments, prefix, lengths, scale, cap, causal, train):
+    return q.new_empty(q.shape), q.new_empty((q.shape[0], q.shape[2], q.shape[1]) if train else (0,), dtype=F32)

@@ -1,0 +1,279 @@
+// Shared parts of the attention kernels (attn_fwd.hip, attn_bwd.hip), for gfx950.
+//
+//   s(i, j) = cap tanh(scale q_i . k_j / cap) + bias[clamp(j - pos_i, -R, R)],   p = softmax over the allowed j
+//   pos_i = length - Nq + i;  allowed: j < length, segment_i == segment_j >= 0,
+//   and (not causal, or j <= pos_i, or j < prefix)
+//
+// One code for both types.  bf16 operands use v_mfma_f32_32x32x16_bf16; an fp32 operand of the same shape (8 values a
+// lane, 16 of the reduced index) is eight v_mfma_f32_32x32x2_f32, whose k index t takes element t of both lane halves:
+// the order of the reduced index is free as long as both operands use the same, so every layout below holds for both.
+// Scores are kept transposed to the operand that follows: a 32 x 32 accumulator (lane n = column, register 4 r + c =
+// row 8 r + 4 h + c) is, register for register, the B operand of the next product whose reduced index is its rows in
+// the order kappa(h, t) = 4 h + t, 8 + 4 h + t - 4; the A operand of that product comes out of LDS in that order by the
+// transposing 8-byte read (bf16) or by single reads (fp32).  So probabilities never leave registers.
+//
+// Tiles (rows of DP values, DP = 32, 64 or 128 >= D) go global -> LDS by buffer loads that write LDS.  Bytes past D and
+// rows past the end read as zero through the buffer bound, so no lane reads outside its tensor.  16-byte pieces are
+// XOR-swizzled by row.
+#pragma once
+
+#include "common.h"
+#include "internal.h"
+
+namespace bioemu {
+
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kAttnThreads = 256;
+constexpr int kAttnXcds = 8;
+constexpr int kMaxRadius = 512;     // of the distance bias
+constexpr int kListBlocks = 1024;   // key (or query) blocks listed at a time where segments are given
+constexpr float kInf = __builtin_inff();
+
+// The host's view of the arguments (bioemu_attention_args) with 32-bit sizes.
+struct AttnArgs {
+  const void *q, *k, *v;
+  int64_t qb, qn, qh, kb, kn, kh, vb, vn, vh;   // strides in elements
+  const int *q_seg, *k_seg, *prefix, *lengths;
+  const void* table;
+  const uint8_t* buckets;
+  float scale, cap;
+  int B, Nq, Nk, H, Hk, G, D, radius, nb, causal, table_bf16;
+};
+
+template <class T>
+struct Operand;
+template <>
+struct Operand<bf16> {
+  typedef bf16x8 frag;
+  static constexpr int kBlock = 64;   // rows of a staged tile
+};
+template <>
+struct Operand<float> {
+  typedef f32x8 frag;
+  static constexpr int kBlock = 32;
+};
+template <class T>
+using Frag = typename Operand<T>::frag;
+
+__device__ __forceinline__ f32x16 mfma16(bf16x8 a, bf16x8 b, f32x16 c) { return mfma32(a, b, c); }
+__device__ __forceinline__ f32x16 mfma16(f32x8 a, f32x8 b, f32x16 c) {
+#pragma unroll
+  for (int t = 0; t < 8; ++t) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[t], b[t], c, 0, 0, 0);
+  return c;
+}
+
+// Copies from memory into LDS: lane i's BYTES at byte voff of the source go to lds + BYTES i; zeros past its end.
+// Written as instructions: the compiler lets every later LDS read wait for a copy that it knows of, and these are to
+// land while the tile before them is worked on.  They have no result registers; whoever reads what they bring waits
+// for vmcnt first (and for the workgroup's barrier where another wave made the copy).  M0 is set and used within one
+// statement; nothing else in these kernels uses it.
+__device__ __forceinline__ u32x4 copy_source(const void* base, unsigned bytes) {
+  const uint64_t p = reinterpret_cast<uint64_t>(base);
+  return u32x4{(unsigned)p, (unsigned)(p >> 32) & 0xffffu, bytes, 0x00020000u};
+}
+template <int BYTES>
+__device__ __forceinline__ void copy_to_lds(u32x4 source, unsigned voff, void* lds) {
+  const unsigned at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  if constexpr (BYTES == 16)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(voff),
+                 "s"(source)
+                 : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(at), "v"(voff),
+                 "s"(source)
+                 : "memory");
+}
+
+// Row swizzle of 16-byte pieces, by pieces per row (a power of two).
+template <int CPR>
+__device__ __forceinline__ int attn_swz(int r) {
+  return CPR == 4 ? (r >> 2) & 3 : CPR == 8 ? (r >> 1) & 7 : r & 15;
+}
+
+// A tile in LDS: ROWS rows of DP values of T.
+template <class T, int DP, int ROWS>
+struct Tile {
+  static constexpr int RB = DP * (int)sizeof(T), CPR = RB / 16, BYTES = ROWS * RB;
+  __device__ static __forceinline__ int piece(int r, int c) { return r * RB + ((c ^ attn_swz<CPR>(r)) << 4); }
+
+  // Copies of 16 bytes: thread t of `threads` moves pieces t, t + threads, ...; their byte offsets in the source.
+  static constexpr int copies(int threads) { return ROWS * CPR / threads; }
+  template <int N>
+  __device__ static __forceinline__ void offsets(int t, int threads, int64_t stride, int D, unsigned (&voff)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int p = i * threads + t, r = p / CPR, c = (p % CPR) ^ attn_swz<CPR>(r);
+      voff[i] = c * 16 < D * (int)sizeof(T) ? (unsigned)(r * stride * (int)sizeof(T)) + c * 16 : 0xfffffff0u;
+    }
+  }
+  // `rows` (may be <= 0) rows exist behind `base`; wave-uniform arguments apart from voff.
+  template <int N>
+  __device__ static __forceinline__ void copy(const T* base, int rows, int64_t stride, int D, char* lds, int wave,
+                                              int threads, const unsigned (&voff)[N]) {
+    const int n = rows < ROWS ? rows : ROWS;
+    const unsigned bytes = n <= 0 ? 0 : (unsigned)(((n - 1) * stride + D) * (int64_t)sizeof(T));
+    const u32x4 rs = copy_source(base, bytes);
+#pragma unroll
+    for (int i = 0; i < N; ++i) copy_to_lds<16>(rs, voff[i], lds + (i * threads + wave * 64) * 16);
+  }
+
+  // Operand with the tile's rows as its outer index: row `r`, values 16 s + 8 h ..
+  __device__ static __forceinline__ Frag<T> rows(const char* lds, int r, int s, int h) {
+    if constexpr (sizeof(T) == 2) {
+      return *reinterpret_cast<const bf16x8*>(lds + piece(r, 2 * s + h));
+    } else {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(lds + piece(r, 4 * s + 2 * h));
+      const f32x4 b = *reinterpret_cast<const f32x4*>(lds + piece(r, 4 * s + 2 * h + 1));
+      return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    }
+  }
+  // Operand with the tile's columns d0 .. d0 + 31 as its outer index and rows r0 .. r0 + 15 in the order kappa.
+  __device__ static __forceinline__ Frag<T> cols(const char* lds, int r0, int d0, int lane) {
+    if constexpr (sizeof(T) == 2) {
+      const int r = r0 + 4 * (lane >> 5) + ((lane & 15) >> 2), d = d0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+      const char* p0 = lds + piece(r, d >> 3) + (d & 4) * 2;
+      const char* p1 = lds + piece(r + 8, d >> 3) + (d & 4) * 2;
+      typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p0);
+      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p1);
+      typedef short s16x8 __attribute__((ext_vector_type(8)));
+      return __builtin_bit_cast(bf16x8, (s16x8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+    } else {
+      f32x8 o;
+      const int d = d0 + (lane & 31), h = lane >> 5;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const int r = r0 + (t < 4 ? 4 * h + t : 4 + 4 * h + t);
+        o[t] = *reinterpret_cast<const float*>(lds + piece(r, d >> 2) + (d & 3) * 4);
+      }
+      return o;
+    }
+  }
+  // Zeroes row r (whoever calls owns the row's 16-byte pieces first, first + step, ...).
+  __device__ static __forceinline__ void clear(char* lds, int r, int first, int step) {
+    for (int c = first; c < CPR; c += step) *reinterpret_cast<u32x4*>(lds + piece(r, c)) = u32x4{0, 0, 0, 0};
+  }
+};
+
+// Eight values of an accumulator as the next product's operand: rows 16 s .. 16 s + 15 in the order kappa.
+template <class T>
+__device__ __forceinline__ Frag<T> as_operand(const float (&x)[16], int s) {
+  Frag<T> f;
+#pragma unroll
+  for (int t = 0; t < 8; ++t) f[t] = (T)x[8 * s + t];
+  return f;
+}
+
+// A row's values 16 s + 8 h .. + 7 from memory as the operand whose outer index is rows; zero past D or if !live.
+template <class T>
+__device__ __forceinline__ Frag<T> row_operand(const T* row, bool live, int s, int h, int D) {
+  Frag<T> f;
+  const int d = 16 * s + 8 * h;
+  if constexpr (sizeof(T) == 2) {
+    f = live && d < D ? *reinterpret_cast<const bf16x8*>(row + d) : bf16x8{};
+  } else {
+    const f32x4 a = live && d < D ? *reinterpret_cast<const f32x4*>(row + d) : f32x4{};
+    const f32x4 b = live && d + 4 < D ? *reinterpret_cast<const f32x4*>(row + d + 4) : f32x4{};
+    f = f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  }
+  return f;
+}
+
+// 64 32-bit values into LDS, zero from the n-th on (one wave).
+__device__ __forceinline__ void copy_ints(const void* src, int n, void* lds, int lane) {
+  copy_to_lds<4>(copy_source(src, n <= 0 ? 0 : (n < 64 ? n : 64) * 4), lane * 4, lds);
+}
+
+// tanh.  bf16 operands: by the hardware exponential, off by 2e-7, far below the rounding of q and k.
+template <class T>
+__device__ __forceinline__ float attn_tanh(float y) {
+  if constexpr (sizeof(T) == 2)
+    return 1.f - 2.f * fast_rcp(1.f + fast_exp2(y * (2.f * kLog2e)));
+  else
+    return tanhf(y);
+}
+
+// A bias in log2 units.  The type's lowest value stays finite (a row of such scores is a softmax over equal scores);
+// -infinity stays what it is.
+__device__ __forceinline__ float bias_log2(float b) {
+  const float v = b * kLog2e;
+  return v == -kInf && b != -kInf ? -__FLT_MAX__ : v;
+}
+
+__device__ __forceinline__ float table_value(const AttnArgs& a, int entry, int h) {
+  const int64_t at = (int64_t)min((int)a.buckets[entry], a.nb - 1) * a.H + h;
+  return bias_log2(a.table_bf16 ? (float)static_cast<const bf16*>(a.table)[at]
+                                : static_cast<const float*>(a.table)[at]);
+}
+
+// Workgroup minimum or maximum of an int (every thread gets it); red: 4 ints of LDS, free again after the next barrier.
+template <bool MAX>
+__device__ __forceinline__ int wg_extreme(int v, int* red) {
+#pragma unroll
+  for (int m = 32; m > 0; m /= 2) {
+    const int o = __shfl_xor(v, m);
+    v = MAX ? max(v, o) : min(v, o);
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  const int a = MAX ? max(red[0], red[1]) : min(red[0], red[1]), b = MAX ? max(red[2], red[3]) : min(red[2], red[3]);
+  return __builtin_amdgcn_readfirstlane(MAX ? max(a, b) : min(a, b));
+}
+
+// Blocks of a segment list that can hold an allowed pair.  An entry is the block's number with two flags.
+constexpr int kBlockMask = 0x0fffffff, kEntryFull = 0x10000000, kEntryHoles = 0x20000000;
+
+// Lists the blocks [c0, c1) of BLOCK rows of `seg` (`n` of them exist) that hold a segment in [lo, hi], in order;
+// full: every row has segment `lo` == `hi`; holes: some row exists in no segment (or past n).  All 256 threads;
+// returns the entries.  flags: one byte a block, list: one int a block.
+template <int BLOCK>
+__device__ __forceinline__ int list_blocks(const int* __restrict__ seg, int n, int lo, int hi, int c0, int c1,
+                                           uint8_t* flags, int* list, int* red) {
+  const int lane = threadIdx.x & 63, wave = wave_id();
+  constexpr int PER = 64 / BLOCK;   // blocks one wave reads at a time
+  for (int b0 = c0 + wave * PER; b0 < c1; b0 += 4 * PER) {
+    const int r = b0 * BLOCK + lane;
+    const int s = r < n ? seg[r] : -1;
+    const uint64_t hit = __ballot(s >= 0 && s >= lo && s <= hi), one = __ballot(lo == hi && s == lo),
+                   hole = __ballot(s < 0);
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const uint64_t m = BLOCK == 64 ? ~0ull : (uint64_t)0xffffffffu << (32 * p);
+      if (lane == 0 && b0 + p < c1)
+        flags[b0 + p - c0] =
+            (uint8_t)(((hit & m) != 0 ? 1 : 0) | ((one & m) == m ? 2 : 0) | ((hole & m) != 0 ? 4 : 0));
+    }
+  }
+  __syncthreads();
+  if (wave == 0) {
+    int at = 0;
+    for (int b0 = 0; b0 < c1 - c0; b0 += 64) {
+      const int f = b0 + lane < c1 - c0 ? flags[b0 + lane] : 0;
+      const uint64_t m = __ballot(f & 1);
+      if (f & 1)
+        list[at + __popcll(m & ((1ull << lane) - 1))] =
+            (c0 + b0 + lane) | (f & 2 ? kEntryFull : 0) | (f & 4 ? kEntryHoles : 0);
+      at += __popcll(m);
+    }
+    if (lane == 0) red[0] = at;
+  }
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(red[0]);
+}
+
+// XCD-aware order: workgroup w runs on XCD w % 8, each XCD gets a contiguous range of the items (so the workgroups
+// that read the same keys share its L2); -1 for padding workgroups.
+__device__ __forceinline__ int attn_item(int total) {
+  const int w = blockIdx.x, per = (total + kAttnXcds - 1) / kAttnXcds;
+  const int item = (w % kAttnXcds) * per + w / kAttnXcds;
+  return w / kAttnXcds < per && item < total ? item : -1;
+}
+inline unsigned attn_grid(int64_t total) { return (unsigned)(round_up(total, kAttnXcds)); }
+
+// Checks the arguments both directions share and lays them out (attn_fwd.hip).
+int attn_args(const char* what, const bioemu_attention_args* in, AttnArgs* out);
+
+}  // namespace bioemu

@@ -1,0 +1,576 @@
+// Attention forward, for gfx950 (formulas and layouts: attn.h).
+//
+// attn_fwd: a workgroup owns 128 queries of one head, a wave 32 of them; 64-key (bf16) or 32-key (fp32) tiles of K and
+// V are staged in LDS, double-buffered, and shared by the four waves.  Per wave and 32 keys: S^T = K Q^T (DP / 16
+// MFMAs), the running maximum and sum of the softmax per lane (a lane is a query; its other half joins by one
+// shuffle), O^T += V^T P^T with P straight from registers.  The maximum moves only when a score exceeds it by 2^8:
+// until then weights are at most 256 and nothing is rescaled.
+// attn_few: up to 32 (query, head of a group) rows share their keys, as single tokens over a cache do: the rows fill
+// one MFMA operand, every wave takes 32-key tiles of its own (K and V read once, bound by HBM), and the waves join.
+// Both may split the keys over workgroups (few rows, long axis); attn_join adds the parts.
+#include "attn.h"
+
+namespace bioemu {
+namespace {
+
+constexpr int kWaveRows = 32;
+constexpr int kGroupRows = 128;
+constexpr float kRescale = 8.f;   // log2 of the largest weight before the maximum moves
+
+// Per-row partial results of one split: [rows][D] values and [rows][2] (maximum in log2 units, sum).
+struct Parts {
+  float *o, *ml;
+};
+
+__device__ __forceinline__ float row_log_sum(float m, float l) { return l > 0.f ? m + __log2f(l) : kInf; }
+
+template <class T, int DP>
+__global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a, T* __restrict__ out,
+                                                                float* __restrict__ lse, Parts parts, int splits,
+                                                                int qblocks, int total) {
+  constexpr int KB = Operand<T>::kBlock, SUB = KB / 32, STEPS = DP / 16, DB = DP / 32;
+  typedef Tile<T, DP, KB> KV;
+  constexpr int CP = KV::copies(kAttnThreads);
+  __shared__ __attribute__((aligned(1024))) char tiles[2][2][KV::BYTES];
+  __shared__ int segs[2][64];
+  __shared__ float lut[2 * kMaxRadius + 1];
+  __shared__ int list[kListBlocks];
+  __shared__ uint8_t flags[kListBlocks];
+  __shared__ int red[4];
+
+  const int item = attn_item(total);
+  if (item < 0) return;
+  const int lane = threadIdx.x & 63, wave = wave_id(), ln = lane & 31, lh = lane >> 5;
+  const int qblk = qblocks - 1 - item % qblocks;   // long rows of a causal mask first
+  const int rest = item / qblocks, split = rest % splits, bh = rest / splits, h = bh % a.H, b = bh / a.H;
+  const int hk = h / a.G;
+  const int length = a.lengths ? min(max(a.lengths[b], 0), a.Nk) : a.Nk;
+  const int prefix = a.prefix ? a.prefix[b] : 0;
+  const bool seg = a.q_seg != nullptr;
+
+  const int i = qblk * kGroupRows + wave * kWaveRows + ln;
+  const bool live = i < a.Nq;
+  const int pos = length - a.Nq + i;
+  const int qseg = seg && live ? a.q_seg[(int64_t)b * a.Nq + i] : 0;
+  // keys below lim are allowed (their segment aside); rows past the last one restrict nothing
+  int lim = a.causal ? min(max(pos + 1, prefix), length) : length;
+  if (qseg < 0) lim = 0;
+  const int seg_lo = seg ? wg_extreme<false>(live && qseg >= 0 ? qseg : 0x7fffffff, red) : 0;
+  const int seg_hi = seg ? wg_extreme<true>(live ? qseg : -1, red) : 0;
+  const int wg_max = wg_extreme<true>(live ? lim : 0, red);
+  int wave_min = live ? lim : 0x7fffffff, wave_max = live ? lim : 0;
+#pragma unroll
+  for (int m = 16; m > 0; m /= 2) {
+    wave_min = min(wave_min, __shfl_xor(wave_min, m));
+    wave_max = max(wave_max, __shfl_xor(wave_max, m));
+  }
+  wave_min = __builtin_amdgcn_readfirstlane(wave_min);
+  wave_max = __builtin_amdgcn_readfirstlane(wave_max);
+  const int wave_pos = __builtin_amdgcn_readfirstlane(pos);   // of the wave's first row
+  if (!live) lim = 0x7fffffff;
+
+  if (a.table)
+    for (int e = threadIdx.x; e < 2 * a.radius + 1; e += kAttnThreads) lut[e] = table_value(a, e, h);
+
+  Frag<T> qf[STEPS];
+  {
+    const T* row = static_cast<const T*>(a.q) + b * a.qb + (int64_t)(live ? i : 0) * a.qn + h * a.qh;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) qf[s] = row_operand<T>(row, live, s, lh, a.D);
+  }
+  const T* kbase = static_cast<const T*>(a.k) + b * a.kb + hk * a.kh;
+  const T* vbase = static_cast<const T*>(a.v) + b * a.vb + hk * a.vh;
+  unsigned koff[CP], voff[CP];
+  KV::offsets(threadIdx.x, kAttnThreads, a.kn, a.D, koff);
+  KV::offsets(threadIdx.x, kAttnThreads, a.vn, a.D, voff);
+  const int* kseg = seg ? a.k_seg + (int64_t)b * a.Nk : nullptr;
+
+  f32x16 acc[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) acc[d] = zero16();
+  float m = -kInf, mref = 0.f, l = 0.f;   // the running maximum, what weights are taken against, their sum
+  const float s_scale = a.cap > 0.f ? a.scale / a.cap : a.scale * kLog2e;
+  const float s_cap = a.cap * kLog2e;
+
+  auto stage = [&](int entry, int buf) {
+    const int k0 = (entry & kBlockMask) * KB;
+    KV::copy(kbase + (int64_t)k0 * a.kn, length - k0, a.kn, a.D, tiles[buf][0], wave, kAttnThreads, koff);
+    KV::copy(vbase + (int64_t)k0 * a.vn, length - k0, a.vn, a.D, tiles[buf][1], wave, kAttnThreads, voff);
+    if (seg && wave == 0) copy_ints(kseg + k0, length - k0, segs[buf], lane);
+  };
+
+  const int blocks = (wg_max + KB - 1) / KB;
+  for (int c0 = 0; c0 < blocks; c0 += kListBlocks) {
+    const int c1 = seg ? min(blocks, c0 + kListBlocks) : blocks;
+    const int n = seg ? list_blocks<KB>(kseg, length, seg_lo, seg_hi, c0, c1, flags, list, red) : blocks;
+    const int t0 = (int)((int64_t)n * split / splits), t1 = (int)((int64_t)n * (split + 1) / splits);
+    auto entry = [&](int t) { return seg ? __builtin_amdgcn_readfirstlane(list[t]) : t | kEntryFull; };
+    if (t0 < t1) stage(entry(t0), t0 & 1);
+    for (int t = t0; t < t1; ++t) {
+      const int e = entry(t), buf = t & 1, k0 = (e & kBlockMask) * KB;
+      __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's copies landed
+      __syncthreads();                       // ... and everyone's; the other buffer is free
+      if (t + 1 < t1) stage(entry(t + 1), buf ^ 1);
+      if (e & kEntryHoles) {
+        // keys in no segment have weight 0, and 0 times what their values hold has to be 0
+        const int r = threadIdx.x / (kAttnThreads / KB);
+        if (segs[buf][r] < 0) KV::clear(tiles[buf][1], r, threadIdx.x % (kAttnThreads / KB), kAttnThreads / KB);
+        __syncthreads();
+      }
+      if (k0 >= wave_max) continue;
+      const char *kt = tiles[buf][0], *vt = tiles[buf][1];
+      float x[SUB][16];
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        f32x16 s = zero16();
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) s = mfma16(KV::rows(kt, 32 * u + ln, st, lh), qf[st], s);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[u][r] = s[r] * s_scale;
+        if (a.cap > 0.f)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[u][r] = s_cap * attn_tanh<T>(x[u][r]);
+        if (a.table) {
+          const int rel0 = k0 + 32 * u - wave_pos;   // of the wave's first query and the first key
+          if (rel0 - 31 >= a.radius || rel0 + 31 <= -a.radius) {
+            const float far = lut[rel0 > 0 ? 2 * a.radius : 0];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[u][r] += far;
+          } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int rel = rel0 - ln + 8 * (r >> 2) + 4 * lh + (r & 3);
+              x[u][r] += lut[min(max(rel, -a.radius), a.radius) + a.radius];
+            }
+          }
+        }
+      }
+      if (k0 + KB > wave_min || !(e & kEntryFull)) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int kk = 32 * u + 8 * (r >> 2) + 4 * lh + (r & 3);
+            const bool ok = (k0 + kk < lim) & (!seg | (segs[buf][kk] == qseg));
+            x[u][r] = ok ? x[u][r] : -kInf;
+          }
+      }
+      float mx = x[0][0];
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, x[u][r]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      if (__ballot(mx > m + kRescale)) {
+        const float mn = fmaxf(m, mx), to = mn == -kInf ? 0.f : mn;
+        const float f = fast_exp2(m - to);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[d][r] *= f;
+        l *= f;
+        m = mn;
+        mref = to;
+      }
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          x[u][r] = fast_exp2(x[u][r] - mref);
+          l += x[u][r];
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const Frag<T> p = as_operand<T>(x[u], s);
+#pragma unroll
+          for (int d = 0; d < DB; ++d) acc[d] = mfma16(KV::cols(vt, 32 * u + 16 * s, 32 * d, lane), p, acc[d]);
+        }
+      }
+    }
+    __syncthreads();   // the list and both buffers are free
+  }
+
+  l += __shfl_xor(l, 32);
+  if (!live) return;
+  const int64_t row = ((int64_t)b * a.Nq + i) * a.H + h;
+  if (splits == 1) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* po = out + row * a.D;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int at = 32 * d + 8 * r + 4 * lh;
+        if (at < a.D) {
+          typedef T quad __attribute__((ext_vector_type(4)));
+          quad v;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[c] = (T)(acc[d][4 * r + c] * inv);
+          *reinterpret_cast<quad*>(po + at) = v;
+        }
+      }
+    if (lse && lh == 0) lse[((int64_t)b * a.H + h) * a.Nq + i] = row_log_sum(mref, l);
+  } else {
+    const int64_t rows = (int64_t)a.B * a.Nq * a.H, at0 = split * rows + row;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int at = 32 * d + 8 * r + 4 * lh;
+        if (at < a.D)
+          *reinterpret_cast<f32x4*>(parts.o + at0 * a.D + at) =
+              f32x4{acc[d][4 * r], acc[d][4 * r + 1], acc[d][4 * r + 2], acc[d][4 * r + 3]};
+      }
+    if (lh == 0) {
+      parts.ml[2 * at0] = l == 0.f ? -kInf : mref;
+      parts.ml[2 * at0 + 1] = l;
+    }
+  }
+}
+
+// Waves of attn_few: each has two K and two V tiles of its own.
+template <class T>
+constexpr int few_waves() {
+  return sizeof(T) == 2 ? 4 : 2;
+}
+
+template <class T, int DP>
+__global__ __launch_bounds__(64 * few_waves<T>()) void attn_few_kernel(const AttnArgs a, T* __restrict__ out,
+                                                                       float* __restrict__ lse, Parts parts,
+                                                                       int splits, int total) {
+  constexpr int W = few_waves<T>(), STEPS = DP / 16, DB = DP / 32;
+  typedef Tile<T, DP, 32> KV;
+  constexpr int CP = KV::copies(64);
+  __shared__ __attribute__((aligned(1024))) char tiles[W][2][2][KV::BYTES];
+  __shared__ float ml[W][2][32];
+
+  const int item = attn_item(total);
+  if (item < 0) return;
+  const int lane = threadIdx.x & 63, wave = wave_id(), ln = lane & 31, lh = lane >> 5;
+  const int split = item % splits, bh = item / splits, hk = bh % a.Hk, b = bh / a.Hk;
+  const int rows = a.Nq * a.G;
+  const int length = a.lengths ? min(max(a.lengths[b], 0), a.Nk) : a.Nk;
+  const int prefix = a.prefix ? a.prefix[b] : 0;
+  const bool seg = a.q_seg != nullptr;
+
+  // lane n: query i and head g of the group
+  const bool live = ln < rows;
+  const int i = live ? ln / a.G : 0, h = hk * a.G + (live ? ln - i * a.G : 0);
+  const int pos = length - a.Nq + i;
+  const int qseg = seg ? a.q_seg[(int64_t)b * a.Nq + i] : 0;
+  int lim = a.causal ? min(max(pos + 1, prefix), length) : length;
+  if (qseg < 0 || !live) lim = 0;
+  int top = lim, low = live ? lim : 0x7fffffff;
+#pragma unroll
+  for (int m = 16; m > 0; m /= 2) {
+    top = max(top, __shfl_xor(top, m));
+    low = min(low, __shfl_xor(low, m));
+  }
+  top = __builtin_amdgcn_readfirstlane(top);
+  low = __builtin_amdgcn_readfirstlane(low);
+
+  Frag<T> qf[STEPS];
+  {
+    const T* row = static_cast<const T*>(a.q) + b * a.qb + (int64_t)i * a.qn + h * a.qh;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) qf[s] = row_operand<T>(row, live, s, lh, a.D);
+  }
+  const float far_lo = a.table ? table_value(a, 0, h) : 0.f, far_hi = a.table ? table_value(a, 2 * a.radius, h) : 0.f;
+  const T* kbase = static_cast<const T*>(a.k) + b * a.kb + hk * a.kh;
+  const T* vbase = static_cast<const T*>(a.v) + b * a.vb + hk * a.vh;
+  unsigned koff[CP], voff[CP];
+  KV::offsets(lane, 64, a.kn, a.D, koff);
+  KV::offsets(lane, 64, a.vn, a.D, voff);
+  const int* kseg = seg ? a.k_seg + (int64_t)b * a.Nk : nullptr;
+
+  f32x16 acc[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) acc[d] = zero16();
+  float m = -kInf, mref = 0.f, l = 0.f;
+  const float s_scale = a.cap > 0.f ? a.scale / a.cap : a.scale * kLog2e;
+  const float s_cap = a.cap * kLog2e;
+
+  const int blocks = (top + 31) / 32;
+  const int t0 = (int)((int64_t)blocks * split / splits), t1 = (int)((int64_t)blocks * (split + 1) / splits);
+  auto stage = [&](int t, int buf) {
+    const int k0 = t * 32;
+    KV::copy(kbase + (int64_t)k0 * a.kn, length - k0, a.kn, a.D, tiles[wave][buf][0], 0, 64, koff);
+    KV::copy(vbase + (int64_t)k0 * a.vn, length - k0, a.vn, a.D, tiles[wave][buf][1], 0, 64, voff);
+  };
+  int buf = 0;
+  if (t0 + wave < t1) stage(t0 + wave, 0);
+  for (int t = t0 + wave; t < t1; t += W, buf ^= 1) {
+    const int k0 = t * 32;
+    if (t + W < t1) {
+      stage(t + W, buf ^ 1);
+      __builtin_amdgcn_s_waitcnt(0x0f70 | ((2 * CP) & 15) | (((2 * CP) >> 4) << 14));   // all but the next tile's
+    } else {
+      __builtin_amdgcn_s_waitcnt(0x0f70);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    char *kt = tiles[wave][buf][0], *vt = tiles[wave][buf][1];
+    if (seg) {
+      // two lanes a key: values of a key in no segment are zeroed (0 times them has to be 0)
+      const int r = lane >> 1;
+      if (k0 + r < length && kseg[k0 + r] < 0) KV::clear(vt, r, lane & 1, 2);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    f32x16 s = zero16();
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) s = mfma16(KV::rows(kt, ln, st, lh), qf[st], s);
+    float x[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = s[r] * s_scale;
+    if (a.cap > 0.f)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = s_cap * attn_tanh<T>(x[r]);
+    if (a.table) {
+      const int rel0 = k0 - (length - a.Nq);   // the first key from the first query
+      if (rel0 - (a.Nq - 1) >= a.radius || rel0 + 31 <= -a.radius) {
+        const float far = rel0 > 0 ? far_hi : far_lo;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] += far;
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int rel = k0 + 8 * (r >> 2) + 4 * lh + (r & 3) - pos;
+          x[r] += table_value(a, min(max(rel, -a.radius), a.radius) + a.radius, h);
+        }
+      }
+    }
+    if (k0 + 32 > low || seg) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int j = k0 + 8 * (r >> 2) + 4 * lh + (r & 3);
+        bool ok = j < lim;
+        if (seg) ok = ok && kseg[min(j, a.Nk - 1)] == qseg;
+        x[r] = ok ? x[r] : -kInf;
+      }
+    }
+    float mx = x[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, x[r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    if (__ballot(mx > m + kRescale)) {
+      const float mn = fmaxf(m, mx), to = mn == -kInf ? 0.f : mn;
+      const float f = fast_exp2(m - to);
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] *= f;
+      l *= f;
+      m = mn;
+      mref = to;
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      x[r] = fast_exp2(x[r] - mref);
+      l += x[r];
+    }
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const Frag<T> p = as_operand<T>(x, st);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) acc[d] = mfma16(KV::cols(vt, 16 * st, 32 * d, lane), p, acc[d]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the tile is read before the copy after next
+  }
+
+  // the waves' parts through LDS (over the tiles: W x 32 x DP floats are half of them at most)
+  l += __shfl_xor(l, 32);
+  __syncthreads();
+  float* sh = reinterpret_cast<float*>(&tiles[0][0][0][0]);
+  if (lh == 0) {
+    ml[wave][0][ln] = l == 0.f ? -kInf : mref;
+    ml[wave][1][ln] = l;
+  }
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      *reinterpret_cast<f32x4*>(sh + (wave * 32 + ln) * DP + 32 * d + 8 * r + 4 * lh) =
+          f32x4{acc[d][4 * r], acc[d][4 * r + 1], acc[d][4 * r + 2], acc[d][4 * r + 3]};
+  __syncthreads();
+  const int64_t all = (int64_t)a.B * a.Nq * a.H;
+  for (int k = threadIdx.x; k < rows * DP; k += 64 * W) {
+    const int r = k / DP, d = k - r * DP;
+    if (d >= a.D) continue;
+    float top_m = -kInf;
+#pragma unroll
+    for (int w = 0; w < W; ++w) top_m = fmaxf(top_m, ml[w][0][r]);
+    const float to = top_m == -kInf ? 0.f : top_m;
+    float o = 0.f, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float f = fast_exp2(ml[w][0][r] - to);
+      o += f * sh[(w * 32 + r) * DP + d];
+      sum += f * ml[w][1][r];
+    }
+    const int qi = r / a.G, qh = hk * a.G + r - qi * a.G;
+    const int64_t row = ((int64_t)b * a.Nq + qi) * a.H + qh;
+    if (splits == 1) {
+      out[row * a.D + d] = (T)(sum == 0.f ? 0.f : o / sum);
+      if (lse && d == 0) lse[((int64_t)b * a.H + qh) * a.Nq + qi] = row_log_sum(to, sum);
+    } else {
+      parts.o[(split * all + row) * a.D + d] = o;
+      if (d == 0) {
+        parts.ml[2 * (split * all + row)] = sum == 0.f ? -kInf : to;
+        parts.ml[2 * (split * all + row) + 1] = sum;
+      }
+    }
+  }
+}
+
+// One wave a row: the splits' parts added in order.
+template <class T>
+__global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const AttnArgs a, Parts parts, int splits,
+                                                                 T* __restrict__ out, float* __restrict__ lse) {
+  const int64_t rows = (int64_t)a.B * a.Nq * a.H, row = (int64_t)blockIdx.x * 4 + wave_id();
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 63;
+  float top = -kInf;
+  for (int s = lane; s < splits; s += 64) top = fmaxf(top, parts.ml[2 * (s * rows + row)]);
+#pragma unroll
+  for (int m = 32; m > 0; m /= 2) top = fmaxf(top, __shfl_xor(top, m));
+  const float to = top == -kInf ? 0.f : top;
+  float o0 = 0.f, o1 = 0.f, sum = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float* ml = parts.ml + 2 * (s * rows + row);
+    const float* po = parts.o + (s * rows + row) * a.D;
+    const float f = fast_exp2(ml[0] - to);
+    sum += f * ml[1];
+    if (lane < a.D) o0 += f * po[lane];
+    if (lane + 64 < a.D) o1 += f * po[lane + 64];
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  if (lane < a.D) out[row * a.D + lane] = (T)(o0 * inv);
+  if (lane + 64 < a.D) out[row * a.D + lane + 64] = (T)(o1 * inv);
+  if (lse && lane == 0) {
+    const int64_t bi = row / a.H, h = row - bi * a.H, b = bi / a.Nq, i = bi - b * a.Nq;
+    lse[(b * a.H + h) * a.Nq + i] = row_log_sum(to, sum);
+  }
+}
+
+bool few_rows(const AttnArgs& a) { return a.Nq * a.G <= 32; }
+
+// Workgroups that the keys of a query block are split over: as many as bring the launch to two workgroups a CU, each
+// with at least `least` keys.
+int key_splits(const AttnArgs& a, bool f32) {
+  const bool few = few_rows(a);
+  const int64_t base = few ? (int64_t)a.B * a.Hk : (int64_t)a.B * a.H * ((a.Nq + kGroupRows - 1) / kGroupRows);
+  const int64_t least = few ? (f32 ? 128 : 256) : 512;
+  const int64_t want = (2 * (int64_t)compute_units() + base - 1) / base;
+  const int64_t most = (a.Nk + least - 1) / least;
+  const int64_t s = want < most ? want : most;
+  return s < 1 ? 1 : (int)s;
+}
+
+size_t parts_bytes(const AttnArgs& a, int splits) {
+  return splits == 1 ? 0 : (size_t)splits * a.B * a.Nq * a.H * (a.D + 2) * sizeof(float);
+}
+
+template <class T>
+int launch_fwd(const AttnArgs& a, void* o, float* lse, void* ws, hipStream_t stream) {
+  const int splits = key_splits(a, sizeof(T) == 4);
+  const int64_t rows = (int64_t)a.B * a.Nq * a.H;
+  Parts parts{static_cast<float*>(ws), nullptr};
+  parts.ml = parts.o ? parts.o + (int64_t)splits * rows * a.D : nullptr;
+  T* out = static_cast<T*>(o);
+  const int dp = a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128;
+  if (few_rows(a)) {
+    const int64_t total = (int64_t)a.B * a.Hk * splits;
+    KernelTimerScope timer("attn_few", stream);
+    const dim3 grid(attn_grid(total)), wg(64 * few_waves<T>());
+    if (dp == 32)
+      attn_few_kernel<T, 32><<<grid, wg, 0, stream>>>(a, out, lse, parts, splits, (int)total);
+    else if (dp == 64)
+      attn_few_kernel<T, 64><<<grid, wg, 0, stream>>>(a, out, lse, parts, splits, (int)total);
+    else
+      attn_few_kernel<T, 128><<<grid, wg, 0, stream>>>(a, out, lse, parts, splits, (int)total);
+    if (const int rc = check_launch("attn_few")) return rc;
+  } else {
+    const int qblocks = (a.Nq + kGroupRows - 1) / kGroupRows;
+    const int64_t total = (int64_t)a.B * a.H * splits * qblocks;
+    KernelTimerScope timer("attn_fwd", stream);
+    const dim3 grid(attn_grid(total));
+    if (dp == 32)
+      attn_fwd_kernel<T, 32><<<grid, kAttnThreads, 0, stream>>>(a, out, lse, parts, splits, qblocks, (int)total);
+    else if (dp == 64)
+      attn_fwd_kernel<T, 64><<<grid, kAttnThreads, 0, stream>>>(a, out, lse, parts, splits, qblocks, (int)total);
+    else
+      attn_fwd_kernel<T, 128><<<grid, kAttnThreads, 0, stream>>>(a, out, lse, parts, splits, qblocks, (int)total);
+    if (const int rc = check_launch("attn_fwd")) return rc;
+  }
+  if (splits == 1) return BIOEMU_OK;
+  KernelTimerScope timer("attn_join", stream);
+  attn_join_kernel<T><<<dim3((unsigned)((rows + 3) / 4)), kAttnThreads, 0, stream>>>(a, parts, splits, out, lse);
+  return check_launch("attn_join");
+}
+
+}  // namespace
+
+int attn_args(const char* what, const bioemu_attention_args* in, AttnArgs* a) {
+  if (!in) return set_error(BIOEMU_ERR_INVALID_ARG, "%s: null arguments", what);
+  const int64_t B = in->B, Nq = in->Nq, Nk = in->Nk, H = in->H, Hk = in->Hk, D = in->D;
+  if (B < 0 || Nq < 0 || Nk < 0 || H < 1 || Hk < 1 || D < 1)
+    return set_error(BIOEMU_ERR_INVALID_ARG, "%s: B=%ld, Nq=%ld, Nk=%ld, H=%ld, Hk=%ld, D=%ld", what, (long)B, (long)Nq,
+                     (long)Nk, (long)H, (long)Hk, (long)D);
+  if (H % Hk) return set_error(BIOEMU_ERR_INVALID_ARG, "%s: %ld heads over %ld key heads", what, (long)H, (long)Hk);
+  if (D % 8 || D > 128)
+    return set_error(BIOEMU_ERR_UNSUPPORTED, "%s: head width %ld (a multiple of 8, at most 128)", what, (long)D);
+  const int64_t most = int64_t(1) << 27;
+  if (Nq > most || Nk > most || B * H > (1 << 20) || B * Nq * H >= (int64_t(1) << 31) ||
+      B * H * ((Nq + 127) / 128) * 512 >= (int64_t(1) << 31) || B * H * ((Nk + 127) / 128) >= (int64_t(1) << 31))
+    return set_error(BIOEMU_ERR_UNSUPPORTED, "%s: B=%ld, H=%ld, Nq=%ld, Nk=%ld are too many", what, (long)B, (long)H,
+                     (long)Nq, (long)Nk);
+  if (!(in->scale > -kInf && in->scale < kInf) || !(in->cap >= 0.f && in->cap < kInf))
+    return set_error(BIOEMU_ERR_INVALID_ARG, "%s: scale %g, cap %g", what, (double)in->scale, (double)in->cap);
+  const int64_t per = in->f32 ? 4 : 8, far = int64_t(1) << 23;
+  const void* ptr[3] = {in->q, in->k, in->v};
+  const int64_t* st[3] = {in->q_stride, in->k_stride, in->v_stride};
+  const int64_t len[3] = {Nq, Nk, Nk};
+  for (int t = 0; t < 3; ++t) {
+    if (!ptr[t] && B * len[t] > 0) return set_error(BIOEMU_ERR_INVALID_ARG, "%s: null pointer", what);
+    if (!aligned16(ptr[t]) || st[t][0] % per || st[t][1] % per || st[t][2] % per)
+      return set_error(BIOEMU_ERR_INVALID_ARG, "%s: rows of q, k and v start at 16-byte addresses", what);
+    if (st[t][1] > far || (len[t] > 1 && st[t][1] < D))
+      return set_error(BIOEMU_ERR_UNSUPPORTED, "%s: row stride %ld (head width to 2^23)", what, (long)st[t][1]);
+  }
+  if ((in->q_segments == nullptr) != (in->k_segments == nullptr))
+    return set_error(BIOEMU_ERR_INVALID_ARG, "%s: segments of queries and of keys come together", what);
+  if (in->bias_table) {
+    if (!in->bias_buckets) return set_error(BIOEMU_ERR_INVALID_ARG, "%s: null pointer", what);
+    if (in->radius < 0 || in->radius > kMaxRadius || in->num_buckets < 1 || in->num_buckets > 256)
+      return set_error(BIOEMU_ERR_UNSUPPORTED, "%s: radius %ld (at most %d), %ld buckets (at most 256)", what,
+                       (long)in->radius, kMaxRadius, (long)in->num_buckets);
+  }
+  *a = AttnArgs{in->q, in->k, in->v, in->q_stride[0], in->q_stride[1], in->q_stride[2], in->k_stride[0],
+                in->k_stride[1], in->k_stride[2], in->v_stride[0], in->v_stride[1], in->v_stride[2], in->q_segments,
+                in->k_segments, in->prefix, in->lengths, in->bias_table, in->bias_buckets, in->scale, in->cap, (int)B,
+                (int)Nq, (int)Nk, (int)H, (int)Hk, (int)(H / Hk), (int)D, (int)in->radius, (int)in->num_buckets,
+                in->causal, in->table_bf16};
+  return BIOEMU_OK;
+}
+
+}  // namespace bioemu
+
+using namespace bioemu;
+
+extern "C" size_t bioemu_attention_workspace_bytes(const bioemu_attention_args* args) {
+  AttnArgs a;
+  if (attn_args("attention", args, &a) || a.B == 0 || a.Nq == 0) return 0;
+  return parts_bytes(a, key_splits(a, args->f32 != 0));
+}
+
+extern "C" int bioemu_attention_fwd(const bioemu_attention_args* args, void* o, float* lse, void* workspace,
+                                    size_t workspace_bytes, hipStream_t stream) {
+  AttnArgs a;
+  if (const int rc = attn_args("attention", args, &a)) return rc;
+  if (a.B == 0 || a.Nq == 0) return BIOEMU_OK;
+  if (!o || !aligned16(o)) return set_error(BIOEMU_ERR_INVALID_ARG, "attention: o must be 16-byte aligned");
+  const size_t need = parts_bytes(a, key_splits(a, args->f32 != 0));
+  if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need))
+    return set_error(BIOEMU_ERR_WORKSPACE, "attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  return args->f32 ? launch_fwd<float>(a, o, lse, workspace, stream) : launch_fwd<bf16>(a, o, lse, workspace, stream);
+}

@@ -494,6 +494,46 @@ int bioemu_relpos_bwd(const void* dout, const uint8_t* buckets, const int32_t* p
                       void* dtable, void* workspace, size_t workspace_bytes, int64_t B, int64_t N, int64_t C,
                       int64_t radius, int64_t num_buckets, int f32, int table_bf16, hipStream_t stream);
 
+/*
+ * Attention over q [B, Nq, H, D], k and v [B, Nk, Hk, D] (H a multiple of Hk:
+ * H / Hk query heads share a key head), with its gradients:
+ *   s(i,j) = cap tanh(scale q_i.k_j / cap) + bias_table[bias_buckets[clamp(j - pos_i, -radius, radius) + radius], h]
+ *   p = softmax over the allowed j,  o_i = sum_j p_j v_j  (0 where no j is allowed)
+ *   pos_i = length - Nq + i (the queries are the last Nq positions)
+ * Allowed: j < length; segments equal and not negative, where given; where
+ * causal, also j <= pos_i or j < prefix.  A key at or past its length, or of a
+ * negative segment, may hold anything.  cap = 0: no tanh.
+ * Strides (batch, row, head) are in elements, values of a head adjacent, every
+ * row at a 16-byte address, the row stride between D and 2^23.  D is a
+ * multiple of 8 up to 128, radius at most 512, num_buckets at most 256; bucket
+ * values past the table count as its last row.  f32: types of q, k, v, o and
+ * their gradients.  Every pointer of the second group may be NULL.
+ */
+typedef struct bioemu_attention_args {
+  const void *q, *k, *v;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  const int32_t *q_segments, *k_segments; /* [B, Nq], [B, Nk]; both or none */
+  const int32_t *prefix, *lengths;        /* [B] each; lengths are taken into 0 .. Nk (NULL: Nk) */
+  const void* bias_table;                 /* [num_buckets, H] */
+  const uint8_t* bias_buckets;            /* [2 radius + 1] */
+  int64_t B, Nq, Nk, H, Hk, D, radius, num_buckets;
+  float scale, cap;
+  int causal, f32, table_bf16;
+} bioemu_attention_args;
+
+/* o: [B, Nq, H, D] contiguous; lse: NULL or [B, H, Nq] fp32, log2 of the sum of 2^(s log2 e), +infinity for rows that
+ * see nothing (what the backward pass reads). */
+size_t bioemu_attention_workspace_bytes(const bioemu_attention_args* args);
+int bioemu_attention_fwd(const bioemu_attention_args* args, void* o, float* lse, void* workspace,
+                         size_t workspace_bytes, hipStream_t stream);
+
+/* Gradients.  dout: strides as above; dq [B, Nq, H, D], dk and dv [B, Nk, Hk, D]: contiguous; dtable: NULL or
+ * [num_buckets, H] of the table's type.  Nq >= 1. */
+size_t bioemu_attention_bwd_workspace_bytes(const bioemu_attention_args* args, int table_gradient);
+int bioemu_attention_bwd(const bioemu_attention_args* args, const void* o, const float* lse, const void* dout,
+                         const int64_t* dout_stride, void* dq, void* dk, void* dv, void* dtable, void* workspace,
+                         size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

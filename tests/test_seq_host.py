@@ -79,3 +79,50 @@ def test_relpos_c_abi_refusals():
     assert lib.bioemu_relpos_bwd(16, 16, 16, None, 16, None, 0, 1, 8, 16, 2, 5, 1, 0, None) == -3
     assert lib.bioemu_relpos_bwd_workspace_bytes(0, 8, 16, 5) == 0
     assert math.prod((1, 5, 16, 4)) == lib.bioemu_relpos_bwd_workspace_bytes(1, 8, 16, 5)
+
+
+def _attention_args(**over):
+    vals = dict(q=16, k=16, v=16, q_batch=128, q_row=32, q_head=16, k_batch=128, k_row=32, k_head=16, v_batch=128,
+                v_row=32, v_head=16, q_segments=None, k_segments=None, prefix=None, lengths=None, bias_table=None,
+                bias_buckets=None, B=1, Nq=4, Nk=4, H=2, Hk=2, D=16, radius=0, num_buckets=0, scale=0.25, cap=0.0,
+                causal=0, f32=1, table_bf16=0) | over
+    return _lib.AttentionArgs(**vals)
+
+
+@pytest.mark.parametrize("over,code", [
+    (dict(q=None), -1), (dict(q=8), -1), (dict(k_row=30), -1), (dict(k_row=8), -2), (dict(v_row=1 << 24), -2),
+    (dict(D=12), -2), (dict(D=136), -2), (dict(H=3), -1), (dict(H=0), -1), (dict(Nq=1 << 28), -2), (dict(cap=-1.0), -1),
+    (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1), (dict(q_segments=16), -1), (dict(bias_table=16), -1),
+    (dict(bias_table=16, bias_buckets=16, radius=513, num_buckets=4), -2),
+    (dict(bias_table=16, bias_buckets=16, radius=5, num_buckets=257), -2), (dict(B=1 << 20, H=4, Hk=2), -2)])
+def test_attention_c_abi_refusals(over, code):
+    lib = _lib.lib()
+    args = _attention_args(**over)
+    assert lib.bioemu_attention_fwd(args, 16, None, None, 0, None) == code
+    assert lib.bioemu_attention_workspace_bytes(args) == 0
+    assert lib.bioemu_attention_bwd_workspace_bytes(args, 0) == 0
+
+
+def test_attention_c_abi_workspace_and_outputs():
+    lib = _lib.lib()
+    assert lib.bioemu_attention_fwd(None, 16, None, None, 0, None) == -1
+    assert lib.bioemu_attention_fwd(_attention_args(), None, None, None, 0, None) == -1
+    assert lib.bioemu_attention_fwd(_attention_args(B=0), None, None, None, 0, None) == 0
+    strides = (_lib._c_int64 * 3)(128, 32, 16)
+    args = _attention_args()
+    assert lib.bioemu_attention_bwd(args, 16, 16, 16, strides, 16, 16, 16, None, None, 0, None) == -3
+    assert lib.bioemu_attention_bwd(args, 16, 16, 16, strides, 16, 16, None, None, 16, 1 << 20, None) == -1
+    assert lib.bioemu_attention_bwd(args, 16, 16, 16, strides, 16, 16, 16, 16, 16, 1 << 20, None) == -1   # no table
+    assert lib.bioemu_attention_bwd_workspace_bytes(args, 0) == 256   # 1 x 2 x 4 row sums, rounded up
+
+
+def test_attention_rejects_cpu_tensors():
+    from bioemu2_amd.attention import SequenceAttention, attention
+
+    q = torch.randn(1, 4, 2, 16)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        attention(q, q, q)
+    mod = SequenceAttention(2, radius=4)
+    assert set(mod.state_dict()) == {"bias"} and mod.bias.shape == (9, 2)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        mod(q, q, q)
