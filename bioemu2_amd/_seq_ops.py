@@ -10,8 +10,8 @@ are first order.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import struct
 
 import torch
 from torch import Tensor
@@ -20,21 +20,30 @@ from ._lib import AttentionArgs, check, lib
 from ._ops import BF16, F32, _check_tensor, _Op, _ptr, _stream, _unobserved, require_gpu, workspace
 
 _TYPES = (BF16, F32)
+_current_device = torch._C._cuda_getDevice
 
 
-def _on(t: Tensor):
-    """A launch reaches the device of its tensors, current or not."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == t.get_device() else torch.cuda.device(t.device)
+def _call(t: Tensor, what: str, *args) -> None:
+    """The C ABI's ``what`` on t's device (current or not) and its current stream."""
+    fn = getattr(lib(), what)
+    if _current_device() == t.get_device():
+        rc = fn(*args, _stream(t))
+    else:
+        with torch.cuda.device(t.device):
+            rc = fn(*args, _stream(t))
+    if rc:
+        check(rc, what)
 
 
 class _TrainOp(_Op):
-    """An ``_Op`` with a gradient.  ``save`` takes (ctx, args, outputs), ``grad`` (ctx, gradients of the outputs);
-    ``for_grad`` and ``no_grad`` give the body's arguments of a call with and without gradients, where those differ
-    (what the backward pass reads is not written by a serving call).  The op's first output is what callers get."""
+    """An ``_Op`` with a gradient.  ``save`` takes (ctx, args, outputs), ``grad`` (ctx, gradients of the outputs).  The
+    op's last argument says whether a gradient is wanted (what the backward pass reads is not written by a serving
+    call) and is filled in here; callers get the first output."""
 
     def __init__(self, name: str, body, save, grad):
         super().__init__(name, body)
         self.op.register_autograd(grad, setup_context=lambda ctx, inputs, output: save(ctx, inputs, output))
+        once = torch.autograd.function.once_differentiable(lambda ctx, g: grad(ctx, g, None))
 
         def forward(ctx, *args):
             out = body(*args)
@@ -42,15 +51,19 @@ class _TrainOp(_Op):
             return out[0]
 
         def backward(ctx, g):
-            return grad(ctx, g, None)
+            # grad mode is off but where a graph of the gradient is asked for, which there is none of
+            return once(ctx, g) if torch.is_grad_enabled() else grad(ctx, g, None)
 
         self.fn = type(name, (torch.autograd.Function,),
-                       {"forward": staticmethod(forward),
-                        "backward": staticmethod(torch.autograd.function.once_differentiable(backward))})
+                       {"forward": staticmethod(forward), "backward": staticmethod(backward)})
 
     def __call__(self, *args):
-        """args[-1] of the op says whether a gradient is wanted, and is filled in here."""
-        train = torch.is_grad_enabled() and any(isinstance(a, Tensor) and a.requires_grad for a in args)
+        train = False
+        if torch.is_grad_enabled():
+            for a in args:
+                if isinstance(a, Tensor) and a.requires_grad:
+                    train = True
+                    break
         if _unobserved(args) and self._own():
             return self.fn.apply(*args, True) if train else self.body(*args, False)[0]
         return self.op(*args, train)[0]
@@ -77,18 +90,31 @@ def _activation(t: Tensor, what: str) -> int:
 # ----------------------------------------------------------------------------
 # LayerNorm
 # ----------------------------------------------------------------------------
-def _as_rows(x: Tensor) -> Tensor:
-    """``x`` as [rows, c] with neighbouring values adjacent: a view where its strides allow, a copy else."""
+def _as_rows(x: Tensor) -> tuple[Tensor, int]:
+    """``x`` with the stride of its rows (of the last dimension, neighbouring values adjacent): itself where its strides
+    allow, a copy else."""
     c = x.shape[-1]
     if x.is_contiguous():
-        return x.view(-1, c)
+        return x, c
     if x.stride(-1) == 1 or c == 1:
         try:
             rows = x.view(-1, c)
-            return rows if rows.stride(1) == 1 else rows.contiguous()
+            if rows.stride(1) == 1:
+                return rows, rows.stride(0)
         except RuntimeError:
             pass
-    return x.contiguous().view(-1, c)
+    return x.contiguous(), c
+
+
+def _norm_types(x: Tensor, weight: Tensor | None, bias: Tensor | None) -> tuple[int, int]:
+    """(1 for fp32 activations, 1 for bf16 parameters)."""
+    f32, c = _activation(x, "layer_norm"), x.shape[-1]
+    w16 = _param_type(weight, "layer_norm weight", (c,), x.device)
+    if bias is None:
+        return f32, w16
+    if weight is not None and bias.dtype != weight.dtype:
+        raise ValueError(f"layer_norm: weight is {weight.dtype}, bias {bias.dtype}")
+    return f32, _param_type(bias, "layer_norm bias", (c,), x.device)
 
 
 def layer_norm_bwd_workspace_bytes(rows: int, c: int) -> int:
@@ -98,36 +124,29 @@ def layer_norm_bwd_workspace_bytes(rows: int, c: int) -> int:
 def launch_layer_norm(x: Tensor, weight: Tensor | None, bias: Tensor | None, y: Tensor, eps: float,
                       stats: Tensor | None = None) -> Tensor:
     """LayerNorm of the rows ``x`` [rows, c] (any row stride) into contiguous ``y``; ``stats`` [rows, 2] fp32."""
-    f32 = _activation(x, "layer_norm")
     if x.ndim != 2 or x.stride(1) != 1:
         raise ValueError("layer_norm: x must be [rows, c] with adjacent values")
+    f32, w16 = _norm_types(x, weight, bias)
     rows, c = x.shape
     _check_tensor(y, "layer_norm y", x.dtype, (rows, c), x.device)
-    w16 = _param_type(weight, "layer_norm weight", (c,), x.device)
-    if bias is not None and weight is not None and bias.dtype != weight.dtype:
-        raise ValueError(f"layer_norm: weight is {weight.dtype}, bias {bias.dtype}")
-    w16 |= _param_type(bias, "layer_norm bias", (c,), x.device)
     if stats is not None:
         _check_tensor(stats, "layer_norm stats", F32, (rows, 2), x.device)
-    with _on(x):
-        rc = lib().bioemu_layer_norm_fwd(_ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _ptr(stats), rows, c, x.stride(0),
-                                         eps, f32, w16, _stream(x))
-    check(rc, "bioemu_layer_norm_fwd")
+    _call(x, "bioemu_layer_norm_fwd", x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), _ptr(stats), rows, c,
+          x.stride(0), eps, f32, w16)
     return y
 
 
 def launch_layer_norm_bwd(x: Tensor, dy: Tensor, stats: Tensor, weight: Tensor | None, dx: Tensor | None,
                           dweight: Tensor | None, dbias: Tensor | None, ws: Tensor | None = None) -> None:
     """Gradients of ``launch_layer_norm`` into ``dx`` [rows, c], ``dweight``, ``dbias`` (each may be None)."""
-    f32 = _activation(x, "layer_norm_bwd")
     if x.ndim != 2 or x.stride(1) != 1 or dy.shape != x.shape or dy.dtype != x.dtype or dy.stride(1) != 1:
         raise ValueError("layer_norm_bwd: x and dy must be [rows, c] of one type with adjacent values")
+    f32, w16 = _norm_types(x, weight, None)
     rows, c = x.shape
     dev = x.device
     _check_tensor(stats, "layer_norm stats", F32, (rows, 2), dev)
     if dx is not None:
         _check_tensor(dx, "layer_norm dx", x.dtype, (rows, c), dev)
-    w16 = _param_type(weight, "layer_norm weight", (c,), dev)
     for t in (dweight, dbias):
         if t is not None and weight is not None and t.dtype != weight.dtype:
             raise ValueError("layer_norm_bwd: weight gradients take the weight's type")
@@ -135,33 +154,40 @@ def launch_layer_norm_bwd(x: Tensor, dy: Tensor, stats: Tensor, weight: Tensor |
     need = layer_norm_bwd_workspace_bytes(rows, c) if dweight is not None or dbias is not None else 0
     if need and (ws is None or ws.numel() < need):
         ws = workspace(need, dev)
-    with _on(x):
-        rc = lib().bioemu_layer_norm_bwd(
-            _ptr(x), _ptr(dy), _ptr(stats), _ptr(weight), _ptr(dx), _ptr(dweight), _ptr(dbias), _ptr(ws),
-            ctypes.c_size_t(0 if ws is None else ws.numel()), rows, c, x.stride(0), dy.stride(0), f32, w16, _stream(x))
-    check(rc, "bioemu_layer_norm_bwd")
+    _call(x, "bioemu_layer_norm_bwd", x.data_ptr(), dy.data_ptr(), stats.data_ptr(), _ptr(weight), _ptr(dx),
+          _ptr(dweight), _ptr(dbias), _ptr(ws), 0 if ws is None else ws.numel(), rows, c, x.stride(0), dy.stride(0),
+          f32, w16)
 
 
 def _layer_norm(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float, train: bool) -> tuple[Tensor, Tensor]:
-    rows = _as_rows(x)
+    f32, w16 = _norm_types(x, weight, bias)
+    src, stride = _as_rows(x)
+    c = x.shape[-1]
+    rows = x.numel() // c
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((rows.shape[0] if train else 0, 2), dtype=F32, device=x.device)
-    launch_layer_norm(rows, weight, bias, y.view(rows.shape), eps, stats if train else None)
+    stats = torch.empty((rows if train else 0, 2), dtype=F32, device=x.device)
+    _call(x, "bioemu_layer_norm_fwd", src.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(),
+          stats.data_ptr() if train else None, rows, c, stride, eps, f32, w16)
     return y, stats
 
 
 def _layer_norm_backward(x: Tensor, dy: Tensor, stats: Tensor, weight: Tensor | None, want_x: bool, want_w: bool,
                          want_b: bool, bias_bf16: bool) -> tuple[Tensor, Tensor, Tensor]:
-    rows = _as_rows(x)
-    c = x.shape[-1]
+    dev, c = x.device, x.shape[-1]
+    rows = x.numel() // c
     wt = weight.dtype if weight is not None else (BF16 if bias_bf16 else F32)
-    dx = torch.empty(x.shape if want_x else (0,), dtype=x.dtype, device=x.device)
-    dw = torch.empty((c if want_w else 0,), dtype=wt, device=x.device)
-    db = torch.empty((c if want_b else 0,), dtype=wt, device=x.device)
-    if x.numel() == 0:
+    dx = torch.empty(x.shape if want_x else (0,), dtype=x.dtype, device=dev)
+    dw = torch.empty((c if want_w else 0,), dtype=wt, device=dev)
+    db = torch.empty((c if want_b else 0,), dtype=wt, device=dev)
+    if rows == 0:
         return dx, dw.zero_(), db.zero_()
-    launch_layer_norm_bwd(rows, _as_rows(dy), stats, weight, dx.view(rows.shape) if want_x else None,
-                          dw if want_w else None, db if want_b else None)
+    (src, stride), (dsrc, dstride) = _as_rows(x), _as_rows(dy)
+    ws = None
+    if want_w or want_b:
+        ws = workspace(layer_norm_bwd_workspace_bytes(rows, c), dev)
+    _call(x, "bioemu_layer_norm_bwd", src.data_ptr(), dsrc.data_ptr(), stats.data_ptr(), _ptr(weight),
+          dx.data_ptr() if want_x else None, dw.data_ptr() if want_w else None, db.data_ptr() if want_b else None,
+          _ptr(ws), 0 if ws is None else ws.numel(), rows, c, stride, dstride, int(x.dtype == F32), int(wt == BF16))
     return dx, dw, db
 
 
@@ -226,10 +252,8 @@ def launch_relpos(table: Tensor, buckets: Tensor, positions: Tensor, chains: Ten
     _check_tensor(out, "relpos out", out.dtype, (B, N, N, C), out.device)
     if z is not None:
         _check_tensor(z, "relpos z", out.dtype, (B, N, N, C), out.device)
-    with _on(out):
-        rc = lib().bioemu_relpos_fwd(_ptr(table), _ptr(buckets), _ptr(positions), _ptr(chains), _ptr(z), _ptr(out), B, N,
-                                     C, radius, NB, f32, t16, _stream(out))
-    check(rc, "bioemu_relpos_fwd")
+    _call(out, "bioemu_relpos_fwd", table.data_ptr(), buckets.data_ptr(), positions.data_ptr(), _ptr(chains), _ptr(z),
+          out.data_ptr(), B, N, C, radius, NB, f32, t16)
     return out
 
 
@@ -244,10 +268,8 @@ def launch_relpos_bwd(dout: Tensor, buckets: Tensor, positions: Tensor, chains: 
     need = relpos_bwd_workspace_bytes(B, N, C, NB)
     if ws is None or ws.numel() < need:
         ws = workspace(need, dout.device)
-    with _on(dout):
-        rc = lib().bioemu_relpos_bwd(_ptr(dout), _ptr(buckets), _ptr(positions), _ptr(chains), _ptr(dtable), _ptr(ws),
-                                     ctypes.c_size_t(ws.numel()), B, N, C, radius, NB, f32, t16, _stream(dout))
-    check(rc, "bioemu_relpos_bwd")
+    _call(dout, "bioemu_relpos_bwd", dout.data_ptr(), buckets.data_ptr(), positions.data_ptr(), _ptr(chains),
+          dtable.data_ptr(), ws.data_ptr(), ws.numel(), B, N, C, radius, NB, f32, t16)
     return dtable
 
 
@@ -301,13 +323,15 @@ def _(table, z, buckets, positions, chains, dtype, train):
 # Attention
 # ----------------------------------------------------------------------------
 _MAX_ROW_STRIDE = 1 << 23
+_PACKED_ARGS = struct.Struct("@3P9q6P8q2f3i0q").pack   # AttentionArgs, a few times faster than field by field
+assert len(_PACKED_ARGS(*[0] * 31)) == ctypes.sizeof(AttentionArgs)
 
 
 def _heads(t: Tensor) -> Tensor:
     """[B, N, H, D] with adjacent values of a head and rows at 16-byte addresses: ``t`` where it is so, a copy else."""
-    per = 16 // t.element_size()
     b, n, h, d = t.stride()
-    rows, width = t.shape[1], t.shape[3]
+    _, rows, _, width = t.shape
+    per = 16 // t.element_size()
     if (d == 1 and (n >= width or rows <= 1) and n <= _MAX_ROW_STRIDE and not (b % per or n % per or h % per)
             and t.data_ptr() % 16 == 0):
         return t
@@ -342,11 +366,10 @@ def _attention_args(q, k, v, table, buckets, q_segments, k_segments, prefix, len
         radius, nb = buckets.numel() // 2, table.shape[0]
         t16 = _param_type(table, "attention bias table", (nb, H), dev)
     qs, ks, vs = q.stride(), k.stride(), v.stride()
-    return AttentionArgs(
+    return AttentionArgs.from_buffer_copy(_PACKED_ARGS(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-        _ptr(q_segments), _ptr(k_segments), _ptr(prefix), _ptr(lengths), _ptr(table),
-        None if table is None else buckets.data_ptr(), B, Nq, Nk, H, Hk, D, radius, nb, scale, cap, int(causal), f32,
-        t16)
+        _ptr(q_segments) or 0, _ptr(k_segments) or 0, _ptr(prefix) or 0, _ptr(lengths) or 0, _ptr(table) or 0,
+        0 if table is None else buckets.data_ptr(), B, Nq, Nk, H, Hk, D, radius, nb, scale, cap, int(causal), f32, t16))
 
 
 def launch_attention(q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor | None = None, *,
@@ -359,13 +382,10 @@ def launch_attention(q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor |
     _check_tensor(out, "attention out", q.dtype, tuple(q.shape), q.device)
     if lse is not None:
         _check_tensor(lse, "attention lse", F32, (q.shape[0], q.shape[2], q.shape[1]), q.device)
-    with _on(q):
-        need = int(lib().bioemu_attention_workspace_bytes(args))
-        if need and (ws is None or ws.numel() < need):
-            ws = workspace(need, q.device)
-        rc = lib().bioemu_attention_fwd(args, out.data_ptr(), _ptr(lse), _ptr(ws),
-                                        ctypes.c_size_t(0 if ws is None else ws.numel()), _stream(q))
-    check(rc, "bioemu_attention_fwd")
+    need = lib().bioemu_attention_workspace_bytes(args)
+    if need and (ws is None or ws.numel() < need):
+        ws = workspace(need, q.device)
+    _call(q, "bioemu_attention_fwd", args, out.data_ptr(), _ptr(lse), _ptr(ws), 0 if ws is None else ws.numel())
     return out
 
 
@@ -389,15 +409,12 @@ def launch_attention_bwd(q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tens
             raise ValueError("attention_bwd: dtable without a bias table")
         _check_tensor(dtable, "attention dtable", bias_table.dtype, tuple(bias_table.shape), dev)
     st = dout.stride()
-    with _on(q):
-        need = int(lib().bioemu_attention_bwd_workspace_bytes(args, int(dtable is not None)))
-        if ws is None or ws.numel() < need:
-            ws = workspace(need, dev)
-        rc = lib().bioemu_attention_bwd(args, out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
-                                        (ctypes.c_int64 * 3)(st[0], st[1], st[2]), dq.data_ptr(), dk.data_ptr(),
-                                        dv.data_ptr(), _ptr(dtable), ws.data_ptr(), ctypes.c_size_t(ws.numel()),
-                                        _stream(q))
-    check(rc, "bioemu_attention_bwd")
+    need = lib().bioemu_attention_bwd_workspace_bytes(args, int(dtable is not None))
+    if ws is None or ws.numel() < need:
+        ws = workspace(need, dev)
+    _call(q, "bioemu_attention_bwd", args, out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+          (ctypes.c_int64 * 3)(st[0], st[1], st[2]), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dtable),
+          ws.data_ptr(), ws.numel())
 
 
 def _attention(q: Tensor, k: Tensor, v: Tensor, table: Tensor | None, buckets: Tensor | None,

@@ -4,9 +4,10 @@
 //   pos_i = length - Nq + i;  allowed: j < length, segment_i == segment_j >= 0,
 //   and (not causal, or j <= pos_i, or j < prefix)
 //
-// One code for both types.  bf16 operands use v_mfma_f32_32x32x16_bf16; an fp32 operand of the same shape (8 values a
-// lane, 16 of the reduced index) is eight v_mfma_f32_32x32x2_f32, whose k index t takes element t of both lane halves:
-// the order of the reduced index is free as long as both operands use the same, so every layout below holds for both.
+// One code for both types, on v_mfma_f32_32x32x16_bf16 (8 values a lane, 16 of the reduced index).  An fp32 operand is
+// three bf16 parts, hi + mid + lo, which hold its 24 bits; of their nine products the six of 2^-16 of the whole and more
+// are taken, smallest first: 192 cycles where eight v_mfma_f32_32x32x2_f32 take 512, and the same error (the
+// accumulator's rounding).
 // Scores are kept transposed to the operand that follows: a 32 x 32 accumulator (lane n = column, register 4 r + c =
 // row 8 r + 4 h + c) is, register for register, the B operand of the next product whose reduced index is its rows in
 // the order kappa(h, t) = 4 h + t, 8 + 4 h + t - 4; the A operand of that product comes out of LDS in that order by the
@@ -58,10 +59,28 @@ template <class T>
 using Frag = typename Operand<T>::frag;
 
 __device__ __forceinline__ f32x16 mfma16(bf16x8 a, bf16x8 b, f32x16 c) { return mfma32(a, b, c); }
-__device__ __forceinline__ f32x16 mfma16(f32x8 a, f32x8 b, f32x16 c) {
+struct Parts3 {
+  bf16x8 hi, mid, lo;
+};
+__device__ __forceinline__ Parts3 parts3(f32x8 x) {
+  Parts3 p;
 #pragma unroll
-  for (int t = 0; t < 8; ++t) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[t], b[t], c, 0, 0, 0);
-  return c;
+  for (int t = 0; t < 8; ++t) {
+    p.hi[t] = (bf16)x[t];
+    const float r = x[t] - (float)p.hi[t];
+    p.mid[t] = (bf16)r;
+    p.lo[t] = (bf16)(r - (float)p.mid[t]);
+  }
+  return p;
+}
+__device__ __forceinline__ f32x16 mfma16(f32x8 a, f32x8 b, f32x16 c) {
+  const Parts3 x = parts3(a), y = parts3(b);
+  c = mfma32(x.mid, y.mid, c);
+  c = mfma32(x.lo, y.hi, c);
+  c = mfma32(x.hi, y.lo, c);
+  c = mfma32(x.mid, y.hi, c);
+  c = mfma32(x.hi, y.mid, c);
+  return mfma32(x.hi, y.hi, c);
 }
 
 // Copies from memory into LDS: lane i's BYTES at byte voff of the source go to lds + BYTES i; zeros past its end.
@@ -208,19 +227,36 @@ __device__ __forceinline__ float table_value(const AttnArgs& a, int entry, int h
                                 : static_cast<const float*>(a.table)[at]);
 }
 
-// Workgroup minimum or maximum of an int (every thread gets it); red: 4 ints of LDS, free again after the next barrier.
-template <bool MAX>
-__device__ __forceinline__ int wg_extreme(int v, int* red) {
+// Workgroup minimum of `low`, maxima of `high` and `top` (every thread gets them); red: 12 ints of LDS.
+__device__ __forceinline__ void wg_extremes(int& low, int& high, int& top, int (*red)[4]) {
 #pragma unroll
   for (int m = 32; m > 0; m /= 2) {
-    const int o = __shfl_xor(v, m);
-    v = MAX ? max(v, o) : min(v, o);
+    low = min(low, __shfl_xor(low, m));
+    high = max(high, __shfl_xor(high, m));
+    top = max(top, __shfl_xor(top, m));
+  }
+  if ((threadIdx.x & 63) == 0) {
+    red[0][threadIdx.x >> 6] = low;
+    red[1][threadIdx.x >> 6] = high;
+    red[2][threadIdx.x >> 6] = top;
   }
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  const int a = MAX ? max(red[0], red[1]) : min(red[0], red[1]), b = MAX ? max(red[2], red[3]) : min(red[2], red[3]);
-  return __builtin_amdgcn_readfirstlane(MAX ? max(a, b) : min(a, b));
+  low = __builtin_amdgcn_readfirstlane(min(min(red[0][0], red[0][1]), min(red[0][2], red[0][3])));
+  high = __builtin_amdgcn_readfirstlane(max(max(red[1][0], red[1][1]), max(red[1][2], red[1][3])));
+  top = __builtin_amdgcn_readfirstlane(max(max(red[2][0], red[2][1]), max(red[2][2], red[2][3])));
+}
+
+// The bias by offset in LDS, offsets -R - kPad .. R + kPad (beyond the radius its end values): a 32 x 32 block that
+// meets the radius reads it without clamping.  Entry rel + R + kPad.
+constexpr int kPad = 64;
+__device__ __forceinline__ int lut_size(const AttnArgs& a) { return 2 * (a.radius + kPad) + 1; }
+__device__ __forceinline__ void fill_lut(const AttnArgs& a, int h, float* lut) {
+  for (int e = threadIdx.x; e < lut_size(a); e += kAttnThreads)
+    lut[e] = table_value(a, min(max(e - kPad, 0), 2 * a.radius), h);
+}
+// Whether all offsets rel0 - 31 .. rel0 + 31 lie at or beyond the radius.
+__device__ __forceinline__ bool all_far(const AttnArgs& a, int rel0) {
+  return rel0 - 31 >= a.radius || rel0 + 31 <= -a.radius;
 }
 
 // Blocks of a segment list that can hold an allowed pair.  An entry is the block's number with two flags.
@@ -231,12 +267,20 @@ constexpr int kBlockMask = 0x0fffffff, kEntryFull = 0x10000000, kEntryHoles = 0x
 // returns the entries.  flags: one byte a block, list: one int a block.
 template <int BLOCK>
 __device__ __forceinline__ int list_blocks(const int* __restrict__ seg, int n, int lo, int hi, int c0, int c1,
-                                           uint8_t* flags, int* list, int* red) {
+                                           uint8_t* flags, int* list, int* count) {
   const int lane = threadIdx.x & 63, wave = wave_id();
   constexpr int PER = 64 / BLOCK;   // blocks one wave reads at a time
-  for (int b0 = c0 + wave * PER; b0 < c1; b0 += 4 * PER) {
-    const int r = b0 * BLOCK + lane;
-    const int s = r < n ? seg[r] : -1;
+  constexpr int AHEAD = 8;          // reads in flight
+  for (int b8 = c0 + wave * PER; b8 < c1; b8 += 4 * PER * AHEAD) {
+   int got[AHEAD];
+#pragma unroll
+   for (int q = 0; q < AHEAD; ++q) {
+    const int r = (b8 + 4 * PER * q) * BLOCK + lane;
+    got[q] = r < n ? seg[r] : -1;
+   }
+#pragma unroll
+   for (int q = 0; q < AHEAD; ++q) {
+    const int b0 = b8 + 4 * PER * q, s = got[q];
     const uint64_t hit = __ballot(s >= 0 && s >= lo && s <= hi), one = __ballot(lo == hi && s == lo),
                    hole = __ballot(s < 0);
 #pragma unroll
@@ -246,6 +290,7 @@ __device__ __forceinline__ int list_blocks(const int* __restrict__ seg, int n, i
         flags[b0 + p - c0] =
             (uint8_t)(((hit & m) != 0 ? 1 : 0) | ((one & m) == m ? 2 : 0) | ((hole & m) != 0 ? 4 : 0));
     }
+   }
   }
   __syncthreads();
   if (wave == 0) {
@@ -258,10 +303,10 @@ __device__ __forceinline__ int list_blocks(const int* __restrict__ seg, int n, i
             (c0 + b0 + lane) | (f & 2 ? kEntryFull : 0) | (f & 4 ? kEntryHoles : 0);
       at += __popcll(m);
     }
-    if (lane == 0) red[0] = at;
+    if (lane == 0) *count = at;
   }
   __syncthreads();
-  return __builtin_amdgcn_readfirstlane(red[0]);
+  return __builtin_amdgcn_readfirstlane(*count);
 }
 
 // XCD-aware order: workgroup w runs on XCD w % 8, each XCD gets a contiguous range of the items (so the workgroups

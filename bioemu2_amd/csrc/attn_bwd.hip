@@ -9,9 +9,11 @@
 // are so computed twice, 7 products instead of 5; adding dq over workgroups instead would need fp32 atomics (an order
 // that changes results) or as many copies of dq.
 //
+// Either may split its walk over workgroups where the rows alone do not fill the chip; attn_bwd_join adds the parts.
+//
 // The table's gradient: per wave an LDS row of sums by offset, added to with one LDS add an element (a wave's adds are
-// in program order, its 32 queries fall on 32 different offsets, its two halves have rows of their own); offsets at or
-// beyond the radius stay in registers.  Then waves, workgroups and buckets in fixed orders.
+// in program order, its 32 queries fall on 32 different offsets, its two halves have rows of their own); blocks wholly
+// at or beyond the radius stay in registers.  Then waves, workgroups and buckets in fixed orders.
 #include "attn.h"
 
 namespace bioemu {
@@ -19,21 +21,31 @@ namespace {
 
 constexpr int kGroupRows = 128;
 
-// The probability of a masked or unmasked score, and what the gradient of q . k takes beside ds.
-template <class T>
-__device__ __forceinline__ float capped(const AttnArgs& a, float raw, float s_scale, float s_cap, float& slope) {
-  const float y = raw * s_scale;
-  if (a.cap > 0.f) {
-    const float t = attn_tanh<T>(y);
-    slope = 1.f - t * t;
-    return s_cap * t;
-  }
-  return y;
-}
-
 // LDS beyond the tiles: bias values by offset, and sums of ds by offset, 8 rows (4 waves x 2 lane halves).
 inline size_t bias_lds(const AttnArgs& a, bool sums) {
-  return a.table ? (size_t)(2 * a.radius + 1) * sizeof(float) * (sums ? 9 : 1) : 0;
+  return a.table ? (size_t)(2 * (a.radius + kPad) + 1) * sizeof(float) * (sums ? 9 : 1) : 0;
+}
+
+// A lane's row of an accumulator [DB] of 32-value blocks times `scale`, rounded into `out`, or as fp32 into `part`.
+template <class T, int DB>
+__device__ __forceinline__ void store_rows(const f32x16 (&acc)[DB], float scale, T* out, float* part, int lh, int D) {
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int at = 32 * d + 8 * r + 4 * lh;
+      if (at >= D) continue;
+      if (out) {
+        typedef T quad __attribute__((ext_vector_type(4)));
+        quad v;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] = (T)(acc[d][4 * r + c] * scale);
+        *reinterpret_cast<quad*>(out + at) = v;
+      } else {
+        *reinterpret_cast<f32x4*>(part + at) = f32x4{acc[d][4 * r] * scale, acc[d][4 * r + 1] * scale,
+                                                     acc[d][4 * r + 2] * scale, acc[d][4 * r + 3] * scale};
+      }
+    }
 }
 
 template <class T, int DP>
@@ -42,27 +54,29 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
                                                                   const T* __restrict__ dout, int64_t db, int64_t dn,
                                                                   int64_t dh, T* __restrict__ dq,
                                                                   float* __restrict__ delta,
-                                                                  float* __restrict__ bias_part, int qblocks,
-                                                                  int total) {
+                                                                  float* __restrict__ dq_part,
+                                                                  float* __restrict__ bias_part, int splits,
+                                                                  int qblocks, int total) {
   constexpr int KB = Operand<T>::kBlock, SUB = KB / 32, STEPS = DP / 16, DB = DP / 32;
   typedef Tile<T, DP, KB> KV;
   constexpr int CP = KV::copies(kAttnThreads);
   __shared__ __attribute__((aligned(1024))) char tiles[2][2][KV::BYTES];
-  __shared__ int segs[2][64];
+  __shared__ __attribute__((aligned(16))) int segs[2][64];
   __shared__ int list[kListBlocks];
   __shared__ uint8_t flags[kListBlocks];
-  __shared__ int red[4];
+  __shared__ int red[3][4], count;
   __shared__ float ends[4][2];
-  extern __shared__ float dyn[];   // bias values [2 R + 1], then the sums [4][2][2 R + 1]
+  extern __shared__ float dyn[];   // bias values by offset, then the sums [4][2] by offset
 
   const int item = attn_item(total);
   if (item < 0) return;
   const int lane = threadIdx.x & 63, wave = wave_id(), ln = lane & 31, lh = lane >> 5;
-  const int qblk = qblocks - 1 - item % qblocks, bh = item / qblocks, h = bh % a.H, b = bh / a.H, hk = h / a.G;
+  const int qblk = qblocks - 1 - item % qblocks, rest = item / qblocks, split = rest % splits, bh = rest / splits;
+  const int h = bh % a.H, b = bh / a.H, hk = h / a.G;
   const int length = a.lengths ? min(max(a.lengths[b], 0), a.Nk) : a.Nk;
   const int prefix = a.prefix ? a.prefix[b] : 0;
   const bool seg = a.q_seg != nullptr;
-  const int nrel = 2 * a.radius + 1;
+  const int nrel = lut_size(a);
   float *lut = dyn, *sums = dyn + nrel;
 
   const int i = qblk * kGroupRows + wave * 32 + ln;
@@ -71,9 +85,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
   const int qseg = seg && live ? a.q_seg[(int64_t)b * a.Nq + i] : 0;
   int lim = a.causal ? min(max(pos + 1, prefix), length) : length;
   if (qseg < 0 || !live) lim = 0;
-  const int seg_lo = seg ? wg_extreme<false>(live && qseg >= 0 ? qseg : 0x7fffffff, red) : 0;
-  const int seg_hi = seg ? wg_extreme<true>(live ? qseg : -1, red) : 0;
-  const int wg_max = wg_extreme<true>(lim, red);
+  int seg_lo = live && qseg >= 0 ? qseg : 0x7fffffff, seg_hi = live ? qseg : -1, wg_max = lim;
+  wg_extremes(seg_lo, seg_hi, wg_max, red);
   int wave_min = lim, wave_max = lim;
 #pragma unroll
   for (int m = 16; m > 0; m /= 2) {
@@ -85,7 +98,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
   const int wave_pos = __builtin_amdgcn_readfirstlane(pos);
 
   if (a.table) {
-    for (int e = threadIdx.x; e < nrel; e += kAttnThreads) lut[e] = table_value(a, e, h);
+    fill_lut(a, h, lut);
     for (int e = threadIdx.x; e < 8 * nrel; e += kAttnThreads) sums[e] = 0.f;
   }
 
@@ -108,7 +121,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
     }
   }
   dsum += __shfl_xor(dsum, 32);
-  if (live && lh == 0) delta[srow] = dsum;
+  if (live && lh == 0 && split == 0) delta[srow] = -dsum;
 
   const T* kbase = static_cast<const T*>(a.k) + b * a.kb + hk * a.kh;
   const T* vbase = static_cast<const T*>(a.v) + b * a.vb + hk * a.vh;
@@ -121,9 +134,9 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
 #pragma unroll
   for (int d = 0; d < DB; ++d) acc[d] = zero16();
   float far_lo = 0.f, far_hi = 0.f;
-  const float s_scale = a.cap > 0.f ? a.scale / a.cap : a.scale * kLog2e;
-  const float s_cap = a.cap * kLog2e;
-  float* own = sums + (wave * 2 + lh) * nrel + a.radius;
+  const bool cap = a.cap > 0.f;
+  const float s_scale = cap ? a.scale / a.cap : a.scale * kLog2e, s_cap = a.cap * kLog2e, mult = cap ? 1.f : s_scale;
+  float* own = sums + (wave * 2 + lh) * nrel + a.radius + kPad + 4 * lh - ln;   // offset of key 4 lh from this query
 
   auto stage = [&](int entry, int buf) {
     const int k0 = (entry & kBlockMask) * KB;
@@ -135,14 +148,15 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
   const int blocks = (wg_max + KB - 1) / KB;
   for (int c0 = 0; c0 < blocks; c0 += kListBlocks) {
     const int c1 = seg ? min(blocks, c0 + kListBlocks) : blocks;
-    const int n = seg ? list_blocks<KB>(kseg, length, seg_lo, seg_hi, c0, c1, flags, list, red) : blocks;
+    const int n = seg ? list_blocks<KB>(kseg, length, seg_lo, seg_hi, c0, c1, flags, list, &count) : blocks;
     auto entry = [&](int t) { return seg ? __builtin_amdgcn_readfirstlane(list[t]) : t | kEntryFull; };
-    if (n > 0) stage(entry(0), 0);
-    for (int t = 0; t < n; ++t) {
+    const int t0 = (int)((int64_t)n * split / splits), t1 = (int)((int64_t)n * (split + 1) / splits);
+    if (t0 < t1) stage(entry(t0), t0 & 1);
+    for (int t = t0; t < t1; ++t) {
       const int e = entry(t), buf = t & 1, k0 = (e & kBlockMask) * KB;
       __builtin_amdgcn_s_waitcnt(0x0f70);
       __syncthreads();
-      if (t + 1 < n) stage(entry(t + 1), buf ^ 1);
+      if (t + 1 < t1) stage(entry(t + 1), buf ^ 1);
       if (e & kEntryHoles) {
         const int r = threadIdx.x / (kAttnThreads / KB);
         if (segs[buf][r] < 0) {
@@ -153,43 +167,49 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
       }
       if (k0 >= wave_max) continue;
       const char *kt = tiles[buf][0], *vt = tiles[buf][1];
-      const bool full = k0 + KB <= wave_min && (e & kEntryFull);
 #pragma unroll 1
       for (int u = 0; u < SUB; ++u) {
-        f32x16 s = zero16(), dp = zero16();
+        f32x16 s = zero16(), dp;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dp[r] = -dsum;
 #pragma unroll
         for (int st = 0; st < STEPS; ++st) s = mfma16(KV::rows(kt, 32 * u + ln, st, lh), qf[st], s);
 #pragma unroll
         for (int st = 0; st < STEPS; ++st) dp = mfma16(KV::rows(vt, 32 * u + ln, st, lh), df[st], dp);
         float x[16], slope[16];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = capped<T>(a, s[r], s_scale, s_cap, slope[r]);
-        const int rel0 = k0 + 32 * u - wave_pos;   // of the wave's first query and the first key
-        const bool far = rel0 - 31 >= a.radius || rel0 + 31 <= -a.radius;
-        if (a.table) {
-          if (far) {
-            const float v = lut[rel0 > 0 ? 2 * a.radius : 0];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] += v;
-          } else {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int rel = rel0 - ln + 8 * (r >> 2) + 4 * lh + (r & 3);
-              x[r] += lut[min(max(rel, -a.radius), a.radius) + a.radius];
-            }
-          }
-        }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = fast_exp2(x[r] - row_lse) * (dp[r] - dsum);
-        if (!full) {
+        if (cap)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const int kk = 32 * u + 8 * (r >> 2) + 4 * lh + (r & 3);
-            const bool ok = (k0 + kk < lim) & (!seg | (segs[buf][kk] == qseg));
-            x[r] = ok ? x[r] : 0.f;
+            const float t = attn_tanh<T>(s[r] * s_scale);
+            slope[r] = 1.f - t * t;
+            s[r] = s_cap * t;
           }
+        const int rel0 = k0 + 32 * u - wave_pos;   // of the wave's first query and the first key
+        const bool far = all_far(a, rel0);
+        if (a.table && !far) {
+          const float* bias = lut + (rel0 + a.radius + kPad + 4 * lh - ln);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[r] = s[r] * mult + (bias[8 * (r >> 2) + (r & 3)] - row_lse);
+        } else {
+          const float add = (a.table ? lut[rel0 > 0 ? nrel - 1 : 0] : 0.f) - row_lse;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[r] = s[r] * mult + add;
         }
-        if (a.table) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = fast_exp2(x[r]) * dp[r];
+        if (k0 + KB > wave_min)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[r] = k0 + 32 * u + 8 * (r >> 2) + 4 * lh + (r & 3) < lim ? x[r] : 0.f;
+        if (!(e & kEntryFull))
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int4 ks = *reinterpret_cast<const int4*>(&segs[buf][32 * u + 8 * q + 4 * lh]);
+            x[4 * q] = ks.x == qseg ? x[4 * q] : 0.f;
+            x[4 * q + 1] = ks.y == qseg ? x[4 * q + 1] : 0.f;
+            x[4 * q + 2] = ks.z == qseg ? x[4 * q + 2] : 0.f;
+            x[4 * q + 3] = ks.w == qseg ? x[4 * q + 3] : 0.f;
+          }
+        if (bias_part) {
           if (far) {
             float v = 0.f;
 #pragma unroll
@@ -200,18 +220,12 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
               far_lo += v;
           } else {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int rel = rel0 - ln + 8 * (r >> 2) + 4 * lh + (r & 3);
-              if (rel >= a.radius)
-                far_hi += x[r];
-              else if (rel <= -a.radius)
-                far_lo += x[r];
-              else
-                __hip_atomic_fetch_add(own + rel, x[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-            }
+            for (int r = 0; r < 16; ++r)
+              __hip_atomic_fetch_add(own + rel0 + 8 * (r >> 2) + (r & 3), x[r], __ATOMIC_RELAXED,
+                                     __HIP_MEMORY_SCOPE_WORKGROUP);
           }
         }
-        if (a.cap > 0.f)
+        if (cap)
 #pragma unroll
           for (int r = 0; r < 16; ++r) x[r] *= slope[r];
 #pragma unroll
@@ -226,22 +240,10 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
   }
 
   if (live) {
-    T* po = dq + row * a.D;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int at = 32 * d + 8 * r + 4 * lh;
-        if (at < a.D) {
-          typedef T quad __attribute__((ext_vector_type(4)));
-          quad v;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) v[c] = (T)(acc[d][4 * r + c] * a.scale);
-          *reinterpret_cast<quad*>(po + at) = v;
-        }
-      }
+    const int64_t at_row = splits == 1 ? row : split * (int64_t)a.B * a.Nq * a.H + row;
+    store_rows<T, DB>(acc, a.scale, splits == 1 ? dq + row * a.D : nullptr, dq_part + at_row * a.D, lh, a.D);
   }
-  if (a.table && bias_part) {
+  if (bias_part) {
 #pragma unroll
     for (int m = 32; m > 0; m /= 2) {
       far_lo += __shfl_xor(far_lo, m);
@@ -252,7 +254,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
       ends[wave][1] = far_hi;
     }
     __syncthreads();
-    float* out = bias_part + (((int64_t)b * qblocks + qblk) * a.H + h) * nrel;
+    float* out = bias_part + ((((int64_t)b * qblocks + qblk) * splits + split) * a.H + h) * nrel;
     for (int e = threadIdx.x; e < nrel; e += kAttnThreads) {
       float v = 0.f;
 #pragma unroll
@@ -269,36 +271,37 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArg
                                                                    const T* __restrict__ dout, int64_t db, int64_t dn,
                                                                    int64_t dh, const float* __restrict__ delta,
                                                                    T* __restrict__ dk, T* __restrict__ dv,
-                                                                   int kblocks, int total) {
+                                                                   float* __restrict__ part, int splits, int kblocks,
+                                                                   int total) {
   constexpr int QB = Operand<T>::kBlock, SUB = QB / 32, STEPS = DP / 16, DB = DP / 32;
   typedef Tile<T, DP, QB> QD;
   constexpr int CP = QD::copies(kAttnThreads);
   __shared__ __attribute__((aligned(1024))) char tiles[2][2][QD::BYTES];
-  __shared__ int segs[2][64];
-  __shared__ float stats[2][2][64];   // log-sums, do . o
+  __shared__ __attribute__((aligned(16))) int segs[2][64];
+  __shared__ __attribute__((aligned(16))) float stats[2][2][64];   // log-sums, -do . o
   __shared__ int list[kListBlocks];
   __shared__ uint8_t flags[kListBlocks];
-  __shared__ int red[4];
+  __shared__ int red[3][4], count;
   extern __shared__ float lut[];
 
   const int item = attn_item(total);
   if (item < 0) return;
   const int lane = threadIdx.x & 63, wave = wave_id(), ln = lane & 31, lh = lane >> 5;
-  const int kblk = item % kblocks, bh = item / kblocks, hk = bh % a.Hk, b = bh / a.Hk;
+  const int kblk = item % kblocks, rest = item / kblocks, split = rest % splits, bh = rest / splits;
+  const int hk = bh % a.Hk, b = bh / a.Hk;
   const int length = a.lengths ? min(max(a.lengths[b], 0), a.Nk) : a.Nk;
   const int prefix = a.prefix ? a.prefix[b] : 0;
   const bool seg = a.q_seg != nullptr;
   const int first = length - a.Nq;   // position of query 0
-  const int nrel = 2 * a.radius + 1;
 
   const int j = kblk * kGroupRows + wave * 32 + ln;
   const int kseg = seg && j < length ? a.k_seg[(int64_t)b * a.Nk + j] : 0;
   const bool on = j < length && kseg >= 0;
   // queries from imin on see this key (their segment aside)
   const int imin = !on ? 0x7fffffff : (a.causal && j >= prefix ? max(j - first, 0) : 0);
-  const int seg_lo = seg ? wg_extreme<false>(on ? kseg : 0x7fffffff, red) : 0;
-  const int seg_hi = seg ? wg_extreme<true>(on ? kseg : -1, red) : 0;
-  const int wg_min = wg_extreme<false>(imin, red);
+  int seg_lo = on ? kseg : 0x7fffffff, seg_hi = on ? kseg : -1, wg_min = -imin;
+  wg_extremes(seg_lo, seg_hi, wg_min, red);
+  wg_min = -wg_min;
   int wave_min = imin, wave_max = imin;
 #pragma unroll
   for (int m = 16; m > 0; m /= 2) {
@@ -327,8 +330,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArg
   f32x16 ak[DB], av[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) ak[d] = av[d] = zero16();
-  const float s_scale = a.cap > 0.f ? a.scale / a.cap : a.scale * kLog2e;
-  const float s_cap = a.cap * kLog2e;
+  const bool cap = a.cap > 0.f;
+  const float s_scale = cap ? a.scale / a.cap : a.scale * kLog2e, s_cap = a.cap * kLog2e, mult = cap ? 1.f : s_scale;
 
   const T *qbase = nullptr, *dbase = nullptr;   // of the current head, as its row of statistics
   int64_t srow = 0;
@@ -344,21 +347,24 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArg
   const int blocks = (a.Nq + QB - 1) / QB, first_block = min(wg_min, a.Nq) / QB;
   for (int c0 = first_block; c0 < blocks; c0 += kListBlocks) {
     const int c1 = seg ? min(blocks, c0 + kListBlocks) : blocks;
-    const int n = seg ? list_blocks<QB>(qseg, a.Nq, seg_lo, seg_hi, c0, c1, flags, list, red) : blocks - c0;
+    const int n = seg ? list_blocks<QB>(qseg, a.Nq, seg_lo, seg_hi, c0, c1, flags, list, &count) : blocks - c0;
     auto entry = [&](int t) { return seg ? __builtin_amdgcn_readfirstlane(list[t]) : (c0 + t) | kEntryFull; };
-    for (int g = 0; g < a.G; ++g) {
+    // the blocks of all heads of the group, one after the other, are dealt to the splits
+    const int64_t all = (int64_t)n * a.G;
+    const int64_t w0 = all * split / splits, w1 = all * (split + 1) / splits;
+    for (int g = n ? (int)(w0 / n) : 0; g < a.G && g * (int64_t)n < w1; ++g) {
+      const int t0 = (int)max(w0 - g * (int64_t)n, (int64_t)0), t1 = (int)min(w1 - g * (int64_t)n, (int64_t)n);
       const int h = hk * a.G + g;
       qbase = static_cast<const T*>(a.q) + b * a.qb + h * a.qh;
       dbase = dout + b * db + h * dh;
       srow = ((int64_t)b * a.H + h) * a.Nq;
-      if (a.table)
-        for (int e = threadIdx.x; e < nrel; e += kAttnThreads) lut[e] = table_value(a, e, h);
-      if (n > 0) stage(entry(0), 0);
-      for (int t = 0; t < n; ++t) {
+      if (a.table) fill_lut(a, h, lut);
+      if (t0 < t1) stage(entry(t0), t0 & 1);
+      for (int t = t0; t < t1; ++t) {
         const int e = entry(t), buf = t & 1, i0 = (e & kBlockMask) * QB;
         __builtin_amdgcn_s_waitcnt(0x0f70);
         __syncthreads();
-        if (t + 1 < n) stage(entry(t + 1), buf ^ 1);
+        if (t + 1 < t1) stage(entry(t + 1), buf ^ 1);
         // rows that see nothing (their log-sum is infinite) have weight 0, and 0 times what they hold has to be 0
         if (__ballot(lane < QB && stats[buf][0][lane] == kInf)) {
           const int r = threadIdx.x / (kAttnThreads / QB);
@@ -370,41 +376,58 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArg
         }
         if (i0 + QB <= wave_min) continue;
         const char *qt = tiles[buf][0], *dt = tiles[buf][1];
-        const bool full = i0 >= wave_max && (e & kEntryFull) && (!seg || (seg_lo == seg_hi && wave_max != 0x7fffffff));
 #pragma unroll 1
         for (int u = 0; u < SUB; ++u) {
-          f32x16 s = zero16(), dp = zero16();
+          f32x16 s = zero16(), dp;
+          float lsev[16];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int at = 32 * u + 8 * q + 4 * lh;
+            const f32x4 vl = *reinterpret_cast<const f32x4*>(&stats[buf][0][at]);
+            const f32x4 vd = *reinterpret_cast<const f32x4*>(&stats[buf][1][at]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              lsev[4 * q + c] = vl[c];
+              dp[4 * q + c] = vd[c];
+            }
+          }
 #pragma unroll
           for (int st = 0; st < STEPS; ++st) s = mfma16(QD::rows(qt, 32 * u + ln, st, lh), kf[st], s);
 #pragma unroll
           for (int st = 0; st < STEPS; ++st) dp = mfma16(QD::rows(dt, 32 * u + ln, st, lh), vf[st], dp);
           float x[16], slope[16];
-#pragma unroll
-          for (int r = 0; r < 16; ++r) x[r] = capped<T>(a, s[r], s_scale, s_cap, slope[r]);
-          if (a.table) {
-            const int rel0 = wave_key - (first + i0 + 32 * u);   // of the first query and the wave's first key
-            if (rel0 - 31 >= a.radius || rel0 + 31 <= -a.radius) {
-              const float v = lut[rel0 > 0 ? 2 * a.radius : 0];
-#pragma unroll
-              for (int r = 0; r < 16; ++r) x[r] += v;
-            } else {
-#pragma unroll
-              for (int r = 0; r < 16; ++r) {
-                const int rel = rel0 + ln - (8 * (r >> 2) + 4 * lh + (r & 3));
-                x[r] += lut[min(max(rel, -a.radius), a.radius) + a.radius];
-              }
-            }
-          }
-#pragma unroll
-          for (int r = 0; r < 16; ++r) x[r] = fast_exp2(x[r] - stats[buf][0][32 * u + 8 * (r >> 2) + 4 * lh + (r & 3)]);
-          if (!full) {
+          if (cap)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-              const int ii = 32 * u + 8 * (r >> 2) + 4 * lh + (r & 3);
-              const bool ok = (i0 + ii >= imin) & (!seg | (segs[buf][ii] == kseg));
-              x[r] = ok ? x[r] : 0.f;
+              const float t = attn_tanh<T>(s[r] * s_scale);
+              slope[r] = 1.f - t * t;
+              s[r] = s_cap * t;
             }
+          const int rel0 = wave_key - (first + i0 + 32 * u);   // of the first query and the wave's first key
+          if (a.table && !all_far(a, rel0)) {
+            const float* bias = lut + (rel0 + a.radius + kPad + ln - 4 * lh);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] = s[r] * mult + (bias[-(8 * (r >> 2) + (r & 3))] - lsev[r]);
+          } else {
+            const float add = a.table ? lut[rel0 > 0 ? 2 * (a.radius + kPad) : 0] : 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] = s[r] * mult + (add - lsev[r]);
           }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[r] = fast_exp2(x[r]);
+          if (i0 < wave_max)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              x[r] = i0 + 32 * u + 8 * (r >> 2) + 4 * lh + (r & 3) >= imin ? x[r] : 0.f;
+          if (!(e & kEntryFull))
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int4 qs = *reinterpret_cast<const int4*>(&segs[buf][32 * u + 8 * q + 4 * lh]);
+              x[4 * q] = qs.x == kseg ? x[4 * q] : 0.f;
+              x[4 * q + 1] = qs.y == kseg ? x[4 * q + 1] : 0.f;
+              x[4 * q + 2] = qs.z == kseg ? x[4 * q + 2] : 0.f;
+              x[4 * q + 3] = qs.w == kseg ? x[4 * q + 3] : 0.f;
+            }
 #pragma unroll
           for (int st = 0; st < 2; ++st) {
             const Frag<T> p = as_operand<T>(x, st);
@@ -413,8 +436,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArg
           }
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            x[r] *= dp[r] - stats[buf][1][32 * u + 8 * (r >> 2) + 4 * lh + (r & 3)];
-            if (a.cap > 0.f) x[r] *= slope[r];
+            x[r] *= dp[r];
+            if (cap) x[r] *= slope[r];
           }
 #pragma unroll
           for (int st = 0; st < 2; ++st) {
@@ -429,31 +452,54 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArg
   }
 
   if (j >= a.Nk) return;
-  const int64_t row = ((int64_t)b * a.Nk + j) * a.Hk + hk;
+  const int64_t row = ((int64_t)b * a.Nk + j) * a.Hk + hk, rows = (int64_t)a.B * a.Nk * a.Hk;
+  // parts: dk of every split, then dv
+  store_rows<T, DB>(ak, a.scale, splits == 1 ? dk + row * a.D : nullptr, part + (split * rows + row) * a.D, lh, a.D);
+  store_rows<T, DB>(av, 1.f, splits == 1 ? dv + row * a.D : nullptr, part + ((splits + split) * rows + row) * a.D, lh,
+                    a.D);
+}
+
+// out = sum over the splits of part[split][n], four values a thread; up to three arrays (a count of 0: none).
+struct JoinOne {
+  const float* part;
+  void* out;
+  int64_t n;   // values of one part, a multiple of 8
+  int splits;
+};
+struct JoinArgs {
+  JoinOne of[3];
+};
+template <class T>
+__global__ __launch_bounds__(kAttnThreads) void attn_bwd_join_kernel(const JoinArgs j) {
+  int64_t at = ((int64_t)blockIdx.x * kAttnThreads + threadIdx.x) * 4;
 #pragma unroll
-  for (int d = 0; d < DB; ++d)
+  for (int w = 0; w < 3; ++w) {
+    const JoinOne& o = j.of[w];
+    if (at >= 0 && at < o.n) {
+      f32x4 v = *reinterpret_cast<const f32x4*>(o.part + at);
+      for (int s = 1; s < o.splits; ++s) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(o.part + s * o.n + at);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int at = 32 * d + 8 * r + 4 * lh;
-      if (at < a.D) {
-        typedef T quad __attribute__((ext_vector_type(4)));
-        quad vk, vv;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          vk[c] = (T)(ak[d][4 * r + c] * a.scale);
-          vv[c] = (T)av[d][4 * r + c];
-        }
-        *reinterpret_cast<quad*>(dk + row * a.D + at) = vk;
-        *reinterpret_cast<quad*>(dv + row * a.D + at) = vv;
+        for (int c = 0; c < 4; ++c) v[c] += x[c];
       }
+      typedef T quad __attribute__((ext_vector_type(4)));
+      quad q;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) q[c] = (T)v[c];
+      *reinterpret_cast<quad*>(static_cast<T*>(o.out) + at) = q;
     }
+    at -= o.n;
+  }
 }
 
 // One workgroup a head: the parts of all query blocks by offset, then the offsets of each bucket, in order.
 __global__ __launch_bounds__(1024) void attn_bias_reduce_kernel(const AttnArgs a, const float* __restrict__ part,
                                                                 int groups, void* __restrict__ dtable) {
-  __shared__ float rel[2 * kMaxRadius + 1], sh[16][64];
-  const int h = blockIdx.x, nrel = 2 * a.radius + 1, col = threadIdx.x & 63, slice = threadIdx.x >> 6;
+  __shared__ float rel[2 * (kMaxRadius + kPad) + 1], sh[16][64];
+  __shared__ uint8_t which[2 * (kMaxRadius + kPad) + 1];
+  const int h = blockIdx.x, nrel = lut_size(a), col = threadIdx.x & 63, slice = threadIdx.x >> 6;
+  for (int e = threadIdx.x; e < nrel; e += 1024)
+    which[e] = (uint8_t)min((int)a.buckets[min(max(e - kPad, 0), 2 * a.radius)], a.nb - 1);
   for (int e0 = 0; e0 < nrel; e0 += 64) {
     const int e = e0 + col;
     float v = 0.f;
@@ -472,7 +518,8 @@ __global__ __launch_bounds__(1024) void attn_bias_reduce_kernel(const AttnArgs a
   }
   for (int t = threadIdx.x; t < a.nb; t += 1024) {
     float v = 0.f;
-    for (int e = 0; e < nrel; ++e) v += min((int)a.buckets[e], a.nb - 1) == t ? rel[e] : 0.f;
+#pragma unroll 8
+    for (int e = 0; e < nrel; ++e) v += which[e] == t ? rel[e] : 0.f;
     if (a.table_bf16)
       static_cast<bf16*>(dtable)[(int64_t)t * a.H + h] = (bf16)v;
     else
@@ -480,44 +527,72 @@ __global__ __launch_bounds__(1024) void attn_bias_reduce_kernel(const AttnArgs a
   }
 }
 
+// Workgroups that a row block's walk is split over: as many as bring the launch to two workgroups a CU, each with at
+// least two blocks of the walk.
+int walk_splits(int64_t groups, int64_t walk, int block) {
+  const int64_t want = (2 * (int64_t)compute_units() + groups - 1) / groups, most = walk / (2 * block);
+  const int64_t s = want < most ? want : most;
+  return s < 1 ? 1 : (int)(s < 16 ? s : 16);
+}
+
 struct BwdSpace {
-  size_t delta, bias, total;
+  int q_splits, kv_splits;
+  size_t delta, q_part, kv_part, bias, total;   // bytes, in this order
 };
-BwdSpace bwd_space(const AttnArgs& a, bool table) {
-  const int64_t qblocks = (a.Nq + kGroupRows - 1) / kGroupRows;
+BwdSpace bwd_space(const AttnArgs& a, bool f32, bool table) {
+  const int64_t qblocks = (a.Nq + kGroupRows - 1) / kGroupRows, kblocks = (a.Nk + kGroupRows - 1) / kGroupRows;
+  const int block = f32 ? Operand<float>::kBlock : Operand<bf16>::kBlock;
   BwdSpace s;
+  s.q_splits = walk_splits((int64_t)a.B * a.H * qblocks, a.Nk, block);
+  s.kv_splits = kblocks ? walk_splits((int64_t)a.B * a.Hk * kblocks, (int64_t)a.Nq * a.G, block) : 1;
   s.delta = (size_t)round_up((int64_t)a.B * a.H * a.Nq * 4, 256);
-  s.bias = table ? (size_t)(a.B * qblocks * a.H * (2 * a.radius + 1)) * 4 : 0;
-  s.total = s.delta + s.bias;
+  s.q_part = s.q_splits == 1 ? 0 : (size_t)round_up((int64_t)s.q_splits * a.B * a.H * a.Nq * a.D * 4, 256);
+  s.kv_part = s.kv_splits == 1 ? 0 : (size_t)round_up((int64_t)s.kv_splits * 2 * a.B * a.Hk * a.Nk * a.D * 4, 256);
+  s.bias = table ? (size_t)(a.B * qblocks * s.q_splits * a.H * (2 * (a.radius + kPad) + 1)) * 4 : 0;
+  s.total = s.delta + s.q_part + s.kv_part + s.bias;
   return s;
 }
 
 template <class T, int DP>
 int launch_bwd(const AttnArgs& a, const void* o, const float* lse, const void* dout, const int64_t* ds, void* dq,
                void* dk, void* dv, void* dtable, void* ws, hipStream_t stream) {
-  const BwdSpace sp = bwd_space(a, dtable != nullptr);
-  float* delta = static_cast<float*>(ws);
-  float* part = dtable ? reinterpret_cast<float*>(static_cast<char*>(ws) + sp.delta) : nullptr;
+  const BwdSpace sp = bwd_space(a, sizeof(T) == 4, dtable != nullptr);
+  char* at = static_cast<char*>(ws);
+  float* delta = reinterpret_cast<float*>(at);
+  float* q_part = reinterpret_cast<float*>(at + sp.delta);
+  float* kv_part = reinterpret_cast<float*>(at + sp.delta + sp.q_part);
+  float* bias = dtable ? reinterpret_cast<float*>(at + sp.delta + sp.q_part + sp.kv_part) : nullptr;
   const int qblocks = (a.Nq + kGroupRows - 1) / kGroupRows, kblocks = (a.Nk + kGroupRows - 1) / kGroupRows;
   {
-    const int64_t total = (int64_t)a.B * a.H * qblocks;
+    const int64_t total = (int64_t)a.B * a.H * qblocks * sp.q_splits;
     KernelTimerScope timer("attn_bwd_q", stream);
     attn_bwd_q_kernel<T, DP><<<dim3(attn_grid(total)), kAttnThreads, bias_lds(a, true), stream>>>(
         a, static_cast<const T*>(o), lse, static_cast<const T*>(dout), ds[0], ds[1], ds[2], static_cast<T*>(dq), delta,
-        part, qblocks, (int)total);
+        q_part, bias, sp.q_splits, qblocks, (int)total);
     if (const int rc = check_launch("attn_bwd_q")) return rc;
   }
   if (kblocks > 0) {
-    const int64_t total = (int64_t)a.B * a.Hk * kblocks;
+    const int64_t total = (int64_t)a.B * a.Hk * kblocks * sp.kv_splits;
     KernelTimerScope timer("attn_bwd_kv", stream);
     attn_bwd_kv_kernel<T, DP><<<dim3(attn_grid(total)), kAttnThreads, bias_lds(a, false), stream>>>(
         a, lse, static_cast<const T*>(dout), ds[0], ds[1], ds[2], delta, static_cast<T*>(dk), static_cast<T*>(dv),
-        kblocks, (int)total);
+        kv_part, sp.kv_splits, kblocks, (int)total);
     if (const int rc = check_launch("attn_bwd_kv")) return rc;
+  }
+  if (sp.q_splits > 1 || sp.kv_splits > 1) {
+    const int64_t nq = sp.q_splits > 1 ? (int64_t)a.B * a.Nq * a.H * a.D : 0;
+    const int64_t nk = sp.kv_splits > 1 ? (int64_t)a.B * a.Nk * a.Hk * a.D : 0;
+    const JoinArgs join{{{q_part, dq, nq, sp.q_splits},
+                         {kv_part, dk, nk, sp.kv_splits},
+                         {kv_part + sp.kv_splits * nk, dv, nk, sp.kv_splits}}};
+    KernelTimerScope timer("attn_bwd_join", stream);
+    const int64_t groups = (nq + 2 * nk + 4 * kAttnThreads - 1) / (4 * kAttnThreads);
+    attn_bwd_join_kernel<T><<<dim3((unsigned)groups), kAttnThreads, 0, stream>>>(join);
+    if (const int rc = check_launch("attn_bwd_join")) return rc;
   }
   if (!dtable) return BIOEMU_OK;
   KernelTimerScope timer("attn_bias_reduce", stream);
-  attn_bias_reduce_kernel<<<dim3((unsigned)a.H), 1024, 0, stream>>>(a, part, a.B * qblocks, dtable);
+  attn_bias_reduce_kernel<<<dim3((unsigned)a.H), 1024, 0, stream>>>(a, bias, a.B * qblocks * sp.q_splits, dtable);
   return check_launch("attn_bias_reduce");
 }
 
@@ -529,7 +604,7 @@ using namespace bioemu;
 extern "C" size_t bioemu_attention_bwd_workspace_bytes(const bioemu_attention_args* args, int table_gradient) {
   AttnArgs a;
   if (attn_args("attention_bwd", args, &a) || a.B == 0 || a.Nq == 0) return 0;
-  return bwd_space(a, table_gradient && a.table).total;
+  return bwd_space(a, args->f32 != 0, table_gradient && a.table).total;
 }
 
 extern "C" int bioemu_attention_bwd(const bioemu_attention_args* args, const void* o, const float* lse,
@@ -547,7 +622,7 @@ extern "C" int bioemu_attention_bwd(const bioemu_attention_args* args, const voi
     return set_error(BIOEMU_ERR_INVALID_ARG,
                      "attention_bwd: rows start at 16-byte addresses, at least a head's width apart");
   if (dtable && !a.table) return set_error(BIOEMU_ERR_INVALID_ARG, "attention_bwd: dtable without a table");
-  const size_t need = bwd_space(a, dtable != nullptr).total;
+  const size_t need = bwd_space(a, args->f32 != 0, dtable != nullptr).total;
   if (!workspace || !aligned16(workspace) || workspace_bytes < need)
     return set_error(BIOEMU_ERR_WORKSPACE, "attention_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   const int dp = a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128;

@@ -32,11 +32,11 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
   typedef Tile<T, DP, KB> KV;
   constexpr int CP = KV::copies(kAttnThreads);
   __shared__ __attribute__((aligned(1024))) char tiles[2][2][KV::BYTES];
-  __shared__ int segs[2][64];
-  __shared__ float lut[2 * kMaxRadius + 1];
+  __shared__ __attribute__((aligned(16))) int segs[2][64];
+  __shared__ float lut[2 * (kMaxRadius + kPad) + 1];
   __shared__ int list[kListBlocks];
   __shared__ uint8_t flags[kListBlocks];
-  __shared__ int red[4];
+  __shared__ int red[3][4], count;
 
   const int item = attn_item(total);
   if (item < 0) return;
@@ -55,9 +55,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
   // keys below lim are allowed (their segment aside); rows past the last one restrict nothing
   int lim = a.causal ? min(max(pos + 1, prefix), length) : length;
   if (qseg < 0) lim = 0;
-  const int seg_lo = seg ? wg_extreme<false>(live && qseg >= 0 ? qseg : 0x7fffffff, red) : 0;
-  const int seg_hi = seg ? wg_extreme<true>(live ? qseg : -1, red) : 0;
-  const int wg_max = wg_extreme<true>(live ? lim : 0, red);
+  int seg_lo = live && qseg >= 0 ? qseg : 0x7fffffff, seg_hi = live ? qseg : -1, wg_max = live ? lim : 0;
+  wg_extremes(seg_lo, seg_hi, wg_max, red);
   int wave_min = live ? lim : 0x7fffffff, wave_max = live ? lim : 0;
 #pragma unroll
   for (int m = 16; m > 0; m /= 2) {
@@ -69,8 +68,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
   const int wave_pos = __builtin_amdgcn_readfirstlane(pos);   // of the wave's first row
   if (!live) lim = 0x7fffffff;
 
-  if (a.table)
-    for (int e = threadIdx.x; e < 2 * a.radius + 1; e += kAttnThreads) lut[e] = table_value(a, e, h);
+  if (a.table) fill_lut(a, h, lut);
 
   Frag<T> qf[STEPS];
   {
@@ -88,9 +86,10 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
   f32x16 acc[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) acc[d] = zero16();
-  float m = -kInf, mref = 0.f, l = 0.f;   // the running maximum, what weights are taken against, their sum
-  const float s_scale = a.cap > 0.f ? a.scale / a.cap : a.scale * kLog2e;
-  const float s_cap = a.cap * kLog2e;
+  // weights are 2^(x - mref); a row starts with its first finite score, then mref moves when one exceeds limit
+  float mref = 0.f, limit = -kInf, l = 0.f;
+  const bool cap = a.cap > 0.f;
+  const float s_scale = cap ? a.scale / a.cap : a.scale * kLog2e, s_cap = a.cap * kLog2e, mult = cap ? 1.f : s_scale;
 
   auto stage = [&](int entry, int buf) {
     const int k0 = (entry & kBlockMask) * KB;
@@ -102,7 +101,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
   const int blocks = (wg_max + KB - 1) / KB;
   for (int c0 = 0; c0 < blocks; c0 += kListBlocks) {
     const int c1 = seg ? min(blocks, c0 + kListBlocks) : blocks;
-    const int n = seg ? list_blocks<KB>(kseg, length, seg_lo, seg_hi, c0, c1, flags, list, red) : blocks;
+    const int n = seg ? list_blocks<KB>(kseg, length, seg_lo, seg_hi, c0, c1, flags, list, &count) : blocks;
     const int t0 = (int)((int64_t)n * split / splits), t1 = (int)((int64_t)n * (split + 1) / splits);
     auto entry = [&](int t) { return seg ? __builtin_amdgcn_readfirstlane(list[t]) : t | kEntryFull; };
     if (t0 < t1) stage(entry(t0), t0 & 1);
@@ -125,52 +124,55 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
         f32x16 s = zero16();
 #pragma unroll
         for (int st = 0; st < STEPS; ++st) s = mfma16(KV::rows(kt, 32 * u + ln, st, lh), qf[st], s);
+        if (cap)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[u][r] = s[r] * s_scale;
-        if (a.cap > 0.f)
+          for (int r = 0; r < 16; ++r) s[r] = s_cap * attn_tanh<T>(s[r] * s_scale);
+        const int rel0 = k0 + 32 * u - wave_pos;   // of the wave's first query and the first key
+        if (a.table && !all_far(a, rel0)) {
+          const float* bias = lut + (rel0 + a.radius + kPad + 4 * lh - ln);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) x[u][r] = s_cap * attn_tanh<T>(x[u][r]);
-        if (a.table) {
-          const int rel0 = k0 + 32 * u - wave_pos;   // of the wave's first query and the first key
-          if (rel0 - 31 >= a.radius || rel0 + 31 <= -a.radius) {
-            const float far = lut[rel0 > 0 ? 2 * a.radius : 0];
+          for (int r = 0; r < 16; ++r) x[u][r] = s[r] * mult + bias[8 * (r >> 2) + (r & 3)];
+        } else {
+          const float add = a.table ? lut[rel0 > 0 ? 2 * (a.radius + kPad) : 0] : 0.f;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) x[u][r] += far;
-          } else {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int rel = rel0 - ln + 8 * (r >> 2) + 4 * lh + (r & 3);
-              x[u][r] += lut[min(max(rel, -a.radius), a.radius) + a.radius];
-            }
-          }
+          for (int r = 0; r < 16; ++r) x[u][r] = s[r] * mult + add;
         }
       }
-      if (k0 + KB > wave_min || !(e & kEntryFull)) {
+      if (k0 + KB > wave_min)
 #pragma unroll
         for (int u = 0; u < SUB; ++u)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int kk = 32 * u + 8 * (r >> 2) + 4 * lh + (r & 3);
-            const bool ok = (k0 + kk < lim) & (!seg | (segs[buf][kk] == qseg));
-            x[u][r] = ok ? x[u][r] : -kInf;
+          for (int r = 0; r < 16; ++r)
+            x[u][r] = k0 + 32 * u + 8 * (r >> 2) + 4 * lh + (r & 3) < lim ? x[u][r] : -kInf;
+      if (!(e & kEntryFull))
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int4 ks = *reinterpret_cast<const int4*>(&segs[buf][32 * u + 8 * q + 4 * lh]);
+            x[u][4 * q] = ks.x == qseg ? x[u][4 * q] : -kInf;
+            x[u][4 * q + 1] = ks.y == qseg ? x[u][4 * q + 1] : -kInf;
+            x[u][4 * q + 2] = ks.z == qseg ? x[u][4 * q + 2] : -kInf;
+            x[u][4 * q + 3] = ks.w == qseg ? x[u][4 * q + 3] : -kInf;
           }
-      }
       float mx = x[0][0];
 #pragma unroll
       for (int u = 0; u < SUB; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, x[u][r]);
       mx = fmaxf(mx, __shfl_xor(mx, 32));
-      if (__ballot(mx > m + kRescale)) {
-        const float mn = fmaxf(m, mx), to = mn == -kInf ? 0.f : mn;
-        const float f = fast_exp2(m - to);
+      // against mref only now: scores of the type's lowest value may have come first
+      if (__ballot(mx > limit)) {
+        const bool begun = limit > -kInf;
+        const float to = mx == -kInf ? mref : (begun ? fmaxf(mref, mx) : mx);
+        const float f = begun ? fast_exp2(mref - to) : 0.f;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[d][r] *= f;
         l *= f;
-        m = mn;
         mref = to;
+        if (mx > -kInf || begun) limit = mref + kRescale;
       }
 #pragma unroll
       for (int u = 0; u < SUB; ++u) {
