@@ -105,10 +105,13 @@ __device__ __forceinline__ void copy_to_lds(u32x4 source, unsigned voff, void* l
                  : "memory");
 }
 
-// Row swizzle of 16-byte pieces, by pieces per row (a power of two).
+// Row swizzle of 16-byte pieces, by pieces per row (a power of two).  A read of 32 rows' pieces takes rows that differ
+// in bits 0 and 1 and two of bits 2 .. 4 at a time; a transposing read takes four rows' 64 neighbouring bytes.  Both
+// meet every bank once where bits 0 and 1 of the row choose a 64-byte quarter of 256 bytes of LDS and bits 2 and 3 a
+// piece of it (the first row bits are in the address already where rows are 64 or 128 bytes).
 template <int CPR>
 __device__ __forceinline__ int attn_swz(int r) {
-  return CPR == 4 ? (r >> 2) & 3 : CPR == 8 ? (r >> 1) & 7 : r & 15;
+  return CPR == 4 ? (r >> 2) & 3 : CPR == 8 ? ((r >> 1) & 1) * 4 + ((r >> 2) & 3) : (r & 3) * 4 + ((r >> 2) & 3);
 }
 
 // A tile in LDS: ROWS rows of DP values of T.
@@ -309,12 +312,22 @@ __device__ __forceinline__ int list_blocks(const int* __restrict__ seg, int n, i
   return __builtin_amdgcn_readfirstlane(*count);
 }
 
-// XCD-aware order: workgroup w runs on XCD w % 8, each XCD gets a contiguous range of the items (so the workgroups
-// that read the same keys share its L2); -1 for padding workgroups.
-__device__ __forceinline__ int attn_item(int total) {
-  const int w = blockIdx.x, per = (total + kAttnXcds - 1) / kAttnXcds;
-  const int item = (w % kAttnXcds) * per + w / kAttnXcds;
-  return w / kAttnXcds < per && item < total ? item : -1;
+// XCD-aware order of `total` = rows x `cols` items (a row: the blocks of one head): workgroup w runs on XCD w % 8, each
+// XCD gets a contiguous range of the items (so the workgroups that read the same keys share its L2); -1 for padding
+// workgroups.  An XCD with whole rows takes them column by column: with the long blocks of a causal mask in the first
+// columns, long items start first, whatever their head; and the second 32 of them (it has 32 CUs, two workgroups each)
+// go backwards, so that the CU of the longest gets the shortest beside it.
+__device__ __forceinline__ int attn_item(int total, int cols) {
+  const int w = blockIdx.x, per = (total + kAttnXcds - 1) / kAttnXcds, base = (w % kAttnXcds) * per;
+  const int n = min(per, total - base);
+  int p = w / kAttnXcds;
+  if (p >= n) return -1;
+  if (p >= 32 && p < 64) p = 32 + min(64, n) - 1 - p;
+  if (n % cols == 0 && base % cols == 0) {
+    const int rows = n / cols;
+    p = (p % rows) * cols + p / rows;
+  }
+  return base + p;
 }
 inline unsigned attn_grid(int64_t total) { return (unsigned)(round_up(total, kAttnXcds)); }
 

@@ -11,9 +11,11 @@
 //
 // Either may split its walk over workgroups where the rows alone do not fill the chip; attn_bwd_join adds the parts.
 //
-// The table's gradient: per wave an LDS row of sums by offset, added to with one LDS add an element (a wave's adds are
-// in program order, its 32 queries fall on 32 different offsets, its two halves have rows of their own); blocks wholly
-// at or beyond the radius stay in registers.  Then waves, workgroups and buckets in fixed orders.
+// The table's gradient sums ds along the diagonals of every 32 x 32 block that meets the radius: the block goes to LDS,
+// rows 68 values apart with zeros between them, and lane e reads its diagonal (value e + n - 31 of row n) without a
+// bound to check, 16 reads of two values.  (One LDS add an element took 45 cycles each, 8 times the whole.)  Every wave
+// has a row of sums by offset; blocks wholly at or beyond the radius stay in registers.  Then waves, the offsets of a
+// bucket and workgroups are added in fixed orders.
 #include "attn.h"
 
 namespace bioemu {
@@ -21,9 +23,12 @@ namespace {
 
 constexpr int kGroupRows = 128;
 
-// LDS beyond the tiles: bias values by offset, and sums of ds by offset, 8 rows (4 waves x 2 lane halves).
+constexpr int kDiagRow = 68, kDiagBlock = 32 + 32 * kDiagRow;   // floats; 32 zeros in front of row 0
+
+// LDS beyond the tiles: bias values by offset, and for the table's gradient, per wave, sums of ds by offset and a block.
 inline size_t bias_lds(const AttnArgs& a, bool sums) {
-  return a.table ? (size_t)(2 * (a.radius + kPad) + 1) * sizeof(float) * (sums ? 9 : 1) : 0;
+  const size_t n = round_up(2 * (a.radius + kPad) + 1, 4);
+  return a.table ? (n + (sums ? 4 * (n + kDiagBlock) : 0)) * sizeof(float) : 0;
 }
 
 // A lane's row of an accumulator [DB] of 32-value blocks times `scale`, rounded into `out`, or as fp32 into `part`.
@@ -66,9 +71,9 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
   __shared__ uint8_t flags[kListBlocks];
   __shared__ int red[3][4], count;
   __shared__ float ends[4][2];
-  extern __shared__ float dyn[];   // bias values by offset, then the sums [4][2] by offset
+  extern __shared__ __attribute__((aligned(16))) float dyn[];   // bias values, sums by offset [4], blocks [4]
 
-  const int item = attn_item(total);
+  const int item = attn_item(total, qblocks);
   if (item < 0) return;
   const int lane = threadIdx.x & 63, wave = wave_id(), ln = lane & 31, lh = lane >> 5;
   const int qblk = qblocks - 1 - item % qblocks, rest = item / qblocks, split = rest % splits, bh = rest / splits;
@@ -76,8 +81,9 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
   const int length = a.lengths ? min(max(a.lengths[b], 0), a.Nk) : a.Nk;
   const int prefix = a.prefix ? a.prefix[b] : 0;
   const bool seg = a.q_seg != nullptr;
-  const int nrel = lut_size(a);
-  float *lut = dyn, *sums = dyn + nrel;
+  const int nrel = lut_size(a), row4 = (nrel + 3) & ~3;
+  float *lut = dyn, *sums = dyn + row4, *own = sums + wave * row4;
+  float* diag = sums + 4 * row4 + wave * kDiagBlock + 32;
 
   const int i = qblk * kGroupRows + wave * 32 + ln;
   const bool live = i < a.Nq;
@@ -99,7 +105,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
 
   if (a.table) {
     fill_lut(a, h, lut);
-    for (int e = threadIdx.x; e < 8 * nrel; e += kAttnThreads) sums[e] = 0.f;
+    if (bias_part)
+      for (int e = threadIdx.x; e < 4 * (row4 + kDiagBlock); e += kAttnThreads) sums[e] = 0.f;
   }
 
   // a row that sees nothing contributes nothing, whatever it holds
@@ -136,7 +143,6 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
   float far_lo = 0.f, far_hi = 0.f;
   const bool cap = a.cap > 0.f;
   const float s_scale = cap ? a.scale / a.cap : a.scale * kLog2e, s_cap = a.cap * kLog2e, mult = cap ? 1.f : s_scale;
-  float* own = sums + (wave * 2 + lh) * nrel + a.radius + kPad + 4 * lh - ln;   // offset of key 4 lh from this query
 
   auto stage = [&](int entry, int buf) {
     const int k0 = (entry & kBlockMask) * KB;
@@ -220,9 +226,18 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
               far_lo += v;
           } else {
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              __hip_atomic_fetch_add(own + rel0 + 8 * (r >> 2) + (r & 3), x[r], __ATOMIC_RELAXED,
-                                     __HIP_MEMORY_SCOPE_WORKGROUP);
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<f32x4*>(diag + ln * kDiagRow + 8 * q + 4 * lh) =
+                  f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            float v0 = 0.f, v1 = 0.f;
+#pragma unroll
+            for (int n = 0; n < 32; n += 2) {
+              v0 += diag[n * (kDiagRow + 1) + lane - 31];
+              v1 += diag[(n + 1) * (kDiagRow + 1) + lane - 31];
+            }
+            if (lane < 63) own[rel0 + lane - 31 + a.radius + kPad] += v0 + v1;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
           }
         }
         if (cap)
@@ -254,15 +269,29 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
       ends[wave][1] = far_hi;
     }
     __syncthreads();
-    float* out = bias_part + ((((int64_t)b * qblocks + qblk) * splits + split) * a.H + h) * nrel;
+    // waves in order into the first one's row, then each wave a quarter of the offsets into the buckets
+    uint8_t* which = reinterpret_cast<uint8_t*>(lut);
     for (int e = threadIdx.x; e < nrel; e += kAttnThreads) {
-      float v = 0.f;
-#pragma unroll
-      for (int w = 0; w < 8; ++w) v += sums[w * nrel + e];
+      float v = (sums[e] + sums[row4 + e]) + (sums[2 * row4 + e] + sums[3 * row4 + e]);
       if (e == 0) v += (ends[0][0] + ends[1][0]) + (ends[2][0] + ends[3][0]);
       if (e == nrel - 1) v += (ends[0][1] + ends[1][1]) + (ends[2][1] + ends[3][1]);
-      out[e] = v;
+      sums[e] = v;
+      which[e] = (uint8_t)min((int)a.buckets[min(max(e - kPad, 0), 2 * a.radius)], a.nb - 1);
     }
+    __syncthreads();
+    float* quarter = sums + 4 * row4 + wave * 256;   // over the blocks
+    const int e0 = nrel * wave / 4, e1 = nrel * (wave + 1) / 4;
+    for (int t = lane; t < a.nb; t += 64) {
+      float v = 0.f;
+#pragma unroll 4
+      for (int e = e0; e < e1; ++e) v += which[e] == t ? sums[e] : 0.f;
+      quarter[t] = v;
+    }
+    __syncthreads();
+    quarter = sums + 4 * row4;
+    float* out = bias_part + (((int64_t)b * qblocks + qblk) * splits + split) * a.nb * a.H + h;
+    for (int t = threadIdx.x; t < a.nb; t += kAttnThreads)
+      out[(int64_t)t * a.H] = (quarter[t] + quarter[256 + t]) + (quarter[512 + t] + quarter[768 + t]);
   }
 }
 
@@ -284,7 +313,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArg
   __shared__ int red[3][4], count;
   extern __shared__ float lut[];
 
-  const int item = attn_item(total);
+  const int item = attn_item(total, kblocks);
   if (item < 0) return;
   const int lane = threadIdx.x & 63, wave = wave_id(), ln = lane & 31, lh = lane >> 5;
   const int kblk = item % kblocks, rest = item / kblocks, split = rest % splits, bh = rest / splits;
@@ -492,38 +521,26 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_join_kernel(const JoinA
   }
 }
 
-// One workgroup a head: the parts of all query blocks by offset, then the offsets of each bucket, in order.
-__global__ __launch_bounds__(1024) void attn_bias_reduce_kernel(const AttnArgs a, const float* __restrict__ part,
-                                                                int groups, void* __restrict__ dtable) {
-  __shared__ float rel[2 * (kMaxRadius + kPad) + 1], sh[16][64];
-  __shared__ uint8_t which[2 * (kMaxRadius + kPad) + 1];
-  const int h = blockIdx.x, nrel = lut_size(a), col = threadIdx.x & 63, slice = threadIdx.x >> 6;
-  for (int e = threadIdx.x; e < nrel; e += 1024)
-    which[e] = (uint8_t)min((int)a.buckets[min(max(e - kPad, 0), 2 * a.radius)], a.nb - 1);
-  for (int e0 = 0; e0 < nrel; e0 += 64) {
-    const int e = e0 + col;
-    float v = 0.f;
-    if (e < nrel)
+// dtable[k] = sum over the query blocks' parts of part[g][k].  One workgroup: 16 values x 64 slices of the parts.
+__global__ __launch_bounds__(1024) void attn_bias_reduce_kernel(const float* __restrict__ part, int groups, int size,
+                                                                void* __restrict__ dtable, int table_bf16) {
+  __shared__ float sh[64][17];
+  const int k = blockIdx.x * 16 + (threadIdx.x & 15), slice = threadIdx.x >> 4;
+  float s = 0.f;
+  if (k < size)
 #pragma unroll 4
-      for (int g = slice; g < groups; g += 16) v += part[((int64_t)g * a.H + h) * nrel + e];
-    sh[slice][col] = v;
-    __syncthreads();
-    if (slice == 0 && e < nrel) {
-      v = 0.f;
-#pragma unroll
-      for (int s = 0; s < 16; ++s) v += sh[s][col];
-      rel[e] = v;
-    }
+    for (int g = slice; g < groups; g += 64) s += part[(int64_t)g * size + k];
+  sh[slice][threadIdx.x & 15] = s;
+  __syncthreads();
+  for (int m = 32; m > 0; m /= 2) {
+    if (slice < m) sh[slice][threadIdx.x & 15] += sh[slice + m][threadIdx.x & 15];
     __syncthreads();
   }
-  for (int t = threadIdx.x; t < a.nb; t += 1024) {
-    float v = 0.f;
-#pragma unroll 8
-    for (int e = 0; e < nrel; ++e) v += which[e] == t ? rel[e] : 0.f;
-    if (a.table_bf16)
-      static_cast<bf16*>(dtable)[(int64_t)t * a.H + h] = (bf16)v;
+  if (slice == 0 && k < size) {
+    if (table_bf16)
+      static_cast<bf16*>(dtable)[k] = (bf16)sh[0][threadIdx.x];
     else
-      static_cast<float*>(dtable)[(int64_t)t * a.H + h] = v;
+      static_cast<float*>(dtable)[k] = sh[0][threadIdx.x];
   }
 }
 
@@ -548,7 +565,7 @@ BwdSpace bwd_space(const AttnArgs& a, bool f32, bool table) {
   s.delta = (size_t)round_up((int64_t)a.B * a.H * a.Nq * 4, 256);
   s.q_part = s.q_splits == 1 ? 0 : (size_t)round_up((int64_t)s.q_splits * a.B * a.H * a.Nq * a.D * 4, 256);
   s.kv_part = s.kv_splits == 1 ? 0 : (size_t)round_up((int64_t)s.kv_splits * 2 * a.B * a.Hk * a.Nk * a.D * 4, 256);
-  s.bias = table ? (size_t)(a.B * qblocks * s.q_splits * a.H * (2 * (a.radius + kPad) + 1)) * 4 : 0;
+  s.bias = table ? (size_t)(a.B * qblocks * s.q_splits * a.H * a.nb) * 4 : 0;
   s.total = s.delta + s.q_part + s.kv_part + s.bias;
   return s;
 }
@@ -566,7 +583,7 @@ int launch_bwd(const AttnArgs& a, const void* o, const float* lse, const void* d
   {
     const int64_t total = (int64_t)a.B * a.H * qblocks * sp.q_splits;
     KernelTimerScope timer("attn_bwd_q", stream);
-    attn_bwd_q_kernel<T, DP><<<dim3(attn_grid(total)), kAttnThreads, bias_lds(a, true), stream>>>(
+    attn_bwd_q_kernel<T, DP><<<dim3(attn_grid(total)), kAttnThreads, bias_lds(a, dtable != nullptr), stream>>>(
         a, static_cast<const T*>(o), lse, static_cast<const T*>(dout), ds[0], ds[1], ds[2], static_cast<T*>(dq), delta,
         q_part, bias, sp.q_splits, qblocks, (int)total);
     if (const int rc = check_launch("attn_bwd_q")) return rc;
@@ -592,7 +609,9 @@ int launch_bwd(const AttnArgs& a, const void* o, const float* lse, const void* d
   }
   if (!dtable) return BIOEMU_OK;
   KernelTimerScope timer("attn_bias_reduce", stream);
-  attn_bias_reduce_kernel<<<dim3((unsigned)a.H), 1024, 0, stream>>>(a, bias, a.B * qblocks * sp.q_splits, dtable);
+  const int size = a.nb * a.H;
+  attn_bias_reduce_kernel<<<dim3((unsigned)((size + 15) / 16)), 1024, 0, stream>>>(bias, a.B * qblocks * sp.q_splits,
+                                                                                  size, dtable, a.table_bf16);
   return check_launch("attn_bias_reduce");
 }
 

@@ -38,7 +38,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
   __shared__ uint8_t flags[kListBlocks];
   __shared__ int red[3][4], count;
 
-  const int item = attn_item(total);
+  const int item = attn_item(total, qblocks);
   if (item < 0) return;
   const int lane = threadIdx.x & 63, wave = wave_id(), ln = lane & 31, lh = lane >> 5;
   const int qblk = qblocks - 1 - item % qblocks;   // long rows of a causal mask first
@@ -246,7 +246,7 @@ __global__ __launch_bounds__(64 * few_waves<T>()) void attn_few_kernel(const Att
   __shared__ __attribute__((aligned(1024))) char tiles[W][2][2][KV::BYTES];
   __shared__ float ml[W][2][32];
 
-  const int item = attn_item(total);
+  const int item = attn_item(total, splits);
   if (item < 0) return;
   const int lane = threadIdx.x & 63, wave = wave_id(), ln = lane & 31, lh = lane >> 5;
   const int split = item % splits, bh = item / splits, hk = bh % a.Hk, b = bh / a.Hk;
