@@ -11,6 +11,7 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libbioemu2_mi355x.so"
+TORCH_LIB_PATH = LIB_PATH.with_name("libbioemu2_torch.so")   # the trainable operators as torch ops, over the C ABI
 
 _c_void_p = ctypes.c_void_p
 _c_size_t = ctypes.c_size_t
@@ -194,6 +195,28 @@ def lib() -> ctypes.CDLL:
                 fn.argtypes = argtypes
             _lib = handle
     return _lib
+
+
+_torch_ops: dict[str, object] = {}
+
+
+def torch_op(name: str):
+    """``torch.ops.bioemu_mi355x.<name>`` of the trainable operators, whose library is loaded on first use."""
+    op = _torch_ops.get(name)
+    if op is None:
+        import torch
+
+        lib()   # its C ABI, and its message where it is missing
+        with _lock:
+            if not _torch_ops:
+                if not TORCH_LIB_PATH.exists():
+                    raise NativeLibraryError(
+                        f"bioemu2_amd torch library not found at {TORCH_LIB_PATH}; "
+                        "build it with `python -m bioemu2_amd.build`"
+                    )
+                torch.ops.load_library(str(TORCH_LIB_PATH))
+            op = _torch_ops[name] = getattr(torch.ops.bioemu_mi355x, name).default
+    return op
 
 
 def check(rc: int, what: str) -> None:

@@ -19,7 +19,8 @@ import torch
 import torch.nn as nn
 from torch import Tensor
 
-from . import _ops, _seq_ops
+from . import _ops
+from ._lib import torch_op
 from .relative_position import _int32, distance_buckets
 
 
@@ -54,8 +55,6 @@ def attention(
     _ops.require_gpu(q, "attention")
     if q.ndim != 4:
         raise ValueError(f"attention: q must be [B, Nq, H, D], got {tuple(q.shape)}")
-    if bias_buckets is not None and bias_table is None:
-        raise ValueError("attention: a bias table [num_buckets, H] comes with its buckets")
     if key_segments is None:
         key_segments = segments
     elif segments is None:
@@ -75,10 +74,9 @@ def attention(
     dtype = q.dtype
     if dtype == torch.float32 and not _ops.fp32_mode(q):
         q, k, v = (t.to(torch.bfloat16) for t in (q, k, v))
-    out = _seq_ops.attention(
-        q, k, v, None if bias_table is None else bias_table.contiguous(), bias_buckets, segments, key_segments, prefix,
-        cache_lengths, q.shape[-1] ** -0.5 if scale is None else float(scale), 0.0 if cap is None else float(cap),
-        bool(causal))
+    out = torch_op("attention")(
+        q, k, v, bias_table, bias_buckets, segments, key_segments, prefix, cache_lengths,
+        q.shape[-1] ** -0.5 if scale is None else scale, 0.0 if cap is None else cap, causal)
     return out if out.dtype == dtype else out.to(dtype)
 
 

@@ -1,8 +1,9 @@
-"""Builds ``libbioemu2_mi355x.so`` (all HIP kernels + the C ABI) in-tree for gfx950.
+"""Builds ``libbioemu2_mi355x.so`` (all HIP kernels + the C ABI) and ``libbioemu2_torch.so`` (the trainable operators
+as torch ops over it) in-tree for gfx950.
 
 Usage: ``python -m bioemu2_amd.build`` (also called by ``__graft_entry__.build()``).
-Always recompiles; the ``.so`` lands next to this file so it travels with the
-source tree and is what the Python layer loads.
+Always recompiles; both ``.so`` land next to this file so they travel with the
+source tree and are what the Python layer loads.
 """
 
 from __future__ import annotations
@@ -19,6 +20,7 @@ PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 INCLUDE = PKG_DIR.parent / "include"
 LIB_NAME = "libbioemu2_mi355x.so"
+TORCH_LIB_NAME = "libbioemu2_torch.so"
 ARCH = os.environ.get("BIOEMU_OFFLOAD_ARCH", "gfx950")
 
 # Packed-fp32 VALU ops are disabled for device code; the host pass warns that
@@ -66,26 +68,60 @@ def _compile(src: Path, obj: Path) -> None:
         print(out, file=sys.stderr)
 
 
+def _compile_torch(obj: Path) -> None:
+    """The torch ops' glue: host code against the installed torch."""
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    rocm = Path(_hipcc()).resolve().parents[1]
+    cmd = [
+        shutil.which("g++") or _hipcc(), "-O2", "-std=c++17", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        *(f"-isystem{p}" for p in include_paths()), f"-isystem{rocm / 'include'}", f"-I{INCLUDE}",
+        "-c", str(CSRC / "torch_ops.cpp"), "-o", str(obj),
+    ]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for torch_ops.cpp:\n{res.stdout}{res.stderr}")
+
+
+def _install(built: Path, name: str) -> Path:
+    """Atomic replace, so that a running process never maps a half-written file."""
+    target = PKG_DIR / name
+    staged = target.with_suffix(".so.tmp")
+    shutil.copy2(built, staged)
+    os.replace(staged, target)
+    return target
+
+
+def _link(cmd: list[str]) -> None:
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"link failed:\n{res.stdout}{res.stderr}")
+
+
 def build(verbose: bool = True) -> Path:
     sources = sorted(CSRC.glob("*.hip"))
     if not sources:
         raise RuntimeError(f"no HIP sources under {CSRC}")
-    target = PKG_DIR / LIB_NAME
     with tempfile.TemporaryDirectory(prefix="bioemu_build_") as tmp:
         objs = [Path(tmp) / (s.stem + ".o") for s in sources]
-        with cf.ThreadPoolExecutor(max_workers=min(8, len(sources))) as ex:
+        glue = Path(tmp) / "torch_ops.o"
+        with cf.ThreadPoolExecutor(max_workers=min(8, len(sources) + 1)) as ex:
+            torch_done = ex.submit(_compile_torch, glue)   # the longest, first
             list(ex.map(_compile, sources, objs))
-        tmp_lib = Path(tmp) / LIB_NAME
-        cmd = [_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp_lib)]
-        res = subprocess.run(cmd, capture_output=True, text=True)
-        if res.returncode != 0:
-            raise RuntimeError(f"link failed:\n{res.stdout}{res.stderr}")
-        # Atomic replace so a running process never maps a half-written file.
-        staged = target.with_suffix(".so.tmp")
-        shutil.copy2(tmp_lib, staged)
-        os.replace(staged, target)
+            torch_done.result()
+        tmp_lib, tmp_torch = Path(tmp) / LIB_NAME, Path(tmp) / TORCH_LIB_NAME
+        _link([_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp_lib)])
+        import torch
+
+        torch_lib = Path(torch.__file__).resolve().parent / "lib"
+        _link([shutil.which("g++") or _hipcc(), "-shared", "-fPIC", str(glue), "-o", str(tmp_torch), f"-L{tmp}",
+               f"-l:{LIB_NAME}", f"-L{torch_lib}", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-Wl,-rpath,$ORIGIN"])
+        target = _install(tmp_lib, LIB_NAME)
+        _install(tmp_torch, TORCH_LIB_NAME)
     if verbose:
-        print(f"built {target} from {len(sources)} sources for {ARCH}")
+        print(f"built {target} from {len(sources)} sources for {ARCH}, and {TORCH_LIB_NAME}")
     return target
 
 

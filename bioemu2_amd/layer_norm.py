@@ -14,7 +14,8 @@ import torch
 import torch.nn as nn
 from torch import Tensor
 
-from . import _ops, _seq_ops
+from . import _ops
+from ._lib import torch_op
 
 
 def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, eps: float = 1e-5) -> Tensor:
@@ -23,10 +24,7 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
     ``weight`` and ``bias`` ([c], fp32 or bf16, one type) may be absent.  Rows may have any stride; c is at most 16384
     where rows are whole 16-byte vectors and 4096 else."""
     _ops.require_gpu(x, "layer_norm")
-    if x.ndim == 0 or x.shape[-1] == 0:
-        raise ValueError(f"layer_norm: x must have a last dimension, got {tuple(x.shape)}")
-    return _seq_ops.layer_norm(x, None if weight is None else weight.contiguous(),
-                               None if bias is None else bias.contiguous(), float(eps))
+    return torch_op("layer_norm")(x, weight, bias, eps)
 
 
 class LayerNorm(nn.Module):

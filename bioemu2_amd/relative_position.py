@@ -19,7 +19,8 @@ import torch
 import torch.nn as nn
 from torch import Tensor
 
-from . import _ops, _seq_ops
+from . import _ops
+from ._lib import torch_op
 
 
 def distance_buckets(radius: int, num_buckets: int | None = None, device=None) -> Tensor:
@@ -55,9 +56,11 @@ def distance_buckets(radius: int, num_buckets: int | None = None, device=None) -
 
 
 def _int32(t: Tensor, what: str) -> Tensor:
+    if t.dtype == torch.int32:
+        return t
     if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
         raise ValueError(f"{what}: expected whole numbers, got {t.dtype}")
-    return t.to(torch.int32).contiguous()
+    return t.to(torch.int32)
 
 
 def relative_position(table: Tensor, buckets: Tensor, positions: Tensor, chains: Tensor | None = None,
@@ -69,17 +72,13 @@ def relative_position(table: Tensor, buckets: Tensor, positions: Tensor, chains:
     positions, chains: whole numbers [B, N]; the result has z's type, or ``dtype`` (the table's by default), bf16 or
     fp32.  Gradients: ``table`` and ``z``."""
     _ops.require_gpu(table, "relative_position")
-    if table.ndim != 2 or positions.ndim != 2:
-        raise ValueError(f"relative_position: table {tuple(table.shape)}, positions {tuple(positions.shape)}")
     if z is not None:
         if dtype is not None and dtype != z.dtype:
             raise ValueError(f"relative_position: dtype {dtype}, z is {z.dtype}")
         dtype = z.dtype
-    dtype = table.dtype if dtype is None else dtype
-    if dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"relative_position: expected fp32 or bf16, got {dtype}")
-    return _seq_ops.relative_position(table, z, buckets, _int32(positions, "relative_position positions"),
-                                      None if chains is None else _int32(chains, "relative_position chains"), dtype)
+    return torch_op("relative_position")(
+        table, z, buckets, _int32(positions, "relative_position positions"),
+        None if chains is None else _int32(chains, "relative_position chains"), table.dtype if dtype is None else dtype)
 
 
 class RelativePosition(nn.Module):

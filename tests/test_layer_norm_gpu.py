@@ -17,7 +17,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from bioemu2_amd import _seq_ops
+from bioemu2_amd import _lib
 from bioemu2_amd.layer_norm import LayerNorm, layer_norm
 
 pytestmark = pytest.mark.gpu
@@ -257,13 +257,36 @@ def test_refusals(gpu_device):
                        ((torch.zeros(2, 4097, device=gpu_device),), "width")):
         with pytest.raises(ValueError, match=what):
             layer_norm(*args)
-    with pytest.raises(RuntimeError, match="layer_norm_bwd"):
-        stats = torch.zeros(4, 2, device=gpu_device)
-        from bioemu2_amd._lib import check, lib
+    stats = torch.zeros(4, 2, device=gpu_device)
+    with pytest.raises(RuntimeError, match="workspace"):
+        _lib.check(_lib.lib().bioemu_layer_norm_bwd(x.data_ptr(), x.data_ptr(), stats.data_ptr(), None, None,
+                                                    w.data_ptr(), None, None, 0, 4, 64, 64, 64, 1, 0, None), "bwd")
 
-        check(lib().bioemu_layer_norm_bwd(x.data_ptr(), x.data_ptr(), stats.data_ptr(), None, None, w.data_ptr(), None,
-                                          None, 0, 4, 64, 64, 64, 1, 0, None), "layer_norm_bwd")
-    y = layer_norm(x.requires_grad_(True), w)
+
+def test_gradients_are_first_order(gpu_device):
+    x = torch.randn(4, 64, device=gpu_device, requires_grad=True)
+    y = layer_norm(x, torch.ones(64, device=gpu_device))
     (g,) = torch.autograd.grad(y, x, torch.ones_like(y), create_graph=True)
-    assert not g.requires_grad or pytest.raises(RuntimeError, torch.autograd.grad, g.sum(), x)
-    assert _seq_ops.layer_norm_bwd_workspace_bytes(4, 64) == 4 * 2 * 64 * 4
+    with pytest.raises(RuntimeError, match="not implemented"):
+        torch.autograd.grad(g.sum(), x)
+
+
+def test_a_leaf_that_wants_its_gradient_accumulated(gpu_device):
+    """backward() twice: gradients add up, the op's outputs are not overwritten."""
+    x = torch.randn(30, 64, device=gpu_device, requires_grad=True)
+    w = torch.ones(64, device=gpu_device, requires_grad=True)
+    layer_norm(x, w).square().sum().backward()
+    once = x.grad.clone(), w.grad.clone()
+    layer_norm(x, w).square().sum().backward()
+    assert torch.equal(x.grad, 2 * once[0]) and torch.equal(w.grad, 2 * once[1])
+
+
+def test_fake_tensors_and_schema(gpu_device):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        x = torch.empty(3, 5, 64, device="cuda", dtype=BF16, requires_grad=True)
+        w = torch.empty(64, device="cuda", requires_grad=True)
+        y = layer_norm(x, w)
+        dx, dw = torch.autograd.grad(y, (x, w), torch.empty_like(y))
+        assert y.shape == x.shape and dx.dtype == BF16 and dw.shape == (64,) and dw.dtype == F32

@@ -14,7 +14,7 @@ import math
 import pytest
 import torch
 
-from bioemu2_amd import _seq_ops
+from bioemu2_amd import _lib
 from bioemu2_amd.relative_position import RelativePosition, distance_buckets, relative_position
 
 pytestmark = pytest.mark.gpu
@@ -58,7 +58,7 @@ def _check(table, buckets, pos, ch, z, dy, y, dt):
     want = torch.zeros(NB, C, dtype=torch.float64, device=dy.device).index_add_(0, idx, flat)
     size = torch.zeros_like(want).index_add_(0, idx, flat.abs())
     units = B * N * math.ceil(N / 64)
-    groups = _seq_ops.relpos_bwd_workspace_bytes(B, N, C, NB) // (NB * C * 4)
+    groups = _lib.lib().bioemu_relpos_bwd_workspace_bytes(B, N, C, NB) // (NB * C * 4)
     depth = (3 if dy.dtype == F32 else 1) * 64 * math.ceil(units / (8 * groups)) + 8 + groups / 64 + 8
     assert bool(((dt.double() - want).abs() <= depth * U * size + _half(dt.dtype) * want.abs()).all())
 
