@@ -160,11 +160,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_c_void_p] * 6 + [_c_size_t] + [_c_int64] * 5 + [_c_int, _c_int, _c_void_p],
     ),
     "bioemu_attention_workspace_bytes": (_c_size_t, [_attn_p]),
-    "bioemu_attention_fwd": (_c_int, [_attn_p] + [_c_void_p] * 3 + [_c_size_t, _c_void_p]),
+    "bioemu_attention_fwd": (_c_int, [_attn_p] + [_c_void_p] * 4 + [_c_size_t, _c_void_p]),
     "bioemu_attention_bwd_workspace_bytes": (_c_size_t, [_attn_p, _c_int]),
     "bioemu_attention_bwd": (
         _c_int,
-        [_attn_p] + [_c_void_p] * 3 + [ctypes.POINTER(_c_int64 * 3)] + [_c_void_p] * 5 + [_c_size_t, _c_void_p],
+        [_attn_p] + [_c_void_p] * 4 + [ctypes.POINTER(_c_int64 * 3)] + [_c_void_p] * 5 + [_c_size_t, _c_void_p],
     ),
 }
 

@@ -55,6 +55,7 @@ __device__ __forceinline__ void store_rows(const f32x16 (&acc)[DB], float scale,
 
 template <class T, int DP>
 __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs a, const T* __restrict__ o,
+                                                                  const T* __restrict__ o_lo,
                                                                   const float* __restrict__ lse,
                                                                   const T* __restrict__ dout, int64_t db, int64_t dn,
                                                                   int64_t dh, T* __restrict__ dq,
@@ -125,6 +126,11 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
       const Frag<T> of = row_operand<T>(o + row * a.D, on, s, lh, a.D);
 #pragma unroll
       for (int t = 0; t < 8; ++t) dsum += (float)of[t] * (float)df[s][t];
+      if (o_lo) {
+        const Frag<T> ol = row_operand<T>(o_lo + row * a.D, on, s, lh, a.D);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) dsum += (float)ol[t] * (float)df[s][t];
+      }
     }
   }
   dsum += __shfl_xor(dsum, 32);
@@ -571,7 +577,7 @@ BwdSpace bwd_space(const AttnArgs& a, bool f32, bool table) {
 }
 
 template <class T, int DP>
-int launch_bwd(const AttnArgs& a, const void* o, const float* lse, const void* dout, const int64_t* ds, void* dq,
+int launch_bwd(const AttnArgs& a, const void* o, const void* o_lo, const float* lse, const void* dout, const int64_t* ds, void* dq,
                void* dk, void* dv, void* dtable, void* ws, hipStream_t stream) {
   const BwdSpace sp = bwd_space(a, sizeof(T) == 4, dtable != nullptr);
   char* at = static_cast<char*>(ws);
@@ -584,8 +590,8 @@ int launch_bwd(const AttnArgs& a, const void* o, const float* lse, const void* d
     const int64_t total = (int64_t)a.B * a.H * qblocks * sp.q_splits;
     KernelTimerScope timer("attn_bwd_q", stream);
     attn_bwd_q_kernel<T, DP><<<dim3(attn_grid(total)), kAttnThreads, bias_lds(a, dtable != nullptr), stream>>>(
-        a, static_cast<const T*>(o), lse, static_cast<const T*>(dout), ds[0], ds[1], ds[2], static_cast<T*>(dq), delta,
-        q_part, bias, sp.q_splits, qblocks, (int)total);
+        a, static_cast<const T*>(o), static_cast<const T*>(o_lo), lse, static_cast<const T*>(dout), ds[0], ds[1], ds[2],
+        static_cast<T*>(dq), delta, q_part, bias, sp.q_splits, qblocks, (int)total);
     if (const int rc = check_launch("attn_bwd_q")) return rc;
   }
   if (kblocks > 0) {
@@ -626,8 +632,8 @@ extern "C" size_t bioemu_attention_bwd_workspace_bytes(const bioemu_attention_ar
   return bwd_space(a, args->f32 != 0, table_gradient && a.table).total;
 }
 
-extern "C" int bioemu_attention_bwd(const bioemu_attention_args* args, const void* o, const float* lse,
-                                    const void* dout, const int64_t* dout_stride, void* dq, void* dk, void* dv,
+extern "C" int bioemu_attention_bwd(const bioemu_attention_args* args, const void* o, const void* o_lo,
+                                    const float* lse, const void* dout, const int64_t* dout_stride, void* dq, void* dk, void* dv,
                                     void* dtable, void* workspace, size_t workspace_bytes, hipStream_t stream) {
   AttnArgs a;
   if (const int rc = attn_args("attention_bwd", args, &a)) return rc;
@@ -635,18 +641,19 @@ extern "C" int bioemu_attention_bwd(const bioemu_attention_args* args, const voi
   if (!o || !lse || !dout || !dout_stride || !dq || (a.Nk > 0 && (!dk || !dv)))
     return set_error(BIOEMU_ERR_INVALID_ARG, "attention_bwd: null pointer");
   const int64_t per = args->f32 ? 4 : 8;
-  if (!aligned16(o) || !aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) ||
+  if (!aligned16(o) || !aligned16(o_lo) || !aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) ||
       dout_stride[0] % per || dout_stride[1] % per || dout_stride[2] % per || dout_stride[1] > (int64_t(1) << 23) ||
       (a.Nq > 1 && dout_stride[1] < a.D))
     return set_error(BIOEMU_ERR_INVALID_ARG,
                      "attention_bwd: rows start at 16-byte addresses, at least a head's width apart");
+  if (o_lo && args->f32) return set_error(BIOEMU_ERR_INVALID_ARG, "attention_bwd: o_lo is of bf16 calls");
   if (dtable && !a.table) return set_error(BIOEMU_ERR_INVALID_ARG, "attention_bwd: dtable without a table");
   const size_t need = bwd_space(a, args->f32 != 0, dtable != nullptr).total;
   if (!workspace || !aligned16(workspace) || workspace_bytes < need)
     return set_error(BIOEMU_ERR_WORKSPACE, "attention_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   const int dp = a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128;
 #define BIOEMU_BWD(T, P)                                                                                            \
-  if (dp == P) return launch_bwd<T, P>(a, o, lse, dout, dout_stride, dq, dk, dv, dtable, workspace, stream)
+  if (dp == P) return launch_bwd<T, P>(a, o, o_lo, lse, dout, dout_stride, dq, dk, dv, dtable, workspace, stream)
   if (args->f32) {
     BIOEMU_BWD(float, 32);
     BIOEMU_BWD(float, 64);

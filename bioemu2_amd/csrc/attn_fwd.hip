@@ -8,6 +8,10 @@
 // attn_few: up to 32 (query, head of a group) rows share their keys, as single tokens over a cache do: the rows fill
 // one MFMA operand, every wave takes 32-key tiles of its own (K and V read once, bound by HBM), and the waves join.
 // Both may split the keys over workgroups (few rows, long axis); attn_join adds the parts.
+//
+// A training call in bf16 also writes what the rounding of o took off (o_lo): the backward pass needs do . o, and with
+// it from o + o_lo the error of dq and dk falls from 1.50 to 1.46 times what rounding their results alone gives (the
+// rest is the rounding of the probabilities and of ds to the operands of the products).
 #include "attn.h"
 
 namespace bioemu {
@@ -22,11 +26,26 @@ struct Parts {
   float *o, *ml;
 };
 
+// Four values of a row, rounded, and what that took off.
+template <class T>
+__device__ __forceinline__ void store_quad(T* out, T* lo, const float (&v)[4]) {
+  typedef T quad __attribute__((ext_vector_type(4)));
+  quad hi, rest;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    hi[c] = (T)v[c];
+    rest[c] = (T)(v[c] - (float)hi[c]);
+  }
+  *reinterpret_cast<quad*>(out) = hi;
+  if (lo) *reinterpret_cast<quad*>(lo) = rest;
+}
+
 __device__ __forceinline__ float row_log_sum(float m, float l) { return l > 0.f ? m + __log2f(l) : kInf; }
 
 template <class T, int DP>
 __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a, T* __restrict__ out,
-                                                                float* __restrict__ lse, Parts parts, int splits,
+                                                                T* __restrict__ lo, float* __restrict__ lse,
+                                                                Parts parts, int splits,
                                                                 int qblocks, int total) {
   constexpr int KB = Operand<T>::kBlock, SUB = KB / 32, STEPS = DP / 16, DB = DP / 32;
   typedef Tile<T, DP, KB> KV;
@@ -197,18 +216,15 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
   const int64_t row = ((int64_t)b * a.Nq + i) * a.H + h;
   if (splits == 1) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* po = out + row * a.D;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int at = 32 * d + 8 * r + 4 * lh;
-        if (at < a.D) {
-          typedef T quad __attribute__((ext_vector_type(4)));
-          quad v;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) v[c] = (T)(acc[d][4 * r + c] * inv);
-          *reinterpret_cast<quad*>(po + at) = v;
+        const int64_t at = row * a.D + 32 * d + 8 * r + 4 * lh;
+        if (32 * d + 8 * r + 4 * lh < a.D) {
+          const float v[4] = {acc[d][4 * r] * inv, acc[d][4 * r + 1] * inv, acc[d][4 * r + 2] * inv,
+                              acc[d][4 * r + 3] * inv};
+          store_quad(out + at, lo ? lo + at : nullptr, v);
         }
       }
     if (lse && lh == 0) lse[((int64_t)b * a.H + h) * a.Nq + i] = row_log_sum(mref, l);
@@ -230,26 +246,28 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
   }
 }
 
-// Waves of attn_few: each has two K and two V tiles of its own.
-template <class T>
+// Waves of attn_few: each has two K and two V tiles of its own, 128 KB of LDS in all at most.
+template <class T, int DP>
 constexpr int few_waves() {
-  return sizeof(T) == 2 ? 4 : 2;
+  constexpr int w = 131072 / (4 * Tile<T, DP, 32>::BYTES);
+  return w < 8 ? w : 8;
 }
 
+// chunk: 32-key tiles of one split.  Splits are of equal length whatever the sequences' lengths (those past a
+// sequence's end do nothing), and workgroups take them in plain order, round the XCDs: no two share a key.
 template <class T, int DP>
-__global__ __launch_bounds__(64 * few_waves<T>()) void attn_few_kernel(const AttnArgs a, T* __restrict__ out,
-                                                                       float* __restrict__ lse, Parts parts,
-                                                                       int splits, int total) {
-  constexpr int W = few_waves<T>(), STEPS = DP / 16, DB = DP / 32;
+__global__ __launch_bounds__((64 * few_waves<T, DP>())) void attn_few_kernel(const AttnArgs a, T* __restrict__ out,
+                                                                           T* __restrict__ lo,
+                                                                           float* __restrict__ lse, Parts parts,
+                                                                           int splits, int chunk) {
+  constexpr int W = few_waves<T, DP>(), STEPS = DP / 16, DB = DP / 32;
   typedef Tile<T, DP, 32> KV;
   constexpr int CP = KV::copies(64);
   __shared__ __attribute__((aligned(1024))) char tiles[W][2][2][KV::BYTES];
   __shared__ float ml[W][2][32];
 
-  const int item = attn_item(total, splits);
-  if (item < 0) return;
   const int lane = threadIdx.x & 63, wave = wave_id(), ln = lane & 31, lh = lane >> 5;
-  const int split = item % splits, bh = item / splits, hk = bh % a.Hk, b = bh / a.Hk;
+  const int bh = blockIdx.x / splits, split = blockIdx.x - bh * splits, b = bh / a.Hk, hk = bh - b * a.Hk;
   const int rows = a.Nq * a.G;
   const int length = a.lengths ? min(max(a.lengths[b], 0), a.Nk) : a.Nk;
   const int prefix = a.prefix ? a.prefix[b] : 0;
@@ -271,6 +289,19 @@ __global__ __launch_bounds__(64 * few_waves<T>()) void attn_few_kernel(const Att
   top = __builtin_amdgcn_readfirstlane(top);
   low = __builtin_amdgcn_readfirstlane(low);
 
+  const T* kbase = static_cast<const T*>(a.k) + b * a.kb + hk * a.kh;
+  const T* vbase = static_cast<const T*>(a.v) + b * a.vb + hk * a.vh;
+  unsigned koff[CP], voff[CP];
+  KV::offsets(lane, 64, a.kn, a.D, koff);
+  KV::offsets(lane, 64, a.vn, a.D, voff);
+  auto stage = [&](int t, int buf) {
+    const int k0 = t * 32;
+    KV::copy(kbase + (int64_t)k0 * a.kn, length - k0, a.kn, a.D, tiles[wave][buf][0], 0, 64, koff);
+    KV::copy(vbase + (int64_t)k0 * a.vn, length - k0, a.vn, a.D, tiles[wave][buf][1], 0, 64, voff);
+  };
+  const int blocks = (top + 31) / 32, t0 = min(split * chunk, blocks), t1 = min(t0 + chunk, blocks);
+  if (t0 + wave < t1) stage(t0 + wave, 0);   // before the queries and the bias: it takes longest
+
   Frag<T> qf[STEPS];
   {
     const T* row = static_cast<const T*>(a.q) + b * a.qb + (int64_t)i * a.qn + h * a.qh;
@@ -278,11 +309,6 @@ __global__ __launch_bounds__(64 * few_waves<T>()) void attn_few_kernel(const Att
     for (int s = 0; s < STEPS; ++s) qf[s] = row_operand<T>(row, live, s, lh, a.D);
   }
   const float far_lo = a.table ? table_value(a, 0, h) : 0.f, far_hi = a.table ? table_value(a, 2 * a.radius, h) : 0.f;
-  const T* kbase = static_cast<const T*>(a.k) + b * a.kb + hk * a.kh;
-  const T* vbase = static_cast<const T*>(a.v) + b * a.vb + hk * a.vh;
-  unsigned koff[CP], voff[CP];
-  KV::offsets(lane, 64, a.kn, a.D, koff);
-  KV::offsets(lane, 64, a.vn, a.D, voff);
   const int* kseg = seg ? a.k_seg + (int64_t)b * a.Nk : nullptr;
 
   f32x16 acc[DB];
@@ -292,15 +318,7 @@ __global__ __launch_bounds__(64 * few_waves<T>()) void attn_few_kernel(const Att
   const float s_scale = a.cap > 0.f ? a.scale / a.cap : a.scale * kLog2e;
   const float s_cap = a.cap * kLog2e;
 
-  const int blocks = (top + 31) / 32;
-  const int t0 = (int)((int64_t)blocks * split / splits), t1 = (int)((int64_t)blocks * (split + 1) / splits);
-  auto stage = [&](int t, int buf) {
-    const int k0 = t * 32;
-    KV::copy(kbase + (int64_t)k0 * a.kn, length - k0, a.kn, a.D, tiles[wave][buf][0], 0, 64, koff);
-    KV::copy(vbase + (int64_t)k0 * a.vn, length - k0, a.vn, a.D, tiles[wave][buf][1], 0, 64, voff);
-  };
   int buf = 0;
-  if (t0 + wave < t1) stage(t0 + wave, 0);
   for (int t = t0 + wave; t < t1; t += W, buf ^= 1) {
     const int k0 = t * 32;
     if (t + W < t1) {
@@ -411,7 +429,10 @@ __global__ __launch_bounds__(64 * few_waves<T>()) void attn_few_kernel(const Att
     const int qi = r / a.G, qh = hk * a.G + r - qi * a.G;
     const int64_t row = ((int64_t)b * a.Nq + qi) * a.H + qh;
     if (splits == 1) {
-      out[row * a.D + d] = (T)(sum == 0.f ? 0.f : o / sum);
+      const float v = sum == 0.f ? 0.f : o / sum;
+      const T hi = (T)v;
+      out[row * a.D + d] = hi;
+      if (lo) lo[row * a.D + d] = (T)(v - (float)hi);
       if (lse && d == 0) lse[((int64_t)b * a.H + qh) * a.Nq + qi] = row_log_sum(to, sum);
     } else {
       parts.o[(split * all + row) * a.D + d] = o;
@@ -423,10 +444,12 @@ __global__ __launch_bounds__(64 * few_waves<T>()) void attn_few_kernel(const Att
   }
 }
 
-// One wave a row: the splits' parts added in order.
+// One wave a row: the splits' parts added in order (a split that saw nothing wrote no values).  Lane s holds the weight
+// of split s, lane d value d and 64 + d.
 template <class T>
 __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const AttnArgs a, Parts parts, int splits,
-                                                                 T* __restrict__ out, float* __restrict__ lse) {
+                                                                 T* __restrict__ out, T* __restrict__ lo,
+                                                                 float* __restrict__ lse) {
   const int64_t rows = (int64_t)a.B * a.Nq * a.H, row = (int64_t)blockIdx.x * 4 + wave_id();
   if (row >= rows) return;
   const int lane = threadIdx.x & 63;
@@ -436,18 +459,36 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const AttnArgs 
   for (int m = 32; m > 0; m /= 2) top = fmaxf(top, __shfl_xor(top, m));
   const float to = top == -kInf ? 0.f : top;
   float o0 = 0.f, o1 = 0.f, sum = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < splits; ++s) {
-    const float* ml = parts.ml + 2 * (s * rows + row);
-    const float* po = parts.o + (s * rows + row) * a.D;
-    const float f = fast_exp2(ml[0] - to);
-    sum += f * ml[1];
-    if (lane < a.D) o0 += f * po[lane];
-    if (lane + 64 < a.D) o1 += f * po[lane + 64];
+  const int d0 = min(lane, a.D - 1), d1 = min(lane + 64, a.D - 1);
+  for (int s0 = 0; s0 < splits; s0 += 64) {
+    const bool on = s0 + lane < splits;
+    const float* ml = parts.ml + 2 * ((s0 + (on ? lane : 0)) * rows + row);
+    const float f = on ? fast_exp2(ml[0] - to) : 0.f;
+    float l = on ? f * ml[1] : 0.f;
+#pragma unroll
+    for (int m = 32; m > 0; m /= 2) l += __shfl_xor(l, m);
+    sum += l;
+    const uint64_t seen = __ballot(f != 0.f);
+    const int n = min(64, splits - s0);
+#pragma unroll 8
+    for (int s = 0; s < n; ++s) {
+      const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s));
+      const bool there = (seen >> s) & 1;
+      const float* po = parts.o + ((there ? s0 + s : 0) * rows + row) * a.D;
+      const float x0 = po[d0], x1 = po[d1];
+      o0 += there ? w * x0 : 0.f;
+      o1 += there ? w * x1 : 0.f;
+    }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  if (lane < a.D) out[row * a.D + lane] = (T)(o0 * inv);
-  if (lane + 64 < a.D) out[row * a.D + lane + 64] = (T)(o1 * inv);
+  for (int h = 0; h < 2; ++h) {
+    const int d = lane + 64 * h;
+    if (d >= a.D) continue;
+    const float v = (h ? o1 : o0) * inv;
+    const T hi = (T)v;
+    out[row * a.D + d] = hi;
+    if (lo) lo[row * a.D + d] = (T)(v - (float)hi);
+  }
   if (lse && lane == 0) {
     const int64_t bi = row / a.H, h = row - bi * a.H, b = bi / a.Nq, i = bi - b * a.Nq;
     lse[(b * a.H + h) * a.Nq + i] = row_log_sum(to, sum);
@@ -456,13 +497,14 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const AttnArgs 
 
 bool few_rows(const AttnArgs& a) { return a.Nq * a.G <= 32; }
 
-// Workgroups that the keys of a query block are split over: as many as bring the launch to two workgroups a CU, each
-// with at least `least` keys.
-int key_splits(const AttnArgs& a, bool f32) {
+// Workgroups that the keys of a query block are split over: as many as bring the launch to two workgroups a CU (four
+// where rows are few: sequences of a cache are of unequal length), each with at least `least` keys: below it the join
+// costs more than the shorter walk gains (773 keys of 16 heads: 18 us in four parts, 13 in one).
+int key_splits(const AttnArgs& a) {
   const bool few = few_rows(a);
   const int64_t base = few ? (int64_t)a.B * a.Hk : (int64_t)a.B * a.H * ((a.Nq + kGroupRows - 1) / kGroupRows);
-  const int64_t least = few ? (f32 ? 128 : 256) : 512;
-  const int64_t want = (2 * (int64_t)compute_units() + base - 1) / base;
+  const int64_t least = few ? 1024 : 512;
+  const int64_t want = ((few ? 4 : 2) * (int64_t)compute_units() + base - 1) / base;
   const int64_t most = (a.Nk + least - 1) / least;
   const int64_t s = want < most ? want : most;
   return s < 1 ? 1 : (int)s;
@@ -472,41 +514,30 @@ size_t parts_bytes(const AttnArgs& a, int splits) {
   return splits == 1 ? 0 : (size_t)splits * a.B * a.Nq * a.H * (a.D + 2) * sizeof(float);
 }
 
-template <class T>
-int launch_fwd(const AttnArgs& a, void* o, float* lse, void* ws, hipStream_t stream) {
-  const int splits = key_splits(a, sizeof(T) == 4);
+template <class T, int DP>
+int launch_fwd(const AttnArgs& a, void* o, void* o_lo, float* lse, void* ws, hipStream_t stream) {
+  const int splits = key_splits(a);
   const int64_t rows = (int64_t)a.B * a.Nq * a.H;
   Parts parts{static_cast<float*>(ws), nullptr};
   parts.ml = parts.o ? parts.o + (int64_t)splits * rows * a.D : nullptr;
-  T* out = static_cast<T*>(o);
-  const int dp = a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128;
+  T *out = static_cast<T*>(o), *lo = static_cast<T*>(o_lo);
   if (few_rows(a)) {
-    const int64_t total = (int64_t)a.B * a.Hk * splits;
+    const int tiles = (a.Nk + 31) / 32, chunk = (tiles + splits - 1) / splits;
     KernelTimerScope timer("attn_few", stream);
-    const dim3 grid(attn_grid(total)), wg(64 * few_waves<T>());
-    if (dp == 32)
-      attn_few_kernel<T, 32><<<grid, wg, 0, stream>>>(a, out, lse, parts, splits, (int)total);
-    else if (dp == 64)
-      attn_few_kernel<T, 64><<<grid, wg, 0, stream>>>(a, out, lse, parts, splits, (int)total);
-    else
-      attn_few_kernel<T, 128><<<grid, wg, 0, stream>>>(a, out, lse, parts, splits, (int)total);
+    attn_few_kernel<T, DP><<<dim3((unsigned)(a.B * a.Hk * splits)), 64 * few_waves<T, DP>(), 0, stream>>>(
+        a, out, lo, lse, parts, splits, chunk);
     if (const int rc = check_launch("attn_few")) return rc;
   } else {
     const int qblocks = (a.Nq + kGroupRows - 1) / kGroupRows;
     const int64_t total = (int64_t)a.B * a.H * splits * qblocks;
     KernelTimerScope timer("attn_fwd", stream);
-    const dim3 grid(attn_grid(total));
-    if (dp == 32)
-      attn_fwd_kernel<T, 32><<<grid, kAttnThreads, 0, stream>>>(a, out, lse, parts, splits, qblocks, (int)total);
-    else if (dp == 64)
-      attn_fwd_kernel<T, 64><<<grid, kAttnThreads, 0, stream>>>(a, out, lse, parts, splits, qblocks, (int)total);
-    else
-      attn_fwd_kernel<T, 128><<<grid, kAttnThreads, 0, stream>>>(a, out, lse, parts, splits, qblocks, (int)total);
+    attn_fwd_kernel<T, DP><<<dim3(attn_grid(total)), kAttnThreads, 0, stream>>>(a, out, lo, lse, parts, splits, qblocks,
+                                                                               (int)total);
     if (const int rc = check_launch("attn_fwd")) return rc;
   }
   if (splits == 1) return BIOEMU_OK;
   KernelTimerScope timer("attn_join", stream);
-  attn_join_kernel<T><<<dim3((unsigned)((rows + 3) / 4)), kAttnThreads, 0, stream>>>(a, parts, splits, out, lse);
+  attn_join_kernel<T><<<dim3((unsigned)((rows + 3) / 4)), kAttnThreads, 0, stream>>>(a, parts, splits, out, lo, lse);
   return check_launch("attn_join");
 }
 
@@ -562,17 +593,32 @@ using namespace bioemu;
 extern "C" size_t bioemu_attention_workspace_bytes(const bioemu_attention_args* args) {
   AttnArgs a;
   if (attn_args("attention", args, &a) || a.B == 0 || a.Nq == 0) return 0;
-  return parts_bytes(a, key_splits(a, args->f32 != 0));
+  return parts_bytes(a, key_splits(a));
 }
 
-extern "C" int bioemu_attention_fwd(const bioemu_attention_args* args, void* o, float* lse, void* workspace,
-                                    size_t workspace_bytes, hipStream_t stream) {
+extern "C" int bioemu_attention_fwd(const bioemu_attention_args* args, void* o, void* o_lo, float* lse,
+                                    void* workspace, size_t workspace_bytes, hipStream_t stream) {
   AttnArgs a;
   if (const int rc = attn_args("attention", args, &a)) return rc;
   if (a.B == 0 || a.Nq == 0) return BIOEMU_OK;
-  if (!o || !aligned16(o)) return set_error(BIOEMU_ERR_INVALID_ARG, "attention: o must be 16-byte aligned");
-  const size_t need = parts_bytes(a, key_splits(a, args->f32 != 0));
+  if (!o || !aligned16(o) || !aligned16(o_lo))
+    return set_error(BIOEMU_ERR_INVALID_ARG, "attention: o and o_lo must be 16-byte aligned");
+  if (o_lo && args->f32) return set_error(BIOEMU_ERR_INVALID_ARG, "attention: o_lo is of bf16 calls");
+  const size_t need = parts_bytes(a, key_splits(a));
   if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need))
     return set_error(BIOEMU_ERR_WORKSPACE, "attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-  return args->f32 ? launch_fwd<float>(a, o, lse, workspace, stream) : launch_fwd<bf16>(a, o, lse, workspace, stream);
+  const int dp = a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128;
+#define BIOEMU_FWD(T, P) \
+  if (dp == P) return launch_fwd<T, P>(a, o, o_lo, lse, workspace, stream)
+  if (args->f32) {
+    BIOEMU_FWD(float, 32);
+    BIOEMU_FWD(float, 64);
+    BIOEMU_FWD(float, 128);
+  } else {
+    BIOEMU_FWD(bf16, 32);
+    BIOEMU_FWD(bf16, 64);
+    BIOEMU_FWD(bf16, 128);
+  }
+#undef BIOEMU_FWD
+  return BIOEMU_ERR_UNSUPPORTED;
 }

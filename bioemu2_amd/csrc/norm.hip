@@ -86,13 +86,17 @@ __device__ __forceinline__ void load_weight(const void* w, int is_bf16, int c, i
   }
 }
 
+// Rows a lane group works on at a time: two where they are short, so that twice the loads are in flight.
+template <int LPR, int E>
+constexpr int kRowsAtOnce = LPR <= 64 && E <= 8 ? 2 : 1;
+
 // stats: NULL or [rows][2] (mean, 1 / deviation), what the backward pass reads.
 template <class T, int VEC, int LPR, int VPL>
 __global__ __launch_bounds__(kThreads) void norm_fwd_kernel(const T* __restrict__ x, int64_t ldx,
                                                             const void* __restrict__ w, const void* __restrict__ b,
                                                             int w_bf16, T* __restrict__ y, float* __restrict__ stats,
                                                             int64_t rows, int c, float eps) {
-  constexpr int E = VEC * VPL, RPG = kThreads / LPR;
+  constexpr int E = VEC * VPL, RPG = kThreads / LPR, U = kRowsAtOnce<LPR, E>;
   __shared__ float sh[2][4];
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
   float wv[E], bv[E];
@@ -100,51 +104,55 @@ __global__ __launch_bounds__(kThreads) void norm_fwd_kernel(const T* __restrict_
   load_weight<VEC, LPR, VPL>(b, w_bf16, c, lane, 0.f, bv);
   const float inv_c = 1.f / (float)c;
   // every lane of a workgroup makes the same number of turns (barriers where a row spans waves)
-  for (int64_t row0 = (int64_t)blockIdx.x * RPG; row0 < rows; row0 += (int64_t)gridDim.x * RPG) {
-    const int64_t row = row0 + group;
-    const bool live = row < rows;
-    const T* px = x + (live ? row : 0) * ldx;
-    float v[E], s = 0.f;
+  for (int64_t row0 = (int64_t)blockIdx.x * RPG * U; row0 < rows; row0 += (int64_t)gridDim.x * RPG * U) {
+    float v[U][E];
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int at = (i * LPR + lane) * VEC;
-      if (live && at < c) {
-        load_vec<T, VEC>(px + at, v + i * VEC);
-      } else {
-#pragma unroll
-        for (int t = 0; t < VEC; ++t) v[i * VEC + t] = 0.f;
-      }
-#pragma unroll
-      for (int t = 0; t < VEC; ++t) s += v[i * VEC + t];
-    }
-    const float mean = row_sum<LPR>(s, sh[0]) * inv_c;
-    float q = 0.f;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i)
-      if ((i * LPR + lane) * VEC < c)
-#pragma unroll
-        for (int t = 0; t < VEC; ++t) {
-          const float d = v[i * VEC + t] - mean;
-          v[i * VEC + t] = d;
-          q += d * d;
-        }
-    const float var = row_sum<LPR>(q, sh[1]) * inv_c;
-    const float r = 1.f / sqrtf(var + eps);
-    if (live) {
-      T* py = y + row * c;
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = row0 + u * RPG + group;
+      const T* px = x + (row < rows ? row : 0) * ldx;
 #pragma unroll
       for (int i = 0; i < VPL; ++i) {
         const int at = (i * LPR + lane) * VEC;
         if (at < c) {
-          float o[VEC];
+          load_vec<T, VEC>(px + at, v[u] + i * VEC);
+        } else {
 #pragma unroll
-          for (int t = 0; t < VEC; ++t) o[t] = v[i * VEC + t] * r * wv[i * VEC + t] + bv[i * VEC + t];
-          store_vec<T, VEC>(py + at, o);
+          for (int t = 0; t < VEC; ++t) v[u][i * VEC + t] = 0.f;
         }
       }
-      if (stats != nullptr && lane == 0) {
-        stats[2 * row] = mean;
-        stats[2 * row + 1] = r;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = row0 + u * RPG + group;
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) s += v[u][e];
+      const float mean = row_sum<LPR>(s, sh[0]) * inv_c;
+      float q = 0.f;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if ((i * LPR + lane) * VEC < c)
+#pragma unroll
+          for (int t = 0; t < VEC; ++t) {
+            const float d = v[u][i * VEC + t] - mean;
+            v[u][i * VEC + t] = d;
+            q += d * d;
+          }
+      const float var = row_sum<LPR>(q, sh[1]) * inv_c;
+      const float r = 1.f / sqrtf(var + eps);
+      if (row < rows) {
+        T* py = y + row * c;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+          const int at = (i * LPR + lane) * VEC;
+          if (at < c) {
+            float o[VEC];
+#pragma unroll
+            for (int t = 0; t < VEC; ++t) o[t] = v[u][i * VEC + t] * r * wv[i * VEC + t] + bv[i * VEC + t];
+            store_vec<T, VEC>(py + at, o);
+          }
+        }
+        if (stats != nullptr && lane == 0) *reinterpret_cast<f32x2*>(stats + 2 * row) = f32x2{mean, r};
       }
     }
     if constexpr (LPR > 64) __syncthreads();   // sh is read before the next row writes it
@@ -159,7 +167,7 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_kernel(const T* __restrict_
                                                             const void* __restrict__ w, int w_bf16,
                                                             T* __restrict__ dx, float* __restrict__ part,
                                                             int64_t rows, int c) {
-  constexpr int E = VEC * VPL, RPG = kThreads / LPR;
+  constexpr int E = VEC * VPL, RPG = kThreads / LPR, U = kRowsAtOnce<LPR, E>;
   __shared__ float sh[2][4];
   __shared__ float acc[LPR < kThreads ? kThreads * E : 1];
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
@@ -168,43 +176,55 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_kernel(const T* __restrict_
 #pragma unroll
   for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.f;
   const float inv_c = 1.f / (float)c;
-  for (int64_t row0 = (int64_t)blockIdx.x * RPG; row0 < rows; row0 += (int64_t)gridDim.x * RPG) {
-    const int64_t row = row0 + group;
-    const bool live = row < rows;
-    const int64_t r0 = live ? row : 0;
-    const T *px = x + r0 * ldx, *pd = dy + r0 * ldy;
-    const float mean = stats[2 * r0], r = stats[2 * r0 + 1];
-    float xh[E], g[E], sg = 0.f, sgx = 0.f;
+  for (int64_t row0 = (int64_t)blockIdx.x * RPG * U; row0 < rows; row0 += (int64_t)gridDim.x * RPG * U) {
+    float xh[U][E], g[U][E];
+    f32x2 st[U];
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int at = (i * LPR + lane) * VEC;
-      if (live && at < c) {
-        load_vec<T, VEC>(px + at, xh + i * VEC);
-        load_vec<T, VEC>(pd + at, g + i * VEC);
-#pragma unroll
-        for (int t = 0; t < VEC; ++t) {
-          const int e = i * VEC + t;
-          xh[e] = (xh[e] - mean) * r;
-          dw[e] += g[e] * xh[e];
-          db[e] += g[e];
-          g[e] *= wv[e];
-          sg += g[e];
-          sgx += g[e] * xh[e];
-        }
-      }
-    }
-    const float mg = row_sum<LPR>(sg, sh[0]) * inv_c;
-    const float mgx = row_sum<LPR>(sgx, sh[1]) * inv_c;
-    if (live && dx != nullptr) {
-      T* po = dx + row * c;
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = row0 + u * RPG + group, r0 = row < rows ? row : 0;
+      const T *px = x + r0 * ldx, *pd = dy + r0 * ldy;
+      st[u] = *reinterpret_cast<const f32x2*>(stats + 2 * r0);
 #pragma unroll
       for (int i = 0; i < VPL; ++i) {
         const int at = (i * LPR + lane) * VEC;
         if (at < c) {
-          float o[VEC];
+          load_vec<T, VEC>(px + at, xh[u] + i * VEC);
+          load_vec<T, VEC>(pd + at, g[u] + i * VEC);
+        }
+      }
+    }
 #pragma unroll
-          for (int t = 0; t < VEC; ++t) o[t] = r * (g[i * VEC + t] - mg - xh[i * VEC + t] * mgx);
-          store_vec<T, VEC>(po + at, o);
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = row0 + u * RPG + group;
+      const bool live = row < rows;
+      const float mean = st[u][0], r = st[u][1];
+      float sg = 0.f, sgx = 0.f;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (live && (i * LPR + lane) * VEC < c)
+#pragma unroll
+          for (int t = 0; t < VEC; ++t) {
+            const int e = i * VEC + t;
+            xh[u][e] = (xh[u][e] - mean) * r;
+            dw[e] += g[u][e] * xh[u][e];
+            db[e] += g[u][e];
+            g[u][e] *= wv[e];
+            sg += g[u][e];
+            sgx += g[u][e] * xh[u][e];
+          }
+      const float mg = row_sum<LPR>(sg, sh[0]) * inv_c;
+      const float mgx = row_sum<LPR>(sgx, sh[1]) * inv_c;
+      if (live && dx != nullptr) {
+        T* po = dx + row * c;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+          const int at = (i * LPR + lane) * VEC;
+          if (at < c) {
+            float o[VEC];
+#pragma unroll
+            for (int t = 0; t < VEC; ++t) o[t] = r * (g[u][i * VEC + t] - mg - xh[u][i * VEC + t] * mgx);
+            store_vec<T, VEC>(po + at, o);
+          }
         }
       }
     }
@@ -285,9 +305,13 @@ int for_width(bool f32, bool vec, int64_t c, F&& f) {
 
 int64_t max_width(bool f32, bool vec) { return vec ? (f32 ? 256 * 16 * 4 : 256 * 8 * 8) : 256 * 16; }
 
-int row_groups(int64_t rows, int lpr, int64_t cap) {
-  const int64_t need = (rows + kThreads / lpr - 1) / (kThreads / lpr);
-  return (int)(need < cap ? need : cap);
+// Workgroups for `rows` rows: one turn each until there are `cap` of them, whole turns for all from then on.
+int row_groups(int64_t rows, int lpr, int elems, int64_t cap) {
+  const int at_once = (lpr <= 64 && elems <= 8 ? 2 : 1) * (kThreads / lpr);   // kRowsAtOnce
+  const int64_t turns = (rows + at_once - 1) / at_once;
+  if (turns <= cap) return (int)turns;
+  const int64_t each = (turns + cap - 1) / cap;
+  return (int)((turns + each - 1) / each);
 }
 
 template <class T>
@@ -297,7 +321,7 @@ int launch_fwd(const void* x, int64_t ldx, const void* w, const void* b, int w_b
   constexpr int VW = f32 ? 4 : 8;
   return for_width(f32, vec, c, [&](int vw, int lpr, int vpl) {
     // eight workgroups a CU: enough loads in flight, and the weights are read once per workgroup
-    const dim3 grid(row_groups(rows, lpr, (int64_t)compute_units() * 8));
+    const dim3 grid(row_groups(rows, lpr, vw * vpl, (int64_t)compute_units() * 8));
     KernelTimerScope timer("norm_fwd", stream);
 #define BIOEMU_CASE(V, L, P)                                                                                        \
   if (vw == V && lpr == L && vpl == P)                                                                              \
@@ -323,7 +347,7 @@ int launch_bwd(const void* x, int64_t ldx, const void* dy, int64_t ldy, const fl
   constexpr int VW = f32 ? 4 : 8;
   float* part = dw != nullptr || db != nullptr ? static_cast<float*>(ws) : nullptr;
   return for_width(f32, vec, c, [&](int vw, int lpr, int vpl) {
-    const dim3 grid(row_groups(rows, lpr, kMaxBwdGroups));
+    const dim3 grid(row_groups(rows, lpr, vw * vpl, kMaxBwdGroups));
     {
       KernelTimerScope timer("norm_bwd", stream);
 #define BIOEMU_CASE(V, L, P)                                                                                        \

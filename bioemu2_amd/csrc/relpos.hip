@@ -108,6 +108,12 @@ struct ChannelPair<float> {
   typedef f32x2 type;
 };
 
+// Pairs a backward wave holds (and as many on their way): half as many in fp32, which holds their three parts too.
+template <class T>
+constexpr int unit_pairs() {
+  return sizeof(T) == 2 ? 64 : 32;
+}
+
 // The 0/1 operand: element t is 1 where bucket t of bk is `col`.
 __device__ __forceinline__ bf16x8 onehot(u32x4 bk, int col) {
   const u16x2 target = {(unsigned short)col, (unsigned short)col}, one = {1, 1}, neg = {0xc080, 0xc080},
@@ -137,7 +143,7 @@ __global__ __launch_bounds__(kBwdThreads) void relpos_bwd_kernel(const T* __rest
                                                                  int nb, int units, int cols, int paired) {
   typedef typename ChannelPair<T>::type Two;
   constexpr int Waves = kBwdThreads / 64;
-  __shared__ float sum[NBB * 32][kBwdChannels + 1];
+  __shared__ float sum[4][NBB * 32][kBwdChannels + 1];
   __shared__ uint32_t bks[Waves][32];   // the 64 buckets of a wave's unit, two to a word
   const int lane = threadIdx.x & 63, wave = wave_id(), ln = lane & 31, lh = lane >> 5;
   const int c0 = blockIdx.y * kBwdChannels, nb0 = blockIdx.z * (kBwdBlocks * 32);
@@ -147,13 +153,20 @@ __global__ __launch_bounds__(kBwdThreads) void relpos_bwd_kernel(const T* __rest
 #pragma unroll
   for (int q = 0; q < NBB; ++q) acc[q][0] = acc[q][1] = zero16();
 
-  // a unit is 64 pairs of one row: unit u = row * cols + piece
-  for (int u = blockIdx.x * Waves + wave; u < units; u += gridDim.x * Waves) {
-    const int row = u / cols, j0 = (u - row * cols) * 64, b = row / n;
-    Two g[4][8];
+  // a unit is unit_pairs() pairs of one row: unit u = row * cols + piece.  The next one's values and bucket are on their way
+  // while one is multiplied.
+  constexpr int S = unit_pairs<T>() / 16;
+  const auto fetch = [&](int u, Two (&g)[S][8], int& bk) {
+    const int row = u / cols, j0 = (u - row * cols) * (16 * S), b = row / n;
     const T* base = dout + ((int64_t)row * n + j0) * c;
+    bk = 0xffff;
+    if (lane < 16 * S && j0 + lane < n) {
+      const int j = b * n + j0 + lane;
+      bk = pair_bucket(pos[row], pos[j], chains ? chains[row] : 0, chains ? chains[j] : 0, buckets, radius, nb) - nb0;
+      bk = bk < 0 || bk >= kBwdBlocks * 32 ? 0xffff : bk;
+    }
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+    for (int s = 0; s < S; ++s)
 #pragma unroll
       for (int t = 0; t < 8; ++t) {
         const int p = min(16 * s + 8 * lh + t, n - 1 - j0);   // past the row: its last pair, under no bucket
@@ -163,19 +176,26 @@ __global__ __launch_bounds__(kBwdThreads) void relpos_bwd_kernel(const T* __rest
         else
           g[s][t] = Two{src[ch0], src[ch1]};
       }
-    int bk = 0xffff;
-    if (j0 + lane < n) {
-      const int j = b * n + j0 + lane;
-      bk = pair_bucket(pos[row], pos[j], chains ? chains[row] : 0, chains ? chains[j] : 0, buckets, radius, nb) - nb0;
-      bk = bk < 0 || bk >= kBwdBlocks * 32 ? 0xffff : bk;
-    }
+  };
+  const int step = gridDim.x * Waves;
+  int u = blockIdx.x * Waves + wave, next_bk = 0xffff;
+  Two next[S][8];
+  if (u < units) fetch(u, next, next_bk);
+  for (; u < units; u += step) {
+    Two g[S][8];
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int t = 0; t < 8; ++t) g[s][t] = next[s][t];
+    const int bk = next_bk;
+    if (u + step < units) fetch(u + step, next, next_bk);
     reinterpret_cast<u16_alias*>(bks[wave])[lane] = (unsigned short)bk;
     uint64_t there[NBB];
 #pragma unroll
     for (int q = 0; q < NBB; ++q) there[q] = __ballot((bk >> 5) == q);
     wave_fence();   // this wave's own words, which LDS takes in order
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
+    for (int s = 0; s < S; ++s) {
       const u32x4 bv = *reinterpret_cast<const u32x4*>(&bks[wave][8 * s + 4 * lh]);
       bf16x8 a[3][2];
       if constexpr (sizeof(T) == 2) {
@@ -212,23 +232,25 @@ __global__ __launch_bounds__(kBwdThreads) void relpos_bwd_kernel(const T* __rest
   }
 
   // acc[q][e], lane (ln, lh), register 4 r + k: bucket 32 q + ln, channel 2 (8 r + 4 lh + k) + e
-  for (int w = 0; w < Waves; ++w) {
-    if (wave == w) {
+  // waves 0 .. 3 lay theirs down, 4 .. 7 add to them
+  for (int w = 0; w < 2; ++w) {
+    if (wave / 4 == w) {
 #pragma unroll
       for (int q = 0; q < NBB; ++q)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            float* at = &sum[32 * q + ln][2 * (8 * (i >> 2) + 4 * lh + (i & 3)) + e];
+            float* at = &sum[wave & 3][32 * q + ln][2 * (8 * (i >> 2) + 4 * lh + (i & 3)) + e];
             *at = w == 0 ? acc[q][e][i] : *at + acc[q][e][i];
           }
     }
     __syncthreads();
   }
   for (int k = threadIdx.x; k < NBB * 32 * kBwdChannels; k += kBwdThreads) {
-    const int t = nb0 + (k >> 6), ch = c0 + (k & 63);
-    if (t < nb && ch < c) part[((int64_t)blockIdx.x * nb + t) * c + ch] = sum[k >> 6][k & 63];
+    const int r = k >> 6, q = k & 63, t = nb0 + r, ch = c0 + q;
+    if (t < nb && ch < c)
+      part[((int64_t)blockIdx.x * nb + t) * c + ch] = (sum[0][r][q] + sum[1][r][q]) + (sum[2][r][q] + sum[3][r][q]);
   }
 }
 
@@ -261,7 +283,7 @@ int check_sizes(const char* what, int64_t B, int64_t N, int64_t C, int64_t radiu
   if (B < 0 || N < 0 || C < 1 || radius < 0 || NB < 1)
     return set_error(BIOEMU_ERR_INVALID_ARG, "%s: B=%ld, N=%ld, C=%ld, radius=%ld, buckets=%ld", what, (long)B, (long)N,
                      (long)C, (long)radius, (long)NB);
-  if (NB > kMaxBuckets || C > 4096 || radius > (1 << 20) || B * N * ((N + 63) / 64) >= (int64_t(1) << 31) ||
+  if (NB > kMaxBuckets || C > 4096 || radius > (1 << 20) || B * N * ((N + 31) / 32) >= (int64_t(1) << 31) ||
       N > 65535 * 64)
     return set_error(BIOEMU_ERR_UNSUPPORTED, "%s: %ld buckets (at most %d), %ld channels (at most 4096), B=%ld, N=%ld",
                      what, (long)NB, kMaxBuckets, (long)C, (long)B, (long)N);
@@ -336,7 +358,8 @@ extern "C" int bioemu_relpos_bwd(const void* dout, const uint8_t* buckets, const
                      bioemu_relpos_bwd_workspace_bytes(B, N, C, num_buckets));
   const int64_t groups = bwd_groups(B, N, C, num_buckets);
   float* part = static_cast<float*>(workspace);
-  const int cols = (int)((N + 63) / 64), units = (int)(B * N * cols);
+  const int pairs = f32 ? unit_pairs<float>() : unit_pairs<bf16>();
+  const int cols = (int)((N + pairs - 1) / pairs), units = (int)(B * N * cols);
   {
     KernelTimerScope timer("relpos_bwd", stream);
     const dim3 grid((unsigned)groups, (unsigned)((C + kBwdChannels - 1) / kBwdChannels),

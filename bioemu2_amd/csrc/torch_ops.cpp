@@ -408,25 +408,29 @@ struct AttentionCall {
       const optional<Tensor>&lengths, double scale, double cap, bool causal
 #define ATTENTION_ARGS q, k, v, table, buckets, q_seg, k_seg, prefix, lengths, scale, cap, causal
 
-std::pair<Tensor, Tensor> attention_run(ATTENTION_PARAMS, bool train) {
+// o, and for training what its rounding took off (empty in fp32) and the rows' log-sums
+std::tuple<Tensor, Tensor, Tensor> attention_run(ATTENTION_PARAMS, bool train) {
   const c10::OptionalDeviceGuard guard(q.device());
   const AttentionCall c(ATTENTION_ARGS);
-  Tensor out = at::empty(q.sizes(), q.options()), lse, ws;
-  if (train) lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+  Tensor out = at::empty(q.sizes(), q.options()), lo, lse, ws;
+  if (train) {
+    lo = is_f32(q) ? none_like(q) : at::empty(q.sizes(), q.options());
+    lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+  }
   const int64_t need = (int64_t)bioemu_attention_workspace_bytes(&c.args);
   if (need) ws = bytes(need, q);
-  check_rc(bioemu_attention_fwd(&c.args, out.data_ptr(), static_cast<float*>(ptr(lse)), ptr(ws), need, stream_of(q)),
+  check_rc(bioemu_attention_fwd(&c.args, out.data_ptr(), train && !is_f32(q) ? lo.data_ptr() : nullptr,
+                                static_cast<float*>(ptr(lse)), ptr(ws), need, stream_of(q)),
            "bioemu_attention_fwd");
-  return {out, lse};
+  return {out, lo, lse};
 }
-Tensor attention_cuda(ATTENTION_PARAMS) { return attention_run(ATTENTION_ARGS, false).first; }
-std::tuple<Tensor, Tensor> attention_train_cuda(ATTENTION_PARAMS) {
-  auto [out, lse] = attention_run(ATTENTION_ARGS, true);
-  return {out, lse};
+Tensor attention_cuda(ATTENTION_PARAMS) { return std::get<0>(attention_run(ATTENTION_ARGS, false)); }
+std::tuple<Tensor, Tensor, Tensor> attention_train_cuda(ATTENTION_PARAMS) {
+  return attention_run(ATTENTION_ARGS, true);
 }
 // dq, dk, dv and the table's gradient (empty where not wanted)
-std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward_cuda(const Tensor& out, const Tensor& lse,
-                                                                   const Tensor& dout, ATTENTION_PARAMS,
+std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward_cuda(const Tensor& out, const Tensor& lo,
+                                                                   const Tensor& lse, const Tensor& dout, ATTENTION_PARAMS,
                                                                    bool want_table) {
   const c10::OptionalDeviceGuard guard(q.device());
   const AttentionCall c(ATTENTION_ARGS);
@@ -435,29 +439,31 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward_cuda(const Tensor&
                     "attention_backward: out ", out.sizes(), ", dout ", dout.sizes(), " of q ", q.sizes());
   const int64_t lshape[3] = {q.size(0), q.size(2), q.size(1)};
   check_shape(lse, "attention_backward lse", lshape, q);
+  if (!is_f32(q)) check_shape(lo, "attention_backward lo", q.sizes(), q);
   want_table = want_table && table;
   const auto fresh = [](const Tensor& t) { return at::empty(t.sizes(), t.options()); };
   if (q.size(0) == 0 || q.size(1) == 0)
     return {fresh(q), at::zeros(k.sizes(), k.options()), at::zeros(v.sizes(), v.options()),
             want_table ? at::zeros(table->sizes(), table->options()) : none_like(q)};
   Tensor dq = fresh(q), dk = fresh(k), dv = fresh(v), dtable = want_table ? fresh(c.table) : none_like(q);
-  const Tensor o = out.contiguous(), d = heads(dout), l = lse.contiguous();
+  const Tensor o = out.contiguous(), ol = lo.contiguous(), d = heads(dout), l = lse.contiguous();
   const int64_t need = (int64_t)bioemu_attention_bwd_workspace_bytes(&c.args, want_table);
   const Tensor ws = bytes(need, q);
   const int64_t ds[3] = {d.stride(0), d.stride(1), d.stride(2)};
-  check_rc(bioemu_attention_bwd(&c.args, o.data_ptr(), l.data_ptr<float>(), d.data_ptr(), ds, dq.data_ptr(),
-                                dk.data_ptr(), dv.data_ptr(), want_table ? dtable.data_ptr() : nullptr, ws.data_ptr(),
+  check_rc(bioemu_attention_bwd(&c.args, o.data_ptr(), is_f32(q) ? nullptr : ol.data_ptr(), l.data_ptr<float>(),
+                                d.data_ptr(), ds, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), want_table ? dtable.data_ptr() : nullptr, ws.data_ptr(),
                                 need, stream_of(q)),
            "bioemu_attention_bwd");
   return {dq, dk, dv, dtable};
 }
 
 Tensor attention_meta(ATTENTION_PARAMS) { return at::empty_symint(q.sym_sizes(), q.options()); }
-std::tuple<Tensor, Tensor> attention_train_meta(ATTENTION_PARAMS) {
+std::tuple<Tensor, Tensor, Tensor> attention_train_meta(ATTENTION_PARAMS) {
   return {at::empty_symint(q.sym_sizes(), q.options()),
+          is_f32(q) ? none_like(q) : at::empty_symint(q.sym_sizes(), q.options()),
           at::empty_symint({q.sym_size(0), q.sym_size(2), q.sym_size(1)}, q.options().dtype(at::kFloat))};
 }
-std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward_meta(const Tensor&, const Tensor&, const Tensor&,
+std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward_meta(const Tensor&, const Tensor&, const Tensor&, const Tensor&,
                                                                    ATTENTION_PARAMS, bool want_table) {
   const auto fresh = [](const Tensor& t) { return at::empty_symint(t.sym_sizes(), t.options()); };
   return {fresh(q), fresh(k), fresh(v), want_table && table ? fresh(*table) : none_like(q)};
@@ -467,9 +473,9 @@ struct AttentionFn : Function<AttentionFn> {
   static Tensor forward(AutogradContext* ctx, ATTENTION_PARAMS) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = handle<decltype(attention_train_cuda)>("bioemu_mi355x::attention_train");
-    auto [out, lse] = op.call(ATTENTION_ARGS);
+    auto [out, lo, lse] = op.call(ATTENTION_ARGS);
     ctx->save_for_backward({q, k, v, or_undefined(table), or_undefined(buckets), or_undefined(q_seg),
-                            or_undefined(k_seg), or_undefined(prefix), or_undefined(lengths), out, lse});
+                            or_undefined(k_seg), or_undefined(prefix), or_undefined(lengths), out, lo, lse});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["cap"] = cap;
     ctx->saved_data["causal"] = causal;
@@ -480,7 +486,7 @@ struct AttentionFn : Function<AttentionFn> {
     const bool need_table = s[3].defined() && ctx->needs_input_grad(3);
     static auto op = handle<decltype(attention_backward_cuda)>("bioemu_mi355x::attention_backward");
     auto [dq, dk, dv, dtable] =
-        op.call(s[9], s[10], g[0], s[0], s[1], s[2], maybe(s[3]), maybe(s[4]), maybe(s[5]), maybe(s[6]), maybe(s[7]),
+        op.call(s[9], s[10], s[11], g[0], s[0], s[1], s[2], maybe(s[3]), maybe(s[4]), maybe(s[5]), maybe(s[6]), maybe(s[7]),
                 maybe(s[8]), ctx->saved_data["scale"].toDouble(), ctx->saved_data["cap"].toDouble(),
                 ctx->saved_data["causal"].toBool(), need_table);
     variable_list grads(12);
@@ -516,8 +522,8 @@ TORCH_LIBRARY_FRAGMENT(bioemu_mi355x, m) {
   m.def("relative_position_backward(Tensor dout, Tensor buckets, Tensor positions, Tensor? chains, int num_buckets, "
         "ScalarType dtype) -> Tensor");
   m.def("attention(" ATTENTION_SCHEMA ") -> Tensor");
-  m.def("attention_train(" ATTENTION_SCHEMA ") -> (Tensor, Tensor)");
-  m.def("attention_backward(Tensor out, Tensor lse, Tensor dout, " ATTENTION_SCHEMA
+  m.def("attention_train(" ATTENTION_SCHEMA ") -> (Tensor, Tensor, Tensor)");
+  m.def("attention_backward(Tensor out, Tensor out_lo, Tensor lse, Tensor dout, " ATTENTION_SCHEMA
         ", bool want_table) -> (Tensor, Tensor, Tensor, Tensor)");
 }
 

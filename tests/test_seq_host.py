@@ -98,21 +98,22 @@ def _attention_args(**over):
 def test_attention_c_abi_refusals(over, code):
     lib = _lib.lib()
     args = _attention_args(**over)
-    assert lib.bioemu_attention_fwd(args, 16, None, None, 0, None) == code
+    assert lib.bioemu_attention_fwd(args, 16, None, None, None, 0, None) == code
     assert lib.bioemu_attention_workspace_bytes(args) == 0
     assert lib.bioemu_attention_bwd_workspace_bytes(args, 0) == 0
 
 
 def test_attention_c_abi_workspace_and_outputs():
     lib = _lib.lib()
-    assert lib.bioemu_attention_fwd(None, 16, None, None, 0, None) == -1
-    assert lib.bioemu_attention_fwd(_attention_args(), None, None, None, 0, None) == -1
-    assert lib.bioemu_attention_fwd(_attention_args(B=0), None, None, None, 0, None) == 0
+    assert lib.bioemu_attention_fwd(None, 16, None, None, None, 0, None) == -1
+    assert lib.bioemu_attention_fwd(_attention_args(), None, None, None, None, 0, None) == -1
+    assert lib.bioemu_attention_fwd(_attention_args(B=0), None, None, None, None, 0, None) == 0
+    assert lib.bioemu_attention_fwd(_attention_args(), 16, 16, None, None, 0, None) == -1   # o_lo of an fp32 call
     strides = (_lib._c_int64 * 3)(128, 32, 16)
     args = _attention_args()
-    assert lib.bioemu_attention_bwd(args, 16, 16, 16, strides, 16, 16, 16, None, None, 0, None) == -3
-    assert lib.bioemu_attention_bwd(args, 16, 16, 16, strides, 16, 16, None, None, 16, 1 << 20, None) == -1
-    assert lib.bioemu_attention_bwd(args, 16, 16, 16, strides, 16, 16, 16, 16, 16, 1 << 20, None) == -1   # no table
+    assert lib.bioemu_attention_bwd(args, 16, None, 16, 16, strides, 16, 16, 16, None, None, 0, None) == -3
+    assert lib.bioemu_attention_bwd(args, 16, None, 16, 16, strides, 16, 16, None, None, 16, 1 << 20, None) == -1
+    assert lib.bioemu_attention_bwd(args, 16, None, 16, 16, strides, 16, 16, 16, 16, 16, 1 << 20, None) == -1   # no table
     assert lib.bioemu_attention_bwd_workspace_bytes(args, 0) == 256   # 1 x 2 x 4 row sums, rounded up
 
 
