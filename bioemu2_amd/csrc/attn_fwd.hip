@@ -246,12 +246,15 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
   }
 }
 
-// Waves of attn_few: each has two K and two V tiles of its own, 128 KB of LDS in all at most.
+// Waves of attn_few: each has a K and a V tile of its own, 64 KB of LDS in all at most (two workgroups a CU, so that
+// one streams while the other starts or joins: 131 KB with two tiles of each measured 168 us where this takes WW).
 template <class T, int DP>
 constexpr int few_waves() {
-  constexpr int w = 131072 / (4 * Tile<T, DP, 32>::BYTES);
+  constexpr int w = 65536 / (2 * Tile<T, DP, 32>::BYTES);
   return w < 8 ? w : 8;
 }
+constexpr int kLgkm0 = 0xc07f;   // s_waitcnt lgkmcnt(0)
+constexpr int vmcnt(int n) { return 0x0f70 | (n & 15) | ((n >> 4) << 14); }
 
 // chunk: 32-key tiles of one split.  Splits are of equal length whatever the sequences' lengths (those past a
 // sequence's end do nothing), and workgroups take them in plain order, round the XCDs: no two share a key.
@@ -263,11 +266,11 @@ __global__ __launch_bounds__((64 * few_waves<T, DP>())) void attn_few_kernel(con
   constexpr int W = few_waves<T, DP>(), STEPS = DP / 16, DB = DP / 32;
   typedef Tile<T, DP, 32> KV;
   constexpr int CP = KV::copies(64);
-  __shared__ __attribute__((aligned(1024))) char tiles[W][2][2][KV::BYTES];
+  __shared__ __attribute__((aligned(1024))) char tiles[W][2][KV::BYTES];
   __shared__ float ml[W][2][32];
 
   const int lane = threadIdx.x & 63, wave = wave_id(), ln = lane & 31, lh = lane >> 5;
-  const int bh = blockIdx.x / splits, split = blockIdx.x - bh * splits, b = bh / a.Hk, hk = bh - b * a.Hk;
+  const int bs = blockIdx.x / a.Hk, hk = blockIdx.x - bs * a.Hk, b = bs / splits, split = bs - b * splits;
   const int rows = a.Nq * a.G;
   const int length = a.lengths ? min(max(a.lengths[b], 0), a.Nk) : a.Nk;
   const int prefix = a.prefix ? a.prefix[b] : 0;
@@ -294,13 +297,18 @@ __global__ __launch_bounds__((64 * few_waves<T, DP>())) void attn_few_kernel(con
   unsigned koff[CP], voff[CP];
   KV::offsets(lane, 64, a.kn, a.D, koff);
   KV::offsets(lane, 64, a.vn, a.D, voff);
-  auto stage = [&](int t, int buf) {
-    const int k0 = t * 32;
-    KV::copy(kbase + (int64_t)k0 * a.kn, length - k0, a.kn, a.D, tiles[wave][buf][0], 0, 64, koff);
-    KV::copy(vbase + (int64_t)k0 * a.vn, length - k0, a.vn, a.D, tiles[wave][buf][1], 0, 64, voff);
+  char *kt = tiles[wave][0], *vt = tiles[wave][1];
+  auto stage_k = [&](int t) {
+    KV::copy(kbase + (int64_t)t * 32 * a.kn, length - t * 32, a.kn, a.D, kt, 0, 64, koff);
+  };
+  auto stage_v = [&](int t) {
+    KV::copy(vbase + (int64_t)t * 32 * a.vn, length - t * 32, a.vn, a.D, vt, 0, 64, voff);
   };
   const int blocks = (top + 31) / 32, t0 = min(split * chunk, blocks), t1 = min(t0 + chunk, blocks);
-  if (t0 + wave < t1) stage(t0 + wave, 0);   // before the queries and the bias: it takes longest
+  if (t0 + wave < t1) {   // before the queries and the bias: it takes longest
+    stage_k(t0 + wave);
+    stage_v(t0 + wave);
+  }
 
   Frag<T> qf[STEPS];
   {
@@ -318,26 +326,17 @@ __global__ __launch_bounds__((64 * few_waves<T, DP>())) void attn_few_kernel(con
   const float s_scale = a.cap > 0.f ? a.scale / a.cap : a.scale * kLog2e;
   const float s_cap = a.cap * kLog2e;
 
-  int buf = 0;
-  for (int t = t0 + wave; t < t1; t += W, buf ^= 1) {
+  // K of the next tile is on its way while V of this one is waited for and used, and V while K is: a tile's copies are
+  // made as soon as its reader is done with the one before
+  for (int t = t0 + wave; t < t1; t += W) {
     const int k0 = t * 32;
-    if (t + W < t1) {
-      stage(t + W, buf ^ 1);
-      __builtin_amdgcn_s_waitcnt(0x0f70 | ((2 * CP) & 15) | (((2 * CP) >> 4) << 14));   // all but the next tile's
-    } else {
-      __builtin_amdgcn_s_waitcnt(0x0f70);
-    }
+    __builtin_amdgcn_s_waitcnt(vmcnt(CP));   // all but V
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    char *kt = tiles[wave][buf][0], *vt = tiles[wave][buf][1];
-    if (seg) {
-      // two lanes a key: values of a key in no segment are zeroed (0 times them has to be 0)
-      const int r = lane >> 1;
-      if (k0 + r < length && kseg[k0 + r] < 0) KV::clear(vt, r, lane & 1, 2);
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    }
     f32x16 s = zero16();
 #pragma unroll
     for (int st = 0; st < STEPS; ++st) s = mfma16(KV::rows(kt, ln, st, lh), qf[st], s);
+    __builtin_amdgcn_s_waitcnt(kLgkm0);   // the tile has been read
+    if (t + W < t1) stage_k(t + W);
     float x[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) x[r] = s[r] * s_scale;
@@ -387,19 +386,31 @@ __global__ __launch_bounds__((64 * few_waves<T, DP>())) void attn_few_kernel(con
       x[r] = fast_exp2(x[r] - mref);
       l += x[r];
     }
+    if (t + W < t1)
+      __builtin_amdgcn_s_waitcnt(vmcnt(CP));   // all but the next K
+    else
+      __builtin_amdgcn_s_waitcnt(vmcnt(0));
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (seg) {
+      // two lanes a key: values of a key in no segment are zeroed (0 times them has to be 0)
+      const int r = lane >> 1;
+      if (k0 + r < length && kseg[k0 + r] < 0) KV::clear(vt, r, lane & 1, 2);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       const Frag<T> p = as_operand<T>(x, st);
 #pragma unroll
       for (int d = 0; d < DB; ++d) acc[d] = mfma16(KV::cols(vt, 16 * st, 32 * d, lane), p, acc[d]);
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the tile is read before the copy after next
+    __builtin_amdgcn_s_waitcnt(kLgkm0);
+    if (t + W < t1) stage_v(t + W);
   }
 
-  // the waves' parts through LDS (over the tiles: W x 32 x DP floats are half of them at most)
+  // the waves' parts through LDS (over the tiles: W x 32 x DP floats)
   l += __shfl_xor(l, 32);
   __syncthreads();
-  float* sh = reinterpret_cast<float*>(&tiles[0][0][0][0]);
+  float* sh = reinterpret_cast<float*>(&tiles[0][0][0]);
   if (lh == 0) {
     ml[wave][0][ln] = l == 0.f ? -kInf : mref;
     ml[wave][1][ln] = l;
@@ -444,15 +455,15 @@ __global__ __launch_bounds__((64 * few_waves<T, DP>())) void attn_few_kernel(con
   }
 }
 
-// One wave a row: the splits' parts added in order (a split that saw nothing wrote no values).  Lane s holds the weight
-// of split s, lane d value d and 64 + d.
+// A workgroup a row: wave w adds splits w, w + 4, ... in order, then the waves are added in order.  A split that saw
+// nothing wrote no values.  Lane d holds values d and 64 + d.
 template <class T>
 __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const AttnArgs a, Parts parts, int splits,
                                                                  T* __restrict__ out, T* __restrict__ lo,
                                                                  float* __restrict__ lse) {
-  const int64_t rows = (int64_t)a.B * a.Nq * a.H, row = (int64_t)blockIdx.x * 4 + wave_id();
-  if (row >= rows) return;
-  const int lane = threadIdx.x & 63;
+  __shared__ float sh[4][3][64];
+  const int64_t rows = (int64_t)a.B * a.Nq * a.H, row = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = wave_id();
   float top = -kInf;
   for (int s = lane; s < splits; s += 64) top = fmaxf(top, parts.ml[2 * (s * rows + row)]);
 #pragma unroll
@@ -460,36 +471,39 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const AttnArgs 
   const float to = top == -kInf ? 0.f : top;
   float o0 = 0.f, o1 = 0.f, sum = 0.f;
   const int d0 = min(lane, a.D - 1), d1 = min(lane + 64, a.D - 1);
-  for (int s0 = 0; s0 < splits; s0 += 64) {
-    const bool on = s0 + lane < splits;
-    const float* ml = parts.ml + 2 * ((s0 + (on ? lane : 0)) * rows + row);
-    const float f = on ? fast_exp2(ml[0] - to) : 0.f;
-    float l = on ? f * ml[1] : 0.f;
+  for (int s0 = wave; s0 < splits; s0 += 16) {
+    float f[4], l[4], x0[4], x1[4];
 #pragma unroll
-    for (int m = 32; m > 0; m /= 2) l += __shfl_xor(l, m);
-    sum += l;
-    const uint64_t seen = __ballot(f != 0.f);
-    const int n = min(64, splits - s0);
-#pragma unroll 8
-    for (int s = 0; s < n; ++s) {
-      const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s));
-      const bool there = (seen >> s) & 1;
-      const float* po = parts.o + ((there ? s0 + s : 0) * rows + row) * a.D;
-      const float x0 = po[d0], x1 = po[d1];
-      o0 += there ? w * x0 : 0.f;
-      o1 += there ? w * x1 : 0.f;
+    for (int q = 0; q < 4; ++q) {
+      const int s = s0 + 4 * q;
+      const int64_t at = (s < splits ? s : s0) * rows + row;
+      f[q] = s < splits ? fast_exp2(parts.ml[2 * at] - to) : 0.f;
+      l[q] = parts.ml[2 * at + 1];
+      x0[q] = parts.o[at * a.D + d0];
+      x1[q] = parts.o[at * a.D + d1];
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      o0 += f[q] == 0.f ? 0.f : f[q] * x0[q];
+      o1 += f[q] == 0.f ? 0.f : f[q] * x1[q];
+      sum += f[q] == 0.f ? 0.f : f[q] * l[q];
     }
   }
+  sh[wave][0][lane] = o0;
+  sh[wave][1][lane] = o1;
+  sh[wave][2][lane] = sum;
+  __syncthreads();
+  if (wave >= 2) return;
+  sum = (sh[0][2][lane] + sh[1][2][lane]) + (sh[2][2][lane] + sh[3][2][lane]);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  for (int h = 0; h < 2; ++h) {
-    const int d = lane + 64 * h;
-    if (d >= a.D) continue;
-    const float v = (h ? o1 : o0) * inv;
+  const int d = lane + 64 * wave;
+  if (d < a.D) {
+    const float v = ((sh[0][wave][lane] + sh[1][wave][lane]) + (sh[2][wave][lane] + sh[3][wave][lane])) * inv;
     const T hi = (T)v;
     out[row * a.D + d] = hi;
     if (lo) lo[row * a.D + d] = (T)(v - (float)hi);
   }
-  if (lse && lane == 0) {
+  if (lse && threadIdx.x == 0) {
     const int64_t bi = row / a.H, h = row - bi * a.H, b = bi / a.Nq, i = bi - b * a.Nq;
     lse[(b * a.H + h) * a.Nq + i] = row_log_sum(to, sum);
   }
@@ -497,15 +511,16 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const AttnArgs 
 
 bool few_rows(const AttnArgs& a) { return a.Nq * a.G <= 32; }
 
-// Workgroups that the keys of a query block are split over: as many as bring the launch to two workgroups a CU (four
-// where rows are few: sequences of a cache are of unequal length), each with at least `least` keys: below it the join
-// costs more than the shorter walk gains (773 keys of 16 heads: 18 us in four parts, 13 in one).
+// Workgroups that the keys of a query block are split over.  Long rows: as many as bring the launch to two workgroups a
+// CU, 512 keys each at least.  Few rows: sequences of a cache are of unequal length, so up to sixteen a CU that even
+// out, 512 keys each at least (8 sequences of 8200 to 32768 keys, 8 heads: 160 us in parts of 2048, XX in parts of
+// 512), and none for up to 1024 keys, where the join costs what the shorter walk gains (773 keys: 18 us in four parts,
+// 13 in one).
 int key_splits(const AttnArgs& a) {
   const bool few = few_rows(a);
+  if (few && a.Nk <= 1024) return 1;
   const int64_t base = few ? (int64_t)a.B * a.Hk : (int64_t)a.B * a.H * ((a.Nq + kGroupRows - 1) / kGroupRows);
-  const int64_t least = few ? 1024 : 512;
-  const int64_t want = ((few ? 4 : 2) * (int64_t)compute_units() + base - 1) / base;
-  const int64_t most = (a.Nk + least - 1) / least;
+  const int64_t want = ((few ? 16 : 2) * (int64_t)compute_units() + base - 1) / base, most = (a.Nk + 511) / 512;
   const int64_t s = want < most ? want : most;
   return s < 1 ? 1 : (int)s;
 }
@@ -537,7 +552,7 @@ int launch_fwd(const AttnArgs& a, void* o, void* o_lo, float* lse, void* ws, hip
   }
   if (splits == 1) return BIOEMU_OK;
   KernelTimerScope timer("attn_join", stream);
-  attn_join_kernel<T><<<dim3((unsigned)((rows + 3) / 4)), kAttnThreads, 0, stream>>>(a, parts, splits, out, lo, lse);
+  attn_join_kernel<T><<<dim3((unsigned)rows), kAttnThreads, 0, stream>>>(a, parts, splits, out, lo, lse);
   return check_launch("attn_join");
 }
 
