@@ -208,14 +208,37 @@ __device__ __forceinline__ void copy_ints(const void* src, int n, void* lds, int
   copy_to_lds<4>(copy_source(src, n <= 0 ? 0 : (n < 64 ? n : 64) * 4), lane * 4, lds);
 }
 
-// tanh.  bf16 operands: by the hardware exponential, off by 2e-7, far below the rounding of q and k.
+// A capped score in log2 units, x = s_cap tanh(y) + add with s_cap = cap log2 e and y = raw scale / cap, and what the
+// tanh leaves of a gradient: slope times kSlope is 1 - tanh^2.
+// bf16 operands: by r = 1 / (1 + e^2y) of the hardware exponential and reciprocal, tanh = 1 - 2 r, 1 - tanh^2 =
+// 4 (r - r^2): six instructions, off by 2e-7 of the cap, far below the rounding of q and k.  fp32: tanhf.
 template <class T>
-__device__ __forceinline__ float attn_tanh(float y) {
-  if constexpr (sizeof(T) == 2)
-    return 1.f - 2.f * fast_rcp(1.f + fast_exp2(y * (2.f * kLog2e)));
-  else
-    return tanhf(y);
-}
+struct Capped {
+  float k1, k2, k3;
+  static constexpr float kSlope = sizeof(T) == 2 ? 4.f : 1.f;
+  __device__ __forceinline__ explicit Capped(const AttnArgs& a) {
+    if constexpr (sizeof(T) == 2) {
+      k1 = a.scale / a.cap * (2.f * kLog2e);
+      k2 = -2.f * a.cap * kLog2e;
+    } else {
+      k1 = a.scale / a.cap;
+      k2 = a.cap * kLog2e;
+    }
+    k3 = sizeof(T) == 2 ? a.cap * kLog2e : 0.f;
+  }
+  // `add` includes k3
+  __device__ __forceinline__ float score(float raw, float add, float& slope) const {
+    if constexpr (sizeof(T) == 2) {
+      const float r = fast_rcp(1.f + fast_exp2(raw * k1));
+      slope = r - r * r;
+      return r * k2 + add;
+    } else {
+      const float t = tanhf(raw * k1);
+      slope = 1.f - t * t;
+      return t * k2 + add;
+    }
+  }
+};
 
 // A bias in log2 units.  The type's lowest value stays finite (a row of such scores is a softmax over equal scores);
 // -infinity stays what it is.

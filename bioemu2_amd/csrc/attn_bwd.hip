@@ -53,13 +53,13 @@ __device__ __forceinline__ void store_rows(const f32x16 (&acc)[DB], float scale,
     }
 }
 
-template <class T, int DP>
+template <class T, int DP, bool CAP>
 __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs a, const T* __restrict__ o,
                                                                   const T* __restrict__ o_lo,
                                                                   const float* __restrict__ lse,
                                                                   const T* __restrict__ dout, int64_t db, int64_t dn,
                                                                   int64_t dh, T* __restrict__ dq,
-                                                                  float* __restrict__ delta,
+                                                                  float* __restrict__ stats,
                                                                   float* __restrict__ dq_part,
                                                                   float* __restrict__ bias_part, int splits,
                                                                   int qblocks, int total) {
@@ -110,6 +110,13 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
       for (int e = threadIdx.x; e < 4 * (row4 + kDiagBlock); e += kAttnThreads) sums[e] = 0.f;
   }
 
+  const Capped<T> capped(a);
+  const float mult = a.scale * kLog2e, out_scale = a.scale * (CAP ? Capped<T>::kSlope : 1.f);
+  const auto score = [&](float raw, float add, float& slope) {
+    if constexpr (CAP) return capped.score(raw, add, slope);
+    return raw * mult + add;
+  };
+
   // a row that sees nothing contributes nothing, whatever it holds
   const bool on = live && lim > 0;
   const int64_t row = ((int64_t)b * a.Nq + (live ? i : 0)) * a.H + h, srow = ((int64_t)b * a.H + h) * a.Nq + i;
@@ -134,7 +141,12 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
     }
   }
   dsum += __shfl_xor(dsum, 32);
-  if (live && lh == 0 && split == 0) delta[srow] = -dsum;
+  // the constant part of every score of the row, what its weights are taken against included
+  const float base = (CAP ? capped.k3 : 0.f) - row_lse;
+  if (live && lh == 0 && split == 0) {
+    stats[srow] = base;
+    stats[(int64_t)a.B * a.H * a.Nq + srow] = -dsum;
+  }
 
   const T* kbase = static_cast<const T*>(a.k) + b * a.kb + hk * a.kh;
   const T* vbase = static_cast<const T*>(a.v) + b * a.vb + hk * a.vh;
@@ -147,8 +159,6 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
 #pragma unroll
   for (int d = 0; d < DB; ++d) acc[d] = zero16();
   float far_lo = 0.f, far_hi = 0.f;
-  const bool cap = a.cap > 0.f;
-  const float s_scale = cap ? a.scale / a.cap : a.scale * kLog2e, s_cap = a.cap * kLog2e, mult = cap ? 1.f : s_scale;
 
   auto stage = [&](int entry, int buf) {
     const int k0 = (entry & kBlockMask) * KB;
@@ -189,23 +199,16 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
 #pragma unroll
         for (int st = 0; st < STEPS; ++st) dp = mfma16(KV::rows(vt, 32 * u + ln, st, lh), df[st], dp);
         float x[16], slope[16];
-        if (cap)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float t = attn_tanh<T>(s[r] * s_scale);
-            slope[r] = 1.f - t * t;
-            s[r] = s_cap * t;
-          }
         const int rel0 = k0 + 32 * u - wave_pos;   // of the wave's first query and the first key
         const bool far = all_far(a, rel0);
         if (a.table && !far) {
           const float* bias = lut + (rel0 + a.radius + kPad + 4 * lh - ln);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) x[r] = s[r] * mult + (bias[8 * (r >> 2) + (r & 3)] - row_lse);
+          for (int r = 0; r < 16; ++r) x[r] = score(s[r], bias[8 * (r >> 2) + (r & 3)] + base, slope[r]);
         } else {
-          const float add = (a.table ? lut[rel0 > 0 ? nrel - 1 : 0] : 0.f) - row_lse;
+          const float add = base + (a.table ? lut[rel0 > 0 ? nrel - 1 : 0] : 0.f);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) x[r] = s[r] * mult + add;
+          for (int r = 0; r < 16; ++r) x[r] = score(s[r], add, slope[r]);
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) x[r] = fast_exp2(x[r]) * dp[r];
@@ -246,7 +249,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
           }
         }
-        if (cap)
+        if constexpr (CAP)
 #pragma unroll
           for (int r = 0; r < 16; ++r) x[r] *= slope[r];
 #pragma unroll
@@ -262,7 +265,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
 
   if (live) {
     const int64_t at_row = splits == 1 ? row : split * (int64_t)a.B * a.Nq * a.H + row;
-    store_rows<T, DB>(acc, a.scale, splits == 1 ? dq + row * a.D : nullptr, dq_part + at_row * a.D, lh, a.D);
+    store_rows<T, DB>(acc, out_scale, splits == 1 ? dq + row * a.D : nullptr, dq_part + at_row * a.D, lh, a.D);
   }
   if (bias_part) {
 #pragma unroll
@@ -301,10 +304,10 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
   }
 }
 
-template <class T, int DP>
-__global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArgs a, const float* __restrict__ lse,
+template <class T, int DP, bool CAP>
+__global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArgs a, const float* __restrict__ row_stats,
                                                                    const T* __restrict__ dout, int64_t db, int64_t dn,
-                                                                   int64_t dh, const float* __restrict__ delta,
+                                                                   int64_t dh,
                                                                    T* __restrict__ dk, T* __restrict__ dv,
                                                                    float* __restrict__ part, int splits, int kblocks,
                                                                    int total) {
@@ -313,7 +316,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArg
   constexpr int CP = QD::copies(kAttnThreads);
   __shared__ __attribute__((aligned(1024))) char tiles[2][2][QD::BYTES];
   __shared__ __attribute__((aligned(16))) int segs[2][64];
-  __shared__ __attribute__((aligned(16))) float stats[2][2][64];   // log-sums, -do . o
+  __shared__ __attribute__((aligned(16))) float stats[2][2][64];   // what attn_bwd_q wrote of the rows
   __shared__ int list[kListBlocks];
   __shared__ uint8_t flags[kListBlocks];
   __shared__ int red[3][4], count;
@@ -365,8 +368,12 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArg
   f32x16 ak[DB], av[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) ak[d] = av[d] = zero16();
-  const bool cap = a.cap > 0.f;
-  const float s_scale = cap ? a.scale / a.cap : a.scale * kLog2e, s_cap = a.cap * kLog2e, mult = cap ? 1.f : s_scale;
+  const Capped<T> capped(a);
+  const float mult = a.scale * kLog2e, out_scale = a.scale * (CAP ? Capped<T>::kSlope : 1.f);
+  const auto score = [&](float raw, float add, float& slope) {
+    if constexpr (CAP) return capped.score(raw, add, slope);
+    return raw * mult + add;
+  };
 
   const T *qbase = nullptr, *dbase = nullptr;   // of the current head, as its row of statistics
   int64_t srow = 0;
@@ -374,8 +381,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArg
     const int i0 = (en & kBlockMask) * QB;
     QD::copy(qbase + (int64_t)i0 * a.qn, a.Nq - i0, a.qn, a.D, tiles[buf][0], wave, kAttnThreads, qoff);
     QD::copy(dbase + (int64_t)i0 * dn, a.Nq - i0, dn, a.D, tiles[buf][1], wave, kAttnThreads, doff);
-    if (wave == 0) copy_ints(lse + srow + i0, a.Nq - i0, stats[buf][0], lane);
-    if (wave == 1) copy_ints(delta + srow + i0, a.Nq - i0, stats[buf][1], lane);
+    if (wave == 0) copy_ints(row_stats + srow + i0, a.Nq - i0, stats[buf][0], lane);
+    if (wave == 1) copy_ints(row_stats + (int64_t)a.B * a.H * a.Nq + srow + i0, a.Nq - i0, stats[buf][1], lane);
     if (seg && wave == 2) copy_ints(qseg + i0, a.Nq - i0, segs[buf], lane);
   };
 
@@ -400,10 +407,10 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArg
         __builtin_amdgcn_s_waitcnt(0x0f70);
         __syncthreads();
         if (t + 1 < t1) stage(entry(t + 1), buf ^ 1);
-        // rows that see nothing (their log-sum is infinite) have weight 0, and 0 times what they hold has to be 0
-        if (__ballot(lane < QB && stats[buf][0][lane] == kInf)) {
+        // rows that see nothing (their constant is -infinity) have weight 0, and 0 times what they hold has to be 0
+        if (__ballot(lane < QB && stats[buf][0][lane] == -kInf)) {
           const int r = threadIdx.x / (kAttnThreads / QB);
-          if (stats[buf][0][r] == kInf) {
+          if (stats[buf][0][r] == -kInf) {
             QD::clear(tiles[buf][0], r, threadIdx.x % (kAttnThreads / QB), kAttnThreads / QB);
             QD::clear(tiles[buf][1], r, threadIdx.x % (kAttnThreads / QB), kAttnThreads / QB);
           }
@@ -414,7 +421,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArg
 #pragma unroll 1
         for (int u = 0; u < SUB; ++u) {
           f32x16 s = zero16(), dp;
-          float lsev[16];
+          float base[16];
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const int at = 32 * u + 8 * q + 4 * lh;
@@ -422,7 +429,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArg
             const f32x4 vd = *reinterpret_cast<const f32x4*>(&stats[buf][1][at]);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              lsev[4 * q + c] = vl[c];
+              base[4 * q + c] = vl[c];
               dp[4 * q + c] = vd[c];
             }
           }
@@ -431,22 +438,18 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArg
 #pragma unroll
           for (int st = 0; st < STEPS; ++st) dp = mfma16(QD::rows(dt, 32 * u + ln, st, lh), vf[st], dp);
           float x[16], slope[16];
-          if (cap)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const float t = attn_tanh<T>(s[r] * s_scale);
-              slope[r] = 1.f - t * t;
-              s[r] = s_cap * t;
-            }
           const int rel0 = wave_key - (first + i0 + 32 * u);   // of the first query and the wave's first key
           if (a.table && !all_far(a, rel0)) {
             const float* bias = lut + (rel0 + a.radius + kPad + ln - 4 * lh);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] = s[r] * mult + (bias[-(8 * (r >> 2) + (r & 3))] - lsev[r]);
-          } else {
-            const float add = a.table ? lut[rel0 > 0 ? 2 * (a.radius + kPad) : 0] : 0.f;
+            for (int r = 0; r < 16; ++r) x[r] = score(s[r], bias[-(8 * (r >> 2) + (r & 3))] + base[r], slope[r]);
+          } else if (a.table) {
+            const float add = lut[rel0 > 0 ? 2 * (a.radius + kPad) : 0];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] = s[r] * mult + (add - lsev[r]);
+            for (int r = 0; r < 16; ++r) x[r] = score(s[r], add + base[r], slope[r]);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] = score(s[r], base[r], slope[r]);
           }
 #pragma unroll
           for (int r = 0; r < 16; ++r) x[r] = fast_exp2(x[r]);
@@ -472,7 +475,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArg
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             x[r] *= dp[r];
-            if (cap) x[r] *= slope[r];
+            if constexpr (CAP) x[r] *= slope[r];
           }
 #pragma unroll
           for (int st = 0; st < 2; ++st) {
@@ -489,7 +492,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArg
   if (j >= a.Nk) return;
   const int64_t row = ((int64_t)b * a.Nk + j) * a.Hk + hk, rows = (int64_t)a.B * a.Nk * a.Hk;
   // parts: dk of every split, then dv
-  store_rows<T, DB>(ak, a.scale, splits == 1 ? dk + row * a.D : nullptr, part + (split * rows + row) * a.D, lh, a.D);
+  store_rows<T, DB>(ak, out_scale, splits == 1 ? dk + row * a.D : nullptr, part + (split * rows + row) * a.D, lh, a.D);
   store_rows<T, DB>(av, 1.f, splits == 1 ? dv + row * a.D : nullptr, part + ((splits + split) * rows + row) * a.D, lh,
                     a.D);
 }
@@ -560,7 +563,7 @@ int walk_splits(int64_t groups, int64_t walk, int block) {
 
 struct BwdSpace {
   int q_splits, kv_splits;
-  size_t delta, q_part, kv_part, bias, total;   // bytes, in this order
+  size_t stats, q_part, kv_part, bias, total;   // bytes, in this order
 };
 BwdSpace bwd_space(const AttnArgs& a, bool f32, bool table) {
   const int64_t qblocks = (a.Nq + kGroupRows - 1) / kGroupRows, kblocks = (a.Nk + kGroupRows - 1) / kGroupRows;
@@ -568,37 +571,37 @@ BwdSpace bwd_space(const AttnArgs& a, bool f32, bool table) {
   BwdSpace s;
   s.q_splits = walk_splits((int64_t)a.B * a.H * qblocks, a.Nk, block);
   s.kv_splits = kblocks ? walk_splits((int64_t)a.B * a.Hk * kblocks, (int64_t)a.Nq * a.G, block) : 1;
-  s.delta = (size_t)round_up((int64_t)a.B * a.H * a.Nq * 4, 256);
+  s.stats = (size_t)round_up((int64_t)a.B * a.H * a.Nq * 8, 256);
   s.q_part = s.q_splits == 1 ? 0 : (size_t)round_up((int64_t)s.q_splits * a.B * a.H * a.Nq * a.D * 4, 256);
   s.kv_part = s.kv_splits == 1 ? 0 : (size_t)round_up((int64_t)s.kv_splits * 2 * a.B * a.Hk * a.Nk * a.D * 4, 256);
   s.bias = table ? (size_t)(a.B * qblocks * s.q_splits * a.H * a.nb) * 4 : 0;
-  s.total = s.delta + s.q_part + s.kv_part + s.bias;
+  s.total = s.stats + s.q_part + s.kv_part + s.bias;
   return s;
 }
 
-template <class T, int DP>
-int launch_bwd(const AttnArgs& a, const void* o, const void* o_lo, const float* lse, const void* dout, const int64_t* ds, void* dq,
+template <class T, int DP, bool CAP>
+int launch_bwd_as(const AttnArgs& a, const void* o, const void* o_lo, const float* lse, const void* dout, const int64_t* ds, void* dq,
                void* dk, void* dv, void* dtable, void* ws, hipStream_t stream) {
   const BwdSpace sp = bwd_space(a, sizeof(T) == 4, dtable != nullptr);
   char* at = static_cast<char*>(ws);
-  float* delta = reinterpret_cast<float*>(at);
-  float* q_part = reinterpret_cast<float*>(at + sp.delta);
-  float* kv_part = reinterpret_cast<float*>(at + sp.delta + sp.q_part);
-  float* bias = dtable ? reinterpret_cast<float*>(at + sp.delta + sp.q_part + sp.kv_part) : nullptr;
+  float* stats = reinterpret_cast<float*>(at);
+  float* q_part = reinterpret_cast<float*>(at + sp.stats);
+  float* kv_part = reinterpret_cast<float*>(at + sp.stats + sp.q_part);
+  float* bias = dtable ? reinterpret_cast<float*>(at + sp.stats + sp.q_part + sp.kv_part) : nullptr;
   const int qblocks = (a.Nq + kGroupRows - 1) / kGroupRows, kblocks = (a.Nk + kGroupRows - 1) / kGroupRows;
   {
     const int64_t total = (int64_t)a.B * a.H * qblocks * sp.q_splits;
     KernelTimerScope timer("attn_bwd_q", stream);
-    attn_bwd_q_kernel<T, DP><<<dim3(attn_grid(total)), kAttnThreads, bias_lds(a, dtable != nullptr), stream>>>(
+    attn_bwd_q_kernel<T, DP, CAP><<<dim3(attn_grid(total)), kAttnThreads, bias_lds(a, dtable != nullptr), stream>>>(
         a, static_cast<const T*>(o), static_cast<const T*>(o_lo), lse, static_cast<const T*>(dout), ds[0], ds[1], ds[2],
-        static_cast<T*>(dq), delta, q_part, bias, sp.q_splits, qblocks, (int)total);
+        static_cast<T*>(dq), stats, q_part, bias, sp.q_splits, qblocks, (int)total);
     if (const int rc = check_launch("attn_bwd_q")) return rc;
   }
   if (kblocks > 0) {
     const int64_t total = (int64_t)a.B * a.Hk * kblocks * sp.kv_splits;
     KernelTimerScope timer("attn_bwd_kv", stream);
-    attn_bwd_kv_kernel<T, DP><<<dim3(attn_grid(total)), kAttnThreads, bias_lds(a, false), stream>>>(
-        a, lse, static_cast<const T*>(dout), ds[0], ds[1], ds[2], delta, static_cast<T*>(dk), static_cast<T*>(dv),
+    attn_bwd_kv_kernel<T, DP, CAP><<<dim3(attn_grid(total)), kAttnThreads, bias_lds(a, false), stream>>>(
+        a, stats, static_cast<const T*>(dout), ds[0], ds[1], ds[2], static_cast<T*>(dk), static_cast<T*>(dv),
         kv_part, sp.kv_splits, kblocks, (int)total);
     if (const int rc = check_launch("attn_bwd_kv")) return rc;
   }
@@ -619,6 +622,13 @@ int launch_bwd(const AttnArgs& a, const void* o, const void* o_lo, const float* 
   attn_bias_reduce_kernel<<<dim3((unsigned)((size + 15) / 16)), 1024, 0, stream>>>(bias, a.B * qblocks * sp.q_splits,
                                                                                   size, dtable, a.table_bf16);
   return check_launch("attn_bias_reduce");
+}
+
+template <class T, int DP>
+int launch_bwd(const AttnArgs& a, const void* o, const void* o_lo, const float* lse, const void* dout, const int64_t* ds,
+               void* dq, void* dk, void* dv, void* dtable, void* ws, hipStream_t stream) {
+  return a.cap > 0.f ? launch_bwd_as<T, DP, true>(a, o, o_lo, lse, dout, ds, dq, dk, dv, dtable, ws, stream)
+                     : launch_bwd_as<T, DP, false>(a, o, o_lo, lse, dout, ds, dq, dk, dv, dtable, ws, stream);
 }
 
 }  // namespace

@@ -42,7 +42,7 @@ __device__ __forceinline__ void store_quad(T* out, T* lo, const float (&v)[4]) {
 
 __device__ __forceinline__ float row_log_sum(float m, float l) { return l > 0.f ? m + __log2f(l) : kInf; }
 
-template <class T, int DP>
+template <class T, int DP, bool CAP>
 __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a, T* __restrict__ out,
                                                                 T* __restrict__ lo, float* __restrict__ lse,
                                                                 Parts parts, int splits,
@@ -107,8 +107,13 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
   for (int d = 0; d < DB; ++d) acc[d] = zero16();
   // weights are 2^(x - mref); a row starts with its first finite score, then mref moves when one exceeds limit
   float mref = 0.f, limit = -kInf, l = 0.f;
-  const bool cap = a.cap > 0.f;
-  const float s_scale = cap ? a.scale / a.cap : a.scale * kLog2e, s_cap = a.cap * kLog2e, mult = cap ? 1.f : s_scale;
+  const Capped<T> capped(a);
+  const float mult = a.scale * kLog2e, base = CAP ? capped.k3 : 0.f;
+  const auto score = [&](float raw, float add) {
+    float slope;
+    if constexpr (CAP) return capped.score(raw, add, slope);
+    return raw * mult + add;
+  };
 
   auto stage = [&](int entry, int buf) {
     const int k0 = (entry & kBlockMask) * KB;
@@ -143,18 +148,15 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
         f32x16 s = zero16();
 #pragma unroll
         for (int st = 0; st < STEPS; ++st) s = mfma16(KV::rows(kt, 32 * u + ln, st, lh), qf[st], s);
-        if (cap)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = s_cap * attn_tanh<T>(s[r] * s_scale);
         const int rel0 = k0 + 32 * u - wave_pos;   // of the wave's first query and the first key
         if (a.table && !all_far(a, rel0)) {
           const float* bias = lut + (rel0 + a.radius + kPad + 4 * lh - ln);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) x[u][r] = s[r] * mult + bias[8 * (r >> 2) + (r & 3)];
+          for (int r = 0; r < 16; ++r) x[u][r] = score(s[r], bias[8 * (r >> 2) + (r & 3)] + base);
         } else {
-          const float add = a.table ? lut[rel0 > 0 ? 2 * (a.radius + kPad) : 0] : 0.f;
+          const float add = base + (a.table ? lut[rel0 > 0 ? 2 * (a.radius + kPad) : 0] : 0.f);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) x[u][r] = s[r] * mult + add;
+          for (int r = 0; r < 16; ++r) x[u][r] = score(s[r], add);
         }
       }
       if (k0 + KB > wave_min)
@@ -323,8 +325,8 @@ __global__ __launch_bounds__((64 * few_waves<T, DP>())) void attn_few_kernel(con
 #pragma unroll
   for (int d = 0; d < DB; ++d) acc[d] = zero16();
   float m = -kInf, mref = 0.f, l = 0.f;
-  const float s_scale = a.cap > 0.f ? a.scale / a.cap : a.scale * kLog2e;
-  const float s_cap = a.cap * kLog2e;
+  const Capped<T> capped(a);
+  const float mult = a.scale * kLog2e;
 
   // K of the next tile is on its way while V of this one is waited for and used, and V while K is: a tile's copies are
   // made as soon as its reader is done with the one before
@@ -338,11 +340,14 @@ __global__ __launch_bounds__((64 * few_waves<T, DP>())) void attn_few_kernel(con
     __builtin_amdgcn_s_waitcnt(kLgkm0);   // the tile has been read
     if (t + W < t1) stage_k(t + W);
     float x[16];
+    if (a.cap > 0.f) {
+      float slope;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) x[r] = s[r] * s_scale;
-    if (a.cap > 0.f)
+      for (int r = 0; r < 16; ++r) x[r] = capped.score(s[r], capped.k3, slope);
+    } else {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = s_cap * attn_tanh<T>(x[r]);
+      for (int r = 0; r < 16; ++r) x[r] = s[r] * mult;
+    }
     if (a.table) {
       const int rel0 = k0 - (length - a.Nq);   // the first key from the first query
       if (rel0 - (a.Nq - 1) >= a.radius || rel0 + 31 <= -a.radius) {
@@ -455,27 +460,30 @@ __global__ __launch_bounds__((64 * few_waves<T, DP>())) void attn_few_kernel(con
   }
 }
 
-// A workgroup a row: wave w adds splits w, w + 4, ... in order, then the waves are added in order.  A split that saw
-// nothing wrote no values.  Lane d holds values d and 64 + d.
-template <class T>
+// The splits' parts of a row added: by one wave (many rows), or by a workgroup whose wave w takes splits w, w + 4, ...
+// (few rows of many splits; then the waves are added), in a fixed order.  A split that saw nothing wrote no values.
+// Lane d holds values d and 64 + d.
+template <class T, bool SPREAD>
 __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const AttnArgs a, Parts parts, int splits,
                                                                  T* __restrict__ out, T* __restrict__ lo,
                                                                  float* __restrict__ lse) {
   __shared__ float sh[4][3][64];
-  const int64_t rows = (int64_t)a.B * a.Nq * a.H, row = blockIdx.x;
+  constexpr int W = SPREAD ? 4 : 1;
   const int lane = threadIdx.x & 63, wave = wave_id();
+  const int64_t rows = (int64_t)a.B * a.Nq * a.H, row = SPREAD ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+  if (row >= rows) return;
   float top = -kInf;
   for (int s = lane; s < splits; s += 64) top = fmaxf(top, parts.ml[2 * (s * rows + row)]);
 #pragma unroll
   for (int m = 32; m > 0; m /= 2) top = fmaxf(top, __shfl_xor(top, m));
   const float to = top == -kInf ? 0.f : top;
-  float o0 = 0.f, o1 = 0.f, sum = 0.f;
+  float o[2] = {0.f, 0.f}, sum = 0.f;
   const int d0 = min(lane, a.D - 1), d1 = min(lane + 64, a.D - 1);
-  for (int s0 = wave; s0 < splits; s0 += 16) {
+  for (int s0 = SPREAD ? wave : 0; s0 < splits; s0 += 4 * W) {
     float f[4], l[4], x0[4], x1[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int s = s0 + 4 * q;
+      const int s = s0 + W * q;
       const int64_t at = (s < splits ? s : s0) * rows + row;
       f[q] = s < splits ? fast_exp2(parts.ml[2 * at] - to) : 0.f;
       l[q] = parts.ml[2 * at + 1];
@@ -484,26 +492,32 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const AttnArgs 
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      o0 += f[q] == 0.f ? 0.f : f[q] * x0[q];
-      o1 += f[q] == 0.f ? 0.f : f[q] * x1[q];
+      o[0] += f[q] == 0.f ? 0.f : f[q] * x0[q];
+      o[1] += f[q] == 0.f ? 0.f : f[q] * x1[q];
       sum += f[q] == 0.f ? 0.f : f[q] * l[q];
     }
   }
-  sh[wave][0][lane] = o0;
-  sh[wave][1][lane] = o1;
-  sh[wave][2][lane] = sum;
-  __syncthreads();
-  if (wave >= 2) return;
-  sum = (sh[0][2][lane] + sh[1][2][lane]) + (sh[2][2][lane] + sh[3][2][lane]);
+  if constexpr (SPREAD) {
+    sh[wave][0][lane] = o[0];
+    sh[wave][1][lane] = o[1];
+    sh[wave][2][lane] = sum;
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) o[h] = (sh[0][h][lane] + sh[1][h][lane]) + (sh[2][h][lane] + sh[3][h][lane]);
+    sum = (sh[0][2][lane] + sh[1][2][lane]) + (sh[2][2][lane] + sh[3][2][lane]);
+  }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int d = lane + 64 * wave;
-  if (d < a.D) {
-    const float v = ((sh[0][wave][lane] + sh[1][wave][lane]) + (sh[2][wave][lane] + sh[3][wave][lane])) * inv;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int d = lane + 64 * h;
+    if (d >= a.D) continue;
+    const float v = o[h] * inv;
     const T hi = (T)v;
     out[row * a.D + d] = hi;
     if (lo) lo[row * a.D + d] = (T)(v - (float)hi);
   }
-  if (lse && threadIdx.x == 0) {
+  if (lse && lane == 0) {
     const int64_t bi = row / a.H, h = row - bi * a.H, b = bi / a.Nq, i = bi - b * a.Nq;
     lse[(b * a.H + h) * a.Nq + i] = row_log_sum(to, sum);
   }
@@ -512,7 +526,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const AttnArgs 
 bool few_rows(const AttnArgs& a) { return a.Nq * a.G <= 32; }
 
 // Workgroups that the keys of a query block are split over.  Long rows: as many as bring the launch to two workgroups a
-// CU, 512 keys each at least.  Few rows: sequences of a cache are of unequal length, so up to sixteen a CU that even
+// CU, 256 keys each at least.  Few rows: sequences of a cache are of unequal length, so up to sixteen a CU that even
 // out, 512 keys each at least (8 sequences of 8200 to 32768 keys, 8 heads: 160 us in parts of 2048, XX in parts of
 // 512), and none for up to 1024 keys, where the join costs what the shorter walk gains (773 keys: 18 us in four parts,
 // 13 in one).
@@ -520,7 +534,7 @@ int key_splits(const AttnArgs& a) {
   const bool few = few_rows(a);
   if (few && a.Nk <= 1024) return 1;
   const int64_t base = few ? (int64_t)a.B * a.Hk : (int64_t)a.B * a.H * ((a.Nq + kGroupRows - 1) / kGroupRows);
-  const int64_t want = ((few ? 16 : 2) * (int64_t)compute_units() + base - 1) / base, most = (a.Nk + 511) / 512;
+  const int64_t want = ((few ? 16 : 2) * (int64_t)compute_units() + base - 1) / base, most = few ? (a.Nk + 511) / 512 : (a.Nk + 255) / 256;
   const int64_t s = want < most ? want : most;
   return s < 1 ? 1 : (int)s;
 }
@@ -546,13 +560,22 @@ int launch_fwd(const AttnArgs& a, void* o, void* o_lo, float* lse, void* ws, hip
     const int qblocks = (a.Nq + kGroupRows - 1) / kGroupRows;
     const int64_t total = (int64_t)a.B * a.H * splits * qblocks;
     KernelTimerScope timer("attn_fwd", stream);
-    attn_fwd_kernel<T, DP><<<dim3(attn_grid(total)), kAttnThreads, 0, stream>>>(a, out, lo, lse, parts, splits, qblocks,
-                                                                               (int)total);
+    const dim3 grid(attn_grid(total));
+    if (a.cap > 0.f)
+      attn_fwd_kernel<T, DP, true><<<grid, kAttnThreads, 0, stream>>>(a, out, lo, lse, parts, splits, qblocks, (int)total);
+    else
+      attn_fwd_kernel<T, DP, false><<<grid, kAttnThreads, 0, stream>>>(a, out, lo, lse, parts, splits, qblocks,
+                                                                      (int)total);
     if (const int rc = check_launch("attn_fwd")) return rc;
   }
   if (splits == 1) return BIOEMU_OK;
   KernelTimerScope timer("attn_join", stream);
-  attn_join_kernel<T><<<dim3((unsigned)rows), kAttnThreads, 0, stream>>>(a, parts, splits, out, lo, lse);
+  // 256 rows of 64 splits: 6 us spread, 10 not; 16000 rows of 2: 24 us spread
+  if (rows < 4 * compute_units() && splits > 4)
+    attn_join_kernel<T, true><<<dim3((unsigned)rows), kAttnThreads, 0, stream>>>(a, parts, splits, out, lo, lse);
+  else
+    attn_join_kernel<T, false><<<dim3((unsigned)((rows + 3) / 4)), kAttnThreads, 0, stream>>>(a, parts, splits, out, lo,
+                                                                                              lse);
   return check_launch("attn_join");
 }
 
@@ -569,7 +592,7 @@ int attn_args(const char* what, const bioemu_attention_args* in, AttnArgs* a) {
     return set_error(BIOEMU_ERR_UNSUPPORTED, "%s: head width %ld (a multiple of 8, at most 128)", what, (long)D);
   const int64_t most = int64_t(1) << 27;
   if (Nq > most || Nk > most || B * H > (1 << 20) || B * Nq * H >= (int64_t(1) << 31) ||
-      B * H * ((Nq + 127) / 128) * 512 >= (int64_t(1) << 31) || B * H * ((Nk + 127) / 128) >= (int64_t(1) << 31))
+      B * H * ((Nq + 127) / 128) * 512 >= (int64_t(1) << 31) || B * H * ((Nk + 127) / 128) * 32 >= (int64_t(1) << 31))
     return set_error(BIOEMU_ERR_UNSUPPORTED, "%s: B=%ld, H=%ld, Nq=%ld, Nk=%ld are too many", what, (long)B, (long)H,
                      (long)Nq, (long)Nk);
   if (!(in->scale > -kInf && in->scale < kInf) || !(in->cap >= 0.f && in->cap < kInf))

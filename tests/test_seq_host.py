@@ -114,7 +114,7 @@ def test_attention_c_abi_workspace_and_outputs():
     assert lib.bioemu_attention_bwd(args, 16, None, 16, 16, strides, 16, 16, 16, None, None, 0, None) == -3
     assert lib.bioemu_attention_bwd(args, 16, None, 16, 16, strides, 16, 16, None, None, 16, 1 << 20, None) == -1
     assert lib.bioemu_attention_bwd(args, 16, None, 16, 16, strides, 16, 16, 16, 16, 16, 1 << 20, None) == -1   # no table
-    assert lib.bioemu_attention_bwd_workspace_bytes(args, 0) == 256   # 1 x 2 x 4 row sums, rounded up
+    assert lib.bioemu_attention_bwd_workspace_bytes(args, 0) == 256   # 2 x 1 x 2 x 4 row values, rounded up
 
 
 def test_attention_rejects_cpu_tensors():
