@@ -285,11 +285,32 @@ __device__ __forceinline__ bool all_far(const AttnArgs& a, int rel0) {
   return rel0 - 31 >= a.radius || rel0 + 31 <= -a.radius;
 }
 
-// Blocks of a segment list that can hold an allowed pair.  An entry is the block's number with two flags.
-constexpr int kBlockMask = 0x0fffffff, kEntryFull = 0x10000000, kEntryHoles = 0x20000000;
+// The range of the segments of a wave's rows (low above high: none), against the segments of a staged tile.
+struct WaveRange {
+  int lo, hi;
+  __device__ __forceinline__ WaveRange(int low, int high) {
+#pragma unroll
+    for (int m = 32; m > 0; m /= 2) {
+      low = min(low, __shfl_xor(low, m));
+      high = max(high, __shfl_xor(high, m));
+    }
+    lo = __builtin_amdgcn_readfirstlane(low);
+    hi = __builtin_amdgcn_readfirstlane(high);
+  }
+  // Whether some of the tile's N rows is of a segment in the range; `all`: all of them are of the only one.
+  template <int N>
+  __device__ __forceinline__ bool meets(const int* tile, int lane, bool& all) const {
+    const int s = tile[lane & (N - 1)];
+    all = lo == hi && __ballot(s != lo) == 0;
+    return __ballot(s >= lo && s <= hi) != 0;
+  }
+};
+
+// Blocks of a segment list that can hold an allowed pair.  An entry is the block's number with a flag.
+constexpr int kBlockMask = 0x0fffffff, kEntryHoles = 0x20000000;
 
 // Lists the blocks [c0, c1) of BLOCK rows of `seg` (`n` of them exist) that hold a segment in [lo, hi], in order;
-// full: every row has segment `lo` == `hi`; holes: some row exists in no segment (or past n).  All 256 threads;
+// holes: some row is of no segment (or past n).  All 256 threads;
 // returns the entries.  flags: one byte a block, list: one int a block.
 template <int BLOCK>
 __device__ __forceinline__ int list_blocks(const int* __restrict__ seg, int n, int lo, int hi, int c0, int c1,
@@ -307,14 +328,12 @@ __device__ __forceinline__ int list_blocks(const int* __restrict__ seg, int n, i
 #pragma unroll
    for (int q = 0; q < AHEAD; ++q) {
     const int b0 = b8 + 4 * PER * q, s = got[q];
-    const uint64_t hit = __ballot(s >= 0 && s >= lo && s <= hi), one = __ballot(lo == hi && s == lo),
-                   hole = __ballot(s < 0);
+    const uint64_t hit = __ballot(s >= 0 && s >= lo && s <= hi), hole = __ballot(s < 0);
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
       const uint64_t m = BLOCK == 64 ? ~0ull : (uint64_t)0xffffffffu << (32 * p);
       if (lane == 0 && b0 + p < c1)
-        flags[b0 + p - c0] =
-            (uint8_t)(((hit & m) != 0 ? 1 : 0) | ((one & m) == m ? 2 : 0) | ((hole & m) != 0 ? 4 : 0));
+        flags[b0 + p - c0] = (uint8_t)(((hit & m) != 0 ? 1 : 0) | ((hole & m) != 0 ? 2 : 0));
     }
    }
   }
@@ -325,8 +344,7 @@ __device__ __forceinline__ int list_blocks(const int* __restrict__ seg, int n, i
       const int f = b0 + lane < c1 - c0 ? flags[b0 + lane] : 0;
       const uint64_t m = __ballot(f & 1);
       if (f & 1)
-        list[at + __popcll(m & ((1ull << lane) - 1))] =
-            (c0 + b0 + lane) | (f & 2 ? kEntryFull : 0) | (f & 4 ? kEntryHoles : 0);
+        list[at + __popcll(m & ((1ull << lane) - 1))] = (c0 + b0 + lane) | (f & 2 ? kEntryHoles : 0);
       at += __popcll(m);
     }
     if (lane == 0) *count = at;

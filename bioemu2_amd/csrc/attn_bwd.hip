@@ -53,8 +53,15 @@ __device__ __forceinline__ void store_rows(const f32x16 (&acc)[DB], float scale,
     }
 }
 
+// Waves per SIMD that the registers have to allow: two where a few registers more would make it one (attn_bwd_kv at
+// D = 64, 2 x 2048 causal tokens: 107 us with 257 registers, 87 with 255).
+template <class T, int DP, bool KV>
+constexpr int bwd_waves() {
+  return sizeof(T) == 2 && KV && DP == 64 ? 2 : 1;
+}
+
 template <class T, int DP, bool CAP>
-__global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs a, const T* __restrict__ o,
+__global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void attn_bwd_q_kernel(const AttnArgs a, const T* __restrict__ o,
                                                                   const T* __restrict__ o_lo,
                                                                   const float* __restrict__ lse,
                                                                   const T* __restrict__ dout, int64_t db, int64_t dn,
@@ -93,6 +100,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
   int lim = a.causal ? min(max(pos + 1, prefix), length) : length;
   if (qseg < 0 || !live) lim = 0;
   int seg_lo = live && qseg >= 0 ? qseg : 0x7fffffff, seg_hi = live ? qseg : -1, wg_max = lim;
+  const WaveRange own_segs(seg_lo, seg_hi);
   wg_extremes(seg_lo, seg_hi, wg_max, red);
   int wave_min = lim, wave_max = lim;
 #pragma unroll
@@ -171,7 +179,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
   for (int c0 = 0; c0 < blocks; c0 += kListBlocks) {
     const int c1 = seg ? min(blocks, c0 + kListBlocks) : blocks;
     const int n = seg ? list_blocks<KB>(kseg, length, seg_lo, seg_hi, c0, c1, flags, list, &count) : blocks;
-    auto entry = [&](int t) { return seg ? __builtin_amdgcn_readfirstlane(list[t]) : t | kEntryFull; };
+    auto entry = [&](int t) { return seg ? __builtin_amdgcn_readfirstlane(list[t]) : t; };
     const int t0 = (int)((int64_t)n * split / splits), t1 = (int)((int64_t)n * (split + 1) / splits);
     if (t0 < t1) stage(entry(t0), t0 & 1);
     for (int t = t0; t < t1; ++t) {
@@ -188,6 +196,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
         __syncthreads();
       }
       if (k0 >= wave_max) continue;
+      bool all = true;   // every key has the one segment of all queries of this wave
+      if (seg && !own_segs.meets<KB>(segs[buf], lane, all)) continue;
       const char *kt = tiles[buf][0], *vt = tiles[buf][1];
 #pragma unroll 1
       for (int u = 0; u < SUB; ++u) {
@@ -215,7 +225,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
         if (k0 + KB > wave_min)
 #pragma unroll
           for (int r = 0; r < 16; ++r) x[r] = k0 + 32 * u + 8 * (r >> 2) + 4 * lh + (r & 3) < lim ? x[r] : 0.f;
-        if (!(e & kEntryFull))
+        if (!all)
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const int4 ks = *reinterpret_cast<const int4*>(&segs[buf][32 * u + 8 * q + 4 * lh]);
@@ -305,7 +315,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(const AttnArgs
 }
 
 template <class T, int DP, bool CAP>
-__global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArgs a, const float* __restrict__ row_stats,
+__global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, true>())) void attn_bwd_kv_kernel(const AttnArgs a, const float* __restrict__ row_stats,
                                                                    const T* __restrict__ dout, int64_t db, int64_t dn,
                                                                    int64_t dh,
                                                                    T* __restrict__ dk, T* __restrict__ dv,
@@ -338,6 +348,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArg
   // queries from imin on see this key (their segment aside)
   const int imin = !on ? 0x7fffffff : (a.causal && j >= prefix ? max(j - first, 0) : 0);
   int seg_lo = on ? kseg : 0x7fffffff, seg_hi = on ? kseg : -1, wg_min = -imin;
+  const WaveRange own_segs(seg_lo, seg_hi);
   wg_extremes(seg_lo, seg_hi, wg_min, red);
   wg_min = -wg_min;
   int wave_min = imin, wave_max = imin;
@@ -390,7 +401,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArg
   for (int c0 = first_block; c0 < blocks; c0 += kListBlocks) {
     const int c1 = seg ? min(blocks, c0 + kListBlocks) : blocks;
     const int n = seg ? list_blocks<QB>(qseg, a.Nq, seg_lo, seg_hi, c0, c1, flags, list, &count) : blocks - c0;
-    auto entry = [&](int t) { return seg ? __builtin_amdgcn_readfirstlane(list[t]) : (c0 + t) | kEntryFull; };
+    auto entry = [&](int t) { return seg ? __builtin_amdgcn_readfirstlane(list[t]) : c0 + t; };
     // the blocks of all heads of the group, one after the other, are dealt to the splits
     const int64_t all = (int64_t)n * a.G;
     const int64_t w0 = all * split / splits, w1 = all * (split + 1) / splits;
@@ -417,6 +428,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArg
           __syncthreads();
         }
         if (i0 + QB <= wave_min) continue;
+        bool all_same = true;
+        if (seg && !own_segs.meets<QB>(segs[buf], lane, all_same)) continue;
         const char *qt = tiles[buf][0], *dt = tiles[buf][1];
 #pragma unroll 1
         for (int u = 0; u < SUB; ++u) {
@@ -457,7 +470,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(const AttnArg
 #pragma unroll
             for (int r = 0; r < 16; ++r)
               x[r] = i0 + 32 * u + 8 * (r >> 2) + 4 * lh + (r & 3) >= imin ? x[r] : 0.f;
-          if (!(e & kEntryFull))
+          if (!all_same)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
               const int4 qs = *reinterpret_cast<const int4*>(&segs[buf][32 * u + 8 * q + 4 * lh]);

@@ -75,6 +75,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
   int lim = a.causal ? min(max(pos + 1, prefix), length) : length;
   if (qseg < 0) lim = 0;
   int seg_lo = live && qseg >= 0 ? qseg : 0x7fffffff, seg_hi = live ? qseg : -1, wg_max = live ? lim : 0;
+  const WaveRange own_segs(seg_lo, seg_hi);
   wg_extremes(seg_lo, seg_hi, wg_max, red);
   int wave_min = live ? lim : 0x7fffffff, wave_max = live ? lim : 0;
 #pragma unroll
@@ -127,7 +128,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
     const int c1 = seg ? min(blocks, c0 + kListBlocks) : blocks;
     const int n = seg ? list_blocks<KB>(kseg, length, seg_lo, seg_hi, c0, c1, flags, list, &count) : blocks;
     const int t0 = (int)((int64_t)n * split / splits), t1 = (int)((int64_t)n * (split + 1) / splits);
-    auto entry = [&](int t) { return seg ? __builtin_amdgcn_readfirstlane(list[t]) : t | kEntryFull; };
+    auto entry = [&](int t) { return seg ? __builtin_amdgcn_readfirstlane(list[t]) : t; };
     if (t0 < t1) stage(entry(t0), t0 & 1);
     for (int t = t0; t < t1; ++t) {
       const int e = entry(t), buf = t & 1, k0 = (e & kBlockMask) * KB;
@@ -141,6 +142,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
         __syncthreads();
       }
       if (k0 >= wave_max) continue;
+      bool all = true;   // every key has the one segment of all queries of this wave
+      if (seg && !own_segs.meets<KB>(segs[buf], lane, all)) continue;
       const char *kt = tiles[buf][0], *vt = tiles[buf][1];
       float x[SUB][16];
 #pragma unroll
@@ -165,7 +168,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             x[u][r] = k0 + 32 * u + 8 * (r >> 2) + 4 * lh + (r & 3) < lim ? x[u][r] : -kInf;
-      if (!(e & kEntryFull))
+      if (!all)
 #pragma unroll
         for (int u = 0; u < SUB; ++u)
 #pragma unroll
