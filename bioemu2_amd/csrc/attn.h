@@ -372,6 +372,9 @@ __device__ __forceinline__ int attn_item(int total, int cols) {
 }
 inline unsigned attn_grid(int64_t total) { return (unsigned)(round_up(total, kAttnXcds)); }
 
+// Compute units of the current device, remembered.
+int attn_units();
+
 // Checks the arguments both directions share and lays them out (attn_fwd.hip).
 int attn_args(const char* what, const bioemu_attention_args* in, AttnArgs* out);
 

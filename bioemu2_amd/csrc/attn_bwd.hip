@@ -9,7 +9,7 @@
 // are so computed twice, 7 products instead of 5; adding dq over workgroups instead would need fp32 atomics (an order
 // that changes results) or as many copies of dq.
 //
-// Either may split its walk over workgroups where the rows alone do not fill the chip; attn_bwd_join adds the parts.
+// Either may split its walk over workgroups where the rows alone do not fill the chip; attn_bwd_finish adds the parts.
 //
 // The table's gradient sums ds along the diagonals of every 32 x 32 block that meets the radius: the block goes to LDS,
 // rows 68 values apart with zeros between them, and lane e reads its diagonal (value e + n - 31 of row n) without a
@@ -520,14 +520,45 @@ struct JoinOne {
 struct JoinArgs {
   JoinOne of[3];
 };
+// The table's gradient: dtable[k] = sum over the query blocks' parts of part[g][k] (size 0: none).
+struct BiasSum {
+  const float* part;
+  void* dtable;
+  int groups, size, table_bf16;
+};
+// What is left after both walks, in one launch: workgroups from bias_groups on join, the others sum 16 values of the
+// table's gradient each, in 16 slices of the parts.
 template <class T>
-__global__ __launch_bounds__(kAttnThreads) void attn_bwd_join_kernel(const JoinArgs j) {
-  int64_t at = ((int64_t)blockIdx.x * kAttnThreads + threadIdx.x) * 4;
+__global__ __launch_bounds__(kAttnThreads) void attn_bwd_finish_kernel(const JoinArgs j, const BiasSum bias,
+                                                                       int bias_groups) {
+  if ((int)blockIdx.x < bias_groups) {
+    __shared__ float sh[16][17];
+    const int k = blockIdx.x * 16 + (threadIdx.x & 15), slice = threadIdx.x >> 4;
+    float s = 0.f;
+    if (k < bias.size)
+#pragma unroll 8
+      for (int g = slice; g < bias.groups; g += 16) s += bias.part[(int64_t)g * bias.size + k];
+    sh[slice][threadIdx.x & 15] = s;
+    __syncthreads();
+    for (int m = 8; m > 0; m /= 2) {
+      if (slice < m) sh[slice][threadIdx.x & 15] += sh[slice + m][threadIdx.x & 15];
+      __syncthreads();
+    }
+    if (slice == 0 && k < bias.size) {
+      if (bias.table_bf16)
+        static_cast<bf16*>(bias.dtable)[k] = (bf16)sh[0][threadIdx.x];
+      else
+        static_cast<float*>(bias.dtable)[k] = sh[0][threadIdx.x];
+    }
+    return;
+  }
+  int64_t at = ((int64_t)(blockIdx.x - bias_groups) * kAttnThreads + threadIdx.x) * 4;
 #pragma unroll
   for (int w = 0; w < 3; ++w) {
     const JoinOne& o = j.of[w];
     if (at >= 0 && at < o.n) {
       f32x4 v = *reinterpret_cast<const f32x4*>(o.part + at);
+#pragma unroll 4
       for (int s = 1; s < o.splits; ++s) {
         const f32x4 x = *reinterpret_cast<const f32x4*>(o.part + s * o.n + at);
 #pragma unroll
@@ -543,33 +574,11 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_join_kernel(const JoinA
   }
 }
 
-// dtable[k] = sum over the query blocks' parts of part[g][k].  One workgroup: 16 values x 64 slices of the parts.
-__global__ __launch_bounds__(1024) void attn_bias_reduce_kernel(const float* __restrict__ part, int groups, int size,
-                                                                void* __restrict__ dtable, int table_bf16) {
-  __shared__ float sh[64][17];
-  const int k = blockIdx.x * 16 + (threadIdx.x & 15), slice = threadIdx.x >> 4;
-  float s = 0.f;
-  if (k < size)
-#pragma unroll 4
-    for (int g = slice; g < groups; g += 64) s += part[(int64_t)g * size + k];
-  sh[slice][threadIdx.x & 15] = s;
-  __syncthreads();
-  for (int m = 32; m > 0; m /= 2) {
-    if (slice < m) sh[slice][threadIdx.x & 15] += sh[slice + m][threadIdx.x & 15];
-    __syncthreads();
-  }
-  if (slice == 0 && k < size) {
-    if (table_bf16)
-      static_cast<bf16*>(dtable)[k] = (bf16)sh[0][threadIdx.x];
-    else
-      static_cast<float*>(dtable)[k] = sh[0][threadIdx.x];
-  }
-}
-
-// Workgroups that a row block's walk is split over: as many as bring the launch to two workgroups a CU, each with at
-// least two blocks of the walk.
+// Workgroups that a row block's walk is split over: as many as bring the launch to two workgroups a CU (four: no
+// shorter, and the join twice as long), each with at least two blocks of the walk (fp32, 2 x 200 tokens of 16 heads: 21
+// and 15 us in three parts, 29 and 24 whole).
 int walk_splits(int64_t groups, int64_t walk, int block) {
-  const int64_t want = (2 * (int64_t)compute_units() + groups - 1) / groups, most = walk / (2 * block);
+  const int64_t want = (2 * (int64_t)attn_units() + groups - 1) / groups, most = walk / (2 * block);
   const int64_t s = want < most ? want : most;
   return s < 1 ? 1 : (int)(s < 16 ? s : 16);
 }
@@ -618,23 +627,18 @@ int launch_bwd_as(const AttnArgs& a, const void* o, const void* o_lo, const floa
         kv_part, sp.kv_splits, kblocks, (int)total);
     if (const int rc = check_launch("attn_bwd_kv")) return rc;
   }
-  if (sp.q_splits > 1 || sp.kv_splits > 1) {
-    const int64_t nq = sp.q_splits > 1 ? (int64_t)a.B * a.Nq * a.H * a.D : 0;
-    const int64_t nk = sp.kv_splits > 1 ? (int64_t)a.B * a.Nk * a.Hk * a.D : 0;
-    const JoinArgs join{{{q_part, dq, nq, sp.q_splits},
-                         {kv_part, dk, nk, sp.kv_splits},
-                         {kv_part + sp.kv_splits * nk, dv, nk, sp.kv_splits}}};
-    KernelTimerScope timer("attn_bwd_join", stream);
-    const int64_t groups = (nq + 2 * nk + 4 * kAttnThreads - 1) / (4 * kAttnThreads);
-    attn_bwd_join_kernel<T><<<dim3((unsigned)groups), kAttnThreads, 0, stream>>>(join);
-    if (const int rc = check_launch("attn_bwd_join")) return rc;
-  }
-  if (!dtable) return BIOEMU_OK;
-  KernelTimerScope timer("attn_bias_reduce", stream);
-  const int size = a.nb * a.H;
-  attn_bias_reduce_kernel<<<dim3((unsigned)((size + 15) / 16)), 1024, 0, stream>>>(bias, a.B * qblocks * sp.q_splits,
-                                                                                  size, dtable, a.table_bf16);
-  return check_launch("attn_bias_reduce");
+  const int64_t nq = sp.q_splits > 1 ? (int64_t)a.B * a.Nq * a.H * a.D : 0;
+  const int64_t nk = sp.kv_splits > 1 ? (int64_t)a.B * a.Nk * a.Hk * a.D : 0;
+  const BiasSum sum{bias, dtable, a.B * qblocks * sp.q_splits, dtable ? a.nb * a.H : 0, a.table_bf16};
+  const int64_t bias_groups = (sum.size + 15) / 16;
+  const int64_t groups = bias_groups + (nq + 2 * nk + 4 * kAttnThreads - 1) / (4 * kAttnThreads);
+  if (groups == 0) return BIOEMU_OK;
+  const JoinArgs join{{{q_part, dq, nq, sp.q_splits},
+                       {kv_part, dk, nk, sp.kv_splits},
+                       {kv_part + sp.kv_splits * nk, dv, nk, sp.kv_splits}}};
+  KernelTimerScope timer("attn_bwd_finish", stream);
+  attn_bwd_finish_kernel<T><<<dim3((unsigned)groups), kAttnThreads, 0, stream>>>(join, sum, (int)bias_groups);
+  return check_launch("attn_bwd_finish");
 }
 
 template <class T, int DP>

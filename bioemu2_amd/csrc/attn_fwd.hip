@@ -12,6 +12,8 @@
 // A training call in bf16 also writes what the rounding of o took off (o_lo): the backward pass needs do . o, and with
 // it from o + o_lo the error of dq and dk falls from 1.50 to 1.46 times what rounding their results alone gives (the
 // rest is the rounding of the probabilities and of ds to the operands of the products).
+#include <atomic>
+
 #include "attn.h"
 
 namespace bioemu {
@@ -537,7 +539,7 @@ int key_splits(const AttnArgs& a) {
   const bool few = few_rows(a);
   if (few && a.Nk <= 1024) return 1;
   const int64_t base = few ? (int64_t)a.B * a.Hk : (int64_t)a.B * a.H * ((a.Nq + kGroupRows - 1) / kGroupRows);
-  const int64_t want = ((few ? 16 : 2) * (int64_t)compute_units() + base - 1) / base, most = few ? (a.Nk + 511) / 512 : (a.Nk + 255) / 256;
+  const int64_t want = ((few ? 16 : 2) * (int64_t)attn_units() + base - 1) / base, most = few ? (a.Nk + 511) / 512 : (a.Nk + 255) / 256;
   const int64_t s = want < most ? want : most;
   return s < 1 ? 1 : (int)s;
 }
@@ -574,7 +576,7 @@ int launch_fwd(const AttnArgs& a, void* o, void* o_lo, float* lse, void* ws, hip
   if (splits == 1) return BIOEMU_OK;
   KernelTimerScope timer("attn_join", stream);
   // 256 rows of 64 splits: 6 us spread, 10 not; 16000 rows of 2: 24 us spread
-  if (rows < 4 * compute_units() && splits > 4)
+  if (rows < 4 * attn_units() && splits > 4)
     attn_join_kernel<T, true><<<dim3((unsigned)rows), kAttnThreads, 0, stream>>>(a, parts, splits, out, lo, lse);
   else
     attn_join_kernel<T, false><<<dim3((unsigned)((rows + 3) / 4)), kAttnThreads, 0, stream>>>(a, parts, splits, out, lo,
@@ -583,6 +585,16 @@ int launch_fwd(const AttnArgs& a, void* o, void* o_lo, float* lse, void* ws, hip
 }
 
 }  // namespace
+
+int attn_units() {
+  // asking the runtime takes microseconds, as long as a launch
+  static std::atomic<int> units[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return compute_units();
+  int n = units[dev].load(std::memory_order_relaxed);
+  if (n == 0) units[dev].store(n = compute_units(), std::memory_order_relaxed);
+  return n;
+}
 
 int attn_args(const char* what, const bioemu_attention_args* in, AttnArgs* a) {
   if (!in) return set_error(BIOEMU_ERR_INVALID_ARG, "%s: null arguments", what);
