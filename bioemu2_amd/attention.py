@@ -51,7 +51,7 @@ def attention(
     segments ([B, Nq] whole numbers): a query sees keys of its own segment only, and a negative one (padding) neither
     sees nor is seen, whatever it holds; key_segments ([B, Nk]) where the keys are others.  Values that a query does
     not see for another reason have to be finite.
-    causal: only keys j <= p_i, and those below ``prefix[b]``."""
+    causal: only keys j <= p_i, and those below ``prefix[b]`` ([B] whole numbers; nothing to say without causal)."""
     _ops.require_gpu(q, "attention")
     if q.ndim != 4:
         raise ValueError(f"attention: q must be [B, Nq, H, D], got {tuple(q.shape)}")
@@ -64,8 +64,6 @@ def attention(
         segments = _int32(segments, "attention segments")
         key_segments = segments if same else _int32(key_segments, "attention key segments")
     if prefix is not None:
-        if not causal:
-            raise ValueError("attention: a prefix needs causal=True")
         prefix = _int32(prefix, "attention prefix")
     if cache_lengths is not None:
         cache_lengths = _int32(cache_lengths, "attention cache_lengths")

@@ -159,13 +159,15 @@ __global__ __launch_bounds__(kThreads) void norm_fwd_kernel(const T* __restrict_
   }
 }
 
-// part: NULL or [gridDim.x][2][c] fp32, this workgroup's sums of dy * xh and of dy.
+// part: NULL or [gridDim.x][2][c] fp32, this workgroup's sums of dy * xh and of dy.  A launch of one workgroup writes
+// them where they belong instead (dweight, dbias; either may be NULL).
 template <class T, int VEC, int LPR, int VPL>
 __global__ __launch_bounds__(kThreads) void norm_bwd_kernel(const T* __restrict__ x, int64_t ldx,
                                                             const T* __restrict__ dy, int64_t ldy,
                                                             const float* __restrict__ stats,
                                                             const void* __restrict__ w, int w_bf16,
                                                             T* __restrict__ dx, float* __restrict__ part,
+                                                            void* __restrict__ dweight, void* __restrict__ dbias,
                                                             int64_t rows, int c) {
   constexpr int E = VEC * VPL, RPG = kThreads / LPR, U = kRowsAtOnce<LPR, E>;
   __shared__ float sh[2][4];
@@ -230,8 +232,19 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_kernel(const T* __restrict_
     }
     if constexpr (LPR > 64) __syncthreads();
   }
-  if (part == nullptr) return;
-  float* out = part + (int64_t)blockIdx.x * 2 * c;
+  if (part == nullptr && dweight == nullptr && dbias == nullptr) return;
+  const auto put = [&](int which, int k, float v) {
+    if (part) {
+      part[((int64_t)blockIdx.x * 2 + which) * c + k] = v;
+      return;
+    }
+    void* out = which ? dbias : dweight;
+    if (out == nullptr) return;
+    if (w_bf16)
+      static_cast<bf16*>(out)[k] = (bf16)v;
+    else
+      static_cast<float*>(out)[k] = v;
+  };
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     const float* src = which ? db : dw;
@@ -245,13 +258,13 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_kernel(const T* __restrict_
         float s = 0.f;
 #pragma unroll
         for (int q = 0; q < RPG; ++q) s += acc[q * (LPR * E) + k];
-        out[which * c + k] = s;
+        put(which, k, s);
       }
     } else {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const int k = (e / VEC * LPR + lane) * VEC + e % VEC;
-        if (k < c) out[which * c + k] = src[e];
+        if (k < c) put(which, k, src[e]);
       }
     }
   }
@@ -345,16 +358,18 @@ int launch_bwd(const void* x, int64_t ldx, const void* dy, int64_t ldy, const fl
                void* dx, void* dw, void* db, void* ws, int64_t rows, int64_t c, bool vec, hipStream_t stream) {
   constexpr bool f32 = sizeof(T) == 4;
   constexpr int VW = f32 ? 4 : 8;
-  float* part = dw != nullptr || db != nullptr ? static_cast<float*>(ws) : nullptr;
   return for_width(f32, vec, c, [&](int vw, int lpr, int vpl) {
-    const dim3 grid(row_groups(rows, lpr, vw * vpl, kMaxBwdGroups));
+    dim3 grid(row_groups(rows, lpr, vw * vpl, kMaxBwdGroups));
+    if (grid.x <= 4) grid.x = 1;   // four turns of one workgroup take less than the second launch
+    const bool weights = dw != nullptr || db != nullptr;
+    float* part = weights && grid.x > 1 ? static_cast<float*>(ws) : nullptr;
     {
       KernelTimerScope timer("norm_bwd", stream);
 #define BIOEMU_CASE(V, L, P)                                                                                        \
   if (vw == V && lpr == L && vpl == P)                                                                              \
     norm_bwd_kernel<T, V, L, P><<<grid, kThreads, 0, stream>>>(static_cast<const T*>(x), ldx,                       \
                                                                static_cast<const T*>(dy), ldy, stats, w, w_bf16,    \
-                                                               static_cast<T*>(dx), part, rows, (int)c);
+                                                               static_cast<T*>(dx), part, dw, db, rows, (int)c);
       BIOEMU_WIDTHS(VW)
       BIOEMU_WIDTHS(1)
 #undef BIOEMU_CASE

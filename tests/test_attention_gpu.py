@@ -343,6 +343,12 @@ def test_fp32_under_autocast_and_mixed_table(gpu_device):
     check(low.step(), low.exact())
 
 
+def test_prefix_without_a_causal_mask_changes_nothing(gpu_device):
+    c = Case(gpu_device, BF16, B=2, Nq=80, H=2, D=32)
+    want = c.call()
+    assert torch.equal(c.call(prefix=torch.tensor([7, 0], device=gpu_device)), want)
+
+
 @pytest.mark.parametrize("kw", [dict(B=1, Nq=400, H=2, D=64, radius=64, segments=packed(1, 400, [150, 200])),
                                 dict(B=2, Nq=1, Nk=3000, H=8, Hk=2, D=64, causal=True, lengths=[3000, 1200])],
                          ids=["packed", "token"])
@@ -501,7 +507,7 @@ def test_refusals(gpu_device):
         (dict(q=torch.zeros(1, 2, 1, 136, device=gpu_device), k=torch.zeros(1, 2, 1, 136, device=gpu_device),
               v=torch.zeros(1, 2, 1, 136, device=gpu_device)), "multiple of 8"),
         (dict(segments=seg[:, :5]), "shape"), (dict(segments=seg.float()), "whole numbers"),
-        (dict(key_segments=seg), "come together"), (dict(prefix=one), "causal"),
+        (dict(key_segments=seg), "come together"),
         (dict(prefix=one[:1], causal=True), "shape"), (dict(cache_lengths=one[:1]), "shape"), (dict(cap=0.0), "cap"),
         (dict(cap=float("inf")), "cap"), (dict(scale=float("nan")), "scale"),
         (dict(bias_table=c.table), "buckets"), (dict(bias_buckets=c.buckets), "buckets"),
