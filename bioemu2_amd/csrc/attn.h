@@ -11,7 +11,7 @@
 // Scores are kept transposed to the operand that follows: a 32 x 32 accumulator (lane n = column, register 4 r + c =
 // row 8 r + 4 h + c) is, register for register, the B operand of the next product whose reduced index is its rows in
 // the order kappa(h, t) = 4 h + t, 8 + 4 h + t - 4; the A operand of that product comes out of LDS in that order by the
-// transposing 8-byte read (bf16) or by single reads (fp32).  So probabilities never leave registers.
+// transposing 8-byte read (or by single reads where fp32 lies unsplit).  So probabilities never leave registers.
 //
 // Tiles (rows of DP values, DP = 32, 64 or 128 >= D) go global -> LDS by buffer loads that write LDS.  Bytes past D and
 // rows past the end read as zero through the buffer bound, so no lane reads outside its tensor.  16-byte pieces are
@@ -73,8 +73,7 @@ __device__ __forceinline__ Parts3 parts3(f32x8 x) {
   }
   return p;
 }
-__device__ __forceinline__ f32x16 mfma16(f32x8 a, f32x8 b, f32x16 c) {
-  const Parts3 x = parts3(a), y = parts3(b);
+__device__ __forceinline__ f32x16 mfma16(const Parts3& x, const Parts3& y, f32x16 c) {
   c = mfma32(x.mid, y.mid, c);
   c = mfma32(x.lo, y.hi, c);
   c = mfma32(x.hi, y.lo, c);
@@ -82,6 +81,8 @@ __device__ __forceinline__ f32x16 mfma16(f32x8 a, f32x8 b, f32x16 c) {
   c = mfma32(x.hi, y.mid, c);
   return mfma32(x.hi, y.hi, c);
 }
+__device__ __forceinline__ f32x16 mfma16(const Parts3& x, f32x8 y, f32x16 c) { return mfma16(x, parts3(y), c); }
+__device__ __forceinline__ f32x16 mfma16(f32x8 x, f32x8 y, f32x16 c) { return mfma16(parts3(x), parts3(y), c); }
 
 // Copies from memory into LDS: lane i's BYTES at byte voff of the source go to lds + BYTES i; zeros past its end.
 // Written as instructions: the compiler lets every later LDS read wait for a copy that it knows of, and these are to
@@ -176,6 +177,75 @@ struct Tile {
   // Zeroes row r (whoever calls owns the row's 16-byte pieces first, first + step, ...).
   __device__ static __forceinline__ void clear(char* lds, int r, int first, int step) {
     for (int c = first; c < CPR; c += step) *reinterpret_cast<u32x4*>(lds + piece(r, c)) = u32x4{0, 0, 0, 0};
+  }
+};
+
+// A tile that the waves of a workgroup share, as they read it.  bf16: the tile above, copied while the one before it is
+// worked on (two buffers).  fp32: its three bf16 parts in a plane each, split once by the thread that fetched the values
+// into registers (else every wave splits every operand it reads: 1000 x 1000 tokens, 8 heads of 64, forward / q / kv
+// 30 / 48 / 57 us, so 25 / 40 / 46); one buffer, filled between two barriers.
+template <class T, int DP, int ROWS>
+struct Staged;
+template <int DP, int ROWS>
+struct Staged<bf16, DP, ROWS> : Tile<bf16, DP, ROWS> {
+  typedef Tile<bf16, DP, ROWS> Base;
+  static constexpr int BUFFERS = 2, N = Base::copies(kAttnThreads);
+  unsigned off[N];
+  __device__ __forceinline__ Staged(int64_t stride, int D) { Base::offsets(threadIdx.x, kAttnThreads, stride, D, off); }
+  __device__ __forceinline__ void fetch(const bf16* base, int rows, int64_t stride, int D, char* lds, int wave) {
+    Base::copy(base, rows, stride, D, lds, wave, kAttnThreads, off);
+  }
+  __device__ __forceinline__ void store(char*) const {}
+};
+template <int DP, int ROWS>
+struct Staged<float, DP, ROWS> {
+  typedef Tile<bf16, DP, ROWS> Plane;
+  static constexpr int BUFFERS = 1, BYTES = 3 * Plane::BYTES, PER = DP / 4, N = ROWS * PER / kAttnThreads;
+  unsigned off[N];
+  f32x4 v[N];
+  // thread t holds the 16-byte pieces t, t + 256, ... of the rows
+  __device__ __forceinline__ Staged(int64_t stride, int D) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int p = i * kAttnThreads + threadIdx.x, r = p / PER, c = p % PER;
+      off[i] = c * 4 < D ? (unsigned)(r * stride * 4) + c * 16 : 0xfffffff0u;
+    }
+  }
+  __device__ __forceinline__ void fetch(const float* base, int rows, int64_t stride, int D, char*, int) {
+    const int n = rows < ROWS ? rows : ROWS;
+    const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(base, n <= 0 ? 0 : (unsigned)(((n - 1) * stride + D) * 4));
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off[i], 0, 0));
+  }
+  __device__ __forceinline__ void store(char* lds) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int p = i * kAttnThreads + threadIdx.x, r = p / PER, c = p % PER;
+      bf16x4 part[3];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = v[i][e];
+        part[0][e] = (bf16)x;
+        const float r1 = x - (float)part[0][e];
+        part[1][e] = (bf16)r1;
+        part[2][e] = (bf16)(r1 - (float)part[1][e]);
+      }
+      char* at = lds + Plane::piece(r, c >> 1) + (c & 1) * 8;
+#pragma unroll
+      for (int q = 0; q < 3; ++q) *reinterpret_cast<bf16x4*>(at + q * Plane::BYTES) = part[q];
+    }
+  }
+  __device__ static __forceinline__ Parts3 rows(const char* lds, int r, int s, int h) {
+    return Parts3{Plane::rows(lds, r, s, h), Plane::rows(lds + Plane::BYTES, r, s, h),
+                  Plane::rows(lds + 2 * Plane::BYTES, r, s, h)};
+  }
+  __device__ static __forceinline__ Parts3 cols(const char* lds, int r0, int d0, int lane) {
+    return Parts3{Plane::cols(lds, r0, d0, lane), Plane::cols(lds + Plane::BYTES, r0, d0, lane),
+                  Plane::cols(lds + 2 * Plane::BYTES, r0, d0, lane)};
+  }
+  __device__ static __forceinline__ void clear(char* lds, int r, int first, int step) {
+#pragma unroll
+    for (int q = 0; q < 3; ++q) Plane::clear(lds + q * Plane::BYTES, r, first, step);
   }
 };
 
@@ -310,8 +380,8 @@ struct WaveRange {
 constexpr int kBlockMask = 0x0fffffff, kEntryHoles = 0x20000000;
 
 // Lists the blocks [c0, c1) of BLOCK rows of `seg` (`n` of them exist) that hold a segment in [lo, hi], in order;
-// holes: some row is of no segment (or past n).  All 256 threads;
-// returns the entries.  flags: one byte a block, list: one int a block.
+// holes: some row is of no segment (or past n).  All 256 threads; returns the entries.  flags: one byte a block, list:
+// one int a block.
 template <int BLOCK>
 __device__ __forceinline__ int list_blocks(const int* __restrict__ seg, int n, int lo, int hi, int c0, int c1,
                                            uint8_t* flags, int* list, int* count) {
@@ -319,23 +389,23 @@ __device__ __forceinline__ int list_blocks(const int* __restrict__ seg, int n, i
   constexpr int PER = 64 / BLOCK;   // blocks one wave reads at a time
   constexpr int AHEAD = 8;          // reads in flight
   for (int b8 = c0 + wave * PER; b8 < c1; b8 += 4 * PER * AHEAD) {
-   int got[AHEAD];
+    int got[AHEAD];
 #pragma unroll
-   for (int q = 0; q < AHEAD; ++q) {
-    const int r = (b8 + 4 * PER * q) * BLOCK + lane;
-    got[q] = r < n ? seg[r] : -1;
-   }
-#pragma unroll
-   for (int q = 0; q < AHEAD; ++q) {
-    const int b0 = b8 + 4 * PER * q, s = got[q];
-    const uint64_t hit = __ballot(s >= 0 && s >= lo && s <= hi), hole = __ballot(s < 0);
-#pragma unroll
-    for (int p = 0; p < PER; ++p) {
-      const uint64_t m = BLOCK == 64 ? ~0ull : (uint64_t)0xffffffffu << (32 * p);
-      if (lane == 0 && b0 + p < c1)
-        flags[b0 + p - c0] = (uint8_t)(((hit & m) != 0 ? 1 : 0) | ((hole & m) != 0 ? 2 : 0));
+    for (int q = 0; q < AHEAD; ++q) {
+      const int r = (b8 + 4 * PER * q) * BLOCK + lane;
+      got[q] = r < n ? seg[r] : -1;
     }
-   }
+#pragma unroll
+    for (int q = 0; q < AHEAD; ++q) {
+      const int b0 = b8 + 4 * PER * q, s = got[q];
+      const uint64_t hit = __ballot(s >= 0 && s >= lo && s <= hi), hole = __ballot(s < 0);
+#pragma unroll
+      for (int p = 0; p < PER; ++p) {
+        const uint64_t m = BLOCK == 64 ? ~0ull : (uint64_t)0xffffffffu << (32 * p);
+        if (lane == 0 && b0 + p < c1)
+          flags[b0 + p - c0] = (uint8_t)(((hit & m) != 0 ? 1 : 0) | ((hole & m) != 0 ? 2 : 0));
+      }
+    }
   }
   __syncthreads();
   if (wave == 0) {

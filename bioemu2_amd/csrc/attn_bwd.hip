@@ -71,9 +71,8 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void att
                                                                   float* __restrict__ bias_part, int splits,
                                                                   int qblocks, int total) {
   constexpr int KB = Operand<T>::kBlock, SUB = KB / 32, STEPS = DP / 16, DB = DP / 32;
-  typedef Tile<T, DP, KB> KV;
-  constexpr int CP = KV::copies(kAttnThreads);
-  __shared__ __attribute__((aligned(1024))) char tiles[2][2][KV::BYTES];
+  typedef Staged<T, DP, KB> KV;
+  __shared__ __attribute__((aligned(1024))) char tiles[KV::BUFFERS][2][KV::BYTES];
   __shared__ __attribute__((aligned(16))) int segs[2][64];
   __shared__ int list[kListBlocks];
   __shared__ uint8_t flags[kListBlocks];
@@ -158,9 +157,7 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void att
 
   const T* kbase = static_cast<const T*>(a.k) + b * a.kb + hk * a.kh;
   const T* vbase = static_cast<const T*>(a.v) + b * a.vb + hk * a.vh;
-  unsigned koff[CP], voff[CP];
-  KV::offsets(threadIdx.x, kAttnThreads, a.kn, a.D, koff);
-  KV::offsets(threadIdx.x, kAttnThreads, a.vn, a.D, voff);
+  KV k_tile(a.kn, a.D), v_tile(a.vn, a.D);
   const int* kseg = seg ? a.k_seg + (int64_t)b * a.Nk : nullptr;
 
   f32x16 acc[DB];
@@ -170,8 +167,9 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void att
 
   auto stage = [&](int entry, int buf) {
     const int k0 = (entry & kBlockMask) * KB;
-    KV::copy(kbase + (int64_t)k0 * a.kn, length - k0, a.kn, a.D, tiles[buf][0], wave, kAttnThreads, koff);
-    KV::copy(vbase + (int64_t)k0 * a.vn, length - k0, a.vn, a.D, tiles[buf][1], wave, kAttnThreads, voff);
+    char(*to)[KV::BYTES] = tiles[buf % KV::BUFFERS];
+    k_tile.fetch(kbase + (int64_t)k0 * a.kn, length - k0, a.kn, a.D, to[0], wave);
+    v_tile.fetch(vbase + (int64_t)k0 * a.vn, length - k0, a.vn, a.D, to[1], wave);
     if (seg && wave == 0) copy_ints(kseg + k0, length - k0, segs[buf], lane);
   };
 
@@ -186,19 +184,25 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void att
       const int e = entry(t), buf = t & 1, k0 = (e & kBlockMask) * KB;
       __builtin_amdgcn_s_waitcnt(0x0f70);
       __syncthreads();
+      char(*tile)[KV::BYTES] = tiles[buf % KV::BUFFERS];
+      if constexpr (KV::BUFFERS == 1) {
+        k_tile.store(tile[0]);
+        v_tile.store(tile[1]);
+        __syncthreads();
+      }
       if (t + 1 < t1) stage(entry(t + 1), buf ^ 1);
       if (e & kEntryHoles) {
         const int r = threadIdx.x / (kAttnThreads / KB);
         if (segs[buf][r] < 0) {
-          KV::clear(tiles[buf][0], r, threadIdx.x % (kAttnThreads / KB), kAttnThreads / KB);
-          KV::clear(tiles[buf][1], r, threadIdx.x % (kAttnThreads / KB), kAttnThreads / KB);
+          KV::clear(tile[0], r, threadIdx.x % (kAttnThreads / KB), kAttnThreads / KB);
+          KV::clear(tile[1], r, threadIdx.x % (kAttnThreads / KB), kAttnThreads / KB);
         }
         __syncthreads();
       }
       if (k0 >= wave_max) continue;
       bool all = true;   // every key has the one segment of all queries of this wave
       if (seg && !own_segs.meets<KB>(segs[buf], lane, all)) continue;
-      const char *kt = tiles[buf][0], *vt = tiles[buf][1];
+      const char *kt = tile[0], *vt = tile[1];
 #pragma unroll 1
       for (int u = 0; u < SUB; ++u) {
         f32x16 s = zero16(), dp;
@@ -322,9 +326,8 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, true>())) void attn
                                                                    float* __restrict__ part, int splits, int kblocks,
                                                                    int total) {
   constexpr int QB = Operand<T>::kBlock, SUB = QB / 32, STEPS = DP / 16, DB = DP / 32;
-  typedef Tile<T, DP, QB> QD;
-  constexpr int CP = QD::copies(kAttnThreads);
-  __shared__ __attribute__((aligned(1024))) char tiles[2][2][QD::BYTES];
+  typedef Staged<T, DP, QB> QD;
+  __shared__ __attribute__((aligned(1024))) char tiles[QD::BUFFERS][2][QD::BYTES];
   __shared__ __attribute__((aligned(16))) int segs[2][64];
   __shared__ __attribute__((aligned(16))) float stats[2][2][64];   // what attn_bwd_q wrote of the rows
   __shared__ int list[kListBlocks];
@@ -371,9 +374,7 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, true>())) void attn
       vf[s] = row_operand<T>(pv, on, s, lh, a.D);
     }
   }
-  unsigned qoff[CP], doff[CP];
-  QD::offsets(threadIdx.x, kAttnThreads, a.qn, a.D, qoff);
-  QD::offsets(threadIdx.x, kAttnThreads, dn, a.D, doff);
+  QD q_tile(a.qn, a.D), d_tile(dn, a.D);
   const int* qseg = seg ? a.q_seg + (int64_t)b * a.Nq : nullptr;
 
   f32x16 ak[DB], av[DB];
@@ -390,8 +391,9 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, true>())) void attn
   int64_t srow = 0;
   auto stage = [&](int en, int buf) {
     const int i0 = (en & kBlockMask) * QB;
-    QD::copy(qbase + (int64_t)i0 * a.qn, a.Nq - i0, a.qn, a.D, tiles[buf][0], wave, kAttnThreads, qoff);
-    QD::copy(dbase + (int64_t)i0 * dn, a.Nq - i0, dn, a.D, tiles[buf][1], wave, kAttnThreads, doff);
+    char(*to)[QD::BYTES] = tiles[buf % QD::BUFFERS];
+    q_tile.fetch(qbase + (int64_t)i0 * a.qn, a.Nq - i0, a.qn, a.D, to[0], wave);
+    d_tile.fetch(dbase + (int64_t)i0 * dn, a.Nq - i0, dn, a.D, to[1], wave);
     if (wave == 0) copy_ints(row_stats + srow + i0, a.Nq - i0, stats[buf][0], lane);
     if (wave == 1) copy_ints(row_stats + (int64_t)a.B * a.H * a.Nq + srow + i0, a.Nq - i0, stats[buf][1], lane);
     if (seg && wave == 2) copy_ints(qseg + i0, a.Nq - i0, segs[buf], lane);
@@ -417,20 +419,26 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, true>())) void attn
         const int e = entry(t), buf = t & 1, i0 = (e & kBlockMask) * QB;
         __builtin_amdgcn_s_waitcnt(0x0f70);
         __syncthreads();
+        char(*tile)[QD::BYTES] = tiles[buf % QD::BUFFERS];
+        if constexpr (QD::BUFFERS == 1) {
+          q_tile.store(tile[0]);
+          d_tile.store(tile[1]);
+          __syncthreads();
+        }
         if (t + 1 < t1) stage(entry(t + 1), buf ^ 1);
         // rows that see nothing (their constant is -infinity) have weight 0, and 0 times what they hold has to be 0
         if (__ballot(lane < QB && stats[buf][0][lane] == -kInf)) {
           const int r = threadIdx.x / (kAttnThreads / QB);
           if (stats[buf][0][r] == -kInf) {
-            QD::clear(tiles[buf][0], r, threadIdx.x % (kAttnThreads / QB), kAttnThreads / QB);
-            QD::clear(tiles[buf][1], r, threadIdx.x % (kAttnThreads / QB), kAttnThreads / QB);
+            QD::clear(tile[0], r, threadIdx.x % (kAttnThreads / QB), kAttnThreads / QB);
+            QD::clear(tile[1], r, threadIdx.x % (kAttnThreads / QB), kAttnThreads / QB);
           }
           __syncthreads();
         }
         if (i0 + QB <= wave_min) continue;
         bool all_same = true;
         if (seg && !own_segs.meets<QB>(segs[buf], lane, all_same)) continue;
-        const char *qt = tiles[buf][0], *dt = tiles[buf][1];
+        const char *qt = tile[0], *dt = tile[1];
 #pragma unroll 1
         for (int u = 0; u < SUB; ++u) {
           f32x16 s = zero16(), dp;

@@ -50,9 +50,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
                                                                 Parts parts, int splits,
                                                                 int qblocks, int total) {
   constexpr int KB = Operand<T>::kBlock, SUB = KB / 32, STEPS = DP / 16, DB = DP / 32;
-  typedef Tile<T, DP, KB> KV;
-  constexpr int CP = KV::copies(kAttnThreads);
-  __shared__ __attribute__((aligned(1024))) char tiles[2][2][KV::BYTES];
+  typedef Staged<T, DP, KB> KV;
+  __shared__ __attribute__((aligned(1024))) char tiles[KV::BUFFERS][2][KV::BYTES];
   __shared__ __attribute__((aligned(16))) int segs[2][64];
   __shared__ float lut[2 * (kMaxRadius + kPad) + 1];
   __shared__ int list[kListBlocks];
@@ -100,9 +99,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
   }
   const T* kbase = static_cast<const T*>(a.k) + b * a.kb + hk * a.kh;
   const T* vbase = static_cast<const T*>(a.v) + b * a.vb + hk * a.vh;
-  unsigned koff[CP], voff[CP];
-  KV::offsets(threadIdx.x, kAttnThreads, a.kn, a.D, koff);
-  KV::offsets(threadIdx.x, kAttnThreads, a.vn, a.D, voff);
+  KV k_tile(a.kn, a.D), v_tile(a.vn, a.D);
   const int* kseg = seg ? a.k_seg + (int64_t)b * a.Nk : nullptr;
 
   f32x16 acc[DB];
@@ -120,8 +117,9 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
 
   auto stage = [&](int entry, int buf) {
     const int k0 = (entry & kBlockMask) * KB;
-    KV::copy(kbase + (int64_t)k0 * a.kn, length - k0, a.kn, a.D, tiles[buf][0], wave, kAttnThreads, koff);
-    KV::copy(vbase + (int64_t)k0 * a.vn, length - k0, a.vn, a.D, tiles[buf][1], wave, kAttnThreads, voff);
+    char(*to)[KV::BYTES] = tiles[buf % KV::BUFFERS];
+    k_tile.fetch(kbase + (int64_t)k0 * a.kn, length - k0, a.kn, a.D, to[0], wave);
+    v_tile.fetch(vbase + (int64_t)k0 * a.vn, length - k0, a.vn, a.D, to[1], wave);
     if (seg && wave == 0) copy_ints(kseg + k0, length - k0, segs[buf], lane);
   };
 
@@ -136,17 +134,23 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
       const int e = entry(t), buf = t & 1, k0 = (e & kBlockMask) * KB;
       __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's copies landed
       __syncthreads();                       // ... and everyone's; the other buffer is free
+      char(*tile)[KV::BYTES] = tiles[buf % KV::BUFFERS];
+      if constexpr (KV::BUFFERS == 1) {
+        k_tile.store(tile[0]);
+        v_tile.store(tile[1]);
+        __syncthreads();
+      }
       if (t + 1 < t1) stage(entry(t + 1), buf ^ 1);
       if (e & kEntryHoles) {
         // keys in no segment have weight 0, and 0 times what their values hold has to be 0
         const int r = threadIdx.x / (kAttnThreads / KB);
-        if (segs[buf][r] < 0) KV::clear(tiles[buf][1], r, threadIdx.x % (kAttnThreads / KB), kAttnThreads / KB);
+        if (segs[buf][r] < 0) KV::clear(tile[1], r, threadIdx.x % (kAttnThreads / KB), kAttnThreads / KB);
         __syncthreads();
       }
       if (k0 >= wave_max) continue;
       bool all = true;   // every key has the one segment of all queries of this wave
       if (seg && !own_segs.meets<KB>(segs[buf], lane, all)) continue;
-      const char *kt = tiles[buf][0], *vt = tiles[buf][1];
+      const char *kt = tile[0], *vt = tile[1];
       float x[SUB][16];
 #pragma unroll
       for (int u = 0; u < SUB; ++u) {
@@ -254,7 +258,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
 }
 
 // Waves of attn_few: each has a K and a V tile of its own, 64 KB of LDS in all at most (two workgroups a CU, so that
-// one streams while the other starts or joins: 131 KB with two tiles of each measured 168 us where this takes WW).
+// one streams while the other starts or joins: 131 KB with two tiles of each measured 168 us where this takes 157).
 template <class T, int DP>
 constexpr int few_waves() {
   constexpr int w = 65536 / (2 * Tile<T, DP, 32>::BYTES);
@@ -532,7 +536,7 @@ bool few_rows(const AttnArgs& a) { return a.Nq * a.G <= 32; }
 
 // Workgroups that the keys of a query block are split over.  Long rows: as many as bring the launch to two workgroups a
 // CU, 256 keys each at least.  Few rows: sequences of a cache are of unequal length, so up to sixteen a CU that even
-// out, 512 keys each at least (8 sequences of 8200 to 32768 keys, 8 heads: 160 us in parts of 2048, XX in parts of
+// out, 512 keys each at least (8 sequences of 8200 to 32768 keys, 8 heads: 160 us in parts of 2048, 157 in parts of
 // 512), and none for up to 1024 keys, where the join costs what the shorter walk gains (773 keys: 18 us in four parts,
 // 13 in one).
 int key_splits(const AttnArgs& a) {
