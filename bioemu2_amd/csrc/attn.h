@@ -346,9 +346,10 @@ __device__ __forceinline__ void wg_extremes(int& low, int& high, int& top, int (
 // meets the radius reads it without clamping.  Entry rel + R + kPad.
 constexpr int kPad = 64;
 __device__ __forceinline__ int lut_size(const AttnArgs& a) { return 2 * (a.radius + kPad) + 1; }
-__device__ __forceinline__ void fill_lut(const AttnArgs& a, int h, float* lut) {
+// `add`: what a capped score takes besides.
+__device__ __forceinline__ void fill_lut(const AttnArgs& a, int h, float add, float* lut) {
   for (int e = threadIdx.x; e < lut_size(a); e += kAttnThreads)
-    lut[e] = table_value(a, min(max(e - kPad, 0), 2 * a.radius), h);
+    lut[e] = table_value(a, min(max(e - kPad, 0), 2 * a.radius), h) + add;
 }
 // Whether all offsets rel0 - 31 .. rel0 + 31 lie at or beyond the radius.
 __device__ __forceinline__ bool all_far(const AttnArgs& a, int rel0) {
@@ -444,6 +445,15 @@ inline unsigned attn_grid(int64_t total) { return (unsigned)(round_up(total, kAt
 
 // Compute units of the current device, remembered.
 int attn_units();
+
+// log2 of a row's sum of weights in two parts: the reference its weights are taken against, and log2 of their sum by it.
+// A bias of the type's lowest value makes a reference in which the second part vanishes, so the backward pass adds them
+// only where the reference is below kWideRow (there 2^-14 of the sum is kept).
+constexpr float kWideRow = 1024.f;
+__device__ __forceinline__ void store_log_sum(float* lse, int64_t plane, int64_t at, float m, float l) {
+  lse[at] = l == 0.f ? 0.f : m;
+  lse[plane + at] = l == 0.f ? kInf : __log2f(l);   // rows that see nothing
+}
 
 // Checks the arguments both directions share and lays them out (attn_fwd.hip).
 int attn_args(const char* what, const bioemu_attention_args* in, AttnArgs* out);

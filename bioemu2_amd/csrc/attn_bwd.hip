@@ -11,6 +11,9 @@
 //
 // Either may split its walk over workgroups where the rows alone do not fill the chip; attn_bwd_finish adds the parts.
 //
+// Rows whose scores' reference is at or beyond kWideRow (attn.h) take their weights against it and multiply them by the
+// inverse sum; all others have log2 of the sum in the constant that is added to a score.
+//
 // The table's gradient sums ds along the diagonals of every 32 x 32 block that meets the radius: the block goes to LDS,
 // rows 68 values apart with zeros between them, and lane e reads its diagonal (value e + n - 31 of row n) without a
 // bound to check, 16 reads of two values.  (One LDS add an element took 45 cycles each, 8 times the whole.)  Every wave
@@ -61,15 +64,10 @@ constexpr int bwd_waves() {
 }
 
 template <class T, int DP, bool CAP>
-__global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void attn_bwd_q_kernel(const AttnArgs a, const T* __restrict__ o,
-                                                                  const T* __restrict__ o_lo,
-                                                                  const float* __restrict__ lse,
-                                                                  const T* __restrict__ dout, int64_t db, int64_t dn,
-                                                                  int64_t dh, T* __restrict__ dq,
-                                                                  float* __restrict__ stats,
-                                                                  float* __restrict__ dq_part,
-                                                                  float* __restrict__ bias_part, int splits,
-                                                                  int qblocks, int total) {
+__global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void attn_bwd_q_kernel(
+    const AttnArgs a, const T* __restrict__ o, const T* __restrict__ o_lo, const float* __restrict__ lse, const T*
+    __restrict__ dout, int64_t db, int64_t dn, int64_t dh, T* __restrict__ dq, float* __restrict__ stats, float*
+    __restrict__ dq_part, float* __restrict__ bias_part, int splits, int qblocks, int total) {
   constexpr int KB = Operand<T>::kBlock, SUB = KB / 32, STEPS = DP / 16, DB = DP / 32;
   typedef Staged<T, DP, KB> KV;
   __shared__ __attribute__((aligned(1024))) char tiles[KV::BUFFERS][2][KV::BYTES];
@@ -111,13 +109,13 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void att
   wave_max = __builtin_amdgcn_readfirstlane(wave_max);
   const int wave_pos = __builtin_amdgcn_readfirstlane(pos);
 
+  const Capped<T> capped(a);
   if (a.table) {
-    fill_lut(a, h, lut);
+    fill_lut(a, h, CAP ? capped.k3 : 0.f, lut);
     if (bias_part)
       for (int e = threadIdx.x; e < 4 * (row4 + kDiagBlock); e += kAttnThreads) sums[e] = 0.f;
   }
 
-  const Capped<T> capped(a);
   const float mult = a.scale * kLog2e, out_scale = a.scale * (CAP ? Capped<T>::kSlope : 1.f);
   const auto score = [&](float raw, float add, float& slope) {
     if constexpr (CAP) return capped.score(raw, add, slope);
@@ -127,7 +125,12 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void att
   // a row that sees nothing contributes nothing, whatever it holds
   const bool on = live && lim > 0;
   const int64_t row = ((int64_t)b * a.Nq + (live ? i : 0)) * a.H + h, srow = ((int64_t)b * a.H + h) * a.Nq + i;
-  const float row_lse = live ? lse[srow] : kInf;
+  // weights are 2^(x + base) row_inv; row_inv is 1 but for wide rows
+  const int64_t plane = (int64_t)a.B * a.H * a.Nq;
+  const float row_m = live ? lse[srow] : 0.f, row_l = live ? lse[plane + srow] : kInf;
+  const bool row_wide = a.table && fabsf(row_m) >= kWideRow && row_l < kInf;
+  const float row_inv = row_wide ? fast_exp2(-row_l) : 1.f;
+  const bool wide = __ballot(row_wide) != 0;
   Frag<T> qf[STEPS], df[STEPS];
   float dsum = 0.f;
   {
@@ -148,11 +151,12 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void att
     }
   }
   dsum += __shfl_xor(dsum, 32);
-  // the constant part of every score of the row, what its weights are taken against included
-  const float base = (CAP ? capped.k3 : 0.f) - row_lse;
+  // (without a table the constant part of the scores is in it, as it is in the table else)
+  const float base = (a.table || !CAP ? 0.f : capped.k3) - (row_wide ? row_m : row_m + row_l);
   if (live && lh == 0 && split == 0) {
     stats[srow] = base;
-    stats[(int64_t)a.B * a.H * a.Nq + srow] = -dsum;
+    stats[plane + srow] = -dsum;
+    if (a.table) stats[2 * plane + srow] = row_inv;
   }
 
   const T* kbase = static_cast<const T*>(a.k) + b * a.kb + hk * a.kh;
@@ -218,14 +222,20 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void att
         if (a.table && !far) {
           const float* bias = lut + (rel0 + a.radius + kPad + 4 * lh - ln);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) x[r] = score(s[r], bias[8 * (r >> 2) + (r & 3)] + base, slope[r]);
-        } else {
-          const float add = base + (a.table ? lut[rel0 > 0 ? nrel - 1 : 0] : 0.f);
+          for (int r = 0; r < 16; ++r) x[r] = score(s[r], bias[8 * (r >> 2) + (r & 3)], slope[r]) + base;
+        } else if (a.table) {
+          const float add = lut[rel0 > 0 ? nrel - 1 : 0];
 #pragma unroll
-          for (int r = 0; r < 16; ++r) x[r] = score(s[r], add, slope[r]);
+          for (int r = 0; r < 16; ++r) x[r] = score(s[r], add, slope[r]) + base;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[r] = score(s[r], base, slope[r]);
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) x[r] = fast_exp2(x[r]) * dp[r];
+        if (wide)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[r] *= row_inv;
         if (k0 + KB > wave_min)
 #pragma unroll
           for (int r = 0; r < 16; ++r) x[r] = k0 + 32 * u + 8 * (r >> 2) + 4 * lh + (r & 3) < lim ? x[r] : 0.f;
@@ -319,17 +329,16 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void att
 }
 
 template <class T, int DP, bool CAP>
-__global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, true>())) void attn_bwd_kv_kernel(const AttnArgs a, const float* __restrict__ row_stats,
-                                                                   const T* __restrict__ dout, int64_t db, int64_t dn,
-                                                                   int64_t dh,
-                                                                   T* __restrict__ dk, T* __restrict__ dv,
-                                                                   float* __restrict__ part, int splits, int kblocks,
-                                                                   int total) {
+__global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, true>())) void attn_bwd_kv_kernel(
+    const AttnArgs a, const float* __restrict__ row_stats, const T* __restrict__ dout, int64_t db, int64_t dn,
+    int64_t dh, T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ part, int splits, int kblocks, int
+    total) {
   constexpr int QB = Operand<T>::kBlock, SUB = QB / 32, STEPS = DP / 16, DB = DP / 32;
   typedef Staged<T, DP, QB> QD;
   __shared__ __attribute__((aligned(1024))) char tiles[QD::BUFFERS][2][QD::BYTES];
   __shared__ __attribute__((aligned(16))) int segs[2][64];
   __shared__ __attribute__((aligned(16))) float stats[2][2][64];   // what attn_bwd_q wrote of the rows
+  __shared__ float inverse[64];
   __shared__ int list[kListBlocks];
   __shared__ uint8_t flags[kListBlocks];
   __shared__ int red[3][4], count;
@@ -387,6 +396,7 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, true>())) void attn
     return raw * mult + add;
   };
 
+  const int64_t plane = (int64_t)a.B * a.H * a.Nq;
   const T *qbase = nullptr, *dbase = nullptr;   // of the current head, as its row of statistics
   int64_t srow = 0;
   auto stage = [&](int en, int buf) {
@@ -395,7 +405,7 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, true>())) void attn
     q_tile.fetch(qbase + (int64_t)i0 * a.qn, a.Nq - i0, a.qn, a.D, to[0], wave);
     d_tile.fetch(dbase + (int64_t)i0 * dn, a.Nq - i0, dn, a.D, to[1], wave);
     if (wave == 0) copy_ints(row_stats + srow + i0, a.Nq - i0, stats[buf][0], lane);
-    if (wave == 1) copy_ints(row_stats + (int64_t)a.B * a.H * a.Nq + srow + i0, a.Nq - i0, stats[buf][1], lane);
+    if (wave == 1) copy_ints(row_stats + plane + srow + i0, a.Nq - i0, stats[buf][1], lane);
     if (seg && wave == 2) copy_ints(qseg + i0, a.Nq - i0, segs[buf], lane);
   };
 
@@ -413,7 +423,7 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, true>())) void attn
       qbase = static_cast<const T*>(a.q) + b * a.qb + h * a.qh;
       dbase = dout + b * db + h * dh;
       srow = ((int64_t)b * a.H + h) * a.Nq;
-      if (a.table) fill_lut(a, h, lut);
+      if (a.table) fill_lut(a, h, CAP ? capped.k3 : 0.f, lut);
       if (t0 < t1) stage(entry(t0), t0 & 1);
       for (int t = t0; t < t1; ++t) {
         const int e = entry(t), buf = t & 1, i0 = (e & kBlockMask) * QB;
@@ -426,12 +436,21 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, true>())) void attn
           __syncthreads();
         }
         if (t + 1 < t1) stage(entry(t + 1), buf ^ 1);
-        // rows that see nothing (their constant is -infinity) have weight 0, and 0 times what they hold has to be 0
-        if (__ballot(lane < QB && stats[buf][0][lane] == -kInf)) {
+        // rows that see nothing (their constant is -infinity) and those past the last have weight 0, and 0 times what
+        // they hold has to be 0; wide rows
+        const float row_base = stats[buf][0][lane & (QB - 1)];
+        bool wide = false;
+        if (i0 + QB > a.Nq || __ballot(fabsf(row_base) >= kWideRow)) {
+          wide = a.table && __ballot(fabsf(row_base) >= kWideRow && row_base != -kInf) != 0;
           const int r = threadIdx.x / (kAttnThreads / QB);
           if (stats[buf][0][r] == -kInf) {
             QD::clear(tile[0], r, threadIdx.x % (kAttnThreads / QB), kAttnThreads / QB);
             QD::clear(tile[1], r, threadIdx.x % (kAttnThreads / QB), kAttnThreads / QB);
+          }
+          __syncthreads();
+          if (wave == 0 && lane < QB) {
+            if (i0 + lane >= a.Nq) stats[buf][0][lane] = -kInf;
+            if (wide) inverse[lane] = i0 + lane < a.Nq ? row_stats[2 * plane + srow + i0 + lane] : 0.f;
           }
           __syncthreads();
         }
@@ -463,17 +482,21 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, true>())) void attn
           if (a.table && !all_far(a, rel0)) {
             const float* bias = lut + (rel0 + a.radius + kPad + ln - 4 * lh);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] = score(s[r], bias[-(8 * (r >> 2) + (r & 3))] + base[r], slope[r]);
+            for (int r = 0; r < 16; ++r)
+              x[r] = score(s[r], bias[-(8 * (r >> 2) + (r & 3))], slope[r]) + base[r];
           } else if (a.table) {
             const float add = lut[rel0 > 0 ? 2 * (a.radius + kPad) : 0];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] = score(s[r], add + base[r], slope[r]);
+            for (int r = 0; r < 16; ++r) x[r] = score(s[r], add, slope[r]) + base[r];
           } else {
 #pragma unroll
             for (int r = 0; r < 16; ++r) x[r] = score(s[r], base[r], slope[r]);
           }
 #pragma unroll
           for (int r = 0; r < 16; ++r) x[r] = fast_exp2(x[r]);
+          if (wide)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] *= inverse[32 * u + 8 * (r >> 2) + 4 * lh + (r & 3)];
           if (i0 < wave_max)
 #pragma unroll
             for (int r = 0; r < 16; ++r)
@@ -601,7 +624,7 @@ BwdSpace bwd_space(const AttnArgs& a, bool f32, bool table) {
   BwdSpace s;
   s.q_splits = walk_splits((int64_t)a.B * a.H * qblocks, a.Nk, block);
   s.kv_splits = kblocks ? walk_splits((int64_t)a.B * a.Hk * kblocks, (int64_t)a.Nq * a.G, block) : 1;
-  s.stats = (size_t)round_up((int64_t)a.B * a.H * a.Nq * 8, 256);
+  s.stats = (size_t)round_up((int64_t)a.B * a.H * a.Nq * (a.table ? 12 : 8), 256);
   s.q_part = s.q_splits == 1 ? 0 : (size_t)round_up((int64_t)s.q_splits * a.B * a.H * a.Nq * a.D * 4, 256);
   s.kv_part = s.kv_splits == 1 ? 0 : (size_t)round_up((int64_t)s.kv_splits * 2 * a.B * a.Hk * a.Nk * a.D * 4, 256);
   s.bias = table ? (size_t)(a.B * qblocks * s.q_splits * a.H * a.nb) * 4 : 0;
@@ -610,8 +633,8 @@ BwdSpace bwd_space(const AttnArgs& a, bool f32, bool table) {
 }
 
 template <class T, int DP, bool CAP>
-int launch_bwd_as(const AttnArgs& a, const void* o, const void* o_lo, const float* lse, const void* dout, const int64_t* ds, void* dq,
-               void* dk, void* dv, void* dtable, void* ws, hipStream_t stream) {
+int launch_bwd_as(const AttnArgs& a, const void* o, const void* o_lo, const float* lse, const void* dout,
+                  const int64_t* ds, void* dq, void* dk, void* dv, void* dtable, void* ws, hipStream_t stream) {
   const BwdSpace sp = bwd_space(a, sizeof(T) == 4, dtable != nullptr);
   char* at = static_cast<char*>(ws);
   float* stats = reinterpret_cast<float*>(at);
@@ -668,17 +691,17 @@ extern "C" size_t bioemu_attention_bwd_workspace_bytes(const bioemu_attention_ar
 }
 
 extern "C" int bioemu_attention_bwd(const bioemu_attention_args* args, const void* o, const void* o_lo,
-                                    const float* lse, const void* dout, const int64_t* dout_stride, void* dq, void* dk, void* dv,
-                                    void* dtable, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+                                    const float* lse, const void* dout, const int64_t* dout_stride, void* dq, void* dk,
+                                    void* dv, void* dtable, void* workspace, size_t workspace_bytes, hipStream_t stream) {
   AttnArgs a;
   if (const int rc = attn_args("attention_bwd", args, &a)) return rc;
   if (a.B == 0 || a.Nq == 0) return set_error(BIOEMU_ERR_INVALID_ARG, "attention_bwd: no queries");
   if (!o || !lse || !dout || !dout_stride || !dq || (a.Nk > 0 && (!dk || !dv)))
     return set_error(BIOEMU_ERR_INVALID_ARG, "attention_bwd: null pointer");
   const int64_t per = args->f32 ? 4 : 8;
+  const int64_t ds[3] = {dout_stride[0], a.Nq > 1 ? dout_stride[1] : a.D, dout_stride[2]};
   if (!aligned16(o) || !aligned16(o_lo) || !aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) ||
-      dout_stride[0] % per || dout_stride[1] % per || dout_stride[2] % per || dout_stride[1] > (int64_t(1) << 23) ||
-      (a.Nq > 1 && dout_stride[1] < a.D))
+      ds[0] % per || ds[1] % per || ds[2] % per || ds[1] > (int64_t(1) << 23) || ds[1] < a.D)
     return set_error(BIOEMU_ERR_INVALID_ARG,
                      "attention_bwd: rows start at 16-byte addresses, at least a head's width apart");
   if (o_lo && args->f32) return set_error(BIOEMU_ERR_INVALID_ARG, "attention_bwd: o_lo is of bf16 calls");
@@ -688,7 +711,7 @@ extern "C" int bioemu_attention_bwd(const bioemu_attention_args* args, const voi
     return set_error(BIOEMU_ERR_WORKSPACE, "attention_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   const int dp = a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128;
 #define BIOEMU_BWD(T, P)                                                                                            \
-  if (dp == P) return launch_bwd<T, P>(a, o, o_lo, lse, dout, dout_stride, dq, dk, dv, dtable, workspace, stream)
+  if (dp == P) return launch_bwd<T, P>(a, o, o_lo, lse, dout, ds, dq, dk, dv, dtable, workspace, stream)
   if (args->f32) {
     BIOEMU_BWD(float, 32);
     BIOEMU_BWD(float, 64);

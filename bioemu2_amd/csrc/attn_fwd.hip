@@ -42,8 +42,6 @@ __device__ __forceinline__ void store_quad(T* out, T* lo, const float (&v)[4]) {
   if (lo) *reinterpret_cast<quad*>(lo) = rest;
 }
 
-__device__ __forceinline__ float row_log_sum(float m, float l) { return l > 0.f ? m + __log2f(l) : kInf; }
-
 template <class T, int DP, bool CAP>
 __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a, T* __restrict__ out,
                                                                 T* __restrict__ lo, float* __restrict__ lse,
@@ -89,7 +87,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
   const int wave_pos = __builtin_amdgcn_readfirstlane(pos);   // of the wave's first row
   if (!live) lim = 0x7fffffff;
 
-  if (a.table) fill_lut(a, h, lut);
+  const Capped<T> capped(a);
+  if (a.table) fill_lut(a, h, CAP ? capped.k3 : 0.f, lut);
 
   Frag<T> qf[STEPS];
   {
@@ -107,8 +106,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
   for (int d = 0; d < DB; ++d) acc[d] = zero16();
   // weights are 2^(x - mref); a row starts with its first finite score, then mref moves when one exceeds limit
   float mref = 0.f, limit = -kInf, l = 0.f;
-  const Capped<T> capped(a);
-  const float mult = a.scale * kLog2e, base = CAP ? capped.k3 : 0.f;
+  const float mult = a.scale * kLog2e;
   const auto score = [&](float raw, float add) {
     float slope;
     if constexpr (CAP) return capped.score(raw, add, slope);
@@ -161,9 +159,9 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
         if (a.table && !all_far(a, rel0)) {
           const float* bias = lut + (rel0 + a.radius + kPad + 4 * lh - ln);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) x[u][r] = score(s[r], bias[8 * (r >> 2) + (r & 3)] + base);
+          for (int r = 0; r < 16; ++r) x[u][r] = score(s[r], bias[8 * (r >> 2) + (r & 3)]);
         } else {
-          const float add = base + (a.table ? lut[rel0 > 0 ? 2 * (a.radius + kPad) : 0] : 0.f);
+          const float add = a.table ? lut[rel0 > 0 ? 2 * (a.radius + kPad) : 0] : CAP ? capped.k3 : 0.f;
 #pragma unroll
           for (int r = 0; r < 16; ++r) x[u][r] = score(s[r], add);
         }
@@ -238,7 +236,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
           store_quad(out + at, lo ? lo + at : nullptr, v);
         }
       }
-    if (lse && lh == 0) lse[((int64_t)b * a.H + h) * a.Nq + i] = row_log_sum(mref, l);
+    if (lse && lh == 0)
+      store_log_sum(lse, (int64_t)a.B * a.H * a.Nq, ((int64_t)b * a.H + h) * a.Nq + i, mref, l);
   } else {
     const int64_t rows = (int64_t)a.B * a.Nq * a.H, at0 = split * rows + row;
 #pragma unroll
@@ -458,7 +457,7 @@ __global__ __launch_bounds__((64 * few_waves<T, DP>())) void attn_few_kernel(con
       const T hi = (T)v;
       out[row * a.D + d] = hi;
       if (lo) lo[row * a.D + d] = (T)(v - (float)hi);
-      if (lse && d == 0) lse[((int64_t)b * a.H + qh) * a.Nq + qi] = row_log_sum(to, sum);
+      if (lse && d == 0) store_log_sum(lse, all, ((int64_t)b * a.H + qh) * a.Nq + qi, to, sum);
     } else {
       parts.o[(split * all + row) * a.D + d] = o;
       if (d == 0) {
@@ -528,7 +527,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const AttnArgs 
   }
   if (lse && lane == 0) {
     const int64_t bi = row / a.H, h = row - bi * a.H, b = bi / a.Nq, i = bi - b * a.Nq;
-    lse[(b * a.H + h) * a.Nq + i] = row_log_sum(to, sum);
+    store_log_sum(lse, rows, (b * a.H + h) * a.Nq + i, to, sum);
   }
 }
 
@@ -543,7 +542,8 @@ int key_splits(const AttnArgs& a) {
   const bool few = few_rows(a);
   if (few && a.Nk <= 1024) return 1;
   const int64_t base = few ? (int64_t)a.B * a.Hk : (int64_t)a.B * a.H * ((a.Nq + kGroupRows - 1) / kGroupRows);
-  const int64_t want = ((few ? 16 : 2) * (int64_t)attn_units() + base - 1) / base, most = few ? (a.Nk + 511) / 512 : (a.Nk + 255) / 256;
+  const int64_t want = ((few ? 16 : 2) * (int64_t)attn_units() + base - 1) / base;
+  const int64_t most = few ? (a.Nk + 511) / 512 : (a.Nk + 255) / 256;
   const int64_t s = want < most ? want : most;
   return s < 1 ? 1 : (int)s;
 }
@@ -571,7 +571,8 @@ int launch_fwd(const AttnArgs& a, void* o, void* o_lo, float* lse, void* ws, hip
     KernelTimerScope timer("attn_fwd", stream);
     const dim3 grid(attn_grid(total));
     if (a.cap > 0.f)
-      attn_fwd_kernel<T, DP, true><<<grid, kAttnThreads, 0, stream>>>(a, out, lo, lse, parts, splits, qblocks, (int)total);
+      attn_fwd_kernel<T, DP, true><<<grid, kAttnThreads, 0, stream>>>(a, out, lo, lse, parts, splits, qblocks,
+                                                                     (int)total);
     else
       attn_fwd_kernel<T, DP, false><<<grid, kAttnThreads, 0, stream>>>(a, out, lo, lse, parts, splits, qblocks,
                                                                       (int)total);
@@ -620,12 +621,14 @@ int attn_args(const char* what, const bioemu_attention_args* in, AttnArgs* a) {
   const void* ptr[3] = {in->q, in->k, in->v};
   const int64_t* st[3] = {in->q_stride, in->k_stride, in->v_stride};
   const int64_t len[3] = {Nq, Nk, Nk};
+  int64_t row[3];
   for (int t = 0; t < 3; ++t) {
     if (!ptr[t] && B * len[t] > 0) return set_error(BIOEMU_ERR_INVALID_ARG, "%s: null pointer", what);
-    if (!aligned16(ptr[t]) || st[t][0] % per || st[t][1] % per || st[t][2] % per)
+    row[t] = len[t] > 1 ? st[t][1] : D;   // a single row has none, whatever stands there
+    if (!aligned16(ptr[t]) || st[t][0] % per || row[t] % per || st[t][2] % per)
       return set_error(BIOEMU_ERR_INVALID_ARG, "%s: rows of q, k and v start at 16-byte addresses", what);
-    if (st[t][1] > far || (len[t] > 1 && st[t][1] < D))
-      return set_error(BIOEMU_ERR_UNSUPPORTED, "%s: row stride %ld (head width to 2^23)", what, (long)st[t][1]);
+    if (row[t] > far || row[t] < D)
+      return set_error(BIOEMU_ERR_UNSUPPORTED, "%s: row stride %ld (head width to 2^23)", what, (long)row[t]);
   }
   if ((in->q_segments == nullptr) != (in->k_segments == nullptr))
     return set_error(BIOEMU_ERR_INVALID_ARG, "%s: segments of queries and of keys come together", what);
@@ -635,8 +638,8 @@ int attn_args(const char* what, const bioemu_attention_args* in, AttnArgs* a) {
       return set_error(BIOEMU_ERR_UNSUPPORTED, "%s: radius %ld (at most %d), %ld buckets (at most 256)", what,
                        (long)in->radius, kMaxRadius, (long)in->num_buckets);
   }
-  *a = AttnArgs{in->q, in->k, in->v, in->q_stride[0], in->q_stride[1], in->q_stride[2], in->k_stride[0],
-                in->k_stride[1], in->k_stride[2], in->v_stride[0], in->v_stride[1], in->v_stride[2], in->q_segments,
+  *a = AttnArgs{in->q, in->k, in->v, in->q_stride[0], row[0], in->q_stride[2], in->k_stride[0],
+                row[1], in->k_stride[2], in->v_stride[0], row[2], in->v_stride[2], in->q_segments,
                 in->k_segments, in->prefix, in->lengths, in->bias_table, in->bias_buckets, in->scale, in->cap, (int)B,
                 (int)Nq, (int)Nk, (int)H, (int)Hk, (int)(H / Hk), (int)D, (int)in->radius, (int)in->num_buckets,
                 in->causal, in->table_bf16};

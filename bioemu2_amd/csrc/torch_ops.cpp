@@ -327,8 +327,9 @@ Tensor relative_position_autograd(const Tensor& table, const optional<Tensor>& z
 // copy else.
 Tensor heads(const Tensor& t) {
   const int64_t per = 16 / t.element_size();
-  if (t.stride(3) == 1 && (t.size(1) <= 1 || t.stride(1) >= t.size(3)) && t.stride(1) <= (int64_t(1) << 23) &&
-      t.stride(0) % per == 0 && t.stride(1) % per == 0 && t.stride(2) % per == 0 &&
+  const bool rows = t.size(1) <= 1 || (t.stride(1) >= t.size(3) && t.stride(1) <= (int64_t(1) << 23) &&
+                                       t.stride(1) % per == 0);
+  if (t.stride(3) == 1 && rows && t.stride(0) % per == 0 && t.stride(2) % per == 0 &&
       reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0)
     return t;
   return t.clone(at::MemoryFormat::Contiguous);
@@ -415,7 +416,7 @@ std::tuple<Tensor, Tensor, Tensor> attention_run(ATTENTION_PARAMS, bool train) {
   Tensor out = at::empty(q.sizes(), q.options()), lo, lse, ws;
   if (train) {
     lo = is_f32(q) ? none_like(q) : at::empty(q.sizes(), q.options());
-    lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+    lse = at::empty({2, q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
   }
   const int64_t need = (int64_t)bioemu_attention_workspace_bytes(&c.args);
   if (need) ws = bytes(need, q);
@@ -430,14 +431,15 @@ std::tuple<Tensor, Tensor, Tensor> attention_train_cuda(ATTENTION_PARAMS) {
 }
 // dq, dk, dv and the table's gradient (empty where not wanted)
 std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward_cuda(const Tensor& out, const Tensor& lo,
-                                                                   const Tensor& lse, const Tensor& dout, ATTENTION_PARAMS,
+                                                                   const Tensor& lse, const Tensor& dout,
+                                                                   ATTENTION_PARAMS,
                                                                    bool want_table) {
   const c10::OptionalDeviceGuard guard(q.device());
   const AttentionCall c(ATTENTION_ARGS);
   TORCH_CHECK_VALUE(dout.scalar_type() == q.scalar_type() && dout.sizes() == q.sizes() &&
                         out.scalar_type() == q.scalar_type() && out.sizes() == q.sizes(),
                     "attention_backward: out ", out.sizes(), ", dout ", dout.sizes(), " of q ", q.sizes());
-  const int64_t lshape[3] = {q.size(0), q.size(2), q.size(1)};
+  const int64_t lshape[4] = {2, q.size(0), q.size(2), q.size(1)};
   check_shape(lse, "attention_backward lse", lshape, q);
   if (!is_f32(q)) check_shape(lo, "attention_backward lo", q.sizes(), q);
   want_table = want_table && table;
@@ -451,8 +453,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward_cuda(const Tensor&
   const Tensor ws = bytes(need, q);
   const int64_t ds[3] = {d.stride(0), d.stride(1), d.stride(2)};
   check_rc(bioemu_attention_bwd(&c.args, o.data_ptr(), is_f32(q) ? nullptr : ol.data_ptr(), l.data_ptr<float>(),
-                                d.data_ptr(), ds, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), want_table ? dtable.data_ptr() : nullptr, ws.data_ptr(),
-                                need, stream_of(q)),
+                                d.data_ptr(), ds, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                want_table ? dtable.data_ptr() : nullptr, ws.data_ptr(), need, stream_of(q)),
            "bioemu_attention_bwd");
   return {dq, dk, dv, dtable};
 }
@@ -461,7 +463,7 @@ Tensor attention_meta(ATTENTION_PARAMS) { return at::empty_symint(q.sym_sizes(),
 std::tuple<Tensor, Tensor, Tensor> attention_train_meta(ATTENTION_PARAMS) {
   return {at::empty_symint(q.sym_sizes(), q.options()),
           is_f32(q) ? none_like(q) : at::empty_symint(q.sym_sizes(), q.options()),
-          at::empty_symint({q.sym_size(0), q.sym_size(2), q.sym_size(1)}, q.options().dtype(at::kFloat))};
+          at::empty_symint({2, q.sym_size(0), q.sym_size(2), q.sym_size(1)}, q.options().dtype(at::kFloat))};
 }
 std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward_meta(const Tensor&, const Tensor&, const Tensor&, const Tensor&,
                                                                    ATTENTION_PARAMS, bool want_table) {

@@ -521,18 +521,19 @@ typedef struct bioemu_attention_args {
   int causal, f32, table_bf16;
 } bioemu_attention_args;
 
-/* o: [B, Nq, H, D] contiguous.  For the backward pass (each may be NULL): lse [B, H, Nq] fp32, log2 of the sum of
- * 2^(s log2 e), +infinity for rows that see nothing; o_lo, bf16 calls only, what the rounding of o took off. */
+/* o: [B, Nq, H, D] contiguous.  For the backward pass (each may be NULL): lse [2, B, H, Nq] fp32, two parts
+ * whose sum is log2 of the row's sum of 2^(s log2 e), +infinity for rows that see nothing; o_lo [B, Nq, H, D], bf16
+ * calls only, what the rounding of o took off. */
 size_t bioemu_attention_workspace_bytes(const bioemu_attention_args* args);
 int bioemu_attention_fwd(const bioemu_attention_args* args, void* o, void* o_lo, float* lse, void* workspace,
                          size_t workspace_bytes, hipStream_t stream);
 
-/* Gradients.  o_lo may be NULL.  dout: strides as above; dq [B, Nq, H, D], dk and dv [B, Nk, Hk, D]: contiguous; dtable: NULL or
- * [num_buckets, H] of the table's type.  Nq >= 1. */
+/* Gradients.  o_lo may be NULL.  dout: strides as above; dq [B, Nq, H, D], dk and dv [B, Nk, Hk, D]: contiguous;
+ * dtable: NULL or [num_buckets, H] of the table's type.  Nq >= 1. */
 size_t bioemu_attention_bwd_workspace_bytes(const bioemu_attention_args* args, int table_gradient);
 int bioemu_attention_bwd(const bioemu_attention_args* args, const void* o, const void* o_lo, const float* lse,
-                         const void* dout, const int64_t* dout_stride, void* dq, void* dk, void* dv, void* dtable, void* workspace,
-                         size_t workspace_bytes, hipStream_t stream);
+                         const void* dout, const int64_t* dout_stride, void* dq, void* dk, void* dv, void* dtable,
+                         void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -113,8 +113,12 @@ class Case:
             which = self.buckets.long()[(j - pos[:, :, None]).clamp(-R, R) + R].clamp(max=self.table.shape[0] - 1)
             bias = self.table.detach().double()[which].permute(0, 3, 1, 2)
             s = s + bias
-            e = e + 8 * U * bias.abs()
-        e = e + 8 * U * s.abs()
+            # next to the type's lowest value nothing of a score is left: such keys are equal, or weigh nothing beside others
+            low = bias < -1e30
+            other = (ok & ~low).any(-1, keepdim=True)
+            s = torch.where(low, torch.where(other, -math.inf, 0.0), s)
+            e = torch.where(low, 0.0, e + 8 * U * bias.abs())
+        e = e + 8 * U * torch.where(s == -math.inf, 0.0, s.abs())
         s = s.masked_fill(~ok, -math.inf)
         p = torch.where(ok.any(-1, keepdim=True), torch.softmax(s, -1), 0.0).nan_to_num(0.0)
         e = 2 * torch.where(ok, e, 0.0).amax(-1, keepdim=True) + 2 * Nk * U
@@ -294,6 +298,81 @@ def test_lowest_values_and_infinities_as_bias(gpu_device, dtype):
         else:
             mean = c.v.double().mean(1, keepdim=True).expand(1, 100, 2, 32)
             assert bool(((o.double() - mean).abs() <= 2 * _half(dtype) * c.v.double().abs().mean(1, keepdim=True) + 200 * U * 5).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("kw", [dict(), dict(causal=True), dict(causal=True, cap=3.0),
+                                dict(causal=True, segments=packed(1, 200, [70, 100]))],
+                         ids=["plain", "causal", "capped", "packed"])
+def test_gradients_of_rows_at_the_lowest_bias(gpu_device, dtype, kw):
+    """Keys within reach at the type's lowest value, those beyond ordinary: the first rows of a causal sequence see only
+    the former and average them, with the gradients of an average; and one head at the lowest value throughout."""
+    c = Case(gpu_device, dtype, B=1, Nq=200, H=4, Hk=2, D=32, radius=40, **kw)
+    low = torch.finfo(dtype).min
+    c.table[1:-1] = low
+    c.table[:, 3] = low
+    check(c.step(), c.exact())
+
+
+def test_large_bias_and_lengths_off_a_tile(gpu_device):
+    """Bias values whose exponential overflows: what stands behind the last query of a tile stays without weight."""
+    for Nq in (33, 70, 130):
+        c = Case(gpu_device, F32, B=1, Nq=Nq, H=2, D=32, radius=4)
+        c.table += 150.0
+        check(c.step(), c.exact())
+        c.table.requires_grad_(False).mul_(40.0)
+        check(c.step(), c.exact())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_widest_bias_and_all_buckets(gpu_device, dtype):
+    c = Case(gpu_device, dtype, B=1, Nq=1100, Nk=1150, H=2, Hk=1, D=128, radius=512, num_buckets=256, causal=True)
+    assert c.table.shape[0] == 256
+    check(c.step(), c.exact())
+
+
+def test_more_query_blocks_than_one_list(gpu_device):
+    """More than 1024 blocks of 32 queries in fp32: the keys' walk over the queries is listed in two parts."""
+    seg = packed(1, 34000, [200, 33000, 500])
+    c = Case(gpu_device, F32, B=1, Nq=34000, Nk=130, H=1, D=8, segments=(seg, torch.tensor([[0] * 40 + [1] * 40 + [2] * 45 + [-1] * 5])))
+    check(c.step(), c.exact())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("Nq,H,Hk", [(8, 8, 2), (1, 32, 1), (11, 3, 1), (1, 33, 1), (17, 4, 2)])
+def test_rows_about_one_operand(gpu_device, dtype, Nq, H, Hk):
+    """31 to 34 (query, head) rows over a key head, about the 32 that the cache kernel takes; keys of several
+    workgroups, packed and not."""
+    c = Case(gpu_device, dtype, B=2, Nq=Nq, Nk=2100, H=H, Hk=Hk, D=64, causal=True, lengths=[2100, 1025], radius=16)
+    check([c.call().detach()], c.exact(train=False))
+    c = Case(gpu_device, dtype, B=2, Nq=Nq, Nk=2100, H=H, Hk=Hk, D=64,
+             segments=(torch.full((2, Nq), 1), packed(2, 2100, [300, 1400, 200], hole=9)))
+    check([c.call().detach()], c.exact(train=False))
+    check(c.step(), c.exact())
+
+
+def test_rows_far_apart_in_memory(gpu_device):
+    """Rows of a cache 2^16 values apart, so that the last lie beyond 2^32 bytes; and the widest stride there is."""
+    room = torch.empty(36000 << 16, dtype=BF16, device=gpu_device)
+    for rows, stride, Nq in ((36000, 1 << 16, 1), (36000, 1 << 16, 60), (270, 1 << 23, 40)):
+        c = Case(gpu_device, BF16, B=1, Nq=Nq, Nk=rows, H=1, D=64, causal=True)
+        far = room[:rows * stride].view(1, rows, 1, stride)
+        far[..., :64] = c.k
+        far[..., 64:128] = c.v
+        want = c.step()
+        c.k, c.v = far[..., :64], far[..., 64:128]
+        got = c.step()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_single_row_of_any_stride(gpu_device):
+    """The stride of a dimension of one row says nothing: none, or a huge one."""
+    c = Case(gpu_device, BF16, B=2, Nq=1, H=2, D=32)
+    want = c.step()
+    q, k, v = (t.detach() for t in (c.q, c.k, c.v))
+    for stride in (0, 8, 1 << 40):
+        c.q, c.k, c.v = (t.as_strided(t.shape, (64, stride, 32, 1)) for t in (q, k, v))
+        assert all(torch.equal(a, b) for a, b in zip(c.step(), want))
 
 
 def test_scores_far_apart(gpu_device):
