@@ -281,7 +281,7 @@ __device__ __forceinline__ void copy_ints(const void* src, int n, void* lds, int
 // A capped score in log2 units, x = s_cap tanh(y) + add with s_cap = cap log2 e and y = raw scale / cap, and what the
 // tanh leaves of a gradient: slope times kSlope is 1 - tanh^2.
 // bf16 operands: by r = 1 / (1 + e^2y) of the hardware exponential and reciprocal, tanh = 1 - 2 r, 1 - tanh^2 =
-// 4 (r - r^2): six instructions, off by 2e-7 of the cap, far below the rounding of q and k.  fp32: tanhf.
+// 4 (r - r^2): six instructions, off by 2e-7 of the cap, below the rounding of q and k for caps that do something to scores.  fp32: tanhf.
 template <class T>
 struct Capped {
   float k1, k2, k3;

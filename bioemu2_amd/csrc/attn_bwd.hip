@@ -9,6 +9,10 @@
 // are so computed twice, 7 products instead of 5; adding dq over workgroups instead would need fp32 atomics (an order
 // that changes results) or as many copies of dq.
 //
+// Measured, bf16: 2 x 2048 causal tokens, 16/4 heads of 64, capped, q 71 us, kv 87 us (the capped softmax's vector
+// instructions); 4096 packed tokens, 16 heads of 24, with the table's gradient, q 56, kv 47 (the walk of the longest
+// sequence); fp32: 1000 tokens, 8 heads of 64, q 40, kv 46.
+//
 // Either may split its walk over workgroups where the rows alone do not fill the chip; attn_bwd_finish adds the parts.
 //
 // Rows whose scores' reference is at or beyond kWideRow (attn.h) take their weights against it and multiply them by the

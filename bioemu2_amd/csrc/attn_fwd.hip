@@ -9,6 +9,12 @@
 // one MFMA operand, every wave takes 32-key tiles of its own (K and V read once, bound by HBM), and the waves join.
 // Both may split the keys over workgroups (few rows, long axis); attn_join adds the parts.
 //
+// Measured, attn_fwd, bf16: 8192 causal tokens, 16/4 heads of 128, 310 to 330 us (830 to 900 TFLOP/s of the half that
+// is not masked; a large matrix product reaches 1195); 2 x 2048 causal, 16/4 heads of 64, capped, 57 us (300 TFLOP/s):
+// the vector instructions of the softmax take longer than the MFMAs there.  fp32: 1000 tokens, 8 heads of 64, 25 us
+// (82 TFLOP/s; a large fp32 matrix product 154).  attn_few: 8 single tokens over 8200 to 32768 keys of 8 heads of 128,
+// 157 us (4.9 TB/s); one over 773 keys of 16 heads of 64, 13 us, a walk of 25 tiles' latencies shared by 8 waves.
+//
 // A training call in bf16 also writes what the rounding of o took off (o_lo): the backward pass needs do . o, and with
 // it from o + o_lo the error of dq and dk falls from 1.50 to 1.46 times what rounding their results alone gives (the
 // rest is the rounding of the probabilities and of ds to the operands of the products).
@@ -617,6 +623,9 @@ int attn_args(const char* what, const bioemu_attention_args* in, AttnArgs* a) {
                      (long)Nq, (long)Nk);
   if (!(in->scale > -kInf && in->scale < kInf) || !(in->cap >= 0.f && in->cap < kInf))
     return set_error(BIOEMU_ERR_INVALID_ARG, "%s: scale %g, cap %g", what, (double)in->scale, (double)in->cap);
+  if (in->cap > 0.f && (in->cap > 1e5f || !(fabsf(in->scale) / in->cap < 1e30f)))
+    return set_error(BIOEMU_ERR_UNSUPPORTED, "%s: cap %g with scale %g (a cap is at most 1e5)", what, (double)in->cap,
+                     (double)in->scale);
   const int64_t per = in->f32 ? 4 : 8, far = int64_t(1) << 23;
   const void* ptr[3] = {in->q, in->k, in->v};
   const int64_t* st[3] = {in->q_stride, in->k_stride, in->v_stride};

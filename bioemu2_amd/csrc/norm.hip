@@ -9,6 +9,9 @@
 // y and dx are rounded once.  A lane owns the same channels of every row it meets, so the weight gradients are sums in
 // its registers; a workgroup adds its row groups in a fixed order and writes one partial row, and norm_bwd_reduce adds
 // the partial rows in a fixed order: no atomics, the same bits every time.
+//
+// Measured: 589824 rows of 128, bf16, forward 59 us (5.1 TB/s), backward 92 us (4.9 TB/s) and 5 for the partial rows;
+// 170163 rows of 64, fp32, 17 us (5.1 TB/s), 23 us (5.7 TB/s) and 4; a stream of one read and one write reaches 6.1.
 #include "common.h"
 #include "internal.h"
 
@@ -360,8 +363,8 @@ int launch_bwd(const void* x, int64_t ldx, const void* dy, int64_t ldy, const fl
   constexpr int VW = f32 ? 4 : 8;
   return for_width(f32, vec, c, [&](int vw, int lpr, int vpl) {
     dim3 grid(row_groups(rows, lpr, vw * vpl, kMaxBwdGroups));
-    if (grid.x <= 4) grid.x = 1;   // four turns of one workgroup take less than the second launch
     const bool weights = dw != nullptr || db != nullptr;
+    if (weights && grid.x <= 4) grid.x = 1;   // four turns of one workgroup take less than the second launch
     float* part = weights && grid.x > 1 ? static_cast<float*>(ws) : nullptr;
     {
       KernelTimerScope timer("norm_bwd", stream);

@@ -13,7 +13,12 @@
 // gradient goes in as three bf16 parts (hi + mid + lo hold its 24 bits).  So a wave needs no atomics and no table of
 // its own in LDS, whatever the order of the buckets, and a 32-bucket block that none of 16 pairs falls into is
 // skipped (a row's far pairs share a bucket).  Waves are added in a fixed order through LDS, workgroups by
-// relpos_bwd_reduce: the same bits every time.
+// relpos_bwd_reduce: the same bits every time.  (A gradient that is not finite reaches other buckets too: 0 times it is
+// not 0.)
+//
+// Measured: 768 x 768 pairs of 128 channels, bf16, forward with z 53 us (5.8 TB/s), backward 47 us (3.2 TB/s) and 4 for
+// the partial sums; 200 x 200 fp32, forward without z 7 us.  Backward is held by the units' loads of 4 bytes a lane,
+// one unit ahead: with what two pairs of waves a SIMD hold there is no room for a second.
 #include "common.h"
 #include "internal.h"
 

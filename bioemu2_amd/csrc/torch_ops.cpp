@@ -398,6 +398,7 @@ struct AttentionCall {
     args.D = q.size(3);
     args.scale = (float)scale;
     args.cap = (float)cap;
+    TORCH_CHECK_VALUE(cap == 0 || args.cap > 0, "attention: cap ", cap);
     args.causal = causal;
     args.f32 = is_f32(q);
   }

@@ -69,7 +69,7 @@ def relative_position(table: Tensor, buckets: Tensor, positions: Tensor, chains:
     differ, added to ``z`` if given.
 
     table: [num_buckets, C] fp32 or bf16, at most 256 rows; buckets: uint8 [2 * radius + 1] (``distance_buckets``);
-    positions, chains: whole numbers [B, N]; the result has z's type, or ``dtype`` (the table's by default), bf16 or
+    positions, chains: whole numbers of 32 bits [B, N]; the result has z's type, or ``dtype`` (the table's by default), bf16 or
     fp32.  Gradients: ``table`` and ``z``."""
     _ops.require_gpu(table, "relative_position")
     if z is not None:

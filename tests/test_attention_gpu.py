@@ -588,7 +588,7 @@ def test_refusals(gpu_device):
         (dict(segments=seg[:, :5]), "shape"), (dict(segments=seg.float()), "whole numbers"),
         (dict(key_segments=seg), "come together"),
         (dict(prefix=one[:1], causal=True), "shape"), (dict(cache_lengths=one[:1]), "shape"), (dict(cap=0.0), "cap"),
-        (dict(cap=float("inf")), "cap"), (dict(scale=float("nan")), "scale"),
+        (dict(cap=float("inf")), "cap"), (dict(cap=1e6), "cap"), (dict(cap=1e-60), "cap"), (dict(cap=1e-35), "cap"), (dict(scale=float("nan")), "scale"),
         (dict(bias_table=c.table), "buckets"), (dict(bias_buckets=c.buckets), "buckets"),
         (dict(bias_table=c.table, bias_buckets=c.buckets[:-1]), "radius"),
         (dict(bias_table=c.table[:, :3], bias_buckets=c.buckets), "shape"),
