@@ -80,6 +80,7 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void att
   __shared__ uint8_t flags[kListBlocks];
   __shared__ int red[3][4], count;
   __shared__ float ends[4][2];
+  __shared__ uint8_t which[2 * (kMaxRadius + kPad) + 1];   // buckets by offset
   extern __shared__ __attribute__((aligned(16))) float dyn[];   // bias values, sums by offset [4], blocks [4]
 
   const int item = attn_item(total, qblocks);
@@ -116,8 +117,12 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void att
   const Capped<T> capped(a);
   if (a.table) {
     fill_lut(a, h, CAP ? capped.k3 : 0.f, lut);
-    if (bias_part)
-      for (int e = threadIdx.x; e < 4 * (row4 + kDiagBlock); e += kAttnThreads) sums[e] = 0.f;
+    if (bias_part) {
+      for (int e = threadIdx.x; e < nrel; e += kAttnThreads)
+        which[e] = (uint8_t)min((int)a.buckets[min(max(e - kPad, 0), 2 * a.radius)], a.nb - 1);
+      for (int e = threadIdx.x; e < row4 + kDiagBlock; e += kAttnThreads)   // both are multiples of 4
+        reinterpret_cast<f32x4*>(sums)[e] = f32x4{};
+    }
   }
 
   const float mult = a.scale * kLog2e, out_scale = a.scale * (CAP ? Capped<T>::kSlope : 1.f);
@@ -307,20 +312,18 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void att
     }
     __syncthreads();
     // waves in order into the first one's row, then each wave a quarter of the offsets into the buckets
-    uint8_t* which = reinterpret_cast<uint8_t*>(lut);
     for (int e = threadIdx.x; e < nrel; e += kAttnThreads) {
       float v = (sums[e] + sums[row4 + e]) + (sums[2 * row4 + e] + sums[3 * row4 + e]);
       if (e == 0) v += (ends[0][0] + ends[1][0]) + (ends[2][0] + ends[3][0]);
       if (e == nrel - 1) v += (ends[0][1] + ends[1][1]) + (ends[2][1] + ends[3][1]);
       sums[e] = v;
-      which[e] = (uint8_t)min((int)a.buckets[min(max(e - kPad, 0), 2 * a.radius)], a.nb - 1);
     }
     __syncthreads();
     float* quarter = sums + 4 * row4 + wave * 256;   // over the blocks
     const int e0 = nrel * wave / 4, e1 = nrel * (wave + 1) / 4;
     for (int t = lane; t < a.nb; t += 64) {
       float v = 0.f;
-#pragma unroll 4
+#pragma unroll 16
       for (int e = e0; e < e1; ++e) v += which[e] == t ? sums[e] : 0.f;
       quarter[t] = v;
     }
