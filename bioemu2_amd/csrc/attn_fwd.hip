@@ -474,18 +474,16 @@ __global__ __launch_bounds__((64 * few_waves<T, DP>())) void attn_few_kernel(con
   }
 }
 
-// The splits' parts of a row added: by one wave (many rows), or by a workgroup whose wave w takes splits w, w + 4, ...
-// (few rows of many splits; then the waves are added), in a fixed order.  A split that saw nothing wrote no values.
+// The splits' parts of a row added, in a fixed order; a split that saw nothing wrote no values.
+// attn_join: few rows of many splits, a workgroup a row: wave w takes splits w, w + 4, ..., then the waves are added.
 // Lane d holds values d and 64 + d.
-template <class T, bool SPREAD>
+template <class T>
 __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const AttnArgs a, Parts parts, int splits,
                                                                  T* __restrict__ out, T* __restrict__ lo,
                                                                  float* __restrict__ lse) {
   __shared__ float sh[4][3][64];
-  constexpr int W = SPREAD ? 4 : 1;
   const int lane = threadIdx.x & 63, wave = wave_id();
-  const int64_t rows = (int64_t)a.B * a.Nq * a.H, row = SPREAD ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
-  if (row >= rows) return;
+  const int64_t rows = (int64_t)a.B * a.Nq * a.H, row = blockIdx.x;
   float top = -kInf;
   for (int s = lane; s < splits; s += 64) top = fmaxf(top, parts.ml[2 * (s * rows + row)]);
 #pragma unroll
@@ -493,11 +491,11 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const AttnArgs 
   const float to = top == -kInf ? 0.f : top;
   float o[2] = {0.f, 0.f}, sum = 0.f;
   const int d0 = min(lane, a.D - 1), d1 = min(lane + 64, a.D - 1);
-  for (int s0 = SPREAD ? wave : 0; s0 < splits; s0 += 4 * W) {
+  for (int s0 = wave; s0 < splits; s0 += 16) {
     float f[4], l[4], x0[4], x1[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int s = s0 + W * q;
+      const int s = s0 + 4 * q;
       const int64_t at = (s < splits ? s : s0) * rows + row;
       f[q] = s < splits ? fast_exp2(parts.ml[2 * at] - to) : 0.f;
       l[q] = parts.ml[2 * at + 1];
@@ -511,16 +509,14 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const AttnArgs 
       sum += f[q] == 0.f ? 0.f : f[q] * l[q];
     }
   }
-  if constexpr (SPREAD) {
-    sh[wave][0][lane] = o[0];
-    sh[wave][1][lane] = o[1];
-    sh[wave][2][lane] = sum;
-    __syncthreads();
-    if (wave > 0) return;
+  sh[wave][0][lane] = o[0];
+  sh[wave][1][lane] = o[1];
+  sh[wave][2][lane] = sum;
+  __syncthreads();
+  if (wave > 0) return;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) o[h] = (sh[0][h][lane] + sh[1][h][lane]) + (sh[2][h][lane] + sh[3][h][lane]);
-    sum = (sh[0][2][lane] + sh[1][2][lane]) + (sh[2][2][lane] + sh[3][2][lane]);
-  }
+  for (int h = 0; h < 2; ++h) o[h] = (sh[0][h][lane] + sh[1][h][lane]) + (sh[2][h][lane] + sh[3][h][lane]);
+  sum = (sh[0][2][lane] + sh[1][2][lane]) + (sh[2][2][lane] + sh[3][2][lane]);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -532,6 +528,37 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const AttnArgs 
     if (lo) lo[row * a.D + d] = (T)(v - (float)hi);
   }
   if (lse && lane == 0) {
+    const int64_t bi = row / a.H, h = row - bi * a.H, b = bi / a.Nq, i = bi - b * a.Nq;
+    store_log_sum(lse, rows, (b * a.H + h) * a.Nq + i, to, sum);
+  }
+}
+
+// attn_join_rows: many rows, four values of one a thread.
+template <class T>
+__global__ __launch_bounds__(kAttnThreads) void attn_join_rows_kernel(const AttnArgs a, Parts parts, int splits,
+                                                                      int rows, T* __restrict__ out,
+                                                                      T* __restrict__ lo, float* __restrict__ lse) {
+  const unsigned quads = a.D / 4, k = blockIdx.x * kAttnThreads + threadIdx.x, row = k / quads, d = (k - row * quads) * 4;
+  if ((int)row >= rows) return;
+  const f32x2* ml = reinterpret_cast<const f32x2*>(parts.ml) + row;
+  float top = -kInf;
+  for (int s = 0; s < splits; ++s) top = fmaxf(top, ml[(int64_t)s * rows][0]);
+  const float to = top == -kInf ? 0.f : top;
+  float o[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const f32x2 w = ml[(int64_t)s * rows];
+    const f32x4 x = *reinterpret_cast<const f32x4*>(parts.o + ((int64_t)s * rows + row) * a.D + d);
+    const float f = fast_exp2(w[0] - to);
+    sum += f == 0.f ? 0.f : f * w[1];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] += f == 0.f ? 0.f : f * x[c];
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+  const int64_t at = (int64_t)row * a.D + d;
+  store_quad(out + at, lo ? lo + at : nullptr, v);
+  if (lse && d == 0) {
     const int64_t bi = row / a.H, h = row - bi * a.H, b = bi / a.Nq, i = bi - b * a.Nq;
     store_log_sum(lse, rows, (b * a.H + h) * a.Nq + i, to, sum);
   }
@@ -586,12 +613,12 @@ int launch_fwd(const AttnArgs& a, void* o, void* o_lo, float* lse, void* ws, hip
   }
   if (splits == 1) return BIOEMU_OK;
   KernelTimerScope timer("attn_join", stream);
-  // 256 rows of 64 splits: 6 us spread, 10 not; 16000 rows of 2: 24 us spread
+  // 256 rows of 64 splits: 6 us by a workgroup each, 35 by quads; 32000 rows of 2: 5.6 us by quads, 13 by a wave each
   if (rows < 4 * attn_units() && splits > 4)
-    attn_join_kernel<T, true><<<dim3((unsigned)rows), kAttnThreads, 0, stream>>>(a, parts, splits, out, lo, lse);
+    attn_join_kernel<T><<<dim3((unsigned)rows), kAttnThreads, 0, stream>>>(a, parts, splits, out, lo, lse);
   else
-    attn_join_kernel<T, false><<<dim3((unsigned)((rows + 3) / 4)), kAttnThreads, 0, stream>>>(a, parts, splits, out, lo,
-                                                                                              lse);
+    attn_join_rows_kernel<T><<<dim3((unsigned)((rows * (a.D / 4) + kAttnThreads - 1) / kAttnThreads)), kAttnThreads, 0,
+                               stream>>>(a, parts, splits, (int)rows, out, lo, lse);
   return check_launch("attn_join");
 }
 
