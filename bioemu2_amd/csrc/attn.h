@@ -195,7 +195,6 @@ struct Staged<bf16, DP, ROWS> : Tile<bf16, DP, ROWS> {
   __device__ __forceinline__ void fetch(const bf16* base, int rows, int64_t stride, int D, char* lds, int wave) {
     Base::copy(base, rows, stride, D, lds, wave, kAttnThreads, off);
   }
-  __device__ __forceinline__ void store(char*) const {}
 };
 template <int DP, int ROWS>
 struct Staged<float, DP, ROWS> {
