@@ -550,6 +550,60 @@ def test_norm_relative_positions_and_attention_together(gpu_device):
         assert (g.double() - t).abs().max() <= 1e-4 * t.abs().max()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_prompt_then_tokens_as_one_pass(gpu_device, dtype):
+    """Serving: a prompt of 150 rows, then eleven single tokens and a pair against the growing cache (room for 300, NaN
+    behind what is written), within the bounds of the one causal pass over all of them."""
+    B, N, H, Hk, D = 2, 163, 8, 2, 64
+    c = Case(gpu_device, dtype, B=B, Nq=N, H=H, Hk=Hk, D=D, causal=True, radius=30, num_buckets=32)
+    (value, bound), = c.exact(train=False)
+    cache = torch.full((2, B, 300, Hk, D), math.nan, dtype=dtype, device=gpu_device)
+    at = 0
+    for n in (150, *([1] * 11), 2):
+        cache[0, :, at:at + n], cache[1, :, at:at + n] = c.k[:, at:at + n], c.v[:, at:at + n]
+        o = attention(c.q[:, at:at + n], cache[0], cache[1], causal=True, bias_table=c.table, bias_buckets=c.buckets,
+                      cache_lengths=torch.full((B,), at + n, device=gpu_device))
+        check([o], [(value[:, at:at + n], bound[:, at:at + n])])
+        at += n
+    assert at == N
+
+
+def test_two_threads_at_once(gpu_device):
+    """Two threads train on streams of their own; every step gives the bits of the same step alone."""
+    import threading
+
+    cases = [Case(gpu_device, BF16, B=1, Nq=300, H=2, D=64, radius=16, segments=packed(1, 300, [100, 150])),
+             Case(gpu_device, F32, B=2, Nq=1, Nk=2500, H=8, Hk=2, D=32, causal=True)]
+    want = [c.step() for c in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(c, w):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = c.step()
+                torch.cuda.current_stream().synchronize()
+                wrong.extend(n for n, (g, t) in enumerate(zip(got, w)) if not torch.equal(g, t))
+
+    threads = [threading.Thread(target=work, args=p) for p in zip(cases, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_gradients_of_some_inputs_only(gpu_device):
+    c = Case(gpu_device, BF16, B=1, Nq=130, H=4, Hk=2, D=32, radius=8, causal=True)
+    want = c.step()
+    leaves = (c.q, c.k, c.v, c.table)
+    for on in ((0,), (1, 2), (3,)):
+        for n, t in enumerate(leaves):
+            t.requires_grad_(n in on)
+        got = torch.autograd.grad(c.call(), [leaves[n] for n in on], c.do)
+        assert all(torch.equal(g, want[1 + n]) for g, n in zip(got, on))
+
+
 def test_fake_tensors(gpu_device):
     from torch._subclasses.fake_tensor import FakeTensorMode
 
