@@ -604,6 +604,37 @@ def test_gradients_of_some_inputs_only(gpu_device):
         assert all(torch.equal(g, want[1 + n]) for g, n in zip(got, on))
 
 
+@pytest.mark.parametrize("seed", range(40))
+def test_arguments_in_any_combination(gpu_device, seed):
+    """Sizes, types, head layouts, masks, lengths, bias and cap drawn together."""
+    import random
+
+    r = random.Random(seed)
+    B, Hk, D = r.randint(1, 3), r.randint(1, 3), r.choice([8, 16, 24, 32, 40, 64, 72, 96, 128])
+    H, Nq, Nk = Hk * r.randint(1, 4), r.choice([1, 2, 7, 31, 33, 64, 100, 129, 200, 257]), r.choice([1, 5, 32, 63, 65, 130, 255, 400, 700])
+    kw = {}
+    if r.random() < 0.5:
+        kw["causal"] = True
+        if r.random() < 0.5:
+            kw["prefix"] = [r.randint(-1, Nk + 3) for _ in range(B)]
+    if r.random() < 0.5:
+        kw["lengths"] = [r.choice([0, 1, Nk, Nk + 9, r.randint(0, Nk)]) for _ in range(B)]
+    if r.random() < 0.5:
+        ids = [-1, *range(r.randint(1, 4))]
+        order = sorted if r.random() < 0.5 else list
+        kw["segments"] = tuple(torch.tensor([order(r.choices(ids, k=n)) for _ in range(B)]) for n in (Nq, Nk))
+    if r.random() < 0.6:
+        radius = r.choice([0, 1, 9, 64, 200])
+        kw |= dict(radius=radius, num_buckets=None if radius < 120 else 32, tdtype=r.choice([None, F32, BF16]))
+    if r.random() < 0.4:
+        kw["cap"] = r.choice([0.5, 3.0, 40.0])
+    c = Case(gpu_device, r.choice([BF16, F32]), B=B, Nq=Nq, Nk=Nk, H=H, Hk=Hk, D=D, seed=seed,
+             scale=r.choice([None, None, 0.3, -0.2]), spread=r.choice([1.0, 3.0]), **kw)
+    print(seed, c.q.dtype, B, Nq, Nk, H, Hk, D, {k: v for k, v in kw.items() if k != "segments"}, flush=True)
+    check([c.call().detach()], c.exact(train=False))
+    check(c.step(), c.exact())
+
+
 def test_fake_tensors(gpu_device):
     from torch._subclasses.fake_tensor import FakeTensorMode
 
