@@ -23,6 +23,8 @@
 // bound to check, 16 reads of two values.  (One LDS add an element took 45 cycles each, 8 times the whole.)  Every wave
 // has a row of sums by offset; blocks wholly at or beyond the radius stay in registers.  Then waves, the offsets of a
 // bucket and workgroups are added in fixed orders.
+#include <algorithm>
+
 #include "attn.h"
 
 namespace bioemu {
@@ -612,12 +614,15 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_finish_kernel(const Joi
   }
 }
 
-// Workgroups that a row block's walk is split over: as many as bring the launch to two workgroups a CU (four: no
-// shorter, and the join twice as long), each with at least two blocks of the walk (fp32, 2 x 200 tokens of 16 heads: 21
-// and 15 us in three parts, 29 and 24 whole).
-int walk_splits(int64_t groups, int64_t walk, int block) {
+// Workgroups that a row block's walk is split over: as many as bring the launch to two workgroups a CU, each with at
+// least two blocks of the walk (fp32, 2 x 200 tokens of 16 heads: 21 and 15 us in three parts, 29 and 24 whole).  Long
+// causal walks (`far`; the longest takes twice the mean, and nothing is left to start beside it): up to four a CU, 1024
+// rows each at least.  q, kv and finish, bf16: 1 x 4096, 8 heads of 64, 128 us and 143 without; 1 x 8192 369 and 451;
+// 1 x 16384, 4 heads, 548 and 807; 16/4 heads of 128, 4096: 457 and 460; fp32, 8 heads of 64, 4096: 431 and 473.
+int walk_splits(int64_t groups, int64_t walk, int block, bool far) {
   const int64_t want = (2 * (int64_t)attn_units() + groups - 1) / groups, most = walk / (2 * block);
-  const int64_t s = want < most ? want : most;
+  int64_t s = want < most ? want : most;
+  if (far) s = std::max(s, std::min(4 * (int64_t)attn_units() / groups, walk / 1024));
   return s < 1 ? 1 : (int)(s < 16 ? s : 16);
 }
 
@@ -628,9 +633,10 @@ struct BwdSpace {
 BwdSpace bwd_space(const AttnArgs& a, bool f32, bool table) {
   const int64_t qblocks = (a.Nq + kGroupRows - 1) / kGroupRows, kblocks = (a.Nk + kGroupRows - 1) / kGroupRows;
   const int block = f32 ? Operand<float>::kBlock : Operand<bf16>::kBlock;
+  const bool far = a.causal && !a.q_seg && a.Nk >= 4096;
   BwdSpace s;
-  s.q_splits = walk_splits((int64_t)a.B * a.H * qblocks, a.Nk, block);
-  s.kv_splits = kblocks ? walk_splits((int64_t)a.B * a.Hk * kblocks, (int64_t)a.Nq * a.G, block) : 1;
+  s.q_splits = walk_splits((int64_t)a.B * a.H * qblocks, a.Nk, block, far);
+  s.kv_splits = kblocks ? walk_splits((int64_t)a.B * a.Hk * kblocks, (int64_t)a.Nq * a.G, block, far) : 1;
   s.stats = (size_t)round_up((int64_t)a.B * a.H * a.Nq * (a.table ? 12 : 8), 256);
   s.q_part = s.q_splits == 1 ? 0 : (size_t)round_up((int64_t)s.q_splits * a.B * a.H * a.Nq * a.D * 4, 256);
   s.kv_part = s.kv_splits == 1 ? 0 : (size_t)round_up((int64_t)s.kv_splits * 2 * a.B * a.Hk * a.Nk * a.D * 4, 256);

@@ -18,6 +18,7 @@
 // A training call in bf16 also writes what the rounding of o took off (o_lo): the backward pass needs do . o, and with
 // it from o + o_lo the error of dq and dk falls from 1.50 to 1.46 times what rounding their results alone gives (the
 // rest is the rounding of the probabilities and of ds to the operands of the products).
+#include <algorithm>
 #include <atomic>
 
 #include "attn.h"
@@ -567,17 +568,25 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_rows_kernel(const Attn
 bool few_rows(const AttnArgs& a) { return a.Nq * a.G <= 32; }
 
 // Workgroups that the keys of a query block are split over.  Long rows: as many as bring the launch to two workgroups a
-// CU, 256 keys each at least.  Few rows: sequences of a cache are of unequal length, so up to sixteen a CU that even
-// out, 512 keys each at least (8 sequences of 8200 to 32768 keys, 8 heads: 160 us in parts of 2048, 157 in parts of
-// 512), and none for up to 1024 keys, where the join costs what the shorter walk gains (773 keys: 18 us in four parts,
-// 13 in one).
-int key_splits(const AttnArgs& a) {
+// CU, 256 keys each at least.  Long causal walks (the last rows' takes twice the mean, and nothing is left to start
+// beside it): up to four a CU, 1024 keys each at least (1 x 8192, 8 heads of 64, bf16: 109 us with the join, 163 in one
+// part; heads of 128: 191 and 212; fp32, 64: 427 and 523), from where the join costs less than that gains (4096 keys,
+// heads of 64: 46 and 53; of 128: 79 and 73; 2048, 64: 58 and 59).  So too where more than two run on a CU (bf16, heads
+// of up to 32: 4096 x 4096 of 24, all seen: 80 and 90).  Segments: as short as most are, no (4096 in parts of 256: 23
+// and 16).
+// Few rows: sequences of a cache are of unequal length, so up to sixteen a CU that even out, 512 keys each at least (8
+// sequences of 8200 to 32768 keys, 8 heads: 160 us in parts of 2048, 157 in parts of 512), and none for up to 1024 keys,
+// where the join costs what the shorter walk gains (773 keys: 18 us in four parts, 13 in one).
+int key_splits(const AttnArgs& a, bool f32) {
   const bool few = few_rows(a);
   if (few && a.Nk <= 1024) return 1;
   const int64_t base = few ? (int64_t)a.B * a.Hk : (int64_t)a.B * a.H * ((a.Nq + kGroupRows - 1) / kGroupRows);
-  const int64_t want = ((few ? 16 : 2) * (int64_t)attn_units() + base - 1) / base;
-  const int64_t most = few ? (a.Nk + 511) / 512 : (a.Nk + 255) / 256;
-  const int64_t s = want < most ? want : most;
+  const int64_t units = attn_units();
+  const auto at_most = [&](int64_t want, int64_t keys) { return std::min(want, (a.Nk + keys - 1) / keys); };
+  int64_t s = few ? at_most((16 * units + base - 1) / base, 512) : at_most((2 * units + base - 1) / base, 256);
+  const int far = !f32 && a.D <= 64 ? 4096 : 8192;
+  if (!few && !a.q_seg && a.Nk >= far && (a.causal || (!f32 && a.D <= 32)))
+    s = std::max(s, std::min(4 * units / base, (int64_t)a.Nk / 1024));
   return s < 1 ? 1 : (int)s;
 }
 
@@ -587,7 +596,7 @@ size_t parts_bytes(const AttnArgs& a, int splits) {
 
 template <class T, int DP>
 int launch_fwd(const AttnArgs& a, void* o, void* o_lo, float* lse, void* ws, hipStream_t stream) {
-  const int splits = key_splits(a);
+  const int splits = key_splits(a, sizeof(T) == 4);
   const int64_t rows = (int64_t)a.B * a.Nq * a.H;
   Parts parts{static_cast<float*>(ws), nullptr};
   parts.ml = parts.o ? parts.o + (int64_t)splits * rows * a.D : nullptr;
@@ -689,7 +698,7 @@ using namespace bioemu;
 extern "C" size_t bioemu_attention_workspace_bytes(const bioemu_attention_args* args) {
   AttnArgs a;
   if (attn_args("attention", args, &a) || a.B == 0 || a.Nq == 0) return 0;
-  return parts_bytes(a, key_splits(a));
+  return parts_bytes(a, key_splits(a, args->f32 != 0));
 }
 
 extern "C" int bioemu_attention_fwd(const bioemu_attention_args* args, void* o, void* o_lo, float* lse,
@@ -700,7 +709,7 @@ extern "C" int bioemu_attention_fwd(const bioemu_attention_args* args, void* o, 
   if (!o || !aligned16(o) || !aligned16(o_lo))
     return set_error(BIOEMU_ERR_INVALID_ARG, "attention: o and o_lo must be 16-byte aligned");
   if (o_lo && args->f32) return set_error(BIOEMU_ERR_INVALID_ARG, "attention: o_lo is of bf16 calls");
-  const size_t need = parts_bytes(a, key_splits(a));
+  const size_t need = parts_bytes(a, key_splits(a, args->f32 != 0));
   if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need))
     return set_error(BIOEMU_ERR_WORKSPACE, "attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   const int dp = a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128;

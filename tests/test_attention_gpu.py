@@ -254,6 +254,21 @@ def test_long_keys_split_and_joined(gpu_device):
     check(c.step(), c.exact())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("kw", [dict(causal=True), dict(causal=True, cap=4.0, radius=30), dict()], ids=["causal", "bias_capped", "plain"])
+def test_long_walks_in_parts(gpu_device, dtype, kw):
+    """Walks long enough to be dealt to several workgroups beside those that fill the card."""
+    c = Case(gpu_device, dtype, B=1, Nq=4133, H=2, Hk=1, D=24, **kw)
+    check(c.step(), c.exact())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_longest_walks_of_wide_heads(gpu_device, dtype):
+    """A few rows at the end of 8200 keys (the gradients of all of them), heads of 128."""
+    c = Case(gpu_device, dtype, B=1, Nq=300, Nk=8200, H=2, Hk=2, D=128, causal=True)
+    check(c.step(), c.exact())
+
+
 def test_more_blocks_than_one_list(gpu_device):
     """More than 1024 blocks of 32 keys in fp32: the list of active blocks is made in two parts."""
     seg = packed(1, 34000, [200, 33000, 500])
