@@ -128,9 +128,10 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
     if (seg && wave == 0) copy_ints(kseg + k0, length - k0, segs[buf], lane);
   };
 
+  // a turn walks all blocks, or with segments those that one list can hold
   const int blocks = (wg_max + KB - 1) / KB;
-  for (int c0 = 0; c0 < blocks; c0 += kListBlocks) {
-    const int c1 = seg ? min(blocks, c0 + kListBlocks) : blocks;
+  for (int c0 = 0, c1; c0 < blocks; c0 = c1) {
+    c1 = seg ? min(blocks, c0 + kListBlocks) : blocks;
     const int n = seg ? list_blocks<KB>(kseg, length, seg_lo, seg_hi, c0, c1, flags, list, &count) : blocks;
     const int t0 = (int)((int64_t)n * split / splits), t1 = (int)((int64_t)n * (split + 1) / splits);
     auto entry = [&](int t) { return seg ? __builtin_amdgcn_readfirstlane(list[t]) : t; };

@@ -21,6 +21,7 @@ import math
 import pytest
 import torch
 
+from bioemu2_amd._lib import torch_op
 from bioemu2_amd.attention import SequenceAttention, attention
 from bioemu2_amd.layer_norm import LayerNorm
 from bioemu2_amd.relative_position import RelativePosition, distance_buckets
@@ -699,3 +700,24 @@ def test_refusals(gpu_device):
         args = dict(q=q, k=k, v=v) | kw
         with pytest.raises(ValueError, match=what):
             attention(args.pop("q"), args.pop("k"), args.pop("v"), **args)
+
+
+LONG = [(F32, 34000), (BF16, 65600)]   # just past 1024 blocks of 32 and of 64 rows
+
+
+@pytest.mark.parametrize("dtype,Nk", LONG)
+@pytest.mark.parametrize("kw", [dict(), dict(causal=True)], ids=["plain", "causal"])
+def test_log_sums_past_1024_blocks_of_keys(gpu_device, dtype, Nk, kw):
+    """Without segments every key counts once in the saved log-sum too, which dk and dv are made from.  A log-sum is off
+    by a score's error e, by n u, the adds of n weights, and by 4 u of its two parts, each below 64."""
+    c = Case(gpu_device, dtype, B=1, Nq=130, Nk=Nk, H=1, D=8, **kw)
+    got, want = c.step(), c.exact()
+    lse = torch_op("attention_train")(c.q.detach(), c.k.detach(), c.v.detach(), None, None, None, None, None, None,
+                                      8 ** -0.5, 0.0, c.causal)[2].double().sum(0) * math.log(2)
+    q, k = (t.detach().double().transpose(1, 2) for t in (c.q, c.k))
+    s = torch.matmul(q, k.transpose(2, 3).contiguous()) * 8 ** -0.5
+    size = torch.matmul(q.abs(), k.abs().transpose(2, 3).contiguous()) * 8 ** -0.5
+    exact = s.masked_fill(~c.allowed()[0][:, None], -math.inf).logsumexp(-1)
+    off = (16 * U * size + 8 * U * s.abs()).amax(-1) + Nk * U + 4 * 64 * U
+    assert bool(((lse - exact).abs() <= off).all()), (lse - exact).abs().max().item()
+    check([got[n] for n in (0, 2, 3)], [want[n] for n in (0, 2, 3)], ("o", "dk", "dv"))
