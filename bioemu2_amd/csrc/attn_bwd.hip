@@ -189,8 +189,8 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void att
   };
 
   const int blocks = (wg_max + KB - 1) / KB;
-  for (int c0 = 0; c0 < blocks; c0 += kListBlocks) {
-    const int c1 = seg ? min(blocks, c0 + kListBlocks) : blocks;
+  for (int c0 = 0, c1; c0 < blocks; c0 = c1) {   // one turn, or with segments one for each list
+    c1 = seg ? min(blocks, c0 + kListBlocks) : blocks;
     const int n = seg ? list_blocks<KB>(kseg, length, seg_lo, seg_hi, c0, c1, flags, list, &count) : blocks;
     auto entry = [&](int t) { return seg ? __builtin_amdgcn_readfirstlane(list[t]) : t; };
     const int t0 = (int)((int64_t)n * split / splits), t1 = (int)((int64_t)n * (split + 1) / splits);

@@ -721,3 +721,12 @@ def test_log_sums_past_1024_blocks_of_keys(gpu_device, dtype, Nk, kw):
     off = (16 * U * size + 8 * U * s.abs()).amax(-1) + Nk * U + 4 * 64 * U
     assert bool(((lse - exact).abs() <= off).all()), (lse - exact).abs().max().item()
     check([got[n] for n in (0, 2, 3)], [want[n] for n in (0, 2, 3)], ("o", "dk", "dv"))
+
+
+@pytest.mark.parametrize("dtype,Nk", LONG)
+@pytest.mark.parametrize("Nq,kw", [(130, dict()), (130, dict(causal=True, radius=20)), (1, dict(radius=16)),
+                                   (1, dict(causal=True, cap=4.0))], ids=["plain", "causal_bias", "token_bias", "token_capped"])
+def test_gradients_past_1024_blocks_of_keys(gpu_device, dtype, Nk, Nq, kw):
+    """Every key counts once in dq and in the table's gradient, after either form of the forward pass."""
+    c = Case(gpu_device, dtype, B=1, Nq=Nq, Nk=Nk, H=1, D=8, **kw)
+    check(c.step(), c.exact())
