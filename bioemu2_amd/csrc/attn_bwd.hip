@@ -419,8 +419,8 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, true>())) void attn
   };
 
   const int blocks = (a.Nq + QB - 1) / QB, first_block = min(wg_min, a.Nq) / QB;
-  for (int c0 = first_block; c0 < blocks; c0 += kListBlocks) {
-    const int c1 = seg ? min(blocks, c0 + kListBlocks) : blocks;
+  for (int c0 = first_block, c1; c0 < blocks; c0 = c1) {   // one turn, or with segments one for each list
+    c1 = seg ? min(blocks, c0 + kListBlocks) : blocks;
     const int n = seg ? list_blocks<QB>(qseg, a.Nq, seg_lo, seg_hi, c0, c1, flags, list, &count) : blocks - c0;
     auto entry = [&](int t) { return seg ? __builtin_amdgcn_readfirstlane(list[t]) : c0 + t; };
     // the blocks of all heads of the group, one after the other, are dealt to the splits

@@ -730,3 +730,12 @@ def test_gradients_past_1024_blocks_of_keys(gpu_device, dtype, Nk, Nq, kw):
     """Every key counts once in dq and in the table's gradient, after either form of the forward pass."""
     c = Case(gpu_device, dtype, B=1, Nq=Nq, Nk=Nk, H=1, D=8, **kw)
     check(c.step(), c.exact())
+
+
+@pytest.mark.parametrize("dtype,Nq", LONG)
+@pytest.mark.parametrize("kw", [dict(), dict(causal=True, prefix=[50]), dict(cap=4.0, radius=20)],
+                         ids=["plain", "prefix", "bias_capped"])
+def test_gradients_past_1024_blocks_of_queries(gpu_device, dtype, Nq, kw):
+    """Every query counts once in dk and dv."""
+    c = Case(gpu_device, dtype, B=1, Nq=Nq, Nk=130, H=2, Hk=1, D=8, **kw)
+    check(c.step(), c.exact())
