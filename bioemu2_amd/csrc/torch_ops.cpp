@@ -74,6 +74,14 @@ c10::TypedOperatorHandle<F> handle(const char* name) {
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants_grad(const optional<Tensor>& t) { return t && wants_grad(*t); }
 
+// Forward-mode derivatives are refused: below autograd a tangent would be dropped without a word.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool has_tangent(const optional<Tensor>& t) { return t && has_tangent(*t); }
+template <class... T>
+void check_no_tangents(const char* what, const T&... inputs) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(inputs) || ...), what, ": no forward-mode derivative");
+}
+
 // ---------------------------------------------------------------------------
 // LayerNorm
 // ---------------------------------------------------------------------------
@@ -210,6 +218,7 @@ struct LayerNormFn : Function<LayerNormFn> {
 };
 
 Tensor layer_norm_autograd(const Tensor& x, const optional<Tensor>& w, const optional<Tensor>& b, double eps) {
+  check_no_tangents("layer_norm", x, w, b);
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b)))
     return LayerNormFn::apply(x, w, b, eps);
   at::AutoDispatchBelowADInplaceOrView below;
@@ -313,6 +322,7 @@ struct RelativePositionFn : Function<RelativePositionFn> {
 
 Tensor relative_position_autograd(const Tensor& table, const optional<Tensor>& z, const Tensor& buckets,
                                   const Tensor& positions, const optional<Tensor>& chains, at::ScalarType dtype) {
+  check_no_tangents("relative_position", table, z);
   if (at::GradMode::is_enabled() && (wants_grad(table) || wants_grad(z)))
     return RelativePositionFn::apply(table, z, buckets, positions, chains, dtype);
   at::AutoDispatchBelowADInplaceOrView below;
@@ -502,6 +512,7 @@ struct AttentionFn : Function<AttentionFn> {
 };
 
 Tensor attention_autograd(ATTENTION_PARAMS) {
+  check_no_tangents("attention", q, k, v, table);
   if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(v) || wants_grad(table)))
     return AttentionFn::apply(ATTENTION_ARGS);
   at::AutoDispatchBelowADInplaceOrView below;

@@ -127,3 +127,45 @@ def test_attention_rejects_cpu_tensors():
     assert set(mod.state_dict()) == {"bias"} and mod.bias.shape == (9, 2)
     with pytest.raises(RuntimeError, match="no CPU path"):
         mod(q, q, q)
+
+
+def _op_calls():
+    """name -> (call on meta tensors, its differentiable inputs)."""
+    op = {n: _lib.torch_op(n) for n in ("layer_norm", "relative_position", "attention")}
+    meta = lambda *s, dtype=torch.float32: torch.zeros(s, dtype=dtype, device="meta")  # noqa: E731
+    buckets, positions = meta(5, dtype=torch.uint8), meta(1, 4, dtype=torch.int32)
+    return {
+        "layer_norm": (lambda x, w, b: op["layer_norm"](x, w, b, 1e-5), [meta(4, 8), meta(8), meta(8)]),
+        "relative_position": (lambda t, z: op["relative_position"](t, z, buckets, positions, None, torch.float32),
+                              [meta(6, 8), meta(1, 4, 4, 8)]),
+        "attention": (lambda q, k, v, t: op["attention"](q, k, v, t, buckets, None, None, None, None, 1.0, 0.0, False),
+                      [meta(1, 4, 2, 8) for _ in range(3)] + [meta(5, 2)]),
+    }
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "relative_position", "attention"])
+@pytest.mark.parametrize("train", [False, True])
+def test_forward_mode_derivatives_are_refused(name, train):
+    """A tangent on any input raises, with and without gradients; it is never dropped."""
+    import torch.autograd.forward_ad as fw
+
+    call, inputs = _op_calls()[name]
+    assert call(*inputs).shape is not None
+    for n, t in enumerate(inputs):
+        with fw.dual_level():
+            args = list(inputs)
+            args[n] = fw.make_dual(t.clone().requires_grad_(train), torch.zeros_like(t))
+            with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+                call(*args)
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+                call(*args)
+    with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        torch.func.jvp(call, tuple(inputs), tuple(inputs))
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "relative_position", "attention"])
+def test_functional_gradients_are_refused(name):
+    """torch.func.grad and vjp do not see the gradients; they raise."""
+    call, inputs = _op_calls()[name]
+    with pytest.raises(RuntimeError, match="functorch"):
+        torch.func.grad(lambda x: call(x, *inputs[1:]).sum())(inputs[0])
