@@ -106,13 +106,17 @@ std::pair<Tensor, int64_t> as_rows(const Tensor& x) {
   return {x.contiguous(), c};
 }
 
+void check_rows(const Tensor& x) {
+  TORCH_CHECK_VALUE(x.dim() > 0 && x.sym_size(-1) > 0, "layer_norm: x must have a last dimension, got ", x.sym_sizes());
+}
+
 struct NormParams {
   Tensor w, b;
   int bf16 = 0;
 };
 NormParams norm_params(const Tensor& x, const optional<Tensor>& w, const optional<Tensor>& b) {
   check_activation(x, "layer_norm x");
-  TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) > 0, "layer_norm: x must have a last dimension, got ", x.sizes());
+  check_rows(x);
   const int64_t c[1] = {x.size(-1)};
   NormParams p;
   if (w) p.w = parameter(*w, "layer_norm weight", c, x);
@@ -153,6 +157,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_cuda(const Tensor& x, con
                                                             const optional<Tensor>& w, bool want_x, bool want_w,
                                                             bool want_b, bool bias_bf16) {
   const c10::OptionalDeviceGuard guard(x.device());
+  check_rows(x);
   const int64_t c = x.size(-1), rows = x.numel() / c;
   check_activation(x, "layer_norm x");
   TORCH_CHECK_VALUE(dy.scalar_type() == x.scalar_type() && dy.sizes() == x.sizes(), "layer_norm_backward: dy is ",
@@ -178,16 +183,19 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_cuda(const Tensor& x, con
 }
 
 Tensor layer_norm_meta(const Tensor& x, const optional<Tensor>&, const optional<Tensor>&, double) {
+  check_rows(x);
   return at::empty_symint(x.sym_sizes(), x.options());
 }
 std::tuple<Tensor, Tensor> layer_norm_train_meta(const Tensor& x, const optional<Tensor>&, const optional<Tensor>&,
                                                  double) {
+  check_rows(x);   // rows are counted by division
   return {at::empty_symint(x.sym_sizes(), x.options()),
           at::empty_symint({x.sym_numel() / x.sym_size(-1), 2}, x.options().dtype(at::kFloat))};
 }
 std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_meta(const Tensor& x, const Tensor&, const Tensor&,
                                                             const optional<Tensor>& w, bool want_x, bool want_w,
                                                             bool want_b, bool bias_bf16) {
+  check_rows(x);
   const auto popt = x.options().dtype(norm_grad_type(w, bias_bf16));
   const c10::SymInt c = x.sym_size(-1), none = 0;
   return {want_x ? at::empty_symint(x.sym_sizes(), x.options()) : none_like(x),

@@ -169,3 +169,18 @@ def test_functional_gradients_are_refused(name):
     call, inputs = _op_calls()[name]
     with pytest.raises(RuntimeError, match="functorch"):
         torch.func.grad(lambda x: call(x, *inputs[1:]).sum())(inputs[0])
+
+
+def test_layer_norm_without_channels_is_refused():
+    """Zero channels (or none) raise, in traced calls and in their gradients too, where rows are counted by division."""
+    norm, back = _lib.torch_op("layer_norm"), _lib.torch_op("layer_norm_backward")
+    for shape in ((2, 0), (0,), ()):
+        for train in (False, True):
+            x = torch.empty(shape, device="meta", requires_grad=train)
+            with pytest.raises(ValueError, match="last dimension"):
+                norm(x, None, None, 1e-5)
+    x = torch.empty(0, 8, device="meta", requires_grad=True)
+    assert torch.autograd.grad(norm(x, None, None, 1e-5).sum(), x)[0].shape == (0, 8)
+    x = torch.empty(2, 0, device="meta")
+    with pytest.raises(ValueError, match="last dimension"):
+        back(x, x, torch.empty(2, 2, device="meta"), None, True, False, False, False)
