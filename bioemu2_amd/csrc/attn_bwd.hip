@@ -133,12 +133,12 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void att
     return raw * mult + add;
   };
 
-  // a row that sees nothing contributes nothing, whatever it holds
-  const bool on = live && lim > 0;
   const int64_t row = ((int64_t)b * a.Nq + (live ? i : 0)) * a.H + h, srow = ((int64_t)b * a.H + h) * a.Nq + i;
   // weights are 2^(x + base) row_inv; row_inv is 1 but for wide rows
   const int64_t plane = (int64_t)a.B * a.H * a.Nq;
   const float row_m = live ? lse[srow] : 0.f, row_l = live ? lse[plane + srow] : kInf;
+  // a row that sees nothing, for whatever reason, contributes nothing, whatever it holds
+  const bool on = live && lim > 0 && row_l != kInf;
   const bool row_wide = a.table && fabsf(row_m) >= kWideRow && row_l < kInf;
   const float row_inv = row_wide ? fast_exp2(-row_l) : 1.f;
   const bool wide = __ballot(row_wide) != 0;

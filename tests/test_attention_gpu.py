@@ -739,3 +739,27 @@ def test_gradients_past_1024_blocks_of_queries(gpu_device, dtype, Nq, kw):
     """Every query counts once in dk and dv."""
     c = Case(gpu_device, dtype, B=1, Nq=Nq, Nk=130, H=2, Hk=1, D=8, **kw)
     check(c.step(), c.exact())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_what_rows_that_see_nothing_hold_does_not_count(gpu_device, dtype):
+    """A query of a segment that no key has, and one whose keys all have a bias of -infinity: whatever its gradient
+    holds, it has none and gives none."""
+    k_seg = packed(2, 150, [70, 75])
+    q_seg = k_seg.clone()
+    q_seg[:, 20:25] = q_seg[:, 90] = 7
+    c = Case(gpu_device, dtype, B=2, Nq=150, H=2, D=64, segments=(q_seg, k_seg), radius=16)
+    orphan = (q_seg == 7).to(gpu_device)
+    want = c.step()
+    for value in (math.nan, math.inf):
+        c.do[orphan] = value
+        c.q.data[orphan] = value
+        got = c.step()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert all(bool((t[orphan] == 0).all()) for t in got[:2])
+    c = Case(gpu_device, dtype, B=1, Nq=60, H=2, D=32, radius=3)
+    c.table[:, 1] = -math.inf
+    want = c.step()
+    c.do[:, :, 1] = math.nan
+    got = c.step()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and bool((got[1][:, :, 1] == 0).all())
