@@ -321,10 +321,11 @@ extern "C" int bioemu_relpos_fwd(const void* table, const uint8_t* buckets, cons
   const int jt = (int)(C >= 128 ? 64 : (C >= 64 ? 128 : 256));
   const dim3 grid((unsigned)(B * N), (unsigned)((N + jt - 1) / jt));
   const int vw = f32 ? 4 : 8;
-  // 16-byte pieces; a row of more pieces than threads takes single values too
-  const bool vec = C % vw == 0 && C / vw <= kThreads && aligned16(table) && aligned16(out) && (!z || aligned16(z));
+  // 16-byte pieces of z and out (more than threads in a row, a column takes several turns); the table is read by values
+  const bool vec = C % vw == 0 && aligned16(out) && (!z || aligned16(z));
   if (!vec && C > kThreads)
-    return set_error(BIOEMU_ERR_UNSUPPORTED, "relpos: %ld channels (at most %d where they are not whole 16-byte pieces)",
+    return set_error(BIOEMU_ERR_UNSUPPORTED,
+                     "relpos: %ld channels (at most %d where rows are not whole 16-byte pieces at 16-byte addresses)",
                      (long)C, kThreads);
 #define BIOEMU_RELPOS(T, V)                                                                                         \
   relpos_fwd_kernel<T, V><<<grid, kThreads, 0, stream>>>(table, table_bf16, buckets, positions, chains,             \

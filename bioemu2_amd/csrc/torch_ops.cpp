@@ -265,7 +265,10 @@ Tensor relative_position_cuda(const Tensor& table, const optional<Tensor>& z, co
   if (z) {
     TORCH_CHECK_VALUE(z->scalar_type() == dtype, "relative_position: dtype ", dtype, ", z is ", z->scalar_type());
     check_shape(*z, "relative_position z", shape, table);
-    zc = z->contiguous();
+    // the kernel's 16-byte pieces; rows of other widths are read by values, at any address
+    zc = z->is_contiguous() && (C * z->element_size()) % 16 == 0 && reinterpret_cast<uintptr_t>(z->data_ptr()) % 16 != 0
+             ? z->clone()
+             : z->contiguous();
   }
   Tensor out = at::empty(shape, t.options().dtype(dtype));
   check_rc(bioemu_relpos_fwd(t.data_ptr(), p.buckets.data_ptr<uint8_t>(), p.positions.data_ptr<int>(),

@@ -68,7 +68,8 @@ def relative_position(table: Tensor, buckets: Tensor, positions: Tensor, chains:
     """[B, N, N, C]: ``table[bucket(positions[b, j] - positions[b, i])]``, the table's last row where ``chains``
     differ, added to ``z`` if given.
 
-    table: [num_buckets, C] fp32 or bf16, at most 256 rows; buckets: uint8 [2 * radius + 1] (``distance_buckets``);
+    table: [num_buckets, C] fp32 or bf16, at most 256 rows, C at most 4096 (256 where rows of the result are not whole
+    16-byte pieces); buckets: uint8 [2 * radius + 1] (``distance_buckets``);
     positions, chains: whole numbers of 32 bits [B, N]; the result has z's type, or ``dtype`` (the table's by default), bf16 or
     fp32.  Gradients: ``table`` and ``z``."""
     _ops.require_gpu(table, "relative_position")

@@ -483,8 +483,8 @@ int bioemu_layer_norm_bwd(const void* x, const void* dy, const float* stats, con
  * uint8, values past num_buckets - 1 count as that; positions, chains: [B, N]
  * int32 (chains may be NULL: one chain); z (may be NULL), out, dout:
  * [B, N, N, C] of the type f32 names; dtable: of table's type.
- * num_buckets is at most 256; C at most 4096, or 256 where rows are not whole
- * 16-byte vectors.
+ * num_buckets is at most 256; C at most 4096, or forward 256 where rows of z
+ * and out are not whole 16-byte vectors at 16-byte addresses.
  */
 int bioemu_relpos_fwd(const void* table, const uint8_t* buckets, const int32_t* positions, const int32_t* chains,
                       const void* z, void* out, int64_t B, int64_t N, int64_t C, int64_t radius, int64_t num_buckets,

@@ -170,3 +170,26 @@ def test_refusals(gpu_device):
         args = dict(table=table, buckets=buckets, positions=pos, chains=ch) | kw
         with pytest.raises(ValueError, match=what):
             relative_position(**args)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("C", [1016, 1024, 1028, 1032, 2048, 2056, 4096])
+def test_wide_rows(gpu_device, dtype, C):
+    """Rows of more 16-byte pieces than a workgroup has threads, up to the limit; tables and z at any address."""
+    if C % 8 and dtype == BF16:
+        pytest.skip("not whole 16-byte pieces")
+    args = _inputs(gpu_device, 2, 9, C, dtype, radius=3, chains=2, add=True)
+    want = _step(*args)
+    _check(*args, *want)
+    table, buckets, pos, ch, z, dy = args
+    odd = lambda t: torch.cat([t.new_zeros(1), t.detach().flatten()])[1:].view(t.shape)  # noqa: E731
+    moved = (odd(table).requires_grad_(True), buckets, pos, ch, odd(z), odd(dy))
+    assert moved[0].data_ptr() % 16 and moved[4].data_ptr() % 16
+    assert all(torch.equal(a, b) for a, b in zip(_step(*moved), want))
+
+
+def test_widths_past_the_limit(gpu_device):
+    for C, dtype in ((4104, BF16), (4100, F32), (260, BF16)):
+        table, buckets, pos, *_ = _inputs(gpu_device, 1, 4, C, dtype, radius=2, add=False)
+        with pytest.raises(ValueError, match="at most"):
+            relative_position(table, buckets, pos, dtype=dtype)
