@@ -88,7 +88,7 @@ __device__ __forceinline__ f32x16 mfma16(f32x8 x, f32x8 y, f32x16 c) { return mf
 // Written as instructions: the compiler lets every later LDS read wait for a copy that it knows of, and these are to
 // land while the tile before them is worked on.  They have no result registers; whoever reads what they bring waits
 // for vmcnt first (and for the workgroup's barrier where another wave made the copy).  M0 is set and used within one
-// statement; nothing else in these kernels uses it.
+// statement, which names it as overwritten.
 __device__ __forceinline__ u32x4 copy_source(const void* base, unsigned bytes) {
   const uint64_t p = reinterpret_cast<uint64_t>(base);
   return u32x4{(unsigned)p, (unsigned)(p >> 32) & 0xffffu, bytes, 0x00020000u};
@@ -99,11 +99,11 @@ __device__ __forceinline__ void copy_to_lds(u32x4 source, unsigned voff, void* l
   if constexpr (BYTES == 16)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(voff),
                  "s"(source)
-                 : "memory");
+                 : "memory", "m0");
   else
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(at), "v"(voff),
                  "s"(source)
-                 : "memory");
+                 : "memory", "m0");
 }
 
 // Row swizzle of 16-byte pieces, by pieces per row (a power of two).  A read of 32 rows' pieces takes rows that differ
