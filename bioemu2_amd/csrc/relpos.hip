@@ -13,8 +13,8 @@
 // gradient goes in as three bf16 parts (hi + mid + lo hold its 24 bits).  So a wave needs no atomics and no table of
 // its own in LDS, whatever the order of the buckets, and a 32-bucket block that none of 16 pairs falls into is
 // skipped (a row's far pairs share a bucket).  Waves are added in a fixed order through LDS, workgroups by
-// relpos_bwd_reduce: the same bits every time.  (A gradient that is not finite reaches other buckets too: 0 times it is
-// not 0.)
+// relpos_bwd_reduce: the same bits every time.  0 times a gradient that is not finite is not 0: a wave whose sums are not
+// finite adds its pairs again one by one.
 //
 // Measured: 768 x 768 pairs of 128 channels, bf16, forward with z 53 us (5.8 TB/s), backward 47 us (3.2 TB/s; 2304 x
 // 2304 pairs 262 us, 5.2 TB/s: the first loads and the sums over waves take some 8 us of any call) and 4 for the
@@ -161,15 +161,17 @@ __global__ __launch_bounds__(kBwdThreads) void relpos_bwd_kernel(const T* __rest
   // a unit is unit_pairs() pairs of one row: unit u = row * cols + piece.  The next one's values and bucket are on their way
   // while one is multiplied.
   constexpr int S = unit_pairs<T>() / 16;
+  const auto lane_bucket = [&](int row, int j0) {   // of the lane's pair, from nb0; 0xffff: none of this workgroup's
+    if (lane >= 16 * S || j0 + lane >= n) return 0xffff;
+    const int j = row / n * n + j0 + lane;
+    const int bk =
+        pair_bucket(pos[row], pos[j], chains ? chains[row] : 0, chains ? chains[j] : 0, buckets, radius, nb) - nb0;
+    return bk < 0 || bk >= kBwdBlocks * 32 ? 0xffff : bk;
+  };
   const auto fetch = [&](int u, Two (&g)[S][8], int& bk) {
-    const int row = u / cols, j0 = (u - row * cols) * (16 * S), b = row / n;
+    const int row = u / cols, j0 = (u - row * cols) * (16 * S);
     const T* base = dout + ((int64_t)row * n + j0) * c;
-    bk = 0xffff;
-    if (lane < 16 * S && j0 + lane < n) {
-      const int j = b * n + j0 + lane;
-      bk = pair_bucket(pos[row], pos[j], chains ? chains[row] : 0, chains ? chains[j] : 0, buckets, radius, nb) - nb0;
-      bk = bk < 0 || bk >= kBwdBlocks * 32 ? 0xffff : bk;
-    }
+    bk = lane_bucket(row, j0);
 #pragma unroll
     for (int s = 0; s < S; ++s)
 #pragma unroll
@@ -237,6 +239,36 @@ __global__ __launch_bounds__(kBwdThreads) void relpos_bwd_kernel(const T* __rest
   }
 
   // acc[q][e], lane (ln, lh), register 4 r + k: bucket 32 q + ln, channel 2 (8 r + 4 lh + k) + e
+  bool finite = true;
+#pragma unroll
+  for (int q = 0; q < NBB; ++q)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        finite = finite && (__builtin_bit_cast(uint32_t, (float)acc[q][e][i]) & 0x7f800000u) != 0x7f800000u;
+  if (__ballot(!finite)) {
+#pragma unroll
+    for (int q = 0; q < NBB; ++q) acc[q][0] = acc[q][1] = zero16();
+    for (u = blockIdx.x * Waves + wave; u < units; u += step) {
+      const int row = u / cols, j0 = (u - row * cols) * (16 * S), bks_here = lane_bucket(row, j0);
+      const T* src = dout + ((int64_t)row * n + j0) * c;
+#pragma unroll 1
+      for (int p = 0; p < min(16 * S, n - j0); ++p, src += c) {
+        const int bk = __shfl(bks_here, p);
+#pragma unroll
+        for (int q = 0; q < NBB; ++q)
+          if (bk == 32 * q + ln)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const int ch = c0 + 2 * (8 * (i >> 2) + 4 * lh + (i & 3)) + e;
+                if (ch < c) acc[q][e][i] += (float)src[ch];
+              }
+      }
+    }
+  }
   // waves 0 .. 3 lay theirs down, 4 .. 7 add to them
   for (int w = 0; w < 2; ++w) {
     if (wave / 4 == w) {

@@ -193,3 +193,26 @@ def test_widths_past_the_limit(gpu_device):
         table, buckets, pos, *_ = _inputs(gpu_device, 1, 4, C, dtype, radius=2, add=False)
         with pytest.raises(ValueError, match="at most"):
             relative_position(table, buckets, pos, dtype=dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("N,C,radius", [(9, 16, 2), (70, 128, 32), (130, 33, 100)])
+def test_gradients_that_are_not_finite_reach_their_own_bucket(gpu_device, dtype, N, C, radius):
+    """Infinities, NaN and the type's largest values in some pairs: the sums of every other bucket and channel are as
+    without them, within the bounds of any order of adds."""
+    table, buckets, pos, ch, z, dy = _inputs(gpu_device, 2, N, C, dtype, radius, chains=2, add=False)
+    pos = torch.arange(N, dtype=torch.int32, device=gpu_device).expand(2, N).contiguous()
+    for i, j, channel, value in ((1, 3, 2, math.inf), (4, 4, C - 1, -math.inf), (5, 7, 0, math.nan),
+                                 (8, 0, 5, torch.finfo(dtype).max), (2, 2, C - 1, math.inf)):
+        dy[1, i, j, channel] = value
+    _, dt = _step(table, buckets, pos, ch, None, dy)
+    t = _which(table, buckets, pos, ch).reshape(-1)
+    flat = dy.double().reshape(-1, C)
+    zeros = torch.zeros(table.shape, dtype=torch.float64, device=gpu_device)
+    want, size = zeros.index_add(0, t, flat), zeros.index_add(0, t, flat.abs())
+    special = ~(want.abs() <= 1e38)
+    assert 3 <= int(special.sum()) <= 5
+    assert bool(((dt.double() - want).abs() <= 2 * N * N * 3 * U * size)[~special].all())
+    assert bool(torch.equal(dt.double()[special].nan_to_num(0.5, 1.0, -1.0).sign(),
+                            want[special].nan_to_num(0.5, 1.0, -1.0).sign()))
+    assert bool((dt.isnan() == want.isnan()).all())
