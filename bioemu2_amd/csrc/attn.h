@@ -87,8 +87,8 @@ __device__ __forceinline__ f32x16 mfma16(f32x8 x, f32x8 y, f32x16 c) { return mf
 // Copies from memory into LDS: lane i's BYTES at byte voff of the source go to lds + BYTES i; zeros past its end.
 // Written as instructions: the compiler lets every later LDS read wait for a copy that it knows of, and these are to
 // land while the tile before them is worked on.  They have no result registers; whoever reads what they bring waits
-// for vmcnt first (and for the workgroup's barrier where another wave made the copy).  M0 is set and used within one
-// statement, which names it as overwritten.
+// for vmcnt first (and for the workgroup's barrier where another wave made the copy).  The LDS address is an operand
+// in M0, which the compiler sets (s_nop: the state between that and its use by a copy).
 __device__ __forceinline__ u32x4 copy_source(const void* base, unsigned bytes) {
   const uint64_t p = reinterpret_cast<uint64_t>(base);
   return u32x4{(unsigned)p, (unsigned)(p >> 32) & 0xffffu, bytes, 0x00020000u};
@@ -97,13 +97,9 @@ template <int BYTES>
 __device__ __forceinline__ void copy_to_lds(u32x4 source, unsigned voff, void* lds) {
   const unsigned at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
   if constexpr (BYTES == 16)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(voff),
-                 "s"(source)
-                 : "memory", "m0");
+    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(source), "{m0}"(at) : "memory");
   else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(at), "v"(voff),
-                 "s"(source)
-                 : "memory", "m0");
+    asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(source), "{m0}"(at) : "memory");
 }
 
 // Row swizzle of 16-byte pieces, by pieces per row (a power of two).  A read of 32 rows' pieces takes rows that differ
