@@ -45,7 +45,8 @@ def attention(
     they come.  The queries are the last Nq of ``cache_lengths[b]`` positions (default Nk): p_i = length - Nq + i.
     Keys at or past the length are not seen, whatever they hold.
 
-    scale: D ** -0.5 by default.  cap: none by default; at most 1e5 (in bf16 scores are off by 2e-7 of it).
+    scale: D ** -0.5 by default.  cap: none by default; at most 1e5 (in bf16 scores are off by 2e-7 of it up to 4096,
+    by fp32 rounding beyond).
     bias_table ([num_buckets, H], fp32 or bf16) and bias_buckets (``distance_buckets``, radius at most 512): the bias is
     ``bias_table[bias_buckets[clamp(j - p_i, -radius, radius) + radius], h]``.
     segments ([B, Nq] whole numbers of 32 bits): a query sees keys of its own segment only, and a negative one

@@ -69,7 +69,7 @@ constexpr int bwd_waves() {
   return sizeof(T) == 2 && KV && DP == 64 ? 2 : 1;
 }
 
-template <class T, int DP, bool CAP>
+template <class T, int DP, int CAP>
 __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void attn_bwd_q_kernel(
     const AttnArgs a, const T* __restrict__ o, const T* __restrict__ o_lo, const float* __restrict__ lse, const T*
     __restrict__ dout, int64_t db, int64_t dn, int64_t dh, T* __restrict__ dq, float* __restrict__ stats, float*
@@ -116,7 +116,7 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void att
   wave_max = __builtin_amdgcn_readfirstlane(wave_max);
   const int wave_pos = __builtin_amdgcn_readfirstlane(pos);
 
-  const Capped<T> capped(a);
+  const Capped<T, CAP> capped(a);
   if (a.table) {
     fill_lut(a, h, CAP ? capped.k3 : 0.f, lut);
     if (bias_part) {
@@ -127,9 +127,9 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void att
     }
   }
 
-  const float mult = a.scale * kLog2e, out_scale = a.scale * (CAP ? Capped<T>::kSlope : 1.f);
+  const float mult = a.scale * kLog2e, out_scale = a.scale * (CAP != kUncapped ? Capped<T, CAP>::kSlope : 1.f);
   const auto score = [&](float raw, float add, float& slope) {
-    if constexpr (CAP) return capped.score(raw, add, slope);
+    if constexpr (CAP != kUncapped) return capped.score(raw, add, slope);
     return raw * mult + add;
   };
 
@@ -284,7 +284,7 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void att
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
           }
         }
-        if constexpr (CAP)
+        if constexpr (CAP != kUncapped)
 #pragma unroll
           for (int r = 0; r < 16; ++r) x[r] *= slope[r];
 #pragma unroll
@@ -337,7 +337,7 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, false>())) void att
   }
 }
 
-template <class T, int DP, bool CAP>
+template <class T, int DP, int CAP>
 __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, true>())) void attn_bwd_kv_kernel(
     const AttnArgs a, const float* __restrict__ row_stats, const T* __restrict__ dout, int64_t db, int64_t dn,
     int64_t dh, T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ part, int splits, int kblocks, int
@@ -398,10 +398,10 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, true>())) void attn
   f32x16 ak[DB], av[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) ak[d] = av[d] = zero16();
-  const Capped<T> capped(a);
-  const float mult = a.scale * kLog2e, out_scale = a.scale * (CAP ? Capped<T>::kSlope : 1.f);
+  const Capped<T, CAP> capped(a);
+  const float mult = a.scale * kLog2e, out_scale = a.scale * (CAP != kUncapped ? Capped<T, CAP>::kSlope : 1.f);
   const auto score = [&](float raw, float add, float& slope) {
-    if constexpr (CAP) return capped.score(raw, add, slope);
+    if constexpr (CAP != kUncapped) return capped.score(raw, add, slope);
     return raw * mult + add;
   };
 
@@ -528,7 +528,7 @@ __global__ __launch_bounds__(kAttnThreads, (bwd_waves<T, DP, true>())) void attn
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             x[r] *= dp[r];
-            if constexpr (CAP) x[r] *= slope[r];
+            if constexpr (CAP != kUncapped) x[r] *= slope[r];
           }
 #pragma unroll
           for (int st = 0; st < 2; ++st) {
@@ -645,7 +645,7 @@ BwdSpace bwd_space(const AttnArgs& a, bool f32, bool table) {
   return s;
 }
 
-template <class T, int DP, bool CAP>
+template <class T, int DP, int CAP>
 int launch_bwd_as(const AttnArgs& a, const void* o, const void* o_lo, const float* lse, const void* dout,
                   const int64_t* ds, void* dq, void* dk, void* dv, void* dtable, void* ws, hipStream_t stream) {
   const BwdSpace sp = bwd_space(a, sizeof(T) == 4, dtable != nullptr);
@@ -688,8 +688,12 @@ int launch_bwd_as(const AttnArgs& a, const void* o, const void* o_lo, const floa
 template <class T, int DP>
 int launch_bwd(const AttnArgs& a, const void* o, const void* o_lo, const float* lse, const void* dout, const int64_t* ds,
                void* dq, void* dk, void* dv, void* dtable, void* ws, hipStream_t stream) {
-  return a.cap > 0.f ? launch_bwd_as<T, DP, true>(a, o, o_lo, lse, dout, ds, dq, dk, dv, dtable, ws, stream)
-                     : launch_bwd_as<T, DP, false>(a, o, o_lo, lse, dout, ds, dq, dk, dv, dtable, ws, stream);
+  if (!(a.cap > 0.f))
+    return launch_bwd_as<T, DP, kUncapped>(a, o, o_lo, lse, dout, ds, dq, dk, dv, dtable, ws, stream);
+  if constexpr (sizeof(T) == 2)
+    if (!fast_cap<T>(a))
+      return launch_bwd_as<T, DP, kCapWide>(a, o, o_lo, lse, dout, ds, dq, dk, dv, dtable, ws, stream);
+  return launch_bwd_as<T, DP, kCapped>(a, o, o_lo, lse, dout, ds, dq, dk, dv, dtable, ws, stream);
 }
 
 }  // namespace

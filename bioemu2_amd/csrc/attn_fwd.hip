@@ -49,7 +49,7 @@ __device__ __forceinline__ void store_quad(T* out, T* lo, const float (&v)[4]) {
   if (lo) *reinterpret_cast<quad*>(lo) = rest;
 }
 
-template <class T, int DP, bool CAP>
+template <class T, int DP, int CAP>
 __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a, T* __restrict__ out,
                                                                 T* __restrict__ lo, float* __restrict__ lse,
                                                                 Parts parts, int splits,
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
   const int wave_pos = __builtin_amdgcn_readfirstlane(pos);   // of the wave's first row
   if (!live) lim = 0x7fffffff;
 
-  const Capped<T> capped(a);
+  const Capped<T, CAP> capped(a);
   if (a.table) fill_lut(a, h, CAP ? capped.k3 : 0.f, lut);
 
   Frag<T> qf[STEPS];
@@ -116,7 +116,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const AttnArgs a
   const float mult = a.scale * kLog2e;
   const auto score = [&](float raw, float add) {
     float slope;
-    if constexpr (CAP) return capped.score(raw, add, slope);
+    if constexpr (CAP != kUncapped) return capped.score(raw, add, slope);
     return raw * mult + add;
   };
 
@@ -276,7 +276,8 @@ constexpr int vmcnt(int n) { return 0x0f70 | (n & 15) | ((n >> 4) << 14); }
 
 // chunk: 32-key tiles of one split.  Splits are of equal length whatever the sequences' lengths (those past a
 // sequence's end do nothing), and workgroups take them in plain order, round the XCDs: no two share a key.
-template <class T, int DP>
+// CAP: kCapped (whether there is a cap is asked at run time, beside the latency of the copies) or kCapWide.
+template <class T, int DP, int CAP>
 __global__ __launch_bounds__((64 * few_waves<T, DP>())) void attn_few_kernel(const AttnArgs a, T* __restrict__ out,
                                                                            T* __restrict__ lo,
                                                                            float* __restrict__ lse, Parts parts,
@@ -341,7 +342,7 @@ __global__ __launch_bounds__((64 * few_waves<T, DP>())) void attn_few_kernel(con
 #pragma unroll
   for (int d = 0; d < DB; ++d) acc[d] = zero16();
   float m = -kInf, mref = 0.f, l = 0.f;
-  const Capped<T> capped(a);
+  const Capped<T, CAP> capped(a);
   const float mult = a.scale * kLog2e;
 
   // K of the next tile is on its way while V of this one is waited for and used, and V while K is: a tile's copies are
@@ -605,20 +606,29 @@ int launch_fwd(const AttnArgs& a, void* o, void* o_lo, float* lse, void* ws, hip
   if (few_rows(a)) {
     const int tiles = (a.Nk + 31) / 32, chunk = (tiles + splits - 1) / splits;
     KernelTimerScope timer("attn_few", stream);
-    attn_few_kernel<T, DP><<<dim3((unsigned)(a.B * a.Hk * splits)), 64 * few_waves<T, DP>(), 0, stream>>>(
-        a, out, lo, lse, parts, splits, chunk);
+    const dim3 grid((unsigned)(a.B * a.Hk * splits));
+    const auto launch = [&](auto kernel) {
+      kernel<<<grid, 64 * few_waves<T, DP>(), 0, stream>>>(a, out, lo, lse, parts, splits, chunk);
+    };
+    if (fast_cap<T>(a))
+      launch(attn_few_kernel<T, DP, kCapped>);
+    else if constexpr (sizeof(T) == 2)
+      launch(attn_few_kernel<T, DP, kCapWide>);
     if (const int rc = check_launch("attn_few")) return rc;
   } else {
     const int qblocks = (a.Nq + kGroupRows - 1) / kGroupRows;
     const int64_t total = (int64_t)a.B * a.H * splits * qblocks;
     KernelTimerScope timer("attn_fwd", stream);
     const dim3 grid(attn_grid(total));
-    if (a.cap > 0.f)
-      attn_fwd_kernel<T, DP, true><<<grid, kAttnThreads, 0, stream>>>(a, out, lo, lse, parts, splits, qblocks,
-                                                                     (int)total);
-    else
-      attn_fwd_kernel<T, DP, false><<<grid, kAttnThreads, 0, stream>>>(a, out, lo, lse, parts, splits, qblocks,
-                                                                      (int)total);
+    const auto launch = [&](auto kernel) {
+      kernel<<<grid, kAttnThreads, 0, stream>>>(a, out, lo, lse, parts, splits, qblocks, (int)total);
+    };
+    if (!(a.cap > 0.f))
+      launch(attn_fwd_kernel<T, DP, kUncapped>);
+    else if (fast_cap<T>(a))
+      launch(attn_fwd_kernel<T, DP, kCapped>);
+    else if constexpr (sizeof(T) == 2)
+      launch(attn_fwd_kernel<T, DP, kCapWide>);
     if (const int rc = check_launch("attn_fwd")) return rc;
   }
   if (splits == 1) return BIOEMU_OK;

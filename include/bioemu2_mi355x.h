@@ -503,7 +503,7 @@ int bioemu_relpos_bwd(const void* dout, const uint8_t* buckets, const int32_t* p
  * Allowed: j < length; segments equal and not negative, where given; where
  * causal, also j <= pos_i or j < prefix.  A key at or past its length, or of a
  * negative segment, may hold anything.  cap = 0: no tanh; at most 1e5 (bf16:
- * scores are off by 2e-7 of it).
+ * scores are off by 2e-7 of it up to 4096, by fp32 rounding beyond).
  * Strides (batch, row, head) are in elements, values of a head adjacent, every
  * row at a 16-byte address, the row stride between D and 2^23.  D is a
  * multiple of 8 up to 128, radius at most 512, num_buckets at most 256; bucket

@@ -763,3 +763,33 @@ def test_what_rows_that_see_nothing_hold_does_not_count(gpu_device, dtype):
     c.do[:, :, 1] = math.nan
     got = c.step()
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and bool((got[1][:, :, 1] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("cap", [30.0, 4096.0, 4097.0, 1e5])
+@pytest.mark.parametrize("Nq", [1, 70])
+def test_capped_scores_themselves(gpu_device, dtype, D, cap, Nq):
+    """Every query sees one key, so its log-sum is its score and its weight is 1 in both directions.  A score is off by
+    (D + 8) u of its product and 16 u of itself (scale, cap, bias, log2 e, the tanh's few last places); up to a cap of
+    4096 in bf16 by 4e-7 of the cap more."""
+    n = torch.arange(Nq)[None]
+    c = Case(gpu_device, dtype, B=1, Nq=Nq, H=2, D=D, segments=n, cap=cap, radius=2, spread=4.0)
+    want = c.exact()
+    lse = torch_op("attention_train")(c.q, c.k, c.v, c.table, c.buckets, c.segments, c.segments, None, None, D ** -0.5,
+                                      cap, False)[2].double().sum(0) * math.log(2)
+    q, k = (t.double().transpose(1, 2) for t in (c.q, c.k))
+    x, size = (q * k).sum(-1) * D ** -0.5, (q * k).abs().sum(-1) * D ** -0.5
+    bias = c.table.double()[2][None, :, None]
+    s = cap * torch.tanh(x / cap)
+    off = (D + 8) * U * size + 16 * U * (s.abs() + bias.abs()) + (4e-7 * cap if dtype == BF16 and cap <= 4096 else 0.0)
+    err = (lse - s - bias).abs()
+    print(f"off {err.max().item():.2e}, allowed {off.max().item():.2e}", flush=True)
+    assert bool((err <= off).all())
+    got = c.step()
+    check(got, want)
+    assert torch.equal(got[0], c.v.detach())
+    # the backward pass takes its weight from a score summed in another order and the log-sum: 1 off by 2 off + 8 u, and
+    # rounded as an operand and as the result
+    off = (2 * off + 8 * U + 2 * _half(dtype)).transpose(1, 2)[..., None]
+    assert bool(((got[3] - c.do).double().abs() <= off * c.do.double().abs()).all())
