@@ -9,8 +9,8 @@
 // are so computed twice, 7 products instead of 5; adding dq over workgroups instead would need fp32 atomics (an order
 // that changes results) or as many copies of dq.
 //
-// Measured, bf16: 2 x 2048 causal tokens, 16/4 heads of 64, capped, q 71 us, kv 87 us (the capped softmax's vector
-// instructions); 4096 packed tokens, 16 heads of 24, with the table's gradient, q 56, kv 47 (the walk of the longest
+// Measured, bf16: 2 x 2048 causal tokens, 16/4 heads of 64, capped, q 72 us, kv 85 us (the capped softmax's vector
+// instructions); 4096 causal tokens, 16/4 heads of 128, q 199, kv 241 (266 and 334 registers: one wave a SIMD); 4096 packed tokens, 16 heads of 24, with the table's gradient, q 56, kv 47 (the walk of the longest
 // sequence); fp32: 1000 tokens, 8 heads of 64, q 40, kv 46.
 //
 // Either may split its walk over workgroups where the rows alone do not fill the chip; attn_bwd_finish adds the parts.

@@ -9,11 +9,13 @@
 // one MFMA operand, every wave takes 32-key tiles of its own (K and V read once, bound by HBM), and the waves join.
 // Both may split the keys over workgroups (few rows, long axis); attn_join adds the parts.
 //
-// Measured, attn_fwd, bf16: 8192 causal tokens, 16/4 heads of 128, 310 to 330 us (830 to 900 TFLOP/s of the half that
-// is not masked; a large matrix product reaches 1195); 2 x 2048 causal, 16/4 heads of 64, capped, 57 us (300 TFLOP/s):
+// Measured, attn_fwd, bf16: 8192 causal tokens behind a prefix of 1000, 16/4 heads of 128, 286 to 298 us called on and on
+// (936 to 975 TFLOP/s of what is not masked; a large matrix product reaches 1195), 306 to 371 under the profiler, whose
+// calls stand apart; 2 x 2048 causal, 16/4 heads of 64, capped, 58 us (300 TFLOP/s):
 // the vector instructions of the softmax take longer than the MFMAs there.  fp32: 1000 tokens, 8 heads of 64, 25 us
 // (82 TFLOP/s; a large fp32 matrix product 154).  attn_few: 8 single tokens over 8200 to 32768 keys of 8 heads of 128,
-// 157 us (4.9 TB/s); one over 773 keys of 16 heads of 64, 13 us, a walk of 25 tiles' latencies shared by 8 waves.
+// 157 us (4.9 TB/s), over 32768 keys each 259 and in fp32 439; one over 773 keys of 16 heads of 64, 13 us, a walk of 25
+// tiles' latencies shared by 8 waves; one over 8192 keys of 8 heads of 128, 19 us, in fp32 (two waves) 45.
 //
 // A training call in bf16 also writes what the rounding of o took off (o_lo): the backward pass needs do . o, and with
 // it from o + o_lo the error of dq and dk falls from 1.50 to 1.46 times what rounding their results alone gives (the
@@ -578,7 +580,8 @@ bool few_rows(const AttnArgs& a) { return a.Nq * a.G <= 32; }
 // and 16).
 // Few rows: sequences of a cache are of unequal length, so up to sixteen a CU that even out, 512 keys each at least (8
 // sequences of 8200 to 32768 keys, 8 heads: 160 us in parts of 2048, 157 in parts of 512), and none for up to 1024 keys,
-// where the join costs what the shorter walk gains (773 keys: 18 us in four parts, 13 in one).
+// where the join costs what the shorter walk gains (773 keys: 18 us in four parts, 13 in one).  Both bounds were measured
+// in bf16 at these sizes only; one or two sequences, and fp32, whose waves are fewer, take them as they are.
 int key_splits(const AttnArgs& a, bool f32) {
   const bool few = few_rows(a);
   if (few && a.Nk <= 1024) return 1;
