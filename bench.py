@@ -4,8 +4,8 @@
 
 A "step" is one forward pass of the selected op over one batch of synthetic,
 HBM-resident input.  The default op is one full bf16 Pairformer block at N=768,
-c_z=128, c_s=384 (the BASELINE metric); the default run then measures every
-BASELINE config the same way (configs 1-5: the N=64 fp32-I/O block, pair-bias
+c_z=128, c_s=384 (the headline metric); the default run then measures five more
+workloads the same way (the N=64 fp32-I/O block, pair-bias
 attention B=8 N=512, the fused OPM, the four triangle ops at N=768 and one pass
 of the 48-block trunk at N=2048) and adds them under ``configs``.  ``--op``
 selects a single op at its config shape instead (a diagnostic line).
@@ -76,7 +76,7 @@ def cpu_baseline(wl) -> dict:
     """
     import torch
 
-    import oracle  # the checker, timed here as the CPU baseline only
+    import oracle  # timed here as the CPU baseline only
 
     threads = os.cpu_count() or 1
     torch.set_num_threads(threads)
@@ -116,7 +116,7 @@ def _cpu_model() -> str:
     return "unknown"
 
 
-# The five BASELINE configs measured after the headline line's own workload (the default run): name ->
+# The five workloads measured after the headline line's own workload (the default run): name ->
 # (workloads.make op, steps, warm-up steps, CPU-baseline warm-ups, CPU-baseline timed calls).  Config 4 is the
 # four triangle ops at N = 768; config 5 one pass of the 48-block trunk at N = 2048, whose CPU baseline is one
 # oracle block at N = 512 scaled to the pass by algorithmic flops.
@@ -218,7 +218,7 @@ def measure(wl, steps: int, warmup: int, with_cpu: bool, kernels_to_stderr: bool
 
 
 def measure_configs(dev, with_cpu: bool) -> dict:
-    """Every BASELINE config on this GPU, one after another (each workload freed before the next)."""
+    """Every workload of CONFIGS on this GPU, one after another (each workload freed before the next)."""
     import torch
 
     from bioemu2_amd import workloads

@@ -227,10 +227,10 @@ def block_flops(n: int, c: int = 128, cs: int = 384, n_valid: int | None = None)
 
 
 class BlockWorkload(Workload):
-    """The BASELINE metric: one full bf16 Pairformer block at N=768 (config 4 + s [1,768,384]).
+    """The headline metric: one full bf16 Pairformer block at N=768 (c_z=128, s [1,768,384]).
 
     With ``tails`` (the default) the residual streams z and s carry int8 tails, the path held to the
-    north_star bound against the fp32 oracle; without them they are plain bf16 (rounded after every add,
+    2e-2 bound against the fp32 oracle; without them they are plain bf16 (rounded after every add,
     as the reference's bf16-autocast trunk stores them)."""
 
     cpu_warmup = 1
@@ -241,8 +241,8 @@ class BlockWorkload(Workload):
 
         self.n = n
         self.tails = tails
-        # padded (masked) trailing tokens: 10 % at the BASELINE size (config 4,
-        # 76 of 768), 5 % at the 48-block trunk size (config 5, 102 of 2048)
+        # padded (masked) trailing tokens: 10 % at N = 768 (76 of them), 5 % at the
+        # 48-block trunk's size (102 of 2048)
         self.n_pad = n // 20 if n >= 2048 else n // 10
         self.name = f"pairformer_block_n{n}" + ("" if tails else "_bf16stream")
         self.metric = f"ms per Pairformer block at N={n} bf16"

@@ -1,6 +1,6 @@
 """CPU oracle for the Pairformer hot path — TEST INFRASTRUCTURE ONLY.
 
-This package is the checker, never the product.  Only ``tests/``,
+This package is what results are tested against, never the product.  Only ``tests/``,
 ``__graft_entry__.smoke()`` and the ``cpu_baseline`` leg of ``bench.py`` may
 import it.  The product path (``bioemu2_amd``) never routes through it and
 fails loudly when its HIP library is missing.
