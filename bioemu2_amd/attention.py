@@ -51,7 +51,8 @@ def attention(
     ``bias_table[bias_buckets[clamp(j - p_i, -radius, radius) + radius], h]``.
     segments ([B, Nq] whole numbers of 32 bits): a query sees keys of its own segment only, and a negative one
     (padding) neither sees nor is seen, whatever it holds; key_segments ([B, Nk]) where the keys are others.  Values
-    that a query does not see for another reason have to be finite.
+    that a query does not see for another reason have to be finite; one that is not, where it is seen, reaches the result
+    (in fp32 an infinity as NaN).
     causal: only keys j <= p_i, and those below ``prefix[b]`` ([B] whole numbers; nothing to say without causal)."""
     _ops.require_gpu(q, "attention")
     if q.ndim != 4:
