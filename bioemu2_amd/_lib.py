@@ -33,7 +33,33 @@ class AttentionArgs(ctypes.Structure):
     )
 
 
+class RotaryArgs(ctypes.Structure):
+    """``bioemu_rotary_args`` (strides one by one)."""
+
+    _fields_ = (
+        [(n, _c_void_p) for n in ("q", "k")]
+        + [(f"{t}_{n}", _c_int64) for t in ("q", "k") for n in ("batch", "row", "head")]
+        + [(n, _c_void_p) for n in ("positions", "frequencies")]
+        + [(n, _c_int64) for n in ("B", "N", "H", "Hk", "D", "pairs")]
+        + [("magnitude", ctypes.c_float)]
+        + [(n, _c_int) for n in ("interleaved", "inverse", "f32")]
+    )
+
+
+class PagedCacheArgs(ctypes.Structure):
+    """``bioemu_paged_cache`` (strides one by one)."""
+
+    _fields_ = (
+        [(n, _c_void_p) for n in ("keys", "values")]
+        + [(f"{t}_{n}", _c_int64) for t in ("keys", "values") for n in ("page", "slot", "head")]
+        + [("page_table", _c_void_p), ("table_stride", _c_int64), ("lengths", _c_void_p), ("counts", _c_void_p)]
+        + [(n, _c_int64) for n in ("pages", "page_size", "table_width")]
+    )
+
+
 _attn_p = ctypes.POINTER(AttentionArgs)
+_rotary_p = ctypes.POINTER(RotaryArgs)
+_cache_p = ctypes.POINTER(PagedCacheArgs)
 
 # name -> (restype, argtypes).  Keep in the order of include/bioemu2_mi355x.h.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -166,6 +192,13 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _c_int,
         [_attn_p] + [_c_void_p] * 4 + [ctypes.POINTER(_c_int64 * 3)] + [_c_void_p] * 5 + [_c_size_t, _c_void_p],
     ),
+    "bioemu_rotary": (_c_int, [_rotary_p] + [_c_void_p] * 3),
+    "bioemu_paged_append": (
+        _c_int,
+        [_cache_p, _rotary_p, _c_void_p, ctypes.POINTER(_c_int64 * 3)] + [_c_void_p] * 2,
+    ),
+    "bioemu_paged_attention_workspace_bytes": (_c_size_t, [_cache_p, _attn_p]),
+    "bioemu_paged_attention": (_c_int, [_cache_p, _attn_p] + [_c_void_p] * 2 + [_c_size_t, _c_void_p]),
 }
 
 _lock = threading.Lock()

@@ -120,4 +120,7 @@ int transition_pair_res(const void* x, const void* res, const float* norm_w, con
                         size_t workspace_bytes, int64_t P, int64_t Dc, int64_t hidden, int use_norm, int residual,
                         hipStream_t stream);
 
+// Checks a paged cache of B sequences and Hk heads (rotary.hip).
+int paged_cache_args(const char* what, const bioemu_paged_cache* c, int64_t B, int64_t Hk, bool f32);
+
 }  // namespace bioemu

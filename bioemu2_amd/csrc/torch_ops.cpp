@@ -1,5 +1,6 @@
-// The trainable operators as torch ops (torch.ops.bioemu_mi355x.{layer_norm, relative_position, attention}): argument
-// checks, output and workspace allocation, the C ABI's calls and the gradients.
+// The trainable operators as torch ops (torch.ops.bioemu_mi355x.{layer_norm, relative_position, attention, rotary}) and
+// those of the paged cache (paged_append, paged_attention): argument checks, output and workspace allocation, the C ABI's
+// calls and the gradients.
 //
 // These run in C++ because a training step's backward pass runs in autograd's own thread: the same glue in Python took
 // 60 to 130 us a step of host time there and back (a step of the smallest sizes computes for 15), and 40 to 70 here.
@@ -535,6 +536,312 @@ Tensor attention_autograd(ATTENTION_PARAMS) {
   "Tensor q, Tensor k, Tensor v, Tensor? table, Tensor? buckets, Tensor? q_segments, Tensor? k_segments, "          \
   "Tensor? prefix, Tensor? lengths, float scale, float cap, bool causal"
 
+// ---------------------------------------------------------------------------
+// Rotary positions
+// ---------------------------------------------------------------------------
+// [B, N, H, D] with adjacent values of a head and rows at 16-byte addresses: t where it is so, a copy else.
+Tensor rows16(const Tensor& t) {
+  const int64_t per = 16 / t.element_size();
+  bool ok = (t.stride(3) == 1 || t.size(3) <= 1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int d = 0; d < 3; ++d) ok = ok && (t.size(d) <= 1 || t.stride(d) % per == 0);
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+void set_strides(int64_t (&out)[3], const Tensor& t) {
+  for (int d = 0; d < 3; ++d) out[d] = t.stride(d);
+}
+Tensor frequencies_of(const Tensor& f, const char* what, const Tensor& like) {
+  TORCH_CHECK_VALUE(f.dim() == 1 && f.scalar_type() == at::kDouble, what, ": frequencies must be [pairs] of 64 bits, got ",
+                    f.sizes(), " ", f.scalar_type());
+  TORCH_CHECK_VALUE(f.device() == like.device(), what, ": frequencies on ", f.device(), ", expected ", like.device());
+  return f.contiguous();
+}
+
+#define ROTARY_PARAMS                                                                                                 \
+  const optional<Tensor>&q, const optional<Tensor>&k, const optional<Tensor>&positions, const Tensor &frequencies,    \
+      bool interleaved, double magnitude, bool inverse
+#define ROTARY_ARGS q, k, positions, frequencies, interleaved, magnitude, inverse
+
+const Tensor& rotary_like(const optional<Tensor>& q, const optional<Tensor>& k) {
+  TORCH_CHECK_VALUE(q || k, "rotary: neither q nor k");
+  return q ? *q : *k;
+}
+
+std::tuple<Tensor, Tensor> rotary_cuda(ROTARY_PARAMS) {
+  const Tensor& like = rotary_like(q, k);
+  check_activation(like, "rotary");
+  TORCH_CHECK_VALUE(like.dim() == 4, "rotary: expected [B, N, heads, D], got ", like.sizes());
+  if (q && k)
+    TORCH_CHECK_VALUE(k->dim() == 4 && k->size(0) == q->size(0) && k->size(1) == q->size(1) && k->size(3) == q->size(3) &&
+                          k->scalar_type() == q->scalar_type() && k->device() == q->device(),
+                      "rotary: q ", q->sizes(), " ", q->scalar_type(), " on ", q->device(), ", k ", k->sizes(), " ",
+                      k->scalar_type(), " on ", k->device());
+  const c10::OptionalDeviceGuard guard(like.device());
+  const int64_t bn[2] = {like.size(0), like.size(1)};
+  const optional<Tensor> pos = whole_numbers(positions, "rotary positions", bn, like);
+  const Tensor f = frequencies_of(frequencies, "rotary", like);
+  bioemu_rotary_args args{};
+  Tensor qs, ks, qo = none_like(like), ko = none_like(like);
+  if (q) {
+    qs = rows16(*q);
+    qo = at::empty(q->sizes(), q->options());
+    args.q = qs.data_ptr();
+    set_strides(args.q_stride, qs);
+    args.H = q->size(2);
+  }
+  if (k) {
+    ks = rows16(*k);
+    ko = at::empty(k->sizes(), k->options());
+    args.k = ks.data_ptr();
+    set_strides(args.k_stride, ks);
+    args.Hk = k->size(2);
+  }
+  args.positions = static_cast<int*>(ptr(pos));
+  args.frequencies = f.data_ptr<double>();
+  args.B = bn[0];
+  args.N = bn[1];
+  args.D = like.size(3);
+  args.pairs = f.numel();
+  args.magnitude = (float)magnitude;
+  args.interleaved = interleaved;
+  args.inverse = inverse;
+  args.f32 = is_f32(like);
+  check_rc(bioemu_rotary(&args, qo.data_ptr(), ko.data_ptr(), stream_of(like)), "bioemu_rotary");
+  return {qo, ko};
+}
+
+std::tuple<Tensor, Tensor> rotary_meta(ROTARY_PARAMS) {
+  const Tensor& like = rotary_like(q, k);
+  const auto fresh = [&](const optional<Tensor>& t) {
+    return t ? at::empty_symint(t->sym_sizes(), t->options()) : none_like(like);
+  };
+  return {fresh(q), fresh(k)};
+}
+
+struct RotaryFn : Function<RotaryFn> {
+  static variable_list forward(AutogradContext* ctx, ROTARY_PARAMS) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = handle<decltype(rotary_cuda)>("bioemu_mi355x::rotary");
+    auto [qo, ko] = op.call(ROTARY_ARGS);
+    ctx->save_for_backward({or_undefined(positions), frequencies});
+    ctx->saved_data["has_q"] = q.has_value();
+    ctx->saved_data["has_k"] = k.has_value();
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["magnitude"] = magnitude;
+    ctx->saved_data["inverse"] = inverse;
+    ctx->set_materialize_grads(false);
+    return {qo, ko};
+  }
+  // the transposed turn; a result that nothing was made of has no gradient
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto s = ctx->get_saved_variables();
+    const bool has_q = ctx->saved_data["has_q"].toBool(), has_k = ctx->saved_data["has_k"].toBool();
+    variable_list grads(7);
+    const bool need_q = has_q && g[0].defined() && ctx->needs_input_grad(0),
+               need_k = has_k && g[1].defined() && ctx->needs_input_grad(has_q);
+    if (!need_q && !need_k) return grads;
+    static auto op = handle<decltype(rotary_cuda)>("bioemu_mi355x::rotary");
+    auto [dq, dk] = op.call(need_q ? optional<Tensor>(g[0]) : std::nullopt, need_k ? optional<Tensor>(g[1]) : std::nullopt,
+                            maybe(s[0]), s[1], ctx->saved_data["interleaved"].toBool(),
+                            ctx->saved_data["magnitude"].toDouble(), !ctx->saved_data["inverse"].toBool());
+    if (need_q) grads[0] = dq;
+    if (need_k) grads[1] = dk;
+    return grads;
+  }
+};
+
+std::tuple<Tensor, Tensor> rotary_autograd(ROTARY_PARAMS) {
+  check_no_tangents("rotary", q, k);
+  if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k))) {
+    auto out = RotaryFn::apply(ROTARY_ARGS);
+    return {out[0], out[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  static auto op = handle<decltype(rotary_cuda)>("bioemu_mi355x::rotary");
+  return op.call(ROTARY_ARGS);
+}
+
+// ---------------------------------------------------------------------------
+// A paged cache
+// ---------------------------------------------------------------------------
+// The C ABI's structure over the cache's tensors, which are used as they are.
+struct CacheCall {
+  Tensor table;
+  Tensor lengths;
+  optional<Tensor> counts;
+  bioemu_paged_cache args{};
+
+  CacheCall(const char* what, const Tensor& keys, const Tensor& values, const Tensor& page_table, const Tensor& lengths_,
+            const optional<Tensor>& counts_, const Tensor& like, int64_t heads) {
+    TORCH_CHECK_VALUE(keys.dim() == 4 && keys.sizes() == values.sizes() && keys.size(2) == heads &&
+                          keys.size(3) == like.size(3),
+                      what, ": keys ", keys.sizes(), ", values ", values.sizes(), ", expected [pages, page_size, ", heads,
+                      ", ", like.size(3), "]");
+    TORCH_CHECK_VALUE(keys.scalar_type() == like.scalar_type() && values.scalar_type() == like.scalar_type(), what,
+                      ": keys are ", keys.scalar_type(), ", values ", values.scalar_type(), ", expected ",
+                      like.scalar_type());
+    TORCH_CHECK_VALUE(keys.device() == like.device() && values.device() == like.device(), what, ": keys on ",
+                      keys.device(), ", values on ", values.device(), ", expected ", like.device());
+    TORCH_CHECK_VALUE(keys.size(1) > 0, what, ": pages of no slots");
+    for (const Tensor* t : {&keys, &values})
+      TORCH_CHECK_VALUE(t->stride(3) == 1, what, ": values of a head must be adjacent, got strides ", t->strides());
+    const int64_t B = like.size(0), b1[1] = {B};
+    TORCH_CHECK_VALUE(page_table.dim() == 2 && page_table.size(0) == B && page_table.scalar_type() == at::kInt &&
+                          page_table.device() == like.device(),
+                      what, ": page_table must be int32 [", B, ", width] on ", like.device(), ", got ",
+                      page_table.scalar_type(), " ", page_table.sizes(), " on ", page_table.device());
+    table = page_table.stride(1) == 1 || page_table.size(1) <= 1 ? page_table : page_table.contiguous();
+    lengths = whole_numbers(lengths_, what, at::kInt, b1, like);
+    counts = whole_numbers(counts_, what, b1, like);
+    args.keys = keys.data_ptr();
+    args.values = values.data_ptr();
+    set_strides(args.keys_stride, keys);
+    set_strides(args.values_stride, values);
+    args.page_table = table.data_ptr<int>();
+    args.table_stride = table.stride(0);
+    args.lengths = lengths.data_ptr<int>();
+    args.counts = static_cast<int*>(ptr(counts));
+    args.pages = keys.size(0);
+    args.page_size = keys.size(1);
+    args.table_width = table.size(1);
+  }
+};
+
+template <class... T>
+void check_no_gradients(const char* what, const T&... inputs) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled() || !(wants_grad(inputs) || ...), what,
+                              ": no backward pass; call it under torch.no_grad()");
+}
+
+#define APPEND_PARAMS                                                                                                 \
+  const Tensor &keys, const Tensor &values, const Tensor &k, const Tensor &v, const Tensor &page_table,               \
+      const Tensor &lengths, const optional<Tensor>&counts, const optional<Tensor>&q,                                 \
+      const optional<Tensor>&frequencies, const optional<Tensor>&positions, bool interleaved, double magnitude
+#define APPEND_ARGS keys, values, k, v, page_table, lengths, counts, q, frequencies, positions, interleaved, magnitude
+
+// Two slots of one tensor in the same place (a dimension of stride 0) cannot both be written.
+void check_writable(const Tensor& t, const char* what) {
+  for (int d = 0; d < 3; ++d)
+    TORCH_CHECK_VALUE(t.size(d) <= 1 || t.stride(d) > 0, what, ": expanded tensors cannot be appended to");
+}
+
+Tensor paged_append_cuda(APPEND_PARAMS) {
+  check_activation(k, "paged_append k");
+  TORCH_CHECK_VALUE(k.dim() == 4 && k.sizes() == v.sizes() && v.scalar_type() == k.scalar_type() &&
+                        v.device() == k.device(),
+                    "paged_append: k ", k.sizes(), " ", k.scalar_type(), " on ", k.device(), ", v ", v.sizes(), " ",
+                    v.scalar_type(), " on ", v.device());
+  if (q) {
+    TORCH_CHECK_VALUE(frequencies.has_value(), "paged_append: q comes with frequencies");
+    TORCH_CHECK_VALUE(q->dim() == 4 && q->size(0) == k.size(0) && q->size(1) == k.size(1) && q->size(3) == k.size(3) &&
+                          q->scalar_type() == k.scalar_type() && q->device() == k.device(),
+                      "paged_append: q ", q->sizes(), " ", q->scalar_type(), " on ", q->device(), ", k ", k.sizes(), " ",
+                      k.scalar_type(), " on ", k.device());
+  }
+  TORCH_CHECK_VALUE(!positions || frequencies, "paged_append: positions come with frequencies");
+  check_writable(keys, "paged_append keys");
+  check_writable(values, "paged_append values");
+  const c10::OptionalDeviceGuard guard(k.device());
+  const CacheCall c("paged_append", keys, values, page_table, lengths, counts, k, k.size(2));
+  const int64_t bn[2] = {k.size(0), k.size(1)};
+  const optional<Tensor> pos = whole_numbers(positions, "paged_append positions", bn, k);
+  Tensor f, qs, out = none_like(k);
+  if (frequencies) f = frequencies_of(*frequencies, "paged_append", k);
+  const Tensor ks = rows16(k), vs = rows16(v);
+  bioemu_rotary_args args{};
+  if (q) {
+    qs = rows16(*q);
+    out = at::empty(q->sizes(), q->options());
+    args.q = qs.data_ptr();
+    set_strides(args.q_stride, qs);
+    args.H = q->size(2);
+  }
+  args.k = ks.data_ptr();
+  set_strides(args.k_stride, ks);
+  args.Hk = k.size(2);
+  args.positions = static_cast<int*>(ptr(pos));
+  args.frequencies = static_cast<double*>(ptr(f));
+  args.B = bn[0];
+  args.N = bn[1];
+  args.D = k.size(3);
+  args.pairs = f.defined() ? f.numel() : 0;
+  args.magnitude = (float)magnitude;
+  args.interleaved = interleaved;
+  args.f32 = is_f32(k);
+  const int64_t vst[3] = {vs.stride(0), vs.stride(1), vs.stride(2)};
+  check_rc(bioemu_paged_append(&c.args, &args, vs.data_ptr(), vst, q ? out.data_ptr() : nullptr, stream_of(k)),
+           "bioemu_paged_append");
+  return out;
+}
+Tensor paged_append_meta(APPEND_PARAMS) {
+  return q ? at::empty_symint(q->sym_sizes(), q->options()) : none_like(k);
+}
+Tensor paged_append_autograd(APPEND_PARAMS) {
+  check_no_tangents("paged_append", keys, values, k, v, q);
+  check_no_gradients("paged_append", keys, values, k, v, q);
+  at::AutoDispatchBelowADInplaceOrView below;
+  static auto op = handle<decltype(paged_append_cuda)>("bioemu_mi355x::paged_append");
+  const Tensor out = op.call(APPEND_ARGS);
+  for (const Tensor* t : {&keys, &values})   // whoever saved them for a backward pass is told
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  return out;
+}
+
+#define PAGED_PARAMS                                                                                                  \
+  const Tensor &q, const Tensor &keys, const Tensor &values, const Tensor &page_table, const Tensor &lengths,         \
+      const optional<Tensor>&counts, const optional<Tensor>&table, const optional<Tensor>&buckets, double scale,      \
+      double cap, bool causal
+#define PAGED_ARGS q, keys, values, page_table, lengths, counts, table, buckets, scale, cap, causal
+
+Tensor paged_attention_cuda(PAGED_PARAMS) {
+  check_activation(q, "paged_attention q");
+  TORCH_CHECK_VALUE(q.dim() == 4, "paged_attention: q must be [B, Nq, H, D], got ", q.sizes());
+  const c10::OptionalDeviceGuard guard(q.device());
+  const CacheCall c("paged_attention", keys, values, page_table, lengths, counts, q,
+                    keys.dim() == 4 ? keys.size(2) : 0);
+  bioemu_attention_args args{};
+  Tensor tab, buck;
+  TORCH_CHECK_VALUE(table.has_value() == buckets.has_value() && (!table || table->dim() == 2),
+                    "paged_attention: a bias table [num_buckets, H] comes with its buckets");
+  if (table) {
+    TORCH_CHECK_VALUE(buckets->dim() == 1 && buckets->numel() % 2 == 1,
+                      "paged_attention: buckets must be [2 * radius + 1], got ", buckets->sizes());
+    buck = whole_numbers(*buckets, "paged_attention buckets", at::kByte, buckets->sizes(), q);
+    const int64_t shape[2] = {table->size(0), q.size(2)};
+    tab = parameter(*table, "paged_attention bias table", shape, q);
+    args.bias_table = tab.data_ptr();
+    args.bias_buckets = buck.data_ptr<uint8_t>();
+    args.radius = buck.numel() / 2;
+    args.num_buckets = tab.size(0);
+    args.table_bf16 = is_bf16(tab);
+  }
+  const Tensor qs = heads(q);
+  args.q = qs.data_ptr();
+  set_strides(args.q_stride, qs);
+  args.B = q.size(0);
+  args.Nq = q.size(1);
+  args.H = q.size(2);
+  args.Hk = keys.size(2);
+  args.D = q.size(3);
+  args.scale = (float)scale;
+  args.cap = (float)cap;
+  TORCH_CHECK_VALUE(cap == 0 || args.cap > 0, "paged_attention: cap ", cap);
+  args.causal = causal;
+  args.f32 = is_f32(q);
+  Tensor out = at::empty(q.sizes(), q.options()), ws;
+  const int64_t need = (int64_t)bioemu_paged_attention_workspace_bytes(&c.args, &args);
+  if (need) ws = bytes(need, q);
+  check_rc(bioemu_paged_attention(&c.args, &args, out.data_ptr(), ptr(ws), need, stream_of(q)), "bioemu_paged_attention");
+  return out;
+}
+Tensor paged_attention_meta(PAGED_PARAMS) { return at::empty_symint(q.sym_sizes(), q.options()); }
+Tensor paged_attention_autograd(PAGED_PARAMS) {
+  check_no_tangents("paged_attention", q, keys, values, table);
+  check_no_gradients("paged_attention", q, keys, values, table);
+  at::AutoDispatchBelowADInplaceOrView below;
+  static auto op = handle<decltype(paged_attention_cuda)>("bioemu_mi355x::paged_attention");
+  return op.call(PAGED_ARGS);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(bioemu_mi355x, m) {
@@ -550,6 +857,12 @@ TORCH_LIBRARY_FRAGMENT(bioemu_mi355x, m) {
   m.def("attention_train(" ATTENTION_SCHEMA ") -> (Tensor, Tensor, Tensor)");
   m.def("attention_backward(Tensor out, Tensor out_lo, Tensor lse, Tensor dout, " ATTENTION_SCHEMA
         ", bool want_table) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("rotary(Tensor? q, Tensor? k, Tensor? positions, Tensor frequencies, bool interleaved, float magnitude, "
+        "bool inverse) -> (Tensor, Tensor)");
+  m.def("paged_append(Tensor(a!) keys, Tensor(b!) values, Tensor k, Tensor v, Tensor page_table, Tensor lengths, "
+        "Tensor? counts, Tensor? q, Tensor? frequencies, Tensor? positions, bool interleaved, float magnitude) -> Tensor");
+  m.def("paged_attention(Tensor q, Tensor keys, Tensor values, Tensor page_table, Tensor lengths, Tensor? counts, "
+        "Tensor? table, Tensor? buckets, float scale, float cap, bool causal) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(bioemu_mi355x, CUDA, m) {
@@ -561,6 +874,9 @@ TORCH_LIBRARY_IMPL(bioemu_mi355x, CUDA, m) {
   m.impl("attention", &attention_cuda);
   m.impl("attention_train", &attention_train_cuda);
   m.impl("attention_backward", &attention_backward_cuda);
+  m.impl("rotary", &rotary_cuda);
+  m.impl("paged_append", &paged_append_cuda);
+  m.impl("paged_attention", &paged_attention_cuda);
 }
 
 TORCH_LIBRARY_IMPL(bioemu_mi355x, Meta, m) {
@@ -572,12 +888,18 @@ TORCH_LIBRARY_IMPL(bioemu_mi355x, Meta, m) {
   m.impl("attention", &attention_meta);
   m.impl("attention_train", &attention_train_meta);
   m.impl("attention_backward", &attention_backward_meta);
+  m.impl("rotary", &rotary_meta);
+  m.impl("paged_append", &paged_append_meta);
+  m.impl("paged_attention", &paged_attention_meta);
 }
 
 TORCH_LIBRARY_IMPL(bioemu_mi355x, Autograd, m) {
   m.impl("layer_norm", &layer_norm_autograd);
   m.impl("relative_position", &relative_position_autograd);
   m.impl("attention", &attention_autograd);
+  m.impl("rotary", &rotary_autograd);
+  m.impl("paged_append", &paged_append_autograd);
+  m.impl("paged_attention", &paged_attention_autograd);
   // a gradient of a gradient raises
   for (const char* name : {"layer_norm_train", "layer_norm_backward", "relative_position_backward", "attention_train",
                            "attention_backward"})

@@ -536,6 +536,70 @@ int bioemu_attention_bwd(const bioemu_attention_args* args, const void* o, const
                          const void* dout, const int64_t* dout_stride, void* dq, void* dk, void* dv, void* dtable,
                          void* workspace, size_t workspace_bytes, hipStream_t stream);
 
+/*
+ * Rotary positions: the first 2 pairs values of every head of q [B, N, H, D]
+ * and k [B, N, Hk, D], taken as pairs (a, b), turn by t = position * frequency:
+ *   a' = m (a cos t - b sin t),  b' = m (a sin t + b cos t);  the rest is copied
+ * Pair i: values i and i + pairs, or 2 i and 2 i + 1 (interleaved).  inverse:
+ * by -t, the gradient.  Angles are 64-bit products, reduced to a quarter turn
+ * before they are rounded.  q or k may be NULL (with its output); positions
+ * [B, N] may be NULL: 0 .. N - 1.  Strides (batch, row, head) are in elements;
+ * rows at 16-byte addresses, D a multiple of 8 up to 512.  Outputs: contiguous.
+ */
+typedef struct bioemu_rotary_args {
+  const void *q, *k;
+  int64_t q_stride[3], k_stride[3];
+  const int32_t* positions;
+  const double* frequencies; /* [pairs], radians a position */
+  int64_t B, N, H, Hk, D, pairs;
+  float magnitude;
+  int interleaved, inverse, f32;
+} bioemu_rotary_args;
+
+int bioemu_rotary(const bioemu_rotary_args* args, void* q_out, void* k_out, hipStream_t stream);
+
+/*
+ * A cache of keys and values in pages: [pages, page_size, Hk, D] each, strides
+ * (page, slot, head) in elements, values of a head adjacent, rows at 16-byte
+ * addresses.  Position p of sequence b is slot p % page_size of page
+ * page_table[b * table_stride + p / page_size].  lengths [B]: positions in use,
+ * the last counts[b] of them new (counts NULL: as many as the call has rows).
+ * A table entry that names no page is not read or written: its keys are not
+ * seen.  Lengths past table_width pages are taken as that many; counts into
+ * 0 .. rows.
+ */
+typedef struct bioemu_paged_cache {
+  void *keys, *values;
+  int64_t keys_stride[3], values_stride[3];
+  const int32_t* page_table;
+  int64_t table_stride;
+  const int32_t *lengths, *counts;
+  int64_t pages, page_size, table_width;
+} bioemu_paged_cache;
+
+/*
+ * New keys and values into their pages: row i < counts[b] of k and v goes to
+ * position lengths[b] - counts[b] + i, k turned as by bioemu_rotary (by that
+ * position, or positions[b, i] where given; pairs = 0: not at all), and q_out =
+ * q turned the same (zeros in rows counts[b] and on; q and q_out may be NULL).
+ * inverse is not taken.  v: [B, N, Hk, D].  Positions that the table does not
+ * hold are left out.  No slot may be named twice in one call.
+ */
+int bioemu_paged_append(const bioemu_paged_cache* cache, const bioemu_rotary_args* args, const void* v,
+                        const int64_t* v_stride, void* q_out, hipStream_t stream);
+
+/*
+ * Attention over the cache: bioemu_attention_fwd's o for Nq queries a sequence,
+ * row i < counts[b] at position lengths[b] - counts[b] + i, zeros behind
+ * (causal: keys up to its own position).  Of args, k, v, Nk, segments, prefix
+ * and lengths are not taken (NULL, 0).  Any number of queries, made for few:
+ * the keys are read once for every 32 rows (queries times H / Hk).  page_size
+ * is at most 2^20, table_width * page_size at most 2^27.
+ */
+size_t bioemu_paged_attention_workspace_bytes(const bioemu_paged_cache* cache, const bioemu_attention_args* args);
+int bioemu_paged_attention(const bioemu_paged_cache* cache, const bioemu_attention_args* args, void* o,
+                           void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,258 @@
+"""Rotary positions and their gradients against float64.
+
+Tolerances, with u = 2^-24: an angle t is a 64-bit product off by 2^-51 t (its three roundings and the reference's), and
+by 2^-25 from rounding what is left of it after whole quarters; cos and sin by 2 units in their last place (2 u) and,
+times the magnitude, one more rounding; the two products and their sum by u each, and the magnitude's own rounding u:
+8 u + 2^-51 t of magnitude (|a| + |b|), and half a step of the result.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from bioemu2_amd._lib import torch_op
+from bioemu2_amd.rotary import RotaryPosition, rotary, rotary_frequencies
+
+pytestmark = pytest.mark.gpu
+BF16, F32, F64, I32 = torch.bfloat16, torch.float32, torch.float64, torch.int32
+U = 2.0 ** -24
+
+
+def exact(x, positions, frequencies, interleaved=False, magnitude=1.0, back=False):
+    """(value, bound) of x [B, N, heads, D] turned."""
+    x = x.detach()
+    half = torch.finfo(x.dtype).eps / 2
+    n = frequencies.numel()
+    B, N = x.shape[:2]
+    if positions is None:
+        positions = torch.arange(N, device=x.device).expand(B, N)
+    t = (positions.double()[..., None] * frequencies)[:, :, None]
+    c, s = magnitude * t.cos(), magnitude * (-t if back else t).sin()
+    xd = x.double()
+    a, b = (xd[..., 0:2 * n:2], xd[..., 1:2 * n:2]) if interleaved else (xd[..., :n], xd[..., n:2 * n])
+    y, z = a * c - b * s, a * s + b * c
+    off = (8 * U + 2.0 ** -51 * t.abs()) * abs(magnitude) * (a.abs() + b.abs())
+    out, bound = xd.clone(), torch.zeros_like(xd)
+    if interleaved:
+        out[..., 0:2 * n:2], out[..., 1:2 * n:2] = y, z
+        bound[..., 0:2 * n:2], bound[..., 1:2 * n:2] = off + half * y.abs(), off + half * z.abs()
+    else:
+        out[..., :n], out[..., n:2 * n] = y, z
+        bound[..., :n], bound[..., n:2 * n] = off + half * y.abs(), off + half * z.abs()
+    return out, bound
+
+
+def check(got, want):
+    value, bound = want
+    off = (got.detach().double() - value).abs()
+    assert got.shape == value.shape and bool((off <= bound + 1e-38).all()), float((off / (bound + 1e-38)).max())
+
+
+def rand(*shape, dtype=BF16, seed=0):
+    g = torch.Generator().manual_seed(seed + 7 * len(shape) + shape[-2])
+    return torch.randn(*shape, generator=g).to(dtype).cuda()
+
+
+SHAPES = [  # B, N, H, Hk, D, rot
+    (1, 1, 1, 1, 8, 8), (2, 7, 3, 1, 24, 24), (1, 130, 16, 16, 24, 12), (2, 33, 8, 2, 64, 64), (3, 5, 7, 7, 80, 40),
+    (1, 257, 4, 4, 128, 128), (1, 40, 2, 2, 128, 6), (2, 9, 3, 3, 512, 512), (1, 3, 2, 2, 16, 2), (1, 2500, 5, 1, 32, 32)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("B,N,H,Hk,D,rot", SHAPES)
+def test_step(gpu_device, dtype, interleaved, B, N, H, Hk, D, rot):
+    q, k = rand(B, N, H, D, dtype=dtype).requires_grad_(), rand(B, N, Hk, D, dtype=dtype, seed=1).requires_grad_()
+    dq, dk = rand(B, N, H, D, dtype=dtype, seed=2), rand(B, N, Hk, D, dtype=dtype, seed=3)
+    g = torch.Generator().manual_seed(N)
+    pos = torch.randint(-5000, 5000, (B, N), generator=g, dtype=I32).cuda()
+    f = rotary_frequencies(rot, device="cuda")
+    kw = dict(interleaved=interleaved, magnitude=1.25)
+    y = rotary(q, k, pos, f, **kw)
+    check(y[0], exact(q, pos, f, **kw))
+    check(y[1], exact(k, pos, f, **kw))
+    gq, gk = torch.autograd.grad(y, (q, k), (dq, dk))
+    check(gq, exact(dq, pos, f, back=True, **kw))
+    check(gk, exact(dk, pos, f, back=True, **kw))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_far_positions(gpu_device, dtype):
+    pos = torch.tensor([[0, 1, -1, 2 ** 20, 2 ** 24 + 1, 10 ** 9 + 7, 2 ** 31 - 1, -2 ** 31, -10 ** 6]], dtype=I32).cuda()
+    q = rand(1, 9, 2, 64, dtype=dtype)
+    f = rotary_frequencies(64, device="cuda")
+    check(rotary(q, None, pos, f)[0], exact(q, pos, f))
+
+
+def test_whole_quarter_turns(gpu_device):
+    """Angles at and about multiples of a quarter turn, where the reduction changes sides."""
+    pos = torch.arange(-40, 41, dtype=I32).cuda()[None]
+    quarter = math.pi / 2
+    f = torch.tensor([quarter, quarter / 2, quarter / 4, quarter * 3, quarter + 1e-9, quarter - 1e-9, 0.0, -quarter / 2],
+                     dtype=F64).cuda()
+    q = rand(1, 81, 1, 16, dtype=F32)
+    check(rotary(q, None, pos, f)[0], exact(q, pos, f))
+
+
+def test_default_positions_and_single_inputs(gpu_device):
+    q, k, f = rand(2, 11, 4, 32), rand(2, 11, 2, 32), rotary_frequencies(32, device="cuda")
+    both = rotary(q, k, None, f)
+    check(both[0], exact(q, None, f))
+    only_q, none = rotary(q, None, None, f)
+    assert none is None and torch.equal(only_q, both[0])
+    none, only_k = rotary(None, k, torch.arange(11, device="cuda").expand(2, 11), f)
+    assert none is None and torch.equal(only_k, both[1])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_strides(gpu_device, dtype):
+    """A projection's thirds, transposed heads, an address off 16 bytes, expanded heads."""
+    f = rotary_frequencies(32, device="cuda")
+    qkv = rand(2, 9, 3, 4, 32, dtype=dtype)
+    for q in (qkv[:, :, 0], qkv[:, :, 2], rand(2, 4, 9, 32, dtype=dtype).transpose(1, 2), rand(9, 2, 4, 32, dtype=dtype).transpose(0, 1),
+              rand(1, 1, 1, 2 * 9 * 4 * 32 + 1, dtype=dtype).flatten()[1:].view(2, 9, 4, 32),
+              rand(2, 9, 1, 32, dtype=dtype).expand(2, 9, 4, 32), rand(2, 9, 4, 64, dtype=dtype)[..., ::2],
+              rand(2, 9, 4, 36, dtype=dtype)[..., 2:34]):
+        check(rotary(q, qkv[:, :, 1], None, f)[0], exact(q, None, f))
+
+
+def test_gradients_of_some(gpu_device):
+    f = rotary_frequencies(16, device="cuda")
+    q, k = rand(1, 6, 2, 16).requires_grad_(), rand(1, 6, 2, 16, seed=4)
+    dy = rand(1, 6, 2, 16, seed=5)
+    y = rotary(q, k, None, f)
+    want = exact(dy, None, f, back=True)
+    check(torch.autograd.grad(y[0], q, dy, retain_graph=True)[0], want)
+    assert torch.autograd.grad((y[1] * 1.0).sum() + (y[0] * 0.0).sum(), q)[0].abs().max() == 0
+    k.requires_grad_()
+    y = rotary(q.detach(), k, None, f)
+    check(torch.autograd.grad(y[1], k, dy, retain_graph=True)[0], want)
+    y = rotary(None, k, None, f)
+    check(torch.autograd.grad(y[1], k, dy)[0], want)
+    y = rotary(q, k, None, f)    # one result used only
+    gq, gk = torch.autograd.grad(y[1], (q, k), dy, allow_unused=True)
+    assert gq is None or gq.abs().max() == 0
+    check(gk, want)
+
+
+def test_gradient_against_differences(gpu_device):
+    """The map is linear: a difference over any step is its derivative but for rounding (2^-20 of the values' size)."""
+    f = rotary_frequencies(24, device="cuda")
+    pos = torch.arange(100, 130, dtype=I32).cuda()[None]
+    q = rand(1, 30, 4, 32, dtype=F32).requires_grad_()
+    way, dy = rand(1, 30, 4, 32, dtype=F32, seed=8), rand(1, 30, 4, 32, dtype=F32, seed=9)
+    g, = torch.autograd.grad(rotary(q, None, pos, f, interleaved=True)[0], q, dy)
+    with torch.no_grad():
+        diff = rotary(q + way, None, pos, f, interleaved=True)[0].double() - rotary(q - way, None, pos, f, interleaved=True)[0].double()
+    a, b = (diff * dy.double()).sum() / 2, (g.double() * way.double()).sum()
+    assert abs(a - b) < 2.0 ** -20 * (dy.abs() * (way.abs() + q.abs()) * 4).double().sum()
+
+
+def test_scores_depend_on_distance(gpu_device):
+    """q.k after turning is the same wherever the two stand, at any length of context."""
+    f = rotary_frequencies(64, scaling="parts", factor=16.0, length=4096, device="cuda")
+    q, k = rand(1, 1, 1, 64, dtype=F32), rand(1, 1, 1, 64, dtype=F32, seed=1)
+    got = []
+    for at in (0, 1000, 1000000):
+        a, _ = rotary(q, None, torch.tensor([[at + 37]], dtype=I32, device="cuda"), f)
+        b, _ = rotary(k, None, torch.tensor([[at]], dtype=I32, device="cuda"), f)
+        got.append(float((a.double() * b.double()).sum()))
+    size = float((q.double().abs().sum() * k.double().abs().max()))
+    assert max(got) - min(got) < 32 * U * size
+
+
+def test_non_finite_values_stay_in_their_pair(gpu_device):
+    f = rotary_frequencies(16, device="cuda")
+    q = rand(1, 4, 2, 16, dtype=F32)
+    want = rotary(q, None, None, f)[0]
+    q[0, 1, 0, 3], q[0, 2, 1, 9] = math.inf, math.nan
+    got = rotary(q, None, None, f)[0]
+    touched = torch.zeros_like(q, dtype=torch.bool)
+    touched[0, 1, 0, [3, 11]] = touched[0, 2, 1, [1, 9]] = True
+    assert torch.equal(got[~touched], want[~touched]) and not bool(got[touched].isfinite().any())
+
+
+def test_same_bits_other_stream_and_replays(gpu_device):
+    f = rotary_frequencies(64, device="cuda")
+    q, k = rand(2, 50, 4, 64).requires_grad_(), rand(2, 50, 2, 64).requires_grad_()
+    dq, dk = rand(2, 50, 4, 64, seed=2), rand(2, 50, 2, 64, seed=3)
+    pos = torch.arange(50, dtype=I32, device="cuda").expand(2, 50).contiguous()
+
+    def step():
+        y = rotary(q, k, pos, f)
+        return [y[0].detach(), y[1].detach(), *torch.autograd.grad(y, (q, k), (dq, dk))]
+
+    want = [t.clone() for t in step()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for a, b in zip(step(), want):
+            assert torch.equal(a, b)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = step()
+    torch.cuda.current_stream().wait_stream(side)
+    for shift in (0, 3, 0):
+        with torch.no_grad():
+            pos.add_(shift)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, step()):
+            assert torch.equal(a, b)
+
+
+def test_module(gpu_device):
+    m = RotaryPosition(32, scaling="parts", factor=8.0, length=512).to(BF16).cuda()
+    assert m.frequencies.dtype == F64 and m.frequencies.is_cuda and not m.state_dict()
+    q, k = rand(1, 9, 2, 64), rand(1, 9, 2, 64, seed=1)
+    y = m(q, k)
+    check(y[0], exact(q, None, m.frequencies, magnitude=m.magnitude))
+    assert m.magnitude == pytest.approx(0.1 * math.log(8.0) + 1.0)
+    check(m(None, k)[1], exact(k, None, m.frequencies, magnitude=m.magnitude))
+
+
+def test_zero_sizes(gpu_device):
+    f = rotary_frequencies(16, device="cuda")
+    for shape in ((0, 4, 2, 16), (2, 0, 2, 16)):
+        q = torch.empty(shape, dtype=BF16, device="cuda", requires_grad=True)
+        y = rotary(q, None, None, f)[0]
+        assert y.shape == shape and torch.autograd.grad(y.sum(), q)[0].shape == shape
+    q = rand(1, 3, 2, 16)
+    assert torch.equal(rotary(q, None, None, f[:0])[0], q)   # no pairs: a copy
+
+
+def test_fake_tensors(gpu_device):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        q = torch.empty(2, 5, 4, 32, dtype=BF16, device="cuda")
+        f = torch.empty(16, dtype=F64, device="cuda")
+        out = torch_op("rotary")(q, None, None, f, False, 1.0, False)
+        assert out[0].shape == q.shape and out[0].dtype == BF16 and out[1].numel() == 0
+
+
+def test_refusals(gpu_device):
+    f, q = rotary_frequencies(32, device="cuda"), rand(2, 5, 4, 32)
+    for args, error in [((None, None, None, f), ValueError), ((q, None, None, f.float()), ValueError),
+                        ((q, None, None, f.cpu()), ValueError), ((q[..., :16], None, None, f), ValueError),
+                        ((q, rand(2, 5, 4, 40), None, f), ValueError), ((q, q.float(), None, f), ValueError),
+                        ((q, rand(2, 4, 4, 32), None, f), ValueError), ((q[0], None, None, f), ValueError),
+                        ((q.half(), None, None, f), ValueError), ((rand(1, 2, 2, 20), None, None, f[:4]), ValueError),
+                        ((rand(1, 2, 2, 520), None, None, f), ValueError),
+                        ((q, None, torch.zeros(2, 4, dtype=I32, device="cuda"), f), ValueError),
+                        ((q, None, torch.zeros(2, 5, device="cuda"), f), ValueError),
+                        ((q, q.cpu(), None, f), ValueError)]:
+        with pytest.raises(error):
+            rotary(*args)
+
+
+def test_gradient_of_the_gradient(gpu_device):
+    """The map is linear: its gradient is a linear map of dy, whose gradient is the map again."""
+    f, q = rotary_frequencies(32, device="cuda"), rand(2, 5, 4, 32).requires_grad_()
+    dy, w = rand(2, 5, 4, 32, seed=1).requires_grad_(), rand(2, 5, 4, 32, seed=2)
+    g, = torch.autograd.grad(rotary(q, None, None, f)[0], q, dy, create_graph=True)
+    check(g, exact(dy, None, f, back=True))
+    check(torch.autograd.grad(g, dy, w)[0], exact(w, None, f))
