@@ -20,7 +20,6 @@
 namespace bioemu {
 namespace {
 
-constexpr int kWaves = 4;
 constexpr float kRescale = 8.f;   // log2 of the largest weight before the maximum moves
 
 struct PagedArgs {
@@ -30,11 +29,14 @@ struct PagedArgs {
   int64_t table_stride;
   const int *lengths, *counts;
   int pages, page_size, table_width, blocks;   // blocks of rows a key head
+  unsigned div_mul, div_shift;                  // key / page_size = key * div_mul >> div_shift, for keys below 2^28
+  int even;                                     // pages are whole blocks of 16 keys
   int groups, least;                            // workgroups that share the keys, of `least` tiles at least; 0: one an item
 };
 
 struct Parts {
   float *o, *ml;   // [slots][rows][D], [slots][rows][2]
+  int* range;      // [items][2]: the first and last workgroup of an item
 };
 
 template <class T>
@@ -59,21 +61,25 @@ __device__ __forceinline__ f32x4 mfma_16x16(float a, float b, f32x4 c) {
 // comparison with 0 would take a NaN for an empty row.
 __device__ __forceinline__ float over_sum(float o, float sum) { return o / fmaxf(sum, 0.5f); }
 
+// The largest of the lanes with the same lane % 16: rows of 16 lanes and halves of the wave swapped between two copies.
+// Written as instructions: from the builtins the compiler takes both results for one.
+__device__ __forceinline__ float max_over_keys(float x) {
+  float y = x;
+  asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(x), "+v"(y));   // x: rows 0 0 2 2, y: 1 1 3 3
+  x = y = fmaxf(x, y);
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));   // x: halves 0 0, y: 1 1
+  return fmaxf(x, y);
+}
+
 // Keys of sequence b; the table and the cache bound them.
 __device__ __forceinline__ int length_of(const PagedArgs& p, int b) {
   const int most = p.pages > 0 ? p.table_width * p.page_size : 0;
   return min(max(p.lengths[b], 0), most);
 }
 
-// Tiles of all items before sequence `upto` (B: of all).  Every wave by itself.
 template <int KEYS>
-__device__ __forceinline__ int64_t tiles_before(const PagedArgs& p, int upto, int items) {
-  const int lane = threadIdx.x & 63;
-  int64_t sum = 0;
-  for (int b = lane; b < upto; b += 64) sum += (length_of(p, b) + KEYS - 1) / KEYS;
-#pragma unroll
-  for (int m = 32; m > 0; m /= 2) sum += __shfl_xor(sum, m);
-  return sum * items;
+__device__ __forceinline__ int tiles_of(const PagedArgs& p, int b) {
+  return (length_of(p, b) + KEYS - 1) / KEYS;
 }
 
 __device__ __forceinline__ int64_t uniform(int64_t x) {
@@ -81,12 +87,41 @@ __device__ __forceinline__ int64_t uniform(int64_t x) {
          (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
 }
 
-template <class T, int DP, int RB, int CAP>
+// The deal of the tiles: how many there are, before sequence `upto` and in all, and among how many workgroups: as many as
+// there are, with at least `least` tiles each, but for items of fewer (an item's start costs some tiles' time).  Every
+// wave by itself.
+struct Deal {
+  int64_t before, total, groups;
+};
+template <int KEYS>
+__device__ __forceinline__ Deal deal(const PagedArgs& p, int B, int upto, int items) {
+  const int lane = threadIdx.x & 63;
+  int64_t before = 0, total = 0;
+  int live = 0;
+  for (int b = lane; b < B; b += 64) {
+    const int tiles = tiles_of<KEYS>(p, b);
+    total += tiles;
+    before += b < upto ? tiles : 0;
+    live += tiles > 0;
+  }
+#pragma unroll
+  for (int m = 32; m > 0; m /= 2) {
+    total += __shfl_xor(total, m);
+    before += __shfl_xor(before, m);
+    live += __shfl_xor(live, m);
+  }
+  total = uniform(total) * items;
+  const int64_t want = max((total + p.least - 1) / p.least, (int64_t)__builtin_amdgcn_readfirstlane(live) * items);
+  return {uniform(before) * items, total, min((int64_t)p.groups, want)};
+}
+
+template <class T, int DP, int RB, int CAP, int W>
 struct Walk {
   static constexpr int KEYS = Cache<T>::KEYS, VC = DP / 16;
   static constexpr int VL = VC * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : VC;   // values a load of V
   static constexpr int KL = sizeof(T) == 2 ? 8 : 4, KS = DP / (4 * KL), KU = KEYS / 16;
   static constexpr int VK = KEYS / 4;   // keys whose values a lane loads
+  static constexpr unsigned kAll = KEYS == 32 ? 0xffffffffu : 0xffffu;
   typedef T kvec __attribute__((ext_vector_type(KL)));
   typedef T vvec __attribute__((ext_vector_type(VL)));
 
@@ -94,57 +129,89 @@ struct Walk {
   const PagedArgs& p;
   const int lane, m, h;
   const char *kbase, *vbase;
-  int64_t koff[KU], voff[VK];
+  // byte offsets of the lane's row among sixteen, and of its pieces of a row (the row's first where it has no more)
+  unsigned krow, vrow, kd[KS], vd[VC / VL];
+  int64_t kat[KU], vat[KU];   // see locate
   kvec kf[KU][KS];
   vvec vf[VK][VC / VL];
-  unsigned mask;   // keys of the tile that are there, as loaded
 
   __device__ __forceinline__ Walk(const AttnArgs& a_, const PagedArgs& p_)
-      : a(a_), p(p_), lane(threadIdx.x & 63), m(lane & 15), h(lane >> 4) {}
+      : a(a_), p(p_), lane(threadIdx.x & 63), m(lane & 15), h(lane >> 4) {
+    krow = p.even ? (unsigned)(m * p.kslot) : 0;
+    vrow = p.even ? (unsigned)(4 * h * p.vslot) : 0;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) kd[s] = KL * (4 * s + h) < a.D ? KL * (4 * s + h) * (int)sizeof(T) : 0;
+#pragma unroll
+    for (int c = 0; c < VC / VL; ++c) vd[c] = 16 * VL * c + VL * m < a.D ? (16 * VL * c + VL * m) * (int)sizeof(T) : 0;
+  }
 
+  __device__ __forceinline__ int page_index(int j) const { return (int)((uint64_t)(unsigned)j * p.div_mul >> p.div_shift); }
   // Page of the lane's key (key lane % KEYS) of tile t; -1: none.
   __device__ __forceinline__ int page_of(const int* table, int t) const {
-    const int j = t * KEYS + (lane & (KEYS - 1)), at = j / p.page_size;
+    const int at = page_index(t * KEYS + (lane & (KEYS - 1)));
     return at < p.table_width ? table[at] : -1;
   }
-  // Rows of the tile's keys, shared among the lanes.  Keys past the end or of no page read the cache's first row.
-  __device__ __forceinline__ void locate(int t, int page, int length, unsigned& there) {
-    const int j = t * KEYS + (lane & (KEYS - 1)), slot = j % p.page_size;
-    const bool ok = j < length && page >= 0 && page < p.pages;
-    there = (unsigned)__ballot(ok) & (KEYS == 32 ? 0xffffffffu : 0xffffu);
-    const int64_t k = ok ? page * p.kpage + slot * p.kslot : 0, v = ok ? page * p.vpage + slot * p.vslot : 0;
+  // Which of a tile's keys are there, and where they lie.  Sixteen keys of one page: where their rows begin, for all lanes;
+  // else each lane's own key, shared as it is loaded.  Keys of no page are read as the first page's.
+  __device__ __forceinline__ unsigned locate(int t, int page, int length) {
+    const int j = t * KEYS + (lane & (KEYS - 1));
+    const bool ok = j < length && (unsigned)page < (unsigned)p.pages;
+    const unsigned there = (unsigned)__ballot(ok) & kAll;
+    const int own = (unsigned)page < (unsigned)p.pages ? page : 0;
+    if (p.even) {
 #pragma unroll
-    for (int u = 0; u < KU; ++u) koff[u] = __shfl(k, 16 * u + m);
-#pragma unroll
-    for (int t = 0; t < VK; ++t) voff[t] = __shfl(v, 16 * (t >> 2) + 4 * h + (t & 3));
+      for (int u = 0; u < KU; ++u) {
+        const int j0 = t * KEYS + 16 * u, slot = j0 - page_index(j0) * p.page_size;
+        const int64_t at = __builtin_amdgcn_readlane(own, 16 * u);
+        kat[u] = at * p.kpage + slot * p.kslot;
+        vat[u] = at * p.vpage + slot * p.vslot;
+      }
+    } else {
+      const int slot = j - page_index(j) * p.page_size;
+      kat[0] = own * p.kpage + slot * p.kslot;
+      vat[0] = own * p.vpage + slot * p.vslot;
+    }
+    return there;
   }
   __device__ __forceinline__ void load_k() {
+    if (p.even) {
 #pragma unroll
-    for (int u = 0; u < KU; ++u)
+      for (int u = 0; u < KU; ++u)
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int d = KL * (4 * s + h);
-        kf[u][s] = *reinterpret_cast<const kvec*>(kbase + koff[u] + (d < a.D ? d : 0) * (int)sizeof(T));
+        for (int s = 0; s < KS; ++s) kf[u][s] = *reinterpret_cast<const kvec*>(kbase + kat[u] + (krow + kd[s]));
+    } else {
+#pragma unroll
+      for (int u = 0; u < KU; ++u) {
+        const char* row = kbase + __shfl(kat[0], 16 * u + m);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) kf[u][s] = *reinterpret_cast<const kvec*>(row + kd[s]);
       }
+    }
+    if (a.D < DP)   // zero times what lies there has to be zero
+#pragma unroll
+      for (int u = 0; u < KU; ++u)
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+          if (KL * (4 * s + h) >= a.D) kf[u][s] = kvec{};
   }
   __device__ __forceinline__ void load_v() {
+    if (p.even) {
 #pragma unroll
-    for (int t = 0; t < VK; ++t)
+      for (int t = 0; t < VK; ++t)
 #pragma unroll
-      for (int c = 0; c < VC / VL; ++c) {
-        const int d = 16 * VL * c + VL * m;
-        vf[t][c] = *reinterpret_cast<const vvec*>(vbase + voff[t] + (d < a.D ? d : 0) * (int)sizeof(T));
+        for (int c = 0; c < VC / VL; ++c)
+          vf[t][c] = *reinterpret_cast<const vvec*>(vbase + vat[t >> 2] + (t & 3) * p.vslot + (vrow + vd[c]));
+    } else {
+#pragma unroll
+      for (int t = 0; t < VK; ++t) {
+        const char* row = vbase + __shfl(vat[0], 16 * (t >> 2) + 4 * h + (t & 3));
+#pragma unroll
+        for (int c = 0; c < VC / VL; ++c) vf[t][c] = *reinterpret_cast<const vvec*>(row + vd[c]);
       }
+    }
   }
-
-  // acc += V^T times the tile's weights; for the lanes that are `mine`, if SOME
-  template <bool SOME>
-  __device__ __forceinline__ void add_values(const float (&x)[RB][KU][4], f32x4 (&acc)[RB][VC],
-                                             const bool (&mine)[RB]) const {
-    const auto put = [&](int q, int c, f32x4 sum) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc[q][c][r] = !SOME || mine[q] ? sum[r] : acc[q][c][r];
-    };
+  // acc += V^T times the tile's weights
+  __device__ __forceinline__ void add_values(const float (&x)[RB][KU][4], f32x4 (&acc)[RB][VC]) const {
     if constexpr (sizeof(T) == 2) {
       bf16x8 hi[RB], lo[RB];
 #pragma unroll
@@ -160,30 +227,37 @@ struct Walk {
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = vf[k][0][c];
 #pragma unroll
-        for (int q = 0; q < RB; ++q) put(q, c, mfma_16x16(v, hi[q], mfma_16x16(v, lo[q], acc[q][c])));
+        for (int q = 0; q < RB; ++q) acc[q][c] = mfma_16x16(v, hi[q], mfma_16x16(v, lo[q], acc[q][c]));
       }
     } else {
 #pragma unroll
-      for (int c = 0; c < VC; ++c)
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int q = 0; q < RB; ++q) {
-          f32x4 sum = acc[q][c];
+        for (int c = 0; c < VC; ++c)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) sum = mfma_16x16(vf[r][c / VL][c % VL], x[q][0][r], sum);
-          put(q, c, sum);
-        }
+          for (int q = 0; q < RB; ++q) acc[q][c] = mfma_16x16(vf[r][c / VL][c % VL], x[q][0][r], acc[q][c]);
     }
   }
-  // Whether the tile's values hold an infinity or NaN: on their bits, and by size, since the compiler, which is told that
-  // there are no NaN, knows the usual test of the exponent for what it is.
-  __device__ __forceinline__ bool any_not_finite() const {
+  // Whether v is an infinity or NaN: on its bits, and by size, since the compiler, which is told that there are no NaN,
+  // knows the usual test of the exponent for what it is.
+  __device__ static __forceinline__ bool not_finite(T v) {
+    return __builtin_bit_cast(uint32_t, (float)v) << 1 >= 0xff000000u;
+  }
+  // Takes the values that are not finite out of the tile; whether there were any.
+  __device__ __forceinline__ bool take_not_finite() {
     bool bad = false;
 #pragma unroll
     for (int k = 0; k < VK; ++k)
 #pragma unroll
-      for (int c = 0; c < VC; ++c) {
-        const uint32_t bits = __builtin_bit_cast(uint32_t, (float)vf[k][c / VL][c % VL]);
-        bad |= bits << 1 >= 0xff000000u;
+      for (int c = 0; c < VC / VL; ++c) {
+        vvec v = vf[k][c];
+#pragma unroll
+        for (int e = 0; e < VL; ++e) {
+          const bool is = not_finite(v[e]);
+          bad |= is;
+          v[e] = is ? (T)0.f : v[e];
+        }
+        vf[k][c] = v;
       }
     return __ballot(bad) != 0;
   }
@@ -194,39 +268,49 @@ struct Walk {
     const int wave = wave_id(), length = length_of(p, b);
     const int rows = a.Nq * a.G, n_rows = min(rows - row0, 16 * RB);
     const int count = p.counts ? min(max(p.counts[b], 0), a.Nq) : a.Nq;
+    const int first = length - count;   // position of the first query
     const int* table = p.page_table + b * p.table_stride;
     kbase = p.keys + hk * p.khead;
     vbase = p.values + hk * p.vhead;
+    int t = t0 + wave, page = page_of(table, t);
 
-    int t = t0 + wave, page = t < t1 ? page_of(table, t) : -1;
-    unsigned there = 0;
-    if (t < t1) {
-      locate(t, page, length, there);
-      load_k();
-      load_v();
-      page = t + kWaves < t1 ? page_of(table, t + kWaves) : -1;
-    }
-
-    int pos[RB], lim[RB], head[RB];
+    int pos[RB], lim[RB];
     kvec qf[RB][KS];
-    float far_lo[RB], far_hi[RB];
 #pragma unroll
     for (int q = 0; q < RB; ++q) {
-      const int r = row0 + 16 * q + m, i = r < rows ? r / a.G : 0;
-      head[q] = hk * a.G + (r < rows ? r - i * a.G : 0);
+      const int r = row0 + 16 * q + m, i = r < rows ? r / a.G : 0, head = hk * a.G + (r < rows ? r - i * a.G : 0);
       const bool live = r < rows && i < count;
-      pos[q] = length - count + i;
+      pos[q] = first + i;
       lim[q] = !live ? 0 : a.causal ? min(pos[q] + 1, length) : length;
-      const T* row = static_cast<const T*>(a.q) + b * a.qb + i * a.qn + head[q] * a.qh;
+      const T* row = static_cast<const T*>(a.q) + b * a.qb + i * a.qn + head * a.qh;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const int d = KL * (4 * s + h);
-        qf[q][s] = live && d < a.D ? *reinterpret_cast<const kvec*>(row + d) : kvec{};
+        qf[q][s] = r < rows && d < a.D ? *reinterpret_cast<const kvec*>(row + d) : kvec{};
       }
-      far_lo[q] = a.table ? table_value(a, 0, head[q]) : 0.f;
-      far_hi[q] = a.table ? table_value(a, 2 * a.radius, head[q]) : 0.f;
     }
-    const int first = length - count;   // position of the first query
+    // every row that counts sees the keys below low
+    const int low = a.causal ? min(first + 1, length) : length;
+    unsigned there = 0;
+    if (t < t1) {
+      there = locate(t, page, length);
+      load_k();
+      load_v();
+      page = t + W < t1 ? page_of(table, t + W) : -1;
+    }
+    // the bias by bucket and row, and the buckets by distance, where the waves' parts go later
+    float* bias = reinterpret_cast<float*>(lds);                         // [buckets][16 RB]
+    uint8_t* buckets = reinterpret_cast<uint8_t*>(bias + 256 * 16 * RB);   // [2 radius + 1]
+    if (a.table) {
+      for (int e = threadIdx.x; e < a.nb * 16 * RB; e += 64 * W) {
+        const int r = row0 + e % (16 * RB), head = hk * a.G + (r < rows ? r % a.G : 0);
+        const int64_t at = (int64_t)(e / (16 * RB)) * a.H + head;
+        bias[e] = bias_log2(a.table_bf16 ? (float)static_cast<const bf16*>(a.table)[at]
+                                         : static_cast<const float*>(a.table)[at]);
+      }
+      for (int e = threadIdx.x; e <= 2 * a.radius; e += 64 * W) buckets[e] = (uint8_t)min((int)a.buckets[e], a.nb - 1);
+      __syncthreads();
+    }
 
     f32x4 acc[RB][VC];
     float top[RB], ref[RB], l[RB];
@@ -236,13 +320,16 @@ struct Walk {
       for (int c = 0; c < VC; ++c) acc[q][c] = f32x4{0.f, 0.f, 0.f, 0.f};
       top[q] = -kInf;
       ref[q] = l[q] = 0.f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) asm volatile("" ::"v"(qf[q][s]));   // waited for here, not in every turn
     }
     const Capped<T, CAP> capped(a);
     const float mult = a.scale * kLog2e;
 
-    for (; t < t1; t += kWaves) {
+    bool taken = false;
+    for (; t < t1; t += W) {
       const int j0 = t * KEYS;
-      const bool next = t + kWaves < t1;
+      const bool next = t + W < t1;
       const unsigned now = there;
       f32x4 s[RB][KU];
 #pragma unroll
@@ -253,8 +340,7 @@ struct Walk {
       for (int u = 0; u < KU; ++u)
 #pragma unroll
         for (int st = 0; st < KS; ++st) {
-          kvec k = kf[u][st];
-          if (KL * (4 * st + h) >= a.D) k = kvec{};   // zero times what lies there has to be zero
+          const kvec k = kf[u][st];
 #pragma unroll
           for (int q = 0; q < RB; ++q) {
             if constexpr (sizeof(T) == 2) {
@@ -265,61 +351,60 @@ struct Walk {
             }
           }
         }
-      int64_t vnext[VK];
+      __builtin_amdgcn_sched_barrier(0);   // K's registers are free
       if (next) {
-        int64_t vnow[VK];
-#pragma unroll
-        for (int k = 0; k < VK; ++k) vnow[k] = voff[k];
-        locate(t + kWaves, page, length, there);
+        there = locate(t + W, page, length);
         load_k();
-        page = t + 2 * kWaves < t1 ? page_of(table, t + 2 * kWaves) : -1;
-#pragma unroll
-        for (int k = 0; k < VK; ++k) {
-          vnext[k] = voff[k];
-          voff[k] = vnow[k];
-        }
+        page = t + 2 * W < t1 ? page_of(table, t + 2 * W) : -1;
       }
 
       float x[RB][KU][4];
+      if (a.cap > 0.f) {
+        float slope;
+#pragma unroll
+        for (int q = 0; q < RB; ++q)
+#pragma unroll
+          for (int u = 0; u < KU; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[q][u][r] = capped.score(s[q][u][r], capped.k3, slope);
+      } else {
+#pragma unroll
+        for (int q = 0; q < RB; ++q)
+#pragma unroll
+          for (int u = 0; u < KU; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[q][u][r] = s[q][u][r] * mult;
+      }
+      if (a.table) {
+        const int rel0 = j0 - first;   // the first key from the first query
+        const bool far = rel0 - (a.Nq - 1) >= a.radius || rel0 + KEYS - 1 <= -a.radius;
+#pragma unroll
+        for (int q = 0; q < RB; ++q)
+#pragma unroll
+          for (int u = 0; u < KU; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int rel = far ? rel0 : j0 + 16 * u + 4 * h + r - pos[q];
+              const int bucket = buckets[min(max(rel, -a.radius), a.radius) + a.radius];
+              x[q][u][r] += bias[bucket * 16 * RB + 16 * q + m];
+            }
+      }
 #pragma unroll
       for (int q = 0; q < RB; ++q) {
+        if (now != kAll || j0 + KEYS > low)
+#pragma unroll
+          for (int u = 0; u < KU; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int k = 16 * u + 4 * h + r;
+              x[q][u][r] = j0 + k < lim[q] && (now >> k & 1) ? x[q][u][r] : -kInf;
+            }
+        float mx = x[q][0][0];
 #pragma unroll
         for (int u = 0; u < KU; ++u)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float slope;
-            x[q][u][r] = a.cap > 0.f ? capped.score(s[q][u][r], capped.k3, slope) : s[q][u][r] * mult;
-          }
-        if (a.table) {
-          const int rel0 = j0 - first;   // the first key from the first query
-          if (rel0 - (a.Nq - 1) >= a.radius || rel0 + KEYS - 1 <= -a.radius) {
-            const float far = rel0 > 0 ? far_hi[q] : far_lo[q];
-#pragma unroll
-            for (int u = 0; u < KU; ++u)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) x[q][u][r] += far;
-          } else {
-#pragma unroll
-            for (int u = 0; u < KU; ++u)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const int rel = j0 + 16 * u + 4 * h + r - pos[q];
-                x[q][u][r] += table_value(a, min(max(rel, -a.radius), a.radius) + a.radius, head[q]);
-              }
-          }
-        }
-        float mx = -kInf;
-#pragma unroll
-        for (int u = 0; u < KU; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int k = 16 * u + 4 * h + r;
-            const bool ok = j0 + k < lim[q] && (now >> k & 1);
-            x[q][u][r] = ok ? x[q][u][r] : -kInf;
-            mx = fmaxf(mx, x[q][u][r]);
-          }
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
+          for (int r = 0; r < 4; ++r) mx = fmaxf(mx, x[q][u][r]);
+        mx = max_over_keys(mx);
         if (__ballot(mx > top[q] + kRescale)) {
           const float mn = fmaxf(top[q], mx), to = mn == -kInf ? 0.f : mn;
           const float f = fast_exp2(top[q] - to);
@@ -340,7 +425,7 @@ struct Walk {
           }
       }
 
-      if (now != (KEYS == 32 ? 0xffffffffu : 0xffffu)) {
+      if (now != kAll) {
         // what a key that is not there holds has to count nothing, whatever it is
 #pragma unroll
         for (int k = 0; k < VK; ++k)
@@ -348,33 +433,19 @@ struct Walk {
 #pragma unroll
             for (int c = 0; c < VC / VL; ++c) vf[k][c] = vvec{};
       }
-      if (a.causal && j0 + KEYS > first + 1 && any_not_finite()) {
-        // a value that is not finite counts for the queries that see it alone (zero times it is not zero): one query
-        // after the other, the last first, with the keys behind each taken away
-        for (int qi = (min(row0 + 16 * RB, rows) - 1) / a.G; qi >= row0 / a.G; --qi) {
-#pragma unroll
-          for (int k = 0; k < VK; ++k)
-            if (j0 + 16 * (k >> 2) + 4 * h + (k & 3) > first + qi)
-#pragma unroll
-              for (int c = 0; c < VC / VL; ++c) vf[k][c] = vvec{};
-          bool mine[RB];
-#pragma unroll
-          for (int q = 0; q < RB; ++q) mine[q] = pos[q] == first + qi;
-          add_values<true>(x, acc, mine);
-        }
-      } else {
-        add_values<false>(x, acc, {});
-      }
-      if (next) {
-#pragma unroll
-        for (int k = 0; k < VK; ++k) voff[k] = vnext[k];
-        load_v();
-      }
+      // where rows differ in what they see, a value that is not finite waits for the end (zero times it is not zero)
+      if (a.causal && a.Nq > 1 && j0 + KEYS > first + 1) taken |= take_not_finite();
+      add_values(x, acc);
+      __builtin_amdgcn_sched_barrier(0);   // and V's
+      if (next) load_v();
     }
 
     // the waves' parts through LDS
-    float* sh = reinterpret_cast<float*>(lds);                       // [waves][16 RB][DP]
-    float* ml = sh + kWaves * 16 * RB * DP;                          // [waves][16 RB][2]
+    if (a.table) __syncthreads();
+    float* sh = reinterpret_cast<float*>(lds);              // [waves][16 RB][DP]
+    float* ml = sh + W * 16 * RB * DP;                      // [waves][16 RB][2]
+    int* flags = reinterpret_cast<int*>(ml + W * 16 * RB * 2);   // [waves]
+    if (lane == 0) flags[wave] = taken;
 #pragma unroll
     for (int q = 0; q < RB; ++q) {
       l[q] += __shfl_xor(l[q], 16);
@@ -390,29 +461,41 @@ struct Walk {
         for (int c = 0; c < VC; ++c) sh[at * DP + 16 * VL * (c / VL) + VL * (4 * h + r) + c % VL] = acc[q][c][r];
     }
     __syncthreads();
-    for (int k = threadIdx.x; k < n_rows * DP; k += 64 * kWaves) {
+    for (int k = threadIdx.x; k < n_rows * DP; k += 64 * W) {
       const int r = k / DP, d = k - r * DP;
       if (d >= a.D) continue;
       float most = -kInf;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) most = fmaxf(most, ml[2 * (w * 16 * RB + r)]);
+      for (int w = 0; w < W; ++w) most = fmaxf(most, ml[2 * (w * 16 * RB + r)]);
       const float to = most == -kInf ? 0.f : most;
       float o = 0.f, sum = 0.f;
+      int any = 0;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
+      for (int w = 0; w < W; ++w) {
         const int at = w * 16 * RB + r;
         const float f = fast_exp2(ml[2 * at] - to);
         o += f * sh[at * DP + d];
         sum += f * ml[2 * at + 1];
+        any |= flags[w];
+      }
+      const int i = (row0 + r) / a.G, g = row0 + r - i * a.G;
+      if (i >= count) o = sum = 0.f;   // padding
+      if (any) {   // its size does not matter: whatever a seen one weighs, so is the result
+        const int seen = i < count ? min(first + i + 1, min(length, t1 * KEYS)) : 0;
+        for (int j = max(max(first + 1, 0) / KEYS, t0) * KEYS; j < seen; ++j) {   // from the first such tile
+          const int at = page_index(j), page = table[at];
+          if (page < 0 || page >= p.pages) continue;
+          const T v = reinterpret_cast<const T*>(vbase + page * p.vpage + (j - at * p.page_size) * p.vslot)[d];
+          if (not_finite(v)) o += (float)v;
+        }
       }
       if (slot < 0) {
-        const int i = (row0 + r) / a.G, g = row0 + r - i * a.G;
         out[(((int64_t)b * a.Nq + i) * a.H + hk * a.G + g) * a.D + d] = (T)over_sum(o, sum);
       } else {
         const int64_t at = slot * min(rows, 16 * RB) + r;
         parts.o[at * a.D + d] = o;
         if (d == 0) {
-          parts.ml[2 * at] = sum == 0.f ? -kInf : to;
+          parts.ml[2 * at] = i >= count || sum == 0.f ? -kInf : to;
           parts.ml[2 * at + 1] = sum;
         }
       }
@@ -421,62 +504,105 @@ struct Walk {
   }
 };
 
+// LDS of a workgroup: the waves' parts, and before them the bias.
+template <int DP, int RB, int W>
+constexpr int lds_bytes() {
+  constexpr int parts = W * (16 * RB * (DP + 2) + 1) * 4, bias = 256 * 16 * RB * 4 + 2 * kMaxRadius + 4;
+  return parts > bias ? parts : bias;
+}
+
 // An item is a block of rows of a key head of a sequence.  Without groups a workgroup takes an item; with them the tiles
 // of all items, one behind the other, are dealt evenly to the workgroups, whatever the sequences' lengths: a workgroup's
 // share of an item is its part (workgroup + item) of the join, or the whole, which is written at once.
-template <class T, int DP, int RB, int CAP>
-__global__ __launch_bounds__(64 * kWaves) void paged_kernel(const AttnArgs a, const PagedArgs p, T* __restrict__ out,
-                                                            Parts parts) {
+template <class T, int DP, int RB, int CAP, int W>
+__global__ __launch_bounds__(64 * W, 2) void paged_kernel(const AttnArgs a, const PagedArgs p, T* __restrict__ out,
+                                                          Parts parts) {
   constexpr int KEYS = Cache<T>::KEYS;
-  __shared__ __attribute__((aligned(16))) char lds[kWaves * 16 * RB * (DP + 2) * 4];
-  Walk<T, DP, RB, CAP> walk(a, p);
+  __shared__ __attribute__((aligned(16))) char lds[lds_bytes<DP, RB, W>()];
+  Walk<T, DP, RB, CAP, W> walk(a, p);
   const int items = a.Hk * p.blocks;   // of a sequence
+  int b = 0, tiles;
+  int64_t at, end, before = 0;   // the tiles to take, and those of the sequences before b
   if (p.groups == 0) {
-    const int b = blockIdx.x / items, item = blockIdx.x - b * items;
-    walk.run(b, item / p.blocks, item % p.blocks * 16 * RB, 0, (length_of(p, b) + KEYS - 1) / KEYS, out, parts, -1, lds);
-    return;
-  }
-  const int64_t total = uniform(tiles_before<KEYS>(p, a.B, items));
-  const int64_t n = min((int64_t)p.groups, (total + p.least - 1) / p.least);
-  if ((int64_t)blockIdx.x >= n) return;
-  int64_t at = total * blockIdx.x / n;
-  const int64_t end = total * (blockIdx.x + 1) / n;
-  // the sequence that holds tile `at`
-  int b = 0;
-  int64_t before = 0;
-  for (const int lane = threadIdx.x & 63;; b += 64) {
-    const int64_t own = b + lane < a.B ? (int64_t)((length_of(p, b + lane) + KEYS - 1) / KEYS) * items : 0;
-    int64_t sum = own;
+    b = blockIdx.x / items;
+    tiles = tiles_of<KEYS>(p, b);
+    at = (int64_t)(blockIdx.x - b * items) * tiles;
+    end = at + tiles;
+    if (tiles == 0) {
+      const int item = blockIdx.x - b * items, hk = item / p.blocks, row0 = item % p.blocks * 16 * RB;
+      const int n = min(a.Nq * a.G - row0, 16 * RB);
+      for (int k = threadIdx.x; k < n * a.D; k += 64 * W) {
+        const int r = row0 + k / a.D, i = r / a.G;
+        out[(((int64_t)b * a.Nq + i) * a.H + hk * a.G + r - i * a.G) * a.D + k % a.D] = (T)0.f;
+      }
+      return;
+    }
+  } else {
+    const Deal all = deal<KEYS>(p, a.B, 0, items);
+    if ((int64_t)blockIdx.x >= all.groups) return;
+    at = all.total * blockIdx.x / all.groups;
+    end = all.total * (blockIdx.x + 1) / all.groups;
+    // the sequence that holds tile `at`
+    for (const int lane = threadIdx.x & 63;; b += 64) {
+      const int64_t own = b + lane < a.B ? (int64_t)tiles_of<KEYS>(p, b + lane) * items : 0;
+      int64_t sum = own;
 #pragma unroll
-    for (int m = 1; m < 64; m *= 2) {
-      const int64_t o = __shfl_up(sum, m);
-      if (lane >= m) sum += o;
+      for (int m = 1; m < 64; m *= 2) {
+        const int64_t o = __shfl_up(sum, m);
+        if (lane >= m) sum += o;
+      }
+      const uint64_t past = __ballot(before + sum > at);
+      if (past) {
+        const int l = __ffsll((unsigned long long)past) - 1;
+        b += l;
+        before = uniform(before + __shfl(sum - own, l));
+        break;
+      }
+      before = uniform(before + __shfl(sum, 63));
+      if (b + 64 >= a.B) return;
     }
-    const uint64_t past = __ballot(before + sum > at);
-    if (past) {
-      const int l = __ffsll((unsigned long long)past) - 1;
-      b += l;
-      before = uniform(before + __shfl(sum - own, l));
-      break;
-    }
-    before = uniform(before + __shfl(sum, 63));
-    if (b + 64 >= a.B) return;
+    tiles = tiles_of<KEYS>(p, b);
   }
-  for (; at < end && b < a.B; ++b) {
-    const int tiles = (length_of(p, b) + KEYS - 1) / KEYS;
-    while (at < end && at - before < (int64_t)tiles * items) {
-      const int item = (int)((at - before) / tiles), t0 = (int)((at - before) - (int64_t)item * tiles);
-      const int t1 = (int)min((int64_t)tiles, t0 + (end - at));
-      const int64_t slot = t0 == 0 && t1 == tiles ? -1 : (int64_t)blockIdx.x + (int64_t)b * items + item;
-      walk.run(b, item / p.blocks, item % p.blocks * 16 * RB, t0, t1, out, parts, slot, lds);
-      at += t1 - t0;
+  while (at < end) {
+    if (at - before >= (int64_t)tiles * items) {
+      before += (int64_t)tiles * items;
+      if (++b >= a.B) return;
+      tiles = tiles_of<KEYS>(p, b);
+      continue;
     }
-    before += (int64_t)tiles * items;
+    const int item = (int)((at - before) / tiles), t0 = (int)((at - before) - (int64_t)item * tiles);
+    const int t1 = (int)min((int64_t)tiles, t0 + (end - at));
+    const int64_t slot = t0 == 0 && t1 == tiles ? -1 : (int64_t)blockIdx.x + (int64_t)b * items + item;
+    if (p.groups && threadIdx.x == 0) {
+      int* range = parts.range + 2 * ((int64_t)b * items + item);
+      if (t0 == 0) range[0] = blockIdx.x;
+      if (t1 == tiles) range[1] = blockIdx.x;
+    }
+    walk.run(b, item / p.blocks, item % p.blocks * 16 * RB, t0, t1, out, parts, slot, lds);
+    at += t1 - t0;
   }
 }
 
-// Adds the parts of a row in a fixed order: wave w takes parts w, w + waves, ..., then the waves are added.  Rows that
-// one workgroup had are there already; rows of empty sequences get zeros.
+// The parts of a row: those of workgroups first .. last of its item, slot workgroup + item; none where the sequence is
+// empty, one where the result is there already.
+struct RowParts {
+  int64_t row0;   // of the first part
+  int n, stride;
+};
+template <int KEYS>
+__device__ __forceinline__ RowParts row_parts(const AttnArgs& a, const PagedArgs& p, const Parts& parts, int64_t row,
+                                              int block_rows) {
+  const int h = (int)(row % a.H), b = (int)(row / a.H / a.Nq), i = (int)(row / a.H - (int64_t)b * a.Nq);
+  const int hk = h / a.G, r = i * a.G + h - hk * a.G, blk = r / block_rows;
+  const int64_t item = ((int64_t)b * a.Hk + hk) * p.blocks + blk;
+  const int stride = min(a.Nq * a.G, block_rows);
+  if (tiles_of<KEYS>(p, b) == 0) return {0, 0, stride};
+  const int first = parts.range[2 * item], last = parts.range[2 * item + 1];
+  return {(first + item) * stride + r - blk * block_rows, last - first + 1, stride};
+}
+
+// paged_join: few rows of many parts, a workgroup a row: wave w takes parts w, w + waves, ..., then the waves are added in
+// order.  Lane d holds values d and 64 + d.
 constexpr int kJoinWaves = 8;
 template <class T, int KEYS>
 __global__ __launch_bounds__(64 * kJoinWaves) void paged_join_kernel(const AttnArgs a, const PagedArgs p,
@@ -484,31 +610,18 @@ __global__ __launch_bounds__(64 * kJoinWaves) void paged_join_kernel(const AttnA
   __shared__ float sh[kJoinWaves][3][64];
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int64_t row = blockIdx.x;   // (b, i, head)
-  const int h = (int)(row % a.H), i = (int)(row / a.H % a.Nq), b = (int)(row / a.H / a.Nq);
-  const int hk = h / a.G, r = i * a.G + h - hk * a.G, items = a.Hk * p.blocks;
-  const int item = hk * p.blocks + r / block_rows;
-  const int tiles = (length_of(p, b) + KEYS - 1) / KEYS;
-  const int64_t total = uniform(tiles_before<KEYS>(p, a.B, items));
-  const int64_t n = min((int64_t)p.groups, (total + p.least - 1) / p.least);
-  int64_t w0 = 0, w1 = -1;
-  if (tiles > 0) {
-    const int64_t at = uniform(tiles_before<KEYS>(p, b, items)) + (int64_t)item * tiles;
-    w0 = ((at + 1) * n - 1) / total;
-    w1 = ((at + tiles) * n - 1) / total;
-    if (w0 == w1) return;
-  }
-  const int64_t slot0 = (int64_t)b * items + item;
-  const int stride = min(a.Nq * a.G, block_rows);
+  const RowParts own = row_parts<KEYS>(a, p, parts, row, block_rows);
+  if (own.n == 1) return;
   float top = -kInf;
-  for (int64_t w = w0 + lane; w <= w1; w += 64) top = fmaxf(top, parts.ml[2 * ((w + slot0) * stride + r % block_rows)]);
+  for (int w = lane; w < own.n; w += 64) top = fmaxf(top, parts.ml[2 * (own.row0 + (int64_t)w * own.stride)]);
 #pragma unroll
   for (int m = 32; m > 0; m /= 2) top = fmaxf(top, __shfl_xor(top, m));
   const float to = top == -kInf ? 0.f : top;
   float o[2] = {0.f, 0.f}, sum = 0.f;
   const int d0 = min(lane, a.D - 1), d1 = min(lane + 64, a.D - 1);
 #pragma unroll 4
-  for (int64_t w = w0 + wave; w <= w1; w += kJoinWaves) {
-    const int64_t at = (w + slot0) * stride + r % block_rows;
+  for (int w = wave; w < own.n; w += kJoinWaves) {
+    const int64_t at = own.row0 + (int64_t)w * own.stride;
     const float f = fast_exp2(parts.ml[2 * at] - to);
     o[0] += f * parts.o[at * a.D + d0];
     o[1] += f * parts.o[at * a.D + d1];
@@ -531,8 +644,38 @@ __global__ __launch_bounds__(64 * kJoinWaves) void paged_join_kernel(const AttnA
     if (lane + 64 * e < a.D) out[row * a.D + lane + 64 * e] = (T)over_sum(o[e], sum);
 }
 
+// paged_join_rows: many rows of few parts, four values of one a thread, in the parts' order.
+template <class T, int KEYS>
+__global__ __launch_bounds__(256) void paged_join_rows_kernel(const AttnArgs a, const PagedArgs p, T* __restrict__ out,
+                                                              Parts parts, int block_rows, int rows) {
+  typedef T quad __attribute__((ext_vector_type(4)));
+  const unsigned quads = a.D / 4, k = blockIdx.x * 256 + threadIdx.x, row = k / quads, d = (k - row * quads) * 4;
+  if ((int)row >= rows) return;
+  const RowParts own = row_parts<KEYS>(a, p, parts, row, block_rows);
+  if (own.n == 1) return;
+  float top = -kInf;
+#pragma unroll 4
+  for (int w = 0; w < own.n; ++w) top = fmaxf(top, parts.ml[2 * (own.row0 + (int64_t)w * own.stride)]);
+  const float to = top == -kInf ? 0.f : top;
+  float o[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+#pragma unroll 4
+  for (int w = 0; w < own.n; ++w) {
+    const int64_t at = own.row0 + (int64_t)w * own.stride;
+    const f32x2 ml = *reinterpret_cast<const f32x2*>(parts.ml + 2 * at);
+    const f32x4 x = *reinterpret_cast<const f32x4*>(parts.o + at * a.D + d);
+    const float f = fast_exp2(ml[0] - to);
+    sum += f * ml[1];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] += f * x[c];
+  }
+  quad v;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) v[c] = (T)over_sum(o[c], sum);
+  *reinterpret_cast<quad*>(out + (int64_t)row * a.D + d) = v;
+}
+
 struct Plan {
-  int rb, blocks, groups, least;
+  int rb, blocks, waves, groups, least;
   int64_t items, slots;
 };
 
@@ -545,15 +688,20 @@ Plan plan(const AttnArgs& a, const bioemu_paged_cache& c, bool f32) {
   p.blocks = (rows + 16 * p.rb - 1) / (16 * p.rb);
   p.items = (int64_t)a.B * a.Hk * p.blocks;
   const int64_t most = c.pages > 0 ? c.table_width * c.page_size : 0;
-  if (most <= 1024 || p.items >= 16 * attn_units()) return p;
+  if (most <= 1024 || p.items >= 16 * attn_units()) {
+    p.waves = p.items <= 2 * attn_units() ? 8 : 4;
+    return p;
+  }
+  p.waves = 4;
   p.groups = 2 * attn_units();
-  p.least = 2 * kWaves;
+  p.least = 2 * p.waves;
   p.slots = p.groups + p.items;
   return p;
 }
 
 size_t parts_bytes(const AttnArgs& a, const Plan& p) {
-  return (size_t)p.slots * std::min(a.Nq * a.G, 16 * p.rb) * (a.D + 2) * sizeof(float);
+  return (size_t)p.slots * std::min(a.Nq * a.G, 16 * p.rb) * (a.D + 2) * sizeof(float) +
+         (p.groups ? (size_t)p.items * 2 * sizeof(int) : 0);
 }
 
 int paged_args(const bioemu_paged_cache* c, const bioemu_attention_args* in, AttnArgs* a, Plan* pl) {
@@ -570,30 +718,40 @@ int paged_args(const bioemu_paged_cache* c, const bioemu_attention_args* in, Att
 template <class T, int DP>
 int launch(const AttnArgs& a, const PagedArgs& p, const Plan& pl, T* out, void* ws, hipStream_t stream) {
   const int block_rows = 16 * pl.rb;
-  Parts parts{static_cast<float*>(ws), nullptr};
-  if (ws) parts.ml = parts.o + pl.slots * std::min(a.Nq * a.G, block_rows) * a.D;
+  Parts parts{static_cast<float*>(ws), nullptr, nullptr};
+  if (ws) {
+    const int64_t part_rows = pl.slots * std::min(a.Nq * a.G, block_rows);
+    parts.ml = parts.o + part_rows * a.D;
+    parts.range = reinterpret_cast<int*>(parts.ml + 2 * part_rows);
+  }
   {
     KernelTimerScope timer("paged_attention", stream);
     const dim3 grid((unsigned)(pl.groups ? pl.groups : pl.items));
-    const auto go = [&](auto kernel) { kernel<<<grid, 64 * kWaves, 0, stream>>>(a, p, out, parts); };
+    const auto go = [&](auto kernel) { kernel<<<grid, 64 * pl.waves, 0, stream>>>(a, p, out, parts); };
     const bool wide = !fast_cap<T>(a);
-    if (pl.rb == 1) {
-      if (!wide)
-        go(paged_kernel<T, DP, 1, kCapped>);
-      else if constexpr (sizeof(T) == 2)
-        go(paged_kernel<T, DP, 1, kCapWide>);
-    } else {
-      if (!wide)
-        go(paged_kernel<T, DP, 2, kCapped>);
-      else if constexpr (sizeof(T) == 2)
-        go(paged_kernel<T, DP, 2, kCapWide>);
-    }
+#define BIOEMU_GO(RB, W)                       \
+  if (pl.rb == RB && pl.waves == W) {          \
+    if (!wide)                                 \
+      go(paged_kernel<T, DP, RB, kCapped, W>); \
+    else if constexpr (sizeof(T) == 2)         \
+      go(paged_kernel<T, DP, RB, kCapWide, W>); \
+  }
+    BIOEMU_GO(1, 4)
+    BIOEMU_GO(2, 4)
+    BIOEMU_GO(1, 8)
+    BIOEMU_GO(2, 8)
+#undef BIOEMU_GO
     if (const int rc = check_launch("paged_attention")) return rc;
   }
   if (!pl.groups) return BIOEMU_OK;
   KernelTimerScope timer("paged_join", stream);
-  paged_join_kernel<T, Cache<T>::KEYS><<<dim3((unsigned)((int64_t)a.B * a.Nq * a.H)), 64 * kJoinWaves, 0, stream>>>(
-      a, p, out, parts, block_rows);
+  const int64_t rows = (int64_t)a.B * a.Nq * a.H;
+  if (pl.groups <= 14 * pl.items)
+    paged_join_rows_kernel<T, Cache<T>::KEYS><<<dim3((unsigned)((rows * (a.D / 4) + 255) / 256)), 256, 0, stream>>>(
+        a, p, out, parts, block_rows, (int)rows);
+  else
+    paged_join_kernel<T, Cache<T>::KEYS><<<dim3((unsigned)rows), 64 * kJoinWaves, 0, stream>>>(a, p, out, parts,
+                                                                                               block_rows);
   return check_launch("paged_join");
 }
 
@@ -622,10 +780,16 @@ extern "C" int bioemu_paged_attention(const bioemu_paged_cache* cache, const bio
     return set_error(BIOEMU_ERR_WORKSPACE, "paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   const int item = args->f32 ? 4 : 2;
   const int64_t *ks = cache->keys_stride, *vs = cache->values_stride;
+  // key / page_size: 2^(28 + l) / page_size rounded up, l = log2 of page_size rounded up, is off by less than 2^l / page_size
+  unsigned l = 0;
+  while ((int64_t(1) << l) < cache->page_size) ++l;
+  const unsigned mul = (unsigned)(((int64_t(1) << (28 + l)) + cache->page_size - 1) / cache->page_size);
+  const int64_t far = int64_t(1) << 27;   // sixteen slots' offsets in 32 bits
+  const int even = cache->page_size % 16 == 0 && ks[1] * item <= far && vs[1] * item <= far;
   const PagedArgs p{static_cast<const char*>(cache->keys), static_cast<const char*>(cache->values), ks[0] * item,
                     ks[1] * item, ks[2] * item, vs[0] * item, vs[1] * item, vs[2] * item, cache->page_table,
                     cache->table_stride, cache->lengths, cache->counts, (int)cache->pages, (int)cache->page_size,
-                    (int)cache->table_width, pl.blocks, pl.groups, pl.least};
+                    (int)cache->table_width, pl.blocks, mul, 28 + l, even, pl.groups, pl.least};
   const int dp = a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128;
   void* ws = need ? workspace : nullptr;
 #define BIOEMU_PAGED(T, P) \
