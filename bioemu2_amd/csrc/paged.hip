@@ -20,6 +20,9 @@
 namespace bioemu {
 namespace {
 
+// the compiler does not see by itself that addresses of two branches are of memory both
+#define GLOBAL __attribute__((address_space(1)))
+
 constexpr float kRescale = 8.f;   // log2 of the largest weight before the maximum moves
 
 struct PagedArgs {
@@ -30,7 +33,7 @@ struct PagedArgs {
   const int *lengths, *counts;
   int pages, page_size, table_width, blocks;   // blocks of rows a key head
   unsigned div_mul, div_shift;                  // key / page_size = key * div_mul >> div_shift, for keys below 2^28
-  int even;                                     // pages are whole blocks of 16 keys
+  bool even;                                    // pages are whole blocks of 16 keys
   int groups, least;                            // workgroups that share the keys, of `least` tiles at least; 0: one an item
 };
 
@@ -115,7 +118,7 @@ __device__ __forceinline__ Deal deal(const PagedArgs& p, int B, int upto, int it
   return {uniform(before) * items, total, min((int64_t)p.groups, want)};
 }
 
-template <class T, int DP, int RB, int CAP, int W>
+template <class T, int DP, int RB, int CAP, int W, bool EVEN>
 struct Walk {
   static constexpr int KEYS = Cache<T>::KEYS, VC = DP / 16;
   static constexpr int VL = VC * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : VC;   // values a load of V
@@ -128,17 +131,17 @@ struct Walk {
   const AttnArgs& a;
   const PagedArgs& p;
   const int lane, m, h;
-  const char *kbase, *vbase;
+  const GLOBAL char *kbase, *vbase;
   // byte offsets of the lane's row among sixteen, and of its pieces of a row (the row's first where it has no more)
   unsigned krow, vrow, kd[KS], vd[VC / VL];
-  int64_t kat[KU], vat[KU];   // see locate
+  int64_t kat, kat1, vat, vat1;   // see locate
   kvec kf[KU][KS];
   vvec vf[VK][VC / VL];
 
   __device__ __forceinline__ Walk(const AttnArgs& a_, const PagedArgs& p_)
       : a(a_), p(p_), lane(threadIdx.x & 63), m(lane & 15), h(lane >> 4) {
-    krow = p.even ? (unsigned)(m * p.kslot) : 0;
-    vrow = p.even ? (unsigned)(4 * h * p.vslot) : 0;
+    krow = EVEN ? (unsigned)(m * p.kslot) : 0;
+    vrow = EVEN ? (unsigned)(4 * h * p.vslot) : 0;
 #pragma unroll
     for (int s = 0; s < KS; ++s) kd[s] = KL * (4 * s + h) < a.D ? KL * (4 * s + h) * (int)sizeof(T) : 0;
 #pragma unroll
@@ -158,56 +161,34 @@ struct Walk {
     const bool ok = j < length && (unsigned)page < (unsigned)p.pages;
     const unsigned there = (unsigned)__ballot(ok) & kAll;
     const int own = (unsigned)page < (unsigned)p.pages ? page : 0;
-    if (p.even) {
-#pragma unroll
-      for (int u = 0; u < KU; ++u) {
-        const int j0 = t * KEYS + 16 * u, slot = j0 - page_index(j0) * p.page_size;
-        const int64_t at = __builtin_amdgcn_readlane(own, 16 * u);
-        kat[u] = at * p.kpage + slot * p.kslot;
-        vat[u] = at * p.vpage + slot * p.vslot;
-      }
+    if constexpr (EVEN) {
+      place(t * KEYS, __builtin_amdgcn_readlane(own, 0), kat, vat);
+      if constexpr (KU == 2) place(t * KEYS + 16, __builtin_amdgcn_readlane(own, 16), kat1, vat1);
     } else {
-      const int slot = j - page_index(j) * p.page_size;
-      kat[0] = own * p.kpage + slot * p.kslot;
-      vat[0] = own * p.vpage + slot * p.vslot;
+      place(j, own, kat, vat);
     }
     return there;
   }
+  __device__ __forceinline__ void place(int j, int64_t page, int64_t& k, int64_t& v) const {
+    const int slot = j - page_index(j) * p.page_size;
+    k = page * p.kpage + slot * p.kslot;
+    v = page * p.vpage + slot * p.vslot;
+  }
   __device__ __forceinline__ void load_k() {
-    if (p.even) {
 #pragma unroll
-      for (int u = 0; u < KU; ++u)
+    for (int u = 0; u < KU; ++u) {
+      const GLOBAL char* row = EVEN ? kbase + (u == 0 ? kat : kat1) : kbase + __shfl(kat, 16 * u + m);
 #pragma unroll
-        for (int s = 0; s < KS; ++s) kf[u][s] = *reinterpret_cast<const kvec*>(kbase + kat[u] + (krow + kd[s]));
-    } else {
-#pragma unroll
-      for (int u = 0; u < KU; ++u) {
-        const char* row = kbase + __shfl(kat[0], 16 * u + m);
-#pragma unroll
-        for (int s = 0; s < KS; ++s) kf[u][s] = *reinterpret_cast<const kvec*>(row + kd[s]);
-      }
+      for (int s = 0; s < KS; ++s) kf[u][s] = *(const GLOBAL kvec*)(row + (krow + kd[s]));
     }
-    if (a.D < DP)   // zero times what lies there has to be zero
-#pragma unroll
-      for (int u = 0; u < KU; ++u)
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-          if (KL * (4 * s + h) >= a.D) kf[u][s] = kvec{};
   }
   __device__ __forceinline__ void load_v() {
-    if (p.even) {
 #pragma unroll
-      for (int t = 0; t < VK; ++t)
+    for (int t = 0; t < VK; ++t) {
+      const GLOBAL char* row =
+          EVEN ? vbase + (t < 4 ? vat : vat1) + (t & 3) * p.vslot : vbase + __shfl(vat, 16 * (t >> 2) + 4 * h + (t & 3));
 #pragma unroll
-        for (int c = 0; c < VC / VL; ++c)
-          vf[t][c] = *reinterpret_cast<const vvec*>(vbase + vat[t >> 2] + (t & 3) * p.vslot + (vrow + vd[c]));
-    } else {
-#pragma unroll
-      for (int t = 0; t < VK; ++t) {
-        const char* row = vbase + __shfl(vat[0], 16 * (t >> 2) + 4 * h + (t & 3));
-#pragma unroll
-        for (int c = 0; c < VC / VL; ++c) vf[t][c] = *reinterpret_cast<const vvec*>(row + vd[c]);
-      }
+      for (int c = 0; c < VC / VL; ++c) vf[t][c] = *(const GLOBAL vvec*)(row + (vrow + vd[c]));
     }
   }
   // acc += V^T times the tile's weights
@@ -270,8 +251,8 @@ struct Walk {
     const int count = p.counts ? min(max(p.counts[b], 0), a.Nq) : a.Nq;
     const int first = length - count;   // position of the first query
     const int* table = p.page_table + b * p.table_stride;
-    kbase = p.keys + hk * p.khead;
-    vbase = p.values + hk * p.vhead;
+    kbase = (const GLOBAL char*)p.keys + hk * p.khead;
+    vbase = (const GLOBAL char*)p.values + hk * p.vhead;
     int t = t0 + wave, page = page_of(table, t);
 
     int pos[RB], lim[RB];
@@ -292,11 +273,13 @@ struct Walk {
     // every row that counts sees the keys below low
     const int low = a.causal ? min(first + 1, length) : length;
     unsigned there = 0;
+    // keys, values and the page after next are requested as soon as there is room; behind the last tile it once more (a
+    // load that may not be made would have to be waited for at once)
+    const auto after = [&](int t) { return t + W < t1 ? t + W : t; };
     if (t < t1) {
       there = locate(t, page, length);
       load_k();
-      load_v();
-      page = t + W < t1 ? page_of(table, t + W) : -1;
+      page = page_of(table, after(t));
     }
     // the bias by bucket and row, and the buckets by distance, where the waves' parts go later
     float* bias = reinterpret_cast<float*>(lds);                         // [buckets][16 RB]
@@ -327,10 +310,17 @@ struct Walk {
     const float mult = a.scale * kLog2e;
 
     bool taken = false;
-    for (; t < t1; t += W) {
-      const int j0 = t * KEYS;
-      const bool next = t + W < t1;
+    for (bool more = t < t1; more;) {
+      const int j0 = t * KEYS, next = after(t);
+      load_v();
+      __builtin_amdgcn_sched_barrier(0);
       const unsigned now = there;
+      if (a.D < DP)   // zero times what lies there has to be zero
+#pragma unroll
+        for (int u = 0; u < KU; ++u)
+#pragma unroll
+          for (int st = 0; st < KS; ++st)
+            if (KL * (4 * st + h) >= a.D) kf[u][st] = kvec{};
       f32x4 s[RB][KU];
 #pragma unroll
       for (int q = 0; q < RB; ++q)
@@ -352,11 +342,9 @@ struct Walk {
           }
         }
       __builtin_amdgcn_sched_barrier(0);   // K's registers are free
-      if (next) {
-        there = locate(t + W, page, length);
-        load_k();
-        page = t + 2 * W < t1 ? page_of(table, t + 2 * W) : -1;
-      }
+      there = locate(next, page, length);
+      load_k();
+      page = page_of(table, after(next));
 
       float x[RB][KU][4];
       if (a.cap > 0.f) {
@@ -437,7 +425,8 @@ struct Walk {
       if (a.causal && a.Nq > 1 && j0 + KEYS > first + 1) taken |= take_not_finite();
       add_values(x, acc);
       __builtin_amdgcn_sched_barrier(0);   // and V's
-      if (next) load_v();
+      more = next != t;
+      t = next;
     }
 
     // the waves' parts through LDS
@@ -485,7 +474,7 @@ struct Walk {
         for (int j = max(max(first + 1, 0) / KEYS, t0) * KEYS; j < seen; ++j) {   // from the first such tile
           const int at = page_index(j), page = table[at];
           if (page < 0 || page >= p.pages) continue;
-          const T v = reinterpret_cast<const T*>(vbase + page * p.vpage + (j - at * p.page_size) * p.vslot)[d];
+          const T v = ((const GLOBAL T*)(vbase + page * p.vpage + (j - at * p.page_size) * p.vslot))[d];
           if (not_finite(v)) o += (float)v;
         }
       }
@@ -514,12 +503,12 @@ constexpr int lds_bytes() {
 // An item is a block of rows of a key head of a sequence.  Without groups a workgroup takes an item; with them the tiles
 // of all items, one behind the other, are dealt evenly to the workgroups, whatever the sequences' lengths: a workgroup's
 // share of an item is its part (workgroup + item) of the join, or the whole, which is written at once.
-template <class T, int DP, int RB, int CAP, int W>
+template <class T, int DP, int RB, int CAP, int W, bool EVEN>
 __global__ __launch_bounds__(64 * W, 2) void paged_kernel(const AttnArgs a, const PagedArgs p, T* __restrict__ out,
                                                           Parts parts) {
   constexpr int KEYS = Cache<T>::KEYS;
   __shared__ __attribute__((aligned(16))) char lds[lds_bytes<DP, RB, W>()];
-  Walk<T, DP, RB, CAP, W> walk(a, p);
+  Walk<T, DP, RB, CAP, W, EVEN> walk(a, p);
   const int items = a.Hk * p.blocks;   // of a sequence
   int b = 0, tiles;
   int64_t at, end, before = 0;   // the tiles to take, and those of the sequences before b
@@ -683,16 +672,16 @@ struct Plan {
 // walk gains) or the items many.
 Plan plan(const AttnArgs& a, const bioemu_paged_cache& c, bool f32) {
   Plan p{};
+  p.waves = 4;
   const int rows = a.Nq * a.G;
   p.rb = rows <= 16 ? 1 : 2;
   p.blocks = (rows + 16 * p.rb - 1) / (16 * p.rb);
   p.items = (int64_t)a.B * a.Hk * p.blocks;
   const int64_t most = c.pages > 0 ? c.table_width * c.page_size : 0;
   if (most <= 1024 || p.items >= 16 * attn_units()) {
-    p.waves = p.items <= 2 * attn_units() ? 8 : 4;
+    p.waves = p.items <= 2 * attn_units() && (f32 || a.cap <= kFastCap) ? 8 : 4;
     return p;
   }
-  p.waves = 4;
   p.groups = 2 * attn_units();
   p.least = 2 * p.waves;
   p.slots = p.groups + p.items;
@@ -729,17 +718,20 @@ int launch(const AttnArgs& a, const PagedArgs& p, const Plan& pl, T* out, void* 
     const dim3 grid((unsigned)(pl.groups ? pl.groups : pl.items));
     const auto go = [&](auto kernel) { kernel<<<grid, 64 * pl.waves, 0, stream>>>(a, p, out, parts); };
     const bool wide = !fast_cap<T>(a);
-#define BIOEMU_GO(RB, W)                       \
-  if (pl.rb == RB && pl.waves == W) {          \
-    if (!wide)                                 \
-      go(paged_kernel<T, DP, RB, kCapped, W>); \
-    else if constexpr (sizeof(T) == 2)         \
-      go(paged_kernel<T, DP, RB, kCapWide, W>); \
+    // few calls have a wide cap: one form for them
+#define BIOEMU_GO(RB, W, EVEN)                                                                  \
+  if (pl.rb == RB && !wide && pl.waves == W && p.even == EVEN) go(paged_kernel<T, DP, RB, kCapped, W, EVEN>);
+#define BIOEMU_GO_RB(RB)                                             \
+  BIOEMU_GO(RB, 4, true)                                             \
+  BIOEMU_GO(RB, 4, false)                                            \
+  BIOEMU_GO(RB, 8, true)                                             \
+  BIOEMU_GO(RB, 8, false)                                            \
+  if constexpr (sizeof(T) == 2) {                                    \
+    if (pl.rb == RB && wide) go(paged_kernel<T, DP, RB, kCapWide, 4, false>); \
   }
-    BIOEMU_GO(1, 4)
-    BIOEMU_GO(2, 4)
-    BIOEMU_GO(1, 8)
-    BIOEMU_GO(2, 8)
+    BIOEMU_GO_RB(1)
+    BIOEMU_GO_RB(2)
+#undef BIOEMU_GO_RB
 #undef BIOEMU_GO
     if (const int rc = check_launch("paged_attention")) return rc;
   }
@@ -785,7 +777,7 @@ extern "C" int bioemu_paged_attention(const bioemu_paged_cache* cache, const bio
   while ((int64_t(1) << l) < cache->page_size) ++l;
   const unsigned mul = (unsigned)(((int64_t(1) << (28 + l)) + cache->page_size - 1) / cache->page_size);
   const int64_t far = int64_t(1) << 27;   // sixteen slots' offsets in 32 bits
-  const int even = cache->page_size % 16 == 0 && ks[1] * item <= far && vs[1] * item <= far;
+  const bool even = cache->page_size % 16 == 0 && ks[1] * item <= far && vs[1] * item <= far;
   const PagedArgs p{static_cast<const char*>(cache->keys), static_cast<const char*>(cache->values), ks[0] * item,
                     ks[1] * item, ks[2] * item, vs[0] * item, vs[1] * item, vs[2] * item, cache->page_table,
                     cache->table_stride, cache->lengths, cache->counts, (int)cache->pages, (int)cache->page_size,
