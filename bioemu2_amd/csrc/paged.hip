@@ -85,37 +85,63 @@ __device__ __forceinline__ int tiles_of(const PagedArgs& p, int b) {
   return (length_of(p, b) + KEYS - 1) / KEYS;
 }
 
-__device__ __forceinline__ int64_t uniform(int64_t x) {
-  return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
-         (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
+// Inclusive sums over the wave's lanes.
+__device__ __forceinline__ int scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // from 1, 2, 4, 8 lanes before, in rows of 16
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // the last lane of the row before
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // of the first two rows
+  return x;
 }
 
-// The deal of the tiles: how many there are, before sequence `upto` and in all, and among how many workgroups: as many as
-// there are, with at least `least` tiles each, but for items of fewer (an item's start costs some tiles' time).  Every
-// wave by itself.
-struct Deal {
-  int64_t before, total, groups;
+// A workgroup's share of the tiles of all items (their number is below 2^31): `left` of them, the first being tile t0 of
+// item `item` of sequence b.  Every wave by itself.  Two ways of dealing them:
+// long walks: all tiles, one item behind the other, in equal shares, whatever the sequences' lengths;
+// short ones: every item in equal parts of its own, at most `part` tiles, so that no share has two items' ends: what an
+// item's start and end cost, some kItemCost tiles' time, is then more than what the shares are longer.
+struct Share {
+  int b, item, t0, left;
 };
+constexpr int kItemCost = 16;
 template <int KEYS>
-__device__ __forceinline__ Deal deal(const PagedArgs& p, int B, int upto, int items) {
-  const int lane = threadIdx.x & 63;
-  int64_t before = 0, total = 0;
-  int live = 0;
-  for (int b = lane; b < B; b += 64) {
-    const int tiles = tiles_of<KEYS>(p, b);
-    total += tiles;
-    before += b < upto ? tiles : 0;
-    live += tiles > 0;
+__device__ __forceinline__ Share share_of(const PagedArgs& p, int B, int items) {
+  const int lane = threadIdx.x & 63, groups = p.groups, w = blockIdx.x;
+  int total = 0, live = 0, sums = 0, own = 0;
+  for (int b0 = 0; b0 < B; b0 += 64) {
+    own = b0 + lane < B ? tiles_of<KEYS>(p, b0 + lane) : 0;
+    sums = scan(own);
+    total += __builtin_amdgcn_readlane(sums, 63);
+    live += __popcll(__ballot(own > 0));
   }
-#pragma unroll
-  for (int m = 32; m > 0; m /= 2) {
-    total += __shfl_xor(total, m);
-    before += __shfl_xor(before, m);
-    live += __shfl_xor(live, m);
+  total *= items;
+  live *= items;
+  const Share none{0, 0, 0, 0};
+  const unsigned spare = max(groups - live, 1), part = max(((unsigned)total + spare - 1) / spare, (unsigned)p.least);
+  const unsigned each = (unsigned)total / (unsigned)groups;
+  const bool parts = live < groups && part < each + kItemCost;
+  // where the share starts, in tiles, or the number of the part
+  const int more = total - (int)each * groups, at = parts ? w : w * (int)each + min(w, more);
+  int before = 0, b = 0;
+  for (;; b += 64) {
+    if (B > 64) own = b + lane < B ? tiles_of<KEYS>(p, b + lane) : 0;
+    int mine = own;
+    if (parts) mine = ((unsigned)own + part - 1) / part;
+    if (B > 64 || parts) sums = scan(mine);
+    const uint64_t past = __ballot(before + sums * items > at);
+    if (past) {
+      const int l = __ffsll((unsigned long long)past) - 1;
+      b += l;
+      before += __builtin_amdgcn_readlane(sums - mine, l) * items;
+      const unsigned in = at - before, n = __builtin_amdgcn_readlane(mine, l), item = in / n;
+      if (!parts) return {b, (int)item, (int)(in - item * n), (int)each + (w < more)};
+      const unsigned tiles = __builtin_amdgcn_readlane(own, l), i = in - item * n, size = tiles / n, rest = tiles - size * n;
+      return {b, (int)item, (int)(i * size + min(i, rest)), (int)(size + (i < rest))};
+    }
+    before += __builtin_amdgcn_readlane(sums, 63) * items;
+    if (b + 64 >= B) return none;   // more workgroups than parts
   }
-  total = uniform(total) * items;
-  const int64_t want = max((total + p.least - 1) / p.least, (int64_t)__builtin_amdgcn_readfirstlane(live) * items);
-  return {uniform(before) * items, total, min((int64_t)p.groups, want)};
 }
 
 template <class T, int DP, int RB, int CAP, int W, bool EVEN>
@@ -124,6 +150,12 @@ struct Walk {
   static constexpr int VL = VC * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : VC;   // values a load of V
   static constexpr int KL = sizeof(T) == 2 ? 8 : 4, KS = DP / (4 * KL), KU = KEYS / 16;
   static constexpr int VK = KEYS / 4;   // keys whose values a lane loads
+  // Four lanes' pieces of a key are 64 bytes, half a cache line, and a second load of the line would wait for the first
+  // one's in the cache.  So the lanes of two keys read a line of one key, then that line of the other: of the first load an
+  // even lane has its key's first half and an odd lane the other key's second half, and of the second load the reverse.
+  // The first halves make one product, the second halves another, whose rows (keys) are then swapped in pairs.  (One token
+  // over 773 keys of 16 heads of 64: 11.4 us, 11.9 by halves; 64 over up to 4000, 72 and 73.  In fp32 it gains nothing.)
+  static constexpr bool LINES = sizeof(T) == 2 && KS % 2 == 0;
   static constexpr unsigned kAll = KEYS == 32 ? 0xffffffffu : 0xffffu;
   typedef T kvec __attribute__((ext_vector_type(KL)));
   typedef T vvec __attribute__((ext_vector_type(VL)));
@@ -132,22 +164,30 @@ struct Walk {
   const PagedArgs& p;
   const int lane, m, h;
   const GLOBAL char *kbase, *vbase;
-  // byte offsets of the lane's row among sixteen, and of its pieces of a row (the row's first where it has no more)
-  unsigned krow, vrow, kd[KS], vd[VC / VL];
+  // byte offsets of the lane's rows among sixteen, and of its pieces of a row (the row's first where it has no more)
+  unsigned krow[LINES ? 2 : 1], vrow, kd[LINES ? 2 : 1][LINES ? KS / 2 : KS], vd[VC / VL];
   int64_t kat, kat1, vat, vat1;   // see locate
   kvec kf[KU][KS];
   vvec vf[VK][VC / VL];
 
   __device__ __forceinline__ Walk(const AttnArgs& a_, const PagedArgs& p_)
       : a(a_), p(p_), lane(threadIdx.x & 63), m(lane & 15), h(lane >> 4) {
-    krow = EVEN ? (unsigned)(m * p.kslot) : 0;
     vrow = EVEN ? (unsigned)(4 * h * p.vslot) : 0;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) kd[s] = KL * (4 * s + h) < a.D ? KL * (4 * s + h) * (int)sizeof(T) : 0;
+    for (int e = 0; e < (LINES ? 2 : 1); ++e) {
+      krow[e] = EVEN ? (unsigned)(key_of(e) * p.kslot) : 0;
+#pragma unroll
+      for (int s = 0; s < (LINES ? KS / 2 : KS); ++s) {
+        const int d = KL * (LINES ? 8 * s + 4 * ((m ^ e) & 1) + h : 4 * s + h);
+        kd[e][s] = d < a.D ? d * (int)sizeof(T) : 0;
+      }
+    }
 #pragma unroll
     for (int c = 0; c < VC / VL; ++c) vd[c] = 16 * VL * c + VL * m < a.D ? (16 * VL * c + VL * m) * (int)sizeof(T) : 0;
   }
 
+  // key of the lane's load e, among sixteen
+  __device__ __forceinline__ int key_of(int e) const { return LINES ? (m & ~1) + e : m; }
   __device__ __forceinline__ int page_index(int j) const { return (int)((uint64_t)(unsigned)j * p.div_mul >> p.div_shift); }
   // Page of the lane's key (key lane % KEYS) of tile t; -1: none.
   __device__ __forceinline__ int page_of(const int* table, int t) const {
@@ -176,11 +216,37 @@ struct Walk {
   }
   __device__ __forceinline__ void load_k() {
 #pragma unroll
-    for (int u = 0; u < KU; ++u) {
-      const GLOBAL char* row = EVEN ? kbase + (u == 0 ? kat : kat1) : kbase + __shfl(kat, 16 * u + m);
+    for (int u = 0; u < KU; ++u)
 #pragma unroll
-      for (int s = 0; s < KS; ++s) kf[u][s] = *(const GLOBAL kvec*)(row + (krow + kd[s]));
+      for (int e = 0; e < (LINES ? 2 : 1); ++e) {
+        const GLOBAL char* row = EVEN ? kbase + (u == 0 ? kat : kat1) : kbase + __shfl(kat, 16 * u + key_of(e));
+#pragma unroll
+        for (int s = 0; s < (LINES ? KS / 2 : KS); ++s)
+          kf[u][LINES ? 2 * s + e : s] = *(const GLOBAL kvec*)(row + (krow[e] + kd[e][s]));
+      }
+  }
+  // s = K Q^T of rows q, sixteen keys u
+  __device__ __forceinline__ f32x4 product(const kvec (&qf)[KS], int u) const {
+    f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int st = 0; st < KS; ++st) {
+      kvec k = kf[u][st];
+      if constexpr (LINES) {
+        const u32x4 own = __builtin_bit_cast(u32x4, k), other = __builtin_bit_cast(u32x4, kf[u][st ^ 1]);
+        u32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = m & 1 ? other[e] : own[e];
+        k = __builtin_bit_cast(kvec, w);
+      }
+      if constexpr (sizeof(T) == 2) {
+        s[st & 1] = mfma_16x16(k, qf[st], s[st & 1]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < KL; ++e) s[st & 1] = mfma_16x16(k[e], qf[st][e], s[st & 1]);
+      }
     }
+    if constexpr (KS > 1) s[0] += LINES ? f32x4{s[1][1], s[1][0], s[1][3], s[1][2]} : s[1];
+    return s[0];
   }
   __device__ __forceinline__ void load_v() {
 #pragma unroll
@@ -246,9 +312,9 @@ struct Walk {
   // Tiles [t0, t1) of head hk of sequence b, rows from row0 on; to the output or to part `slot`.
   __device__ __forceinline__ void run(int b, int hk, int row0, int t0, int t1, T* out, Parts parts, int64_t slot,
                                       char* lds) {
-    const int wave = wave_id(), length = length_of(p, b);
+    const int wave = wave_id(), length = __builtin_amdgcn_readfirstlane(length_of(p, b));
     const int rows = a.Nq * a.G, n_rows = min(rows - row0, 16 * RB);
-    const int count = p.counts ? min(max(p.counts[b], 0), a.Nq) : a.Nq;
+    const int count = __builtin_amdgcn_readfirstlane(p.counts ? min(max(p.counts[b], 0), a.Nq) : a.Nq);
     const int first = length - count;   // position of the first query
     const int* table = p.page_table + b * p.table_stride;
     kbase = (const GLOBAL char*)p.keys + hk * p.khead;
@@ -276,6 +342,10 @@ struct Walk {
     // keys, values and the page after next are requested as soon as there is room; behind the last tile it once more (a
     // load that may not be made would have to be waited for at once)
     const auto after = [&](int t) { return t + W < t1 ? t + W : t; };
+#pragma unroll
+    for (int u = 0; u < KU; ++u)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) kf[u][s] = kvec{};   // without a tile: else the last item's are kept for this
     if (t < t1) {
       there = locate(t, page, length);
       load_k();
@@ -285,13 +355,17 @@ struct Walk {
     float* bias = reinterpret_cast<float*>(lds);                         // [buckets][16 RB]
     uint8_t* buckets = reinterpret_cast<uint8_t*>(bias + 256 * 16 * RB);   // [2 radius + 1]
     if (a.table) {
-      for (int e = threadIdx.x; e < a.nb * 16 * RB; e += 64 * W) {
+      int self = threadIdx.x;
+      asm volatile("" : "+v"(self));
+#pragma unroll 1
+      for (int e = self; e < a.nb * 16 * RB; e += 64 * W) {
         const int r = row0 + e % (16 * RB), head = hk * a.G + (r < rows ? r % a.G : 0);
         const int64_t at = (int64_t)(e / (16 * RB)) * a.H + head;
         bias[e] = bias_log2(a.table_bf16 ? (float)static_cast<const bf16*>(a.table)[at]
                                          : static_cast<const float*>(a.table)[at]);
       }
-      for (int e = threadIdx.x; e <= 2 * a.radius; e += 64 * W) buckets[e] = (uint8_t)min((int)a.buckets[e], a.nb - 1);
+#pragma unroll 1
+      for (int e = self; e <= 2 * a.radius; e += 64 * W) buckets[e] = (uint8_t)min((int)a.buckets[e], a.nb - 1);
       __syncthreads();
     }
 
@@ -320,27 +394,12 @@ struct Walk {
         for (int u = 0; u < KU; ++u)
 #pragma unroll
           for (int st = 0; st < KS; ++st)
-            if (KL * (4 * st + h) >= a.D) kf[u][st] = kvec{};
+            if (KL * (LINES ? 8 * (st / 2) + 4 * ((m ^ st) & 1) + h : 4 * st + h) >= a.D) kf[u][st] = kvec{};
       f32x4 s[RB][KU];
-#pragma unroll
-      for (int q = 0; q < RB; ++q)
-#pragma unroll
-        for (int u = 0; u < KU; ++u) s[q][u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int u = 0; u < KU; ++u)
 #pragma unroll
-        for (int st = 0; st < KS; ++st) {
-          const kvec k = kf[u][st];
-#pragma unroll
-          for (int q = 0; q < RB; ++q) {
-            if constexpr (sizeof(T) == 2) {
-              s[q][u] = mfma_16x16(k, qf[q][st], s[q][u]);
-            } else {
-#pragma unroll
-              for (int e = 0; e < KL; ++e) s[q][u] = mfma_16x16(k[e], qf[q][st][e], s[q][u]);
-            }
-          }
-        }
+        for (int q = 0; q < RB; ++q) s[q][u] = product(qf[q], u);
       __builtin_amdgcn_sched_barrier(0);   // K's registers are free
       there = locate(next, page, length);
       load_k();
@@ -429,10 +488,13 @@ struct Walk {
       t = next;
     }
 
-    // the waves' parts through LDS
+    // the waves' parts through LDS.  What follows from the thread's number is worked out here, not kept since the start.
     if (a.table) __syncthreads();
-    float* sh = reinterpret_cast<float*>(lds);              // [waves][16 RB][DP]
-    float* ml = sh + W * 16 * RB * DP;                      // [waves][16 RB][2]
+    int self = threadIdx.x;
+    asm volatile("" : "+v"(self));
+    const int lane = self & 63, m = lane & 15, h = lane >> 4;
+    float* sh = reinterpret_cast<float*>(lds);                   // [waves][16 RB][DP]
+    float* ml = sh + W * 16 * RB * DP;                           // [waves][16 RB][2]
     int* flags = reinterpret_cast<int*>(ml + W * 16 * RB * 2);   // [waves]
     if (lane == 0) flags[wave] = taken;
 #pragma unroll
@@ -450,39 +512,51 @@ struct Walk {
         for (int c = 0; c < VC; ++c) sh[at * DP + 16 * VL * (c / VL) + VL * (4 * h + r) + c % VL] = acc[q][c][r];
     }
     __syncthreads();
-    for (int k = threadIdx.x; k < n_rows * DP; k += 64 * W) {
-      const int r = k / DP, d = k - r * DP;
+    typedef T quad __attribute__((ext_vector_type(4)));
+#pragma unroll 1
+    for (int k = self; k < n_rows * (DP / 4); k += 64 * W) {
+      const int r = k / (DP / 4), d = (k - r * (DP / 4)) * 4;
       if (d >= a.D) continue;
+      f32x2 mls[W];
       float most = -kInf;
 #pragma unroll
-      for (int w = 0; w < W; ++w) most = fmaxf(most, ml[2 * (w * 16 * RB + r)]);
+      for (int w = 0; w < W; ++w) {
+        mls[w] = *reinterpret_cast<const f32x2*>(ml + 2 * (w * 16 * RB + r));
+        most = fmaxf(most, mls[w][0]);
+      }
       const float to = most == -kInf ? 0.f : most;
-      float o = 0.f, sum = 0.f;
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+      float sum = 0.f;
       int any = 0;
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        const int at = w * 16 * RB + r;
-        const float f = fast_exp2(ml[2 * at] - to);
-        o += f * sh[at * DP + d];
-        sum += f * ml[2 * at + 1];
+        const float f = fast_exp2(mls[w][0] - to);
+        o += f * *reinterpret_cast<const f32x4*>(sh + (w * 16 * RB + r) * DP + d);
+        sum += f * mls[w][1];
         any |= flags[w];
       }
       const int i = (row0 + r) / a.G, g = row0 + r - i * a.G;
-      if (i >= count) o = sum = 0.f;   // padding
+      if (i >= count) o = f32x4{0.f, 0.f, 0.f, 0.f}, sum = 0.f;   // padding
       if (any) {   // its size does not matter: whatever a seen one weighs, so is the result
         const int seen = i < count ? min(first + i + 1, min(length, t1 * KEYS)) : 0;
+#pragma unroll 1
         for (int j = max(max(first + 1, 0) / KEYS, t0) * KEYS; j < seen; ++j) {   // from the first such tile
           const int at = page_index(j), page = table[at];
           if (page < 0 || page >= p.pages) continue;
-          const T v = ((const GLOBAL T*)(vbase + page * p.vpage + (j - at * p.page_size) * p.vslot))[d];
-          if (not_finite(v)) o += (float)v;
+          const GLOBAL T* v = (const GLOBAL T*)(vbase + page * p.vpage + (j - at * p.page_size) * p.vslot) + d;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (not_finite(v[e])) o[e] += (float)v[e];
         }
       }
       if (slot < 0) {
-        out[(((int64_t)b * a.Nq + i) * a.H + hk * a.G + g) * a.D + d] = (T)over_sum(o, sum);
+        quad v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (T)over_sum(o[e], sum);
+        *reinterpret_cast<quad*>(out + (((int64_t)b * a.Nq + i) * a.H + hk * a.G + g) * a.D + d) = v;
       } else {
         const int64_t at = slot * min(rows, 16 * RB) + r;
-        parts.o[at * a.D + d] = o;
+        *reinterpret_cast<f32x4*>(parts.o + at * a.D + d) = o;
         if (d == 0) {
           parts.ml[2 * at] = i >= count || sum == 0.f ? -kInf : to;
           parts.ml[2 * at + 1] = sum;
@@ -508,18 +582,13 @@ __global__ __launch_bounds__(64 * W, 2) void paged_kernel(const AttnArgs a, cons
                                                           Parts parts) {
   constexpr int KEYS = Cache<T>::KEYS;
   __shared__ __attribute__((aligned(16))) char lds[lds_bytes<DP, RB, W>()];
-  Walk<T, DP, RB, CAP, W, EVEN> walk(a, p);
   const int items = a.Hk * p.blocks;   // of a sequence
-  int b = 0, tiles;
-  int64_t at, end, before = 0;   // the tiles to take, and those of the sequences before b
+  Share s;
   if (p.groups == 0) {
-    b = blockIdx.x / items;
-    tiles = tiles_of<KEYS>(p, b);
-    at = (int64_t)(blockIdx.x - b * items) * tiles;
-    end = at + tiles;
+    const int b = blockIdx.x / items, item = blockIdx.x - b * items, tiles = tiles_of<KEYS>(p, b);
+    s = {b, item, 0, tiles};
     if (tiles == 0) {
-      const int item = blockIdx.x - b * items, hk = item / p.blocks, row0 = item % p.blocks * 16 * RB;
-      const int n = min(a.Nq * a.G - row0, 16 * RB);
+      const int hk = item / p.blocks, row0 = item % p.blocks * 16 * RB, n = min(a.Nq * a.G - row0, 16 * RB);
       for (int k = threadIdx.x; k < n * a.D; k += 64 * W) {
         const int r = row0 + k / a.D, i = r / a.G;
         out[(((int64_t)b * a.Nq + i) * a.H + hk * a.G + r - i * a.G) * a.D + k % a.D] = (T)0.f;
@@ -527,48 +596,25 @@ __global__ __launch_bounds__(64 * W, 2) void paged_kernel(const AttnArgs a, cons
       return;
     }
   } else {
-    const Deal all = deal<KEYS>(p, a.B, 0, items);
-    if ((int64_t)blockIdx.x >= all.groups) return;
-    at = all.total * blockIdx.x / all.groups;
-    end = all.total * (blockIdx.x + 1) / all.groups;
-    // the sequence that holds tile `at`
-    for (const int lane = threadIdx.x & 63;; b += 64) {
-      const int64_t own = b + lane < a.B ? (int64_t)tiles_of<KEYS>(p, b + lane) * items : 0;
-      int64_t sum = own;
-#pragma unroll
-      for (int m = 1; m < 64; m *= 2) {
-        const int64_t o = __shfl_up(sum, m);
-        if (lane >= m) sum += o;
-      }
-      const uint64_t past = __ballot(before + sum > at);
-      if (past) {
-        const int l = __ffsll((unsigned long long)past) - 1;
-        b += l;
-        before = uniform(before + __shfl(sum - own, l));
-        break;
-      }
-      before = uniform(before + __shfl(sum, 63));
-      if (b + 64 >= a.B) return;
-    }
-    tiles = tiles_of<KEYS>(p, b);
+    s = share_of<KEYS>(p, a.B, items);
   }
-  while (at < end) {
-    if (at - before >= (int64_t)tiles * items) {
-      before += (int64_t)tiles * items;
-      if (++b >= a.B) return;
-      tiles = tiles_of<KEYS>(p, b);
+  while (s.left > 0) {
+    const int tiles = __builtin_amdgcn_readfirstlane(tiles_of<KEYS>(p, s.b));
+    if (s.item == items || tiles == 0) {
+      s.item = 0;
+      if (++s.b >= a.B) return;
       continue;
     }
-    const int item = (int)((at - before) / tiles), t0 = (int)((at - before) - (int64_t)item * tiles);
-    const int t1 = (int)min((int64_t)tiles, t0 + (end - at));
-    const int64_t slot = t0 == 0 && t1 == tiles ? -1 : (int64_t)blockIdx.x + (int64_t)b * items + item;
+    const int t1 = min(tiles, s.t0 + s.left);
+    const int64_t item = (int64_t)s.b * items + s.item, slot = s.t0 == 0 && t1 == tiles ? -1 : blockIdx.x + item;
     if (p.groups && threadIdx.x == 0) {
-      int* range = parts.range + 2 * ((int64_t)b * items + item);
-      if (t0 == 0) range[0] = blockIdx.x;
-      if (t1 == tiles) range[1] = blockIdx.x;
+      if (s.t0 == 0) parts.range[2 * item] = blockIdx.x;
+      if (t1 == tiles) parts.range[2 * item + 1] = blockIdx.x;
     }
-    walk.run(b, item / p.blocks, item % p.blocks * 16 * RB, t0, t1, out, parts, slot, lds);
-    at += t1 - t0;
+    Walk<T, DP, RB, CAP, W, EVEN>(a, p).run(s.b, s.item / p.blocks, s.item % p.blocks * 16 * RB, s.t0, t1, out, parts, slot, lds);
+    s.left -= t1 - s.t0;
+    s.t0 = 0;
+    ++s.item;
   }
 }
 
@@ -678,12 +724,14 @@ Plan plan(const AttnArgs& a, const bioemu_paged_cache& c, bool f32) {
   p.blocks = (rows + 16 * p.rb - 1) / (16 * p.rb);
   p.items = (int64_t)a.B * a.Hk * p.blocks;
   const int64_t most = c.pages > 0 ? c.table_width * c.page_size : 0;
-  if (most <= 1024 || p.items >= 16 * attn_units()) {
+  // what a walk of one workgroup takes less than the join: 1024 keys of 64 values in bf16
+  if (most * std::max(a.D, 64) * (f32 ? 4 : 2) <= 1024 * 64 * 2 || p.items >= 16 * attn_units()) {
     p.waves = p.items <= 2 * attn_units() && (f32 || a.cap <= kFastCap) ? 8 : 4;
     return p;
   }
+  // two a CU: with three or four, where registers allow them, 64 sequences of 4096 keys took 206 us, with these 184
   p.groups = 2 * attn_units();
-  p.least = 2 * p.waves;
+  p.least = p.waves;
   p.slots = p.groups + p.items;
   return p;
 }
@@ -699,8 +747,10 @@ int paged_args(const bioemu_paged_cache* c, const bioemu_attention_args* in, Att
     return set_error(BIOEMU_ERR_INVALID_ARG, "paged_attention: keys, lengths and masks come from the cache");
   if (const int rc = paged_cache_args("paged_attention", c, a->B, a->Hk, in->f32 != 0)) return rc;
   *pl = plan(*a, *c, in->f32 != 0);
-  if (pl->items >= (int64_t(1) << 30) || (int64_t)a->B * a->Nq * a->H >= (int64_t(1) << 31))
-    return set_error(BIOEMU_ERR_UNSUPPORTED, "paged_attention: B=%d, Nq=%d, H=%d are too many", a->B, a->Nq, a->H);
+  const int64_t tiles = (c->table_width * c->page_size + 15) / 16;
+  if (pl->items * std::max(tiles, (int64_t)1) >= (int64_t(1) << 31) || (int64_t)a->B * a->Nq * a->H >= (int64_t(1) << 31))
+    return set_error(BIOEMU_ERR_UNSUPPORTED, "paged_attention: B=%d, Nq=%d, H=%d over %ld keys are too many", a->B,
+                     a->Nq, a->H, (long)(c->table_width * c->page_size));
   return BIOEMU_OK;
 }
 
