@@ -8,6 +8,8 @@
 // A workgroup takes a few tokens.  Its threads first request the values that they will turn, then compute cos and sin of
 // every (token, pair) once, into LDS, and every head of the token reads them there.  Appending is the same with k's rows
 // going to their slots and v's copied beside them.
+#include <algorithm>
+
 #include "common.h"
 #include "internal.h"
 
@@ -15,8 +17,23 @@ namespace bioemu {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnits = 4;          // pieces a thread holds at once
+// pieces a thread holds at once; in the half layout a piece is of both halves
+template <bool INTERLEAVED>
+constexpr int kUnits = INTERLEAVED ? 8 : 4;
 constexpr int kMaxWidth = 512;
+
+// n / d for n below 2^31: n mul >> shift, mul = 2^(31 + l) / d rounded up, l = log2 of d rounded up.
+struct Divisor {
+  uint32_t mul = 0, shift = 0;
+  Divisor() = default;
+  explicit Divisor(int64_t d) {
+    uint32_t l = 0;
+    while ((int64_t(1) << l) < d) ++l;
+    mul = (uint32_t)(((uint64_t(1) << (31 + l)) + d - 1) / d);
+    shift = 31 + l;
+  }
+  __device__ __forceinline__ int operator()(int n) const { return (int)((uint64_t)(uint32_t)n * mul >> shift); }
+};
 
 struct RotaryArgs {
   const void *q, *k, *v;
@@ -30,6 +47,8 @@ struct RotaryArgs {
   float magnitude;
   int N, H, Hk, D, pairs, tokens, per, interleaved, inverse;
   int pages, page_size, table_width;
+  int heads, pieces;                    // rows of a token, pieces of a row
+  Divisor by_n, by_heads, by_pieces, by_pairs;
 };
 
 // cos and sin of `position` times `frequency` radians.
@@ -51,7 +70,8 @@ struct Token {
 };
 
 // V values at a time; a piece is V values, or in the half layout V values of each half.  APPEND: with v and a cache.
-template <class T, int V, bool INTERLEAVED, bool APPEND>
+// STREAM: results go past the caches.
+template <class T, int V, bool INTERLEAVED, bool APPEND, bool STREAM>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
   typedef T vec __attribute__((ext_vector_type(V)));
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -59,20 +79,20 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
   f32x2* turn = reinterpret_cast<f32x2*>(lds + a.per * sizeof(Token));   // [per][pairs]
 
   const int t0 = blockIdx.x * a.per, n = min(a.per, a.tokens - t0);
-  const int turned = INTERLEAVED ? 2 * a.pairs / V : a.pairs / V;   // pieces of a head that turn
-  const int plain = (a.D - 2 * a.pairs) / V, pieces = turned + plain;
-  const int heads = (a.q ? a.H : 0) + (a.k ? (APPEND ? 2 : 1) * a.Hk : 0), units = n * heads * pieces;
+  const int turned = INTERLEAVED ? 2 * a.pairs / V : a.pairs / V;   // pieces of a row that turn
+  const int q_heads = a.q ? a.H : 0, units = n * a.heads * a.pieces;
+  constexpr int U = kUnits<INTERLEAVED>;
 
-  for (int u0 = 0; u0 == 0 || u0 < units; u0 += kThreads * kUnits) {
-    vec x[kUnits], y[kUnits];
+  for (int u0 = 0; u0 == 0 || u0 < units; u0 += kThreads * U) {
+    vec x[U], y[U];
 #pragma unroll
-    for (int e = 0; e < kUnits; ++e) {
+    for (int e = 0; e < U; ++e) {
       const int u = u0 + e * kThreads + threadIdx.x;
       x[e] = y[e] = vec{};
       if (u >= units) continue;
-      const int row = u / pieces, p = u - row * pieces, t = row / heads, head = row - t * heads;
-      const int b = (t0 + t) / a.N, i = t0 + t - b * a.N;
-      const int hk = head - (a.q ? a.H : 0);
+      const int row = a.by_pieces(u), p = u - row * a.pieces, t = a.by_heads(row), head = row - t * a.heads;
+      const int b = a.by_n(t0 + t), i = t0 + t - b * a.N, hk = head - q_heads;
+      if (APPEND && a.counts && i >= a.counts[b]) continue;   // padding: nothing to read
       const T* src;
       if (hk < 0)
         src = static_cast<const T*>(a.q) + b * a.q_st[0] + i * a.q_st[1] + head * a.q_st[2];
@@ -89,7 +109,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
     }
     if (u0 == 0) {
       if (APPEND && threadIdx.x < n) {
-        const int b = (t0 + threadIdx.x) / a.N, i = t0 + threadIdx.x - b * a.N;
+        const int b = a.by_n(t0 + threadIdx.x), i = t0 + threadIdx.x - b * a.N;
         const int count = a.counts ? min(max(a.counts[b], 0), a.N) : a.N;
         // 64 bits: lengths may hold anything
         const int64_t at = (int64_t)a.lengths[b] - count + i;
@@ -105,7 +125,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
         tok[threadIdx.x] = to;
       }
       for (int k = threadIdx.x; k < n * a.pairs; k += kThreads) {
-        const int t = k / a.pairs, b = (t0 + t) / a.N, i = t0 + t - b * a.N;
+        const int t = a.by_pairs(k), b = a.by_n(t0 + t), i = t0 + t - b * a.N;
         int position = i;
         if (a.positions)
           position = a.positions[t0 + t];
@@ -116,11 +136,11 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
       __syncthreads();
     }
 #pragma unroll
-    for (int e = 0; e < kUnits; ++e) {
+    for (int e = 0; e < U; ++e) {
       const int u = u0 + e * kThreads + threadIdx.x;
       if (u >= units) continue;
-      const int row = u / pieces, p = u - row * pieces, t = row / heads, head = row - t * heads;
-      const int hk = head - (a.q ? a.H : 0);
+      const int row = a.by_pieces(u), p = u - row * a.pieces, t = a.by_heads(row), head = row - t * a.heads;
+      const int hk = head - q_heads;
       const bool value = APPEND && hk >= a.Hk;
       const f32x2* cs = turn + t * a.pairs;
       vec r = x[e], w = y[e];
@@ -155,11 +175,14 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
       } else {
         dst = static_cast<T*>(a.k_out) + ((int64_t)(t0 + t) * a.Hk + hk) * a.D;
       }
-      if constexpr (INTERLEAVED) {
-        *reinterpret_cast<vec*>(dst + p * V) = r;
+      vec* to = reinterpret_cast<vec*>(dst + (INTERLEAVED || p < turned ? p * V : a.pairs + p * V));
+      vec* too = reinterpret_cast<vec*>(dst + a.pairs + p * V);
+      if constexpr (STREAM) {
+        __builtin_nontemporal_store(r, to);
+        if (!INTERLEAVED && p < turned) __builtin_nontemporal_store(w, too);
       } else {
-        *reinterpret_cast<vec*>(dst + (p < turned ? p * V : a.pairs + p * V)) = r;
-        if (p < turned) *reinterpret_cast<vec*>(dst + a.pairs + p * V) = w;
+        *to = r;
+        if (!INTERLEAVED && p < turned) *too = w;
       }
     }
   }
@@ -173,15 +196,24 @@ int piece(const RotaryArgs& a, bool f32) {
   return v;
 }
 
-template <class T, int V, bool APPEND>
+template <class T, int V, bool APPEND, bool STREAM>
 void launch(const RotaryArgs& a, hipStream_t stream) {
   const dim3 grid((unsigned)((a.tokens + a.per - 1) / a.per));
   const size_t lds = a.per * (sizeof(Token) + a.pairs * sizeof(f32x2));
   if (a.interleaved) {
-    if constexpr (V > 1) rotary_kernel<T, V, true, APPEND><<<grid, kThreads, lds, stream>>>(a);
+    if constexpr (V > 1) rotary_kernel<T, V, true, APPEND, STREAM><<<grid, kThreads, lds, stream>>>(a);
   } else {
-    rotary_kernel<T, V, false, APPEND><<<grid, kThreads, lds, stream>>>(a);
+    rotary_kernel<T, V, false, APPEND, STREAM><<<grid, kThreads, lds, stream>>>(a);
   }
+}
+template <class T, int V, bool APPEND>
+void launch(const RotaryArgs& a, hipStream_t stream) {
+  // Results that no cache near the CUs holds (they have 4 MB a XCD) pass them by, so as not to drive out what is being
+  // read: 16384 tokens of 16/4 heads of 128 in bf16 27 us (6.1 TB/s), 39 the other way.
+  if ((int64_t)a.tokens * a.heads * a.D * (int64_t)sizeof(T) >= 32 << 20)
+    launch<T, V, APPEND, true>(a, stream);
+  else
+    launch<T, V, APPEND, false>(a, stream);
 }
 
 template <bool APPEND>
@@ -192,6 +224,12 @@ int run(const char* what, RotaryArgs& a, bool f32, hipStream_t stream) {
   while (a.per > 1 && a.tokens / a.per < 1024) a.per /= 2;
   KernelTimerScope timer(what, stream);
   const int v = piece(a, f32);
+  a.heads = (a.q ? a.H : 0) + (a.k ? (APPEND ? 2 : 1) * a.Hk : 0);
+  a.pieces = (a.interleaved ? a.D : a.D - a.pairs) / v;
+  a.by_n = Divisor(a.N);
+  a.by_heads = Divisor(a.heads);
+  a.by_pieces = Divisor(a.pieces);
+  a.by_pairs = Divisor(std::max(a.pairs, 1));
   if (f32) {
     if (v == 4) launch<float, 4, APPEND>(a, stream);
     else if (v == 2) launch<float, 2, APPEND>(a, stream);

@@ -580,7 +580,7 @@ std::tuple<Tensor, Tensor> rotary_cuda(ROTARY_PARAMS) {
   const optional<Tensor> pos = whole_numbers(positions, "rotary positions", bn, like);
   const Tensor f = frequencies_of(frequencies, "rotary", like);
   bioemu_rotary_args args{};
-  Tensor qs, ks, qo = none_like(like), ko = none_like(like);
+  Tensor qs, ks, qo, ko;
   if (q) {
     qs = rows16(*q);
     qo = at::empty(q->sizes(), q->options());
@@ -605,8 +605,8 @@ std::tuple<Tensor, Tensor> rotary_cuda(ROTARY_PARAMS) {
   args.interleaved = interleaved;
   args.inverse = inverse;
   args.f32 = is_f32(like);
-  check_rc(bioemu_rotary(&args, qo.data_ptr(), ko.data_ptr(), stream_of(like)), "bioemu_rotary");
-  return {qo, ko};
+  check_rc(bioemu_rotary(&args, ptr(qo), ptr(ko), stream_of(like)), "bioemu_rotary");
+  return {q ? qo : none_like(like), k ? ko : none_like(like)};
 }
 
 std::tuple<Tensor, Tensor> rotary_meta(ROTARY_PARAMS) {
@@ -744,7 +744,7 @@ Tensor paged_append_cuda(APPEND_PARAMS) {
   const CacheCall c("paged_append", keys, values, page_table, lengths, counts, k, k.size(2));
   const int64_t bn[2] = {k.size(0), k.size(1)};
   const optional<Tensor> pos = whole_numbers(positions, "paged_append positions", bn, k);
-  Tensor f, qs, out = none_like(k);
+  Tensor f, qs, out;
   if (frequencies) f = frequencies_of(*frequencies, "paged_append", k);
   const Tensor ks = rows16(k), vs = rows16(v);
   bioemu_rotary_args args{};
@@ -768,9 +768,8 @@ Tensor paged_append_cuda(APPEND_PARAMS) {
   args.interleaved = interleaved;
   args.f32 = is_f32(k);
   const int64_t vst[3] = {vs.stride(0), vs.stride(1), vs.stride(2)};
-  check_rc(bioemu_paged_append(&c.args, &args, vs.data_ptr(), vst, q ? out.data_ptr() : nullptr, stream_of(k)),
-           "bioemu_paged_append");
-  return out;
+  check_rc(bioemu_paged_append(&c.args, &args, vs.data_ptr(), vst, ptr(out), stream_of(k)), "bioemu_paged_append");
+  return q ? out : none_like(k);
 }
 Tensor paged_append_meta(APPEND_PARAMS) {
   return q ? at::empty_symint(q->sym_sizes(), q->options()) : none_like(k);
