@@ -222,7 +222,7 @@ struct Walk {
         const GLOBAL char* row = EVEN ? kbase + (u == 0 ? kat : kat1) : kbase + __shfl(kat, 16 * u + key_of(e));
 #pragma unroll
         for (int s = 0; s < (LINES ? KS / 2 : KS); ++s)
-          kf[u][LINES ? 2 * s + e : s] = *(const GLOBAL kvec*)(row + (krow[e] + kd[e][s]));
+          kf[u][LINES ? 2 * s + e : s] = __builtin_nontemporal_load((const GLOBAL kvec*)(row + (krow[e] + kd[e][s])));
       }
   }
   // s = K Q^T of rows q, sixteen keys u
@@ -254,7 +254,7 @@ struct Walk {
       const GLOBAL char* row =
           EVEN ? vbase + (t < 4 ? vat : vat1) + (t & 3) * p.vslot : vbase + __shfl(vat, 16 * (t >> 2) + 4 * h + (t & 3));
 #pragma unroll
-      for (int c = 0; c < VC / VL; ++c) vf[t][c] = *(const GLOBAL vvec*)(row + (vrow + vd[c]));
+      for (int c = 0; c < VC / VL; ++c) vf[t][c] = __builtin_nontemporal_load((const GLOBAL vvec*)(row + (vrow + vd[c])));
     }
   }
   // acc += V^T times the tile's weights
