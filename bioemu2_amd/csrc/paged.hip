@@ -359,15 +359,15 @@ struct Walk {
       page = page_of(table, after(t));
     }
     // the bias by bucket and row, and the buckets by distance, where the waves' parts go later
-    float* bias = reinterpret_cast<float*>(lds);                         // [buckets][16 RB]
+    float* bias = reinterpret_cast<float*>(lds);                         // [buckets][n_rows]
     uint8_t* buckets = reinterpret_cast<uint8_t*>(bias + 256 * 16 * RB);   // [2 radius + 1]
     if (a.table) {
       int self = threadIdx.x;
       asm volatile("" : "+v"(self));
 #pragma unroll 1
-      for (int e = self; e < a.nb * 16 * RB; e += 64 * W) {
-        const int r = row0 + e % (16 * RB), head = hk * a.G + (r < rows ? r % a.G : 0);
-        const int64_t at = (int64_t)(e / (16 * RB)) * a.H + head;
+      for (int e = self; e < a.nb * n_rows; e += 64 * W) {
+        const int bucket = e / n_rows, head = hk * a.G + (row0 + e - bucket * n_rows) % a.G;
+        const int64_t at = (int64_t)bucket * a.H + head;
         bias[e] = bias_log2(a.table_bf16 ? (float)static_cast<const bf16*>(a.table)[at]
                                          : static_cast<const float*>(a.table)[at]);
       }
@@ -440,7 +440,7 @@ struct Walk {
             for (int r = 0; r < 4; ++r) {
               const int rel = far ? rel0 : j0 + 16 * u + 4 * h + r - pos[q];
               const int bucket = buckets[min(max(rel, -a.radius), a.radius) + a.radius];
-              x[q][u][r] += bias[bucket * 16 * RB + 16 * q + m];
+              x[q][u][r] += bias[bucket * n_rows + min(16 * q + m, n_rows - 1)];
             }
       }
 #pragma unroll
@@ -638,10 +638,43 @@ __device__ __forceinline__ RowParts row_parts(const AttnArgs& a, const PagedArgs
   const int hk = h / a.G, r = i * a.G + h - hk * a.G, blk = r / block_rows;
   const int64_t item = ((int64_t)b * a.Hk + hk) * p.blocks + blk;
   const int stride = min(a.Nq * a.G, block_rows);
+  const int first = parts.range[2 * item], last = parts.range[2 * item + 1];   // not set where the sequence is empty
   if (tiles_of<KEYS>(p, b) == 0) return {0, 0, stride};
-  const int first = parts.range[2 * item], last = parts.range[2 * item + 1];
   return {(first + item) * stride + r - blk * block_rows, last - first + 1, stride};
 }
+
+// Parts w, w + step, ... of a row added in order, four at a time and in one pass; N values of each.
+template <int N>
+struct Sum {
+  float top = -kInf, sum = 0.f, o[N] = {};
+  __device__ __forceinline__ void merge(float m, float l, const float (&x)[N]) {
+    const float to = fmaxf(top, m), ref = to == -kInf ? 0.f : to, f = fast_exp2(top - ref), g = fast_exp2(m - ref);
+    top = to;
+    sum = sum * f + l * g;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = o[i] * f + x[i] * g;
+  }
+  template <class Load>
+  __device__ __forceinline__ void add(const Parts& parts, const RowParts& own, int w, int step, const Load& load) {
+    for (; w < own.n; w += 4 * step) {
+      f32x2 ml[4];
+      float x[4][N];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const bool there = w + k * step < own.n;
+        const int64_t at = own.row0 + (int64_t)(there ? w + k * step : w) * own.stride;
+        ml[k] = *reinterpret_cast<const f32x2*>(parts.ml + 2 * at);
+        load(at, x[k]);
+        if (there) continue;
+        ml[k] = f32x2{-kInf, 0.f};
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[k][i] = 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) merge(ml[k][0], ml[k][1], x[k]);
+    }
+  }
+};
 
 // paged_join: few rows of many parts, a workgroup a row: wave w takes parts w, w + waves, ..., then the waves are added in
 // order.  Lane d holds values d and 64 + d.
@@ -649,41 +682,30 @@ constexpr int kJoinWaves = 8;
 template <class T, int KEYS>
 __global__ __launch_bounds__(64 * kJoinWaves) void paged_join_kernel(const AttnArgs a, const PagedArgs p,
                                                                      T* __restrict__ out, Parts parts, int block_rows) {
-  __shared__ float sh[kJoinWaves][3][64];
+  __shared__ float sh[kJoinWaves][2][64], ml[kJoinWaves][2];
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int64_t row = blockIdx.x;   // (b, i, head)
   const RowParts own = row_parts<KEYS>(a, p, parts, row, block_rows);
   if (own.n == 1) return;
-  float top = -kInf;
-  for (int w = lane; w < own.n; w += 64) top = fmaxf(top, parts.ml[2 * (own.row0 + (int64_t)w * own.stride)]);
-#pragma unroll
-  for (int m = 32; m > 0; m /= 2) top = fmaxf(top, __shfl_xor(top, m));
-  const float to = top == -kInf ? 0.f : top;
-  float o[2] = {0.f, 0.f}, sum = 0.f;
+  Sum<2> s;
   const int d0 = min(lane, a.D - 1), d1 = min(lane + 64, a.D - 1);
-#pragma unroll 4
-  for (int w = wave; w < own.n; w += kJoinWaves) {
-    const int64_t at = own.row0 + (int64_t)w * own.stride;
-    const float f = fast_exp2(parts.ml[2 * at] - to);
-    o[0] += f * parts.o[at * a.D + d0];
-    o[1] += f * parts.o[at * a.D + d1];
-    sum += f * parts.ml[2 * at + 1];
+  s.add(parts, own, wave, kJoinWaves, [&](int64_t at, float (&x)[2]) {
+    x[0] = parts.o[at * a.D + d0];
+    x[1] = parts.o[at * a.D + d1];
+  });
+  sh[wave][0][lane] = s.o[0];
+  sh[wave][1][lane] = s.o[1];
+  if (lane == 0) {
+    ml[wave][0] = s.top;
+    ml[wave][1] = s.sum;
   }
-  sh[wave][0][lane] = o[0];
-  sh[wave][1][lane] = o[1];
-  sh[wave][2][lane] = sum;
   __syncthreads();
   if (wave > 0) return;
-  o[0] = o[1] = sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < kJoinWaves; ++w) {
-    o[0] += sh[w][0][lane];
-    o[1] += sh[w][1][lane];
-    sum += sh[w][2][lane];
-  }
+  for (int w = 1; w < kJoinWaves; ++w) s.merge(ml[w][0], ml[w][1], {sh[w][0][lane], sh[w][1][lane]});
 #pragma unroll
   for (int e = 0; e < 2; ++e)
-    if (lane + 64 * e < a.D) out[row * a.D + lane + 64 * e] = (T)over_sum(o[e], sum);
+    if (lane + 64 * e < a.D) out[row * a.D + lane + 64 * e] = (T)over_sum(s.o[e], s.sum);
 }
 
 // paged_join_rows: many rows of few parts, four values of one a thread, in the parts' order.
@@ -695,25 +717,22 @@ __global__ __launch_bounds__(256) void paged_join_rows_kernel(const AttnArgs a, 
   if ((int)row >= rows) return;
   const RowParts own = row_parts<KEYS>(a, p, parts, row, block_rows);
   if (own.n == 1) return;
-  float top = -kInf;
-#pragma unroll 4
-  for (int w = 0; w < own.n; ++w) top = fmaxf(top, parts.ml[2 * (own.row0 + (int64_t)w * own.stride)]);
-  const float to = top == -kInf ? 0.f : top;
-  float o[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-#pragma unroll 4
-  for (int w = 0; w < own.n; ++w) {
-    const int64_t at = own.row0 + (int64_t)w * own.stride;
-    const f32x2 ml = *reinterpret_cast<const f32x2*>(parts.ml + 2 * at);
-    const f32x4 x = *reinterpret_cast<const f32x4*>(parts.o + at * a.D + d);
-    const float f = fast_exp2(ml[0] - to);
-    sum += f * ml[1];
+  Sum<4> s;
+  s.add(parts, own, 0, 1, [&](int64_t at, float (&x)[4]) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(parts.o + at * a.D + d);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) o[c] += f * x[c];
-  }
+    for (int c = 0; c < 4; ++c) x[c] = v[c];
+  });
   quad v;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) v[c] = (T)over_sum(o[c], sum);
+  for (int c = 0; c < 4; ++c) v[c] = (T)over_sum(s.o[c], s.sum);
   *reinterpret_cast<quad*>(out + (int64_t)row * a.D + d) = v;
+}
+
+// Whether sixteen keys are always of one page (and their slots' offsets of 32 bits).
+bool even_pages(const bioemu_paged_cache& c, bool f32) {
+  const int64_t far = (int64_t(1) << 27) / (f32 ? 4 : 2);
+  return c.page_size % 16 == 0 && c.keys_stride[1] <= far && c.values_stride[1] <= far;
 }
 
 struct Plan {
@@ -733,7 +752,9 @@ Plan plan(const AttnArgs& a, const bioemu_paged_cache& c, bool f32) {
   const int64_t most = c.pages > 0 ? c.table_width * c.page_size : 0;
   // what a walk of one workgroup takes less than the join: 1024 keys of 64 values in bf16
   if (most * std::max(a.D, 64) * (f32 ? 4 : 2) <= 1024 * 64 * 2 || p.items >= 16 * attn_units()) {
-    p.waves = p.items <= 2 * attn_units() && p.blocks == 1 && (f32 || a.cap <= kFastCap) ? 8 : 4;
+    // with workgroups to spare eight waves share a walk (sixteen, where registers allow it, start 1.5 us later: 12.9 us for
+    // one token over 773 keys of 16 heads of 64, 11.3 with eight, 17 with four)
+    if (p.blocks == 1 && p.items <= 2 * attn_units() && (f32 || a.cap <= kFastCap)) p.waves = 8;
     return p;
   }
   // two a CU: with three or four, where registers allow them, 64 sequences of 4096 keys took 206 us, with these 184
@@ -836,12 +857,10 @@ extern "C" int bioemu_paged_attention(const bioemu_paged_cache* cache, const bio
   unsigned l = 0;
   while ((int64_t(1) << l) < cache->page_size) ++l;
   const unsigned mul = (unsigned)(((int64_t(1) << (28 + l)) + cache->page_size - 1) / cache->page_size);
-  const int64_t far = int64_t(1) << 27;   // sixteen slots' offsets in 32 bits
-  const bool even = cache->page_size % 16 == 0 && ks[1] * item <= far && vs[1] * item <= far;
   const PagedArgs p{static_cast<const char*>(cache->keys), static_cast<const char*>(cache->values), ks[0] * item,
                     ks[1] * item, ks[2] * item, vs[0] * item, vs[1] * item, vs[2] * item, cache->page_table,
                     cache->table_stride, cache->lengths, cache->counts, (int)cache->pages, (int)cache->page_size,
-                    (int)cache->table_width, pl.blocks, mul, 28 + l, even, pl.groups, pl.least};
+                    (int)cache->table_width, pl.blocks, mul, 28 + l, even_pages(*cache, args->f32 != 0), pl.groups, pl.least};
   const int dp = a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128;
   void* ws = need ? workspace : nullptr;
 #define BIOEMU_PAGED(T, P) \
