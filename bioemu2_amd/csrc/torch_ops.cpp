@@ -5,7 +5,7 @@
 // These run in C++ because a training step's backward pass runs in autograd's own thread: the same glue in Python took
 // 60 to 130 us a step of host time there and back (a step of the smallest sizes computes for 15), and 40 to 70 here.
 // Each op has a form with what its backward pass reads (`*_train`) and a backward op of its own, all reached through the
-// dispatcher, so that tracing, fake tensors and modes see them.  Gradients are first order.
+// dispatcher, so that tracing, fake tensors and modes see them.  Gradients are first order (rotary's, a linear map, of any).
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
@@ -746,10 +746,14 @@ Tensor paged_append_cuda(APPEND_PARAMS) {
   const optional<Tensor> pos = whole_numbers(positions, "paged_append positions", bn, k);
   Tensor f, qs, out;
   if (frequencies) f = frequencies_of(*frequencies, "paged_append", k);
-  const Tensor ks = rows16(k), vs = rows16(v);
+  // rows that lie in the cache itself are read before any of them is written over
+  const auto apart = [&](const Tensor& t) {
+    return t.is_alias_of(keys) || t.is_alias_of(values) ? t.clone(at::MemoryFormat::Contiguous) : rows16(t);
+  };
+  const Tensor ks = apart(k), vs = apart(v);
   bioemu_rotary_args args{};
   if (q) {
-    qs = rows16(*q);
+    qs = apart(*q);
     out = at::empty(q->sizes(), q->options());
     args.q = qs.data_ptr();
     set_strides(args.q_stride, qs);
@@ -777,10 +781,16 @@ Tensor paged_append_meta(APPEND_PARAMS) {
 Tensor paged_append_autograd(APPEND_PARAMS) {
   check_no_tangents("paged_append", keys, values, k, v, q);
   check_no_gradients("paged_append", keys, values, k, v, q);
+  at::AutoDispatchBelowAutograd below;
+  static auto op = handle<decltype(paged_append_cuda)>("bioemu_mi355x::paged_append");
+  return op.call(APPEND_ARGS);
+}
+// Whoever saved the cache for a backward pass is told that it has changed.
+Tensor paged_append_in_place(APPEND_PARAMS) {
   at::AutoDispatchBelowADInplaceOrView below;
   static auto op = handle<decltype(paged_append_cuda)>("bioemu_mi355x::paged_append");
   const Tensor out = op.call(APPEND_ARGS);
-  for (const Tensor* t : {&keys, &values})   // whoever saved them for a backward pass is told
+  for (const Tensor* t : {&keys, &values})
     if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   return out;
 }
@@ -891,6 +901,8 @@ TORCH_LIBRARY_IMPL(bioemu_mi355x, Meta, m) {
   m.impl("paged_append", &paged_append_meta);
   m.impl("paged_attention", &paged_attention_meta);
 }
+
+TORCH_LIBRARY_IMPL(bioemu_mi355x, ADInplaceOrView, m) { m.impl("paged_append", &paged_append_in_place); }
 
 TORCH_LIBRARY_IMPL(bioemu_mi355x, Autograd, m) {
   m.impl("layer_norm", &layer_norm_autograd);

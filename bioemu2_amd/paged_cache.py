@@ -40,8 +40,8 @@ def paged_append(keys: Tensor, values: Tensor, k: Tensor, v: Tensor, page_table:
     addresses, the other dimensions in any order in memory.  page_table: whole numbers of 32 bits [B, width]; lengths,
     counts: [B].  With ``frequencies`` k and q are turned as ``rotary`` does, to their positions in the sequence or to
     ``positions`` ([B, N]).  Padding rows write nothing, and are zeros in the result; nor does a position whose table
-    entry names no page (below 0, past the pool, or past the table).  A slot that a call names twice gets one of the
-    two."""
+    entry names no page (below 0, past the pool, or past the table).  A slot that a call names twice gets values of
+    both, in any order."""
     _ops.require_gpu(k, "paged_append")
     page_table, lengths, counts = _ints("paged_append", page_table, lengths, counts)
     dtype = None if q is None else q.dtype
@@ -63,7 +63,9 @@ def paged_attention(q: Tensor, keys: Tensor, values: Tensor, page_table: Tensor,
     default) and sees the keys up to its own (all of the sequence's, not causal); padding rows and rows that see nothing
     give zeros.  Made for a few rows a sequence: keys are read once for every 32 rows of queries times H / Hk.
     Keys whose table entry names no page are not seen; what unused slots hold does not matter.
-    scale, cap, bias_table, bias_buckets: as in ``attention``.  The table's width times the page size is at most 2^27."""
+    Values that are not finite reach the rows that see them, and no others.
+    scale, cap, bias_table, bias_buckets: as in ``attention``.  The table's width times the page size is at most 2^27, and
+    times B Hk (and, past 32 rows, their blocks) below 2^35."""
     _ops.require_gpu(q, "paged_attention")
     if q.ndim != 4:
         raise ValueError(f"paged_attention: q must be [B, Nq, H, D], got {tuple(q.shape)}")

@@ -173,6 +173,8 @@ def test_many_sequences(gpu_device):
     lengths[:3], lengths[64], lengths[-1] = [0, 0, 0], 0, 0
     Case(lengths, H=4, Hk=2).check()
     Case(lengths, H=4, Hk=2, width=90).check()
+    Case(lengths, H=8, Hk=8, width=90).check()          # more items than workgroups that share them
+    Case(lengths * 4, H=8, Hk=8, D=16, width=90).check()   # so many that none is split
 
 
 def test_one_long_sequence(gpu_device):
@@ -402,8 +404,47 @@ def test_append_bumps_versions(gpu_device):
     before = cache.keys._version, cache.values._version
     cache.append(k, k, torch.zeros(1, 1, dtype=I32, device="cuda"), torch.ones(1, dtype=I32, device="cuda"))
     assert cache.keys._version > before[0] and cache.values._version > before[1]
+    before = cache.keys._version
     with torch.inference_mode():
         cache.append(k, k, torch.zeros(1, 1, dtype=I32, device="cuda"), torch.ones(1, dtype=I32, device="cuda"))
+        own = PagedCache(2, 8, 2, 32, device="cuda")
+        own.append(k, k, torch.zeros(1, 1, dtype=I32, device="cuda"), torch.ones(1, dtype=I32, device="cuda"))
+    assert cache.keys._version > before
+
+
+def test_append_of_the_cache_to_itself(gpu_device):
+    """Slots moved by one within the cache: rows are read before they are written over."""
+    cache = PagedCache(3, 16, 2, 32, dtype=F32, device="cuda")
+    cache.keys.normal_()
+    cache.values.normal_()
+    k, v = cache.keys.clone(), cache.values.clone()
+    table = torch.tensor([[0, 1]], dtype=I32, device="cuda")
+    cache.append(cache.keys[:1, :15], cache.values[:1, :15], table, torch.tensor([16], device="cuda"))
+    assert torch.equal(cache.keys[0, 1:], k[0, :15]) and torch.equal(cache.values[0, 1:], v[0, :15])
+    assert torch.equal(cache.keys[0, 0], k[0, 0]) and torch.equal(cache.keys[1:], k[1:])
+
+
+def test_append_past_the_caches(gpu_device):
+    """More results than the caches near the CUs hold are written another way."""
+    B, N, H, Hk, D, page = 2, 1500, 16, 16, 128, 64
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q, k, v = (torch.randn(B, N, h, D, generator=g, device="cuda").to(BF16) for h in (H, Hk, Hk))
+    cache = PagedCache(60, page, Hk, D, device="cuda")
+    cache.keys.zero_()
+    cache.values.zero_()
+    table = torch.randperm(60, generator=torch.Generator().manual_seed(1))[:48].view(2, 24).to(I32)
+    lengths, counts = [1533, 1400], [N, 1333]
+    f = rotary_frequencies(D, device="cuda")
+    got = cache.append(k, v, table.cuda(), torch.tensor(lengths, device="cuda"), counts=torch.tensor(counts, device="cuda"),
+                       q=q, frequencies=f)
+    for b in range(B):
+        pos = torch.arange(lengths[b] - counts[b], lengths[b])
+        at = (table[b][pos // page].long().cuda(), (pos % page).cuda())
+        _close(got[b, :counts[b]], _turned(q[b, :counts[b]], pos.cuda(), f, False, 1.0))
+        _close(cache.keys[at], _turned(k[b, :counts[b]], pos.cuda(), f, False, 1.0))
+        assert torch.equal(cache.values[at], v[b, :counts[b]]) and bool((got[b, counts[b]:] == 0).all())
+        cache.keys[at] = cache.values[at] = 0
+    assert cache.keys.abs().max() == 0 and cache.values.abs().max() == 0
 
 
 # ----------------------------------------------------------------------------

@@ -80,6 +80,18 @@ def test_step(gpu_device, dtype, interleaved, B, N, H, Hk, D, rot):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_results_past_the_caches(gpu_device, dtype, interleaved):
+    """More results than the caches near the CUs hold are written another way."""
+    n = 4001 if dtype == BF16 else 2003
+    q, k = rand(1, n, 32, 128, dtype=dtype), rand(1, n, 8, 128, dtype=dtype, seed=1)
+    f = rotary_frequencies(96, device="cuda")
+    y = rotary(q, k, None, f, interleaved=interleaved)
+    check(y[0], exact(q, None, f, interleaved))
+    check(y[1], exact(k, None, f, interleaved))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_far_positions(gpu_device, dtype):
     pos = torch.tensor([[0, 1, -1, 2 ** 20, 2 ** 24 + 1, 10 ** 9 + 7, 2 ** 31 - 1, -2 ** 31, -10 ** 6]], dtype=I32).cuda()
     q = rand(1, 9, 2, 64, dtype=dtype)
