@@ -80,9 +80,11 @@ __device__ __forceinline__ int length_of(const PagedArgs& p, int b) {
   return min(max(p.lengths[b], 0), most);
 }
 
+// Its tiles; none if it has no query.
 template <int KEYS>
 __device__ __forceinline__ int tiles_of(const PagedArgs& p, int b) {
-  return (length_of(p, b) + KEYS - 1) / KEYS;
+  const int length = length_of(p, b), count = p.counts ? p.counts[b] : 1;
+  return count <= 0 ? 0 : (length + KEYS - 1) / KEYS;
 }
 
 // Inclusive sums over the wave's lanes.
@@ -102,12 +104,18 @@ __device__ __forceinline__ int scan(int x) {
 // short ones: every item in equal parts of its own, at most `part` tiles, so that no share has two items' ends: what an
 // item's start and end cost, some kItemCost tiles' time, is then more than what the shares are longer.
 struct Share {
-  int b, item, t0, left;
+  int b, item, t0, left, w;   // w: the share's number
 };
 constexpr int kItemCost = 16;
+// Shares in order over the XCDs (workgroup i runs on XCD i % 8): neighbours, which may read parts of the same cache lines
+// or the same keys for other rows, get one L2.  -1: none.
+__device__ __forceinline__ int xcd_order(int n) {
+  const int per = (n + kAttnXcds - 1) / kAttnXcds, i = blockIdx.x / kAttnXcds, w = blockIdx.x % kAttnXcds * per + i;
+  return i < per && w < n ? w : -1;
+}
 template <int KEYS>
 __device__ __forceinline__ Share share_of(const PagedArgs& p, int B, int items) {
-  const int lane = threadIdx.x & 63, groups = p.groups, w = blockIdx.x;
+  const int lane = threadIdx.x & 63, groups = p.groups;
   int total = 0, live = 0, sums = 0, own = 0;
   for (int b0 = 0; b0 < B; b0 += 64) {
     own = b0 + lane < B ? tiles_of<KEYS>(p, b0 + lane) : 0;
@@ -117,10 +125,22 @@ __device__ __forceinline__ Share share_of(const PagedArgs& p, int B, int items) 
   }
   total *= items;
   live *= items;
-  const Share none{0, 0, 0, 0};
+  const Share none{0, 0, 0, 0, 0};
   const unsigned spare = max(groups - live, 1), part = max(((unsigned)total + spare - 1) / spare, (unsigned)p.least);
   const unsigned each = (unsigned)total / (unsigned)groups;
   const bool parts = live < groups && part < each + kItemCost;
+  int n = groups;
+  if (parts) {
+    n = 0;
+    for (int b0 = 0; b0 < B; b0 += 64) {
+      if (B > 64) own = b0 + lane < B ? tiles_of<KEYS>(p, b0 + lane) : 0;
+      sums = scan(((unsigned)own + part - 1) / part);
+      n += __builtin_amdgcn_readlane(sums, 63);
+    }
+    n *= items;
+  }
+  const int w = xcd_order(n);
+  if (w < 0) return none;
   // where the share starts, in tiles, or the number of the part
   const int more = total - (int)each * groups, at = parts ? w : w * (int)each + min(w, more);
   int before = 0, b = 0;
@@ -128,19 +148,19 @@ __device__ __forceinline__ Share share_of(const PagedArgs& p, int B, int items) 
     if (B > 64) own = b + lane < B ? tiles_of<KEYS>(p, b + lane) : 0;
     int mine = own;
     if (parts) mine = ((unsigned)own + part - 1) / part;
-    if (B > 64 || parts) sums = scan(mine);
+    if (B > 64) sums = scan(mine);
     const uint64_t past = __ballot(before + sums * items > at);
     if (past) {
       const int l = __ffsll((unsigned long long)past) - 1;
       b += l;
       before += __builtin_amdgcn_readlane(sums - mine, l) * items;
       const unsigned in = at - before, n = __builtin_amdgcn_readlane(mine, l), item = in / n;
-      if (!parts) return {b, (int)item, (int)(in - item * n), (int)each + (w < more)};
+      if (!parts) return {b, (int)item, (int)(in - item * n), (int)each + (w < more), w};
       const unsigned tiles = __builtin_amdgcn_readlane(own, l), i = in - item * n, size = tiles / n, rest = tiles - size * n;
-      return {b, (int)item, (int)(i * size + min(i, rest)), (int)(size + (i < rest))};
+      return {b, (int)item, (int)(i * size + min(i, rest)), (int)(size + (i < rest)), w};
     }
     before += __builtin_amdgcn_readlane(sums, 63) * items;
-    if (b + 64 >= B) return none;   // more workgroups than parts
+    if (b + 64 >= B) return none;   // not with lengths that stay
   }
 }
 
@@ -215,7 +235,8 @@ struct Walk {
     v = page * p.vpage + slot * p.vslot;
   }
   // Keys that no other block of rows reads pass the caches by: eight tokens over 8200 to 32768 keys, 117 us, through the
-  // caches 131.  (64 queries of 16/4 heads, 8 blocks, over 4096 keys: 84 and 58.)
+  // caches 131.  (64 queries of 16/4 heads, 8 blocks, over 4096 keys: 84 and 58.)  Not rows that share lines, with other
+  // loads of a tile or other heads: 28 tokens over up to 8000 keys of 16 heads of 80, 155 and 135.
   template <class V>
   __device__ static __forceinline__ V read(const GLOBAL V* p) {
     if constexpr (ONCE) return __builtin_nontemporal_load(p);
@@ -592,8 +613,10 @@ __global__ __launch_bounds__(64 * W, 2) void paged_kernel(const AttnArgs a, cons
   const int items = a.Hk * p.blocks;   // of a sequence
   Share s;
   if (p.groups == 0) {
-    const int b = blockIdx.x / items, item = blockIdx.x - b * items, tiles = tiles_of<KEYS>(p, b);
-    s = {b, item, 0, tiles};
+    const int w = xcd_order(a.B * items);
+    if (w < 0) return;
+    const int b = w / items, item = w - b * items, tiles = tiles_of<KEYS>(p, b);
+    s = {b, item, 0, tiles, w};
     if (tiles == 0) {
       const int hk = item / p.blocks, row0 = item % p.blocks * 16 * RB, n = min(a.Nq * a.G - row0, 16 * RB);
       for (int k = threadIdx.x; k < n * a.D; k += 64 * W) {
@@ -613,10 +636,10 @@ __global__ __launch_bounds__(64 * W, 2) void paged_kernel(const AttnArgs a, cons
       continue;
     }
     const int t1 = min(tiles, s.t0 + s.left);
-    const int64_t item = (int64_t)s.b * items + s.item, slot = s.t0 == 0 && t1 == tiles ? -1 : blockIdx.x + item;
+    const int64_t item = (int64_t)s.b * items + s.item, slot = s.t0 == 0 && t1 == tiles ? -1 : s.w + item;
     if (p.groups && threadIdx.x == 0) {
-      if (s.t0 == 0) parts.range[2 * item] = blockIdx.x;
-      if (t1 == tiles) parts.range[2 * item + 1] = blockIdx.x;
+      if (s.t0 == 0) parts.range[2 * item] = s.w;
+      if (t1 == tiles) parts.range[2 * item + 1] = s.w;
     }
     Walk<T, DP, RB, CAP, W, EVEN, ONCE>(a, p).run(s.b, s.item / p.blocks, s.item % p.blocks * 16 * RB, s.t0, t1, out, parts, slot, lds);
     s.left -= t1 - s.t0;
@@ -737,6 +760,7 @@ bool even_pages(const bioemu_paged_cache& c, bool f32) {
 
 struct Plan {
   int rb, blocks, waves, groups, least;
+  bool once;   // keys pass the caches by
   int64_t items, slots;
 };
 
@@ -749,12 +773,13 @@ Plan plan(const AttnArgs& a, const bioemu_paged_cache& c, bool f32) {
   p.rb = rows <= 16 ? 1 : 2;
   p.blocks = (rows + 16 * p.rb - 1) / (16 * p.rb);
   p.items = (int64_t)a.B * a.Hk * p.blocks;
+  p.once = p.blocks == 1 && a.D * (f32 ? 4 : 2) % 128 == 0;
   const int64_t most = c.pages > 0 ? c.table_width * c.page_size : 0;
   // what a walk of one workgroup takes less than the join: 1024 keys of 64 values in bf16
   if (most * std::max(a.D, 64) * (f32 ? 4 : 2) <= 1024 * 64 * 2 || p.items >= 16 * attn_units()) {
     // with workgroups to spare eight waves share a walk (sixteen, where registers allow it, start 1.5 us later: 12.9 us for
     // one token over 773 keys of 16 heads of 64, 11.3 with eight, 17 with four)
-    if (p.blocks == 1 && p.items <= 2 * attn_units() && (f32 || a.cap <= kFastCap)) p.waves = 8;
+    if ((p.once || p.rb == 1) && p.items <= 2 * attn_units() && (f32 || a.cap <= kFastCap)) p.waves = 8;
     return p;
   }
   // two a CU: with three or four, where registers allow them, 64 sequences of 4096 keys took 206 us, with these 184
@@ -793,12 +818,12 @@ int launch(const AttnArgs& a, const PagedArgs& p, const Plan& pl, T* out, void* 
   }
   {
     KernelTimerScope timer("paged_attention", stream);
-    const dim3 grid((unsigned)(pl.groups ? pl.groups : pl.items));
+    const dim3 grid((unsigned)round_up(pl.groups ? pl.groups : pl.items, kAttnXcds));
     const auto go = [&](auto kernel) { kernel<<<grid, 64 * pl.waves, 0, stream>>>(a, p, out, parts); };
     const bool wide = !fast_cap<T>(a);
     // few calls have a wide cap: one form for them
 #define BIOEMU_GO(RB, W, EVEN, ONCE)                                                                 \
-  if (pl.rb == RB && !wide && pl.waves == W && p.even == EVEN && (p.blocks == 1) == ONCE)            \
+  if (pl.rb == RB && !wide && pl.waves == W && p.even == EVEN && pl.once == ONCE)                     \
     go(paged_kernel<T, DP, RB, kCapped, W, EVEN, ONCE>);
 #define BIOEMU_GO_RB(RB)                                                            \
   BIOEMU_GO(RB, 4, true, true)                                                      \
@@ -810,6 +835,10 @@ int launch(const AttnArgs& a, const PagedArgs& p, const Plan& pl, T* out, void* 
   }
     BIOEMU_GO_RB(1)
     BIOEMU_GO_RB(2)
+    BIOEMU_GO(1, 4, true, false)
+    BIOEMU_GO(1, 4, false, false)
+    BIOEMU_GO(1, 8, true, false)
+    BIOEMU_GO(1, 8, false, false)
     BIOEMU_GO(2, 4, true, false)
     BIOEMU_GO(2, 4, false, false)
 #undef BIOEMU_GO_RB

@@ -69,7 +69,7 @@ struct Token {
   int b, i, live;
 };
 
-// V values at a time; a piece is V values, or in the half layout V values of each half.  APPEND: with v and a cache.
+// V values at a time; a piece is V values, or in the half layout V of each half, or 2 V of what does not turn.  APPEND: with v and a cache.
 // STREAM: results go past the caches.
 template <class T, int V, bool INTERLEAVED, bool APPEND, bool STREAM>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
@@ -82,6 +82,9 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
   const int turned = INTERLEAVED ? 2 * a.pairs / V : a.pairs / V;   // pieces of a row that turn
   const int q_heads = a.q ? a.H : 0, units = n * a.heads * a.pieces;
   constexpr int U = kUnits<INTERLEAVED>;
+  // where the two parts of a piece begin in its row
+  const auto first_of = [&](int p) { return INTERLEAVED || p < turned ? p * V : 2 * (a.pairs + (p - turned) * V); };
+  const auto second_of = [&](int p, int d) { return p < turned ? a.pairs + d : d + V; };
 
   for (int u0 = 0; u0 == 0 || u0 < units; u0 += kThreads * U) {
     vec x[U], y[U];
@@ -103,8 +106,9 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
       if constexpr (INTERLEAVED) {
         x[e] = *reinterpret_cast<const vec*>(src + p * V);
       } else {
-        x[e] = *reinterpret_cast<const vec*>(src + (p < turned ? p * V : a.pairs + p * V));
-        if (p < turned) y[e] = *reinterpret_cast<const vec*>(src + a.pairs + p * V);
+        const int d = first_of(p), other = second_of(p, d);
+        x[e] = *reinterpret_cast<const vec*>(src + d);
+        if (other < a.D) y[e] = *reinterpret_cast<const vec*>(src + other);
       }
     }
     if (u0 == 0) {
@@ -175,14 +179,14 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
       } else {
         dst = static_cast<T*>(a.k_out) + ((int64_t)(t0 + t) * a.Hk + hk) * a.D;
       }
-      vec* to = reinterpret_cast<vec*>(dst + (INTERLEAVED || p < turned ? p * V : a.pairs + p * V));
-      vec* too = reinterpret_cast<vec*>(dst + a.pairs + p * V);
+      const int d = first_of(p), other = INTERLEAVED ? a.D : second_of(p, d);
+      vec *to = reinterpret_cast<vec*>(dst + d), *too = reinterpret_cast<vec*>(dst + other);
       if constexpr (STREAM) {
         __builtin_nontemporal_store(r, to);
-        if (!INTERLEAVED && p < turned) __builtin_nontemporal_store(w, too);
+        if (other < a.D) __builtin_nontemporal_store(w, too);
       } else {
         *to = r;
-        if (!INTERLEAVED && p < turned) *too = w;
+        if (other < a.D) *too = w;
       }
     }
   }
@@ -225,7 +229,7 @@ int run(const char* what, RotaryArgs& a, bool f32, hipStream_t stream) {
   KernelTimerScope timer(what, stream);
   const int v = piece(a, f32);
   a.heads = (a.q ? a.H : 0) + (a.k ? (APPEND ? 2 : 1) * a.Hk : 0);
-  a.pieces = (a.interleaved ? a.D : a.D - a.pairs) / v;
+  a.pieces = a.interleaved ? a.D / v : a.pairs / v + (a.D - 2 * a.pairs + 2 * v - 1) / (2 * v);
   a.by_n = Divisor(a.N);
   a.by_heads = Divisor(a.heads);
   a.by_pieces = Divisor(a.pieces);
