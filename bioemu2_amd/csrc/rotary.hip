@@ -82,9 +82,10 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
   const int turned = INTERLEAVED ? 2 * a.pairs / V : a.pairs / V;   // pieces of a row that turn
   const int q_heads = a.q ? a.H : 0, units = n * a.heads * a.pieces;
   constexpr int U = kUnits<INTERLEAVED>;
-  // where the two parts of a piece begin in its row
-  const auto first_of = [&](int p) { return INTERLEAVED || p < turned ? p * V : 2 * (a.pairs + (p - turned) * V); };
-  const auto second_of = [&](int p, int d) { return p < turned ? a.pairs + d : d + V; };
+  // where the two parts of a piece begin in its row; past it: there is no second
+  const int apart = (a.D - 2 * a.pairs + 2 * V - 1) / (2 * V) * V;
+  const auto first_of = [&](int p) { return INTERLEAVED || p < turned ? p * V : a.pairs + p * V; };
+  const auto second_of = [&](int p, int d) { return d + (p < turned ? a.pairs : apart); };
 
   for (int u0 = 0; u0 == 0 || u0 < units; u0 += kThreads * U) {
     vec x[U], y[U];
@@ -222,14 +223,15 @@ void launch(const RotaryArgs& a, hipStream_t stream) {
 
 template <bool APPEND>
 int run(const char* what, RotaryArgs& a, bool f32, hipStream_t stream) {
-  // as many tokens as have a cos and sin for each thread, where that leaves the launch wide enough
-  a.per = a.pairs > 0 && a.pairs < kThreads ? kThreads / a.pairs : 1;
-  if (a.per > 16) a.per = 16;
-  while (a.per > 1 && a.tokens / a.per < 1024) a.per /= 2;
   KernelTimerScope timer(what, stream);
   const int v = piece(a, f32);
   a.heads = (a.q ? a.H : 0) + (a.k ? (APPEND ? 2 : 1) * a.Hk : 0);
   a.pieces = a.interleaved ? a.D / v : a.pairs / v + (a.D - 2 * a.pairs + 2 * v - 1) / (2 * v);
+  // a workgroup has as many tokens as its threads hold at once, where that leaves the launch wide enough (16384 tokens of
+  // 16/4 heads of 128: 26.1 us, 27.4 with a rest that takes another turn)
+  const int64_t held = kThreads * (a.interleaved ? kUnits<true> : kUnits<false>);
+  a.per = (int)std::min(std::max(held / ((int64_t)a.heads * a.pieces), (int64_t)1), (int64_t)16);
+  while (a.per > 1 && a.tokens / a.per < 1024) a.per /= 2;
   a.by_n = Divisor(a.N);
   a.by_heads = Divisor(a.heads);
   a.by_pieces = Divisor(a.pieces);
