@@ -221,8 +221,9 @@ def test_empty_pool_or_table(gpu_device):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-def test_what_is_not_finite_reaches_its_rows_only(gpu_device, dtype):
-    c = Case([90, 90], dtype, Nq=2, H=4, Hk=2)
+@pytest.mark.parametrize("width", [None, 90])
+def test_what_is_not_finite_reaches_its_rows_only(gpu_device, dtype, width):
+    c = Case([90, 90], dtype, Nq=2, H=4, Hk=2, width=width)
     want = c.call()
     for store in (c.keys, c.values):
         page, slot = int(c.table[0, 89 // 16]), 89 % 16     # the last key: seen by the last query alone
@@ -260,18 +261,20 @@ def test_lowest_bias(gpu_device, width):
         assert out[b, 0, 1].abs().max() == 0
 
 
-def test_offsets_past_32_bits(gpu_device):
-    """Pages beyond 2^32 bytes (and beyond 2^31 values) of a pool."""
-    pages, page, hk, d = 66000, 64, 4, 128          # 4.3 GB in bf16
-    keys = torch.empty(pages, hk, page, d, dtype=BF16, device="cuda").transpose(1, 2)
-    values = torch.empty(pages, hk, page, d, dtype=BF16, device="cuda").transpose(1, 2)
+@pytest.mark.parametrize("page,slots_outside", [(64, False), (64, True), (60, False)])
+def test_offsets_past_32_bits(gpu_device, page, slots_outside):
+    """Pages beyond 2^32 bytes (and beyond 2^31 values) of a pool, or its slots 2^26 bytes apart and more."""
+    pages, hk, d = 70400, 4, 128          # 4.3 GB in bf16
+    shape = (page, pages, hk, d) if slots_outside else (pages, hk, page, d)
+    keys, values = (torch.empty(shape, dtype=BF16, device="cuda").transpose(*((0, 1) if slots_outside else (1, 2)))
+                    for _ in "kv")
     lengths = torch.tensor([150], dtype=I32, device="cuda")
-    table = torch.tensor([[65999, 3, 65700]], dtype=I32, device="cuda")
+    table = torch.tensor([[pages - 1, 3, pages - 300]], dtype=I32, device="cuda")
     g = torch.Generator(device="cuda").manual_seed(0)
     k, v = (torch.randn(1, 150, hk, d, generator=g, device="cuda").to(BF16) for _ in "kv")
     q = torch.randn(1, 1, hk, d, generator=g, device="cuda").to(BF16)
     paged_append(keys, values, k, v, table, lengths)
-    assert torch.equal(keys[65999], k[0, :64]) and torch.equal(values[65700, :22], v[0, 128:])
+    assert torch.equal(keys[pages - 1], k[0, :page]) and torch.equal(values[pages - 300, :150 - 2 * page], v[0, 2 * page:])
     got = paged_attention(q, keys, values, table, lengths)
     want = attention(q.float(), k.float(), v.float())
     assert (got.float() - want).abs().max() < 2.0 ** -8 * want.abs().max() + 1e-4
@@ -294,6 +297,27 @@ def test_strides(gpu_device, dtype):
     odd = torch.empty(2, 1, 4, 36, dtype=dtype, device="cuda")
     odd[..., 1:33] = c.q
     assert torch.equal(paged_attention(odd[..., 1:33], k, v, c.table, c.lengths), want)
+
+
+def test_slots_far_apart(gpu_device):
+    """Slots more than 2^27 bytes apart (pages of 16, all first slots, then all second ones, ...)."""
+    pages, page, hk, d = 131200, 16, 4, 128          # 2.1 GB
+    keys, values = (torch.empty(page, pages, hk, d, dtype=BF16, device="cuda").transpose(0, 1) for _ in "kv")
+    g = torch.Generator(device="cuda").manual_seed(0)
+    k, v = (torch.randn(1, 40, hk, d, generator=g, device="cuda").to(BF16) for _ in "kv")
+    q = torch.randn(1, 1, hk, d, generator=g, device="cuda").to(BF16)
+    lengths, table = torch.tensor([40], device="cuda"), torch.tensor([[131000, 7, 131199]], device="cuda")
+    paged_append(keys, values, k, v, table, lengths)
+    got, want = paged_attention(q, keys, values, table, lengths), attention(q.float(), k.float(), v.float())
+    assert (got.float() - want).abs().max() < 2.0 ** -8 * want.abs().max() + 1e-4
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_more_queries_than_positions(gpu_device, dtype):
+    """Queries before the first position see nothing."""
+    c = Case([3, 1, 40], dtype, Nq=6, H=4, Hk=2, counts=[5, 6, 6])
+    c.check()
+    assert c.call()[0, :2].abs().max() == 0
 
 
 def test_shared_pages(gpu_device):
