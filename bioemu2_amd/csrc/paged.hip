@@ -13,15 +13,17 @@
 //   share a register, which takes one byte permutation for each; in fp32 nothing.
 // Weights go into the second product as two bf16 parts (16 bits): the matrix cores have time to spare, and the result is
 // then rounded once.
+//
+// Reading the keys and values bounds it; a stream of 2 GB is read at 6.2 TB/s.  Measured, join included, in bf16: 8 tokens
+// over 8200 to 32768 keys, 32/8 heads of 128, 117 us (6.1 TB/s); 64 over up to 4000, 28/4 heads of 128, 65 us (4.9).
+// Short caches take the latency of a walk: one token over 773 keys of 16 heads of 64, 11 us.  In fp32 the 16 x 16 x 4
+// product works as long as the reading: 4 x 5 queries over up to 5000 keys, 8/2 heads of 32, 16 us and a join of 4.
 #include <algorithm>
 
 #include "attn.h"
 
 namespace bioemu {
 namespace {
-
-// the compiler does not see by itself that addresses of two branches are of memory both
-#define GLOBAL __attribute__((address_space(1)))
 
 constexpr float kRescale = 8.f;   // log2 of the largest weight before the maximum moves
 
@@ -102,7 +104,9 @@ __device__ __forceinline__ int scan(int x) {
 // item `item` of sequence b.  Every wave by itself.  Two ways of dealing them:
 // long walks: all tiles, one item behind the other, in equal shares, whatever the sequences' lengths;
 // short ones: every item in equal parts of its own, at most `part` tiles, so that no share has two items' ends: what an
-// item's start and end cost, some kItemCost tiles' time, is then more than what the shares are longer.
+// item's start and end cost, some kItemCost tiles' time, is then more than what the shares are longer.  (In a graph, one
+// token over 773 keys of 16 heads of 64: 13.4 us by the first way, 9.9 by the second; 64 over up to 4000 keys, four key
+// heads of 128: 73 and 86.)
 struct Share {
   int b, item, t0, left, w;   // w: the share's number
 };
@@ -183,7 +187,7 @@ struct Walk {
   const AttnArgs& a;
   const PagedArgs& p;
   const int lane, m, h;
-  const GLOBAL char *kbase, *vbase;
+  const char *kbase, *vbase;
   // byte offsets of the lane's rows among sixteen, and of its pieces of a row (the row's first where it has no more)
   unsigned krow[LINES ? 2 : 1], vrow, kd[LINES ? 2 : 1][LINES ? KS / 2 : KS], vd[VC / VL];
   int64_t kat, kat1, vat, vat1;   // see locate
@@ -238,7 +242,7 @@ struct Walk {
   // caches 131.  (64 queries of 16/4 heads, 8 blocks, over 4096 keys: 84 and 58.)  Not rows that share lines, with other
   // loads of a tile or other heads: 28 tokens over up to 8000 keys of 16 heads of 80, 155 and 135.
   template <class V>
-  __device__ static __forceinline__ V read(const GLOBAL V* p) {
+  __device__ static __forceinline__ V read(const V* p) {
     if constexpr (ONCE) return __builtin_nontemporal_load(p);
     return *p;
   }
@@ -247,10 +251,10 @@ struct Walk {
     for (int u = 0; u < KU; ++u)
 #pragma unroll
       for (int e = 0; e < (LINES ? 2 : 1); ++e) {
-        const GLOBAL char* row = EVEN ? kbase + (u == 0 ? kat : kat1) : kbase + __shfl(kat, 16 * u + key_of(e));
+        const char* row = EVEN ? kbase + (u == 0 ? kat : kat1) : kbase + __shfl(kat, 16 * u + key_of(e));
 #pragma unroll
         for (int s = 0; s < (LINES ? KS / 2 : KS); ++s)
-          kf[u][LINES ? 2 * s + e : s] = read((const GLOBAL kvec*)(row + (krow[e] + kd[e][s])));
+          kf[u][LINES ? 2 * s + e : s] = read((const kvec*)(row + (krow[e] + kd[e][s])));
       }
   }
   // s = K Q^T of rows q, sixteen keys u
@@ -279,10 +283,10 @@ struct Walk {
   __device__ __forceinline__ void load_v() {
 #pragma unroll
     for (int t = 0; t < VK; ++t) {
-      const GLOBAL char* row =
+      const char* row =
           EVEN ? vbase + (t < 4 ? vat : vat1) + (t & 3) * p.vslot : vbase + __shfl(vat, 16 * (t >> 2) + 4 * h + (t & 3));
 #pragma unroll
-      for (int c = 0; c < VC / VL; ++c) vf[t][c] = read((const GLOBAL vvec*)(row + (vrow + vd[c])));
+      for (int c = 0; c < VC / VL; ++c) vf[t][c] = read((const vvec*)(row + (vrow + vd[c])));
     }
   }
   // acc += V^T times the tile's weights
@@ -345,8 +349,8 @@ struct Walk {
     const int count = __builtin_amdgcn_readfirstlane(p.counts ? min(max(p.counts[b], 0), a.Nq) : a.Nq);
     const int first = length - count;   // position of the first query
     const int* table = p.page_table + b * p.table_stride;
-    kbase = (const GLOBAL char*)p.keys + hk * p.khead;
-    vbase = (const GLOBAL char*)p.values + hk * p.vhead;
+    kbase = (const char*)p.keys + hk * p.khead;
+    vbase = (const char*)p.values + hk * p.vhead;
     int t = t0 + wave, page = page_of(table, t);
 
     int pos[RB], lim[RB];
@@ -571,7 +575,7 @@ struct Walk {
         for (int j = max(max(first + 1, 0) / KEYS, t0) * KEYS; j < seen; ++j) {   // from the first such tile
           const int at = page_index(j), page = table[at];
           if (page < 0 || page >= p.pages) continue;
-          const GLOBAL T* v = (const GLOBAL T*)(vbase + page * p.vpage + (j - at * p.page_size) * p.vslot) + d;
+          const T* v = (const T*)(vbase + page * p.vpage + (j - at * p.page_size) * p.vslot) + d;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (not_finite(v[e])) o[e] += (float)v[e];
@@ -641,7 +645,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_kernel(const AttnArgs a, cons
       if (s.t0 == 0) parts.range[2 * item] = s.w;
       if (t1 == tiles) parts.range[2 * item + 1] = s.w;
     }
-    Walk<T, DP, RB, CAP, W, EVEN, ONCE>(a, p).run(s.b, s.item / p.blocks, s.item % p.blocks * 16 * RB, s.t0, t1, out, parts, slot, lds);
+    Walk<T, DP, RB, CAP, W, EVEN, ONCE>(a, p).run(s.b, s.item / p.blocks, s.item % p.blocks * 16 * RB, s.t0, t1, out,
+                                                  parts, slot, lds);
     s.left -= t1 - s.t0;
     s.t0 = 0;
     ++s.item;
@@ -775,7 +780,8 @@ Plan plan(const AttnArgs& a, const bioemu_paged_cache& c, bool f32) {
   p.items = (int64_t)a.B * a.Hk * p.blocks;
   p.once = p.blocks == 1 && a.D * (f32 ? 4 : 2) % 128 == 0;
   const int64_t most = c.pages > 0 ? c.table_width * c.page_size : 0;
-  // what a walk of one workgroup takes less than the join: 1024 keys of 64 values in bf16
+  // what a walk of one workgroup takes no longer than parts and the join: up to 1024 keys of 64 values in bf16 (in a graph
+  // 8.4 us for 512 and 11.0 for 1024; in parts 9.8 and 10.0, and a second launch)
   if (most * std::max(a.D, 64) * (f32 ? 4 : 2) <= 1024 * 64 * 2 || p.items >= 16 * attn_units()) {
     // with workgroups to spare eight waves share a walk (sixteen, where registers allow it, start 1.5 us later: 12.9 us for
     // one token over 773 keys of 16 heads of 64, 11.3 with eight, 17 with four)
@@ -848,6 +854,8 @@ int launch(const AttnArgs& a, const PagedArgs& p, const Plan& pl, T* out, void* 
   if (!pl.groups) return BIOEMU_OK;
   KernelTimerScope timer("paged_join", stream);
   const int64_t rows = (int64_t)a.B * a.Nq * a.H;
+  // by parts a row: some 8 (8 tokens over 8192 keys of 8 heads) 50.8 us by quads, 51.2 by a workgroup a row; 16: 30.4 and
+  // 29.5; 64: 37.8 and 31.6
   if (pl.groups <= 14 * pl.items)
     paged_join_rows_kernel<T, Cache<T>::KEYS><<<dim3((unsigned)((rows * (a.D / 4) + 255) / 256)), 256, 0, stream>>>(
         a, p, out, parts, block_rows, (int)rows);

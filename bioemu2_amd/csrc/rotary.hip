@@ -8,6 +8,10 @@
 // A workgroup takes a few tokens.  Its threads first request the values that they will turn, then compute cos and sin of
 // every (token, pair) once, into LDS, and every head of the token reads them there.  Appending is the same with k's rows
 // going to their slots and v's copied beside them.
+//
+// Reading and writing bounds it (a stream of 2 GB is read at 6.2 TB/s).  In bf16: 16384 tokens of 16/4 heads of 128, 26 us
+// (6.4 TB/s: the inputs, 84 MB, fit the last-level cache); 2 x 4096 of 32/8 heads of 128, 32 us (5.3); appending 4 x up to
+// 4000 of 32/8 heads of 128, 62 us (4.5 of what there is, 5.1 with the zeros of q's padding).  One token, 2 us.
 #include <algorithm>
 
 #include "common.h"
@@ -69,8 +73,8 @@ struct Token {
   int b, i, live;
 };
 
-// V values at a time; a piece is V values, or in the half layout V of each half, or 2 V of what does not turn.  APPEND: with v and a cache.
-// STREAM: results go past the caches.
+// V values at a time; a piece is V values, or in the half layout V of each half, or 2 V of what does not turn.  APPEND:
+// with v and a cache.  STREAM: results go past the caches.
 template <class T, int V, bool INTERLEAVED, bool APPEND, bool STREAM>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
   typedef T vec __attribute__((ext_vector_type(V)));
