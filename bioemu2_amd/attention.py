@@ -21,6 +21,7 @@ from torch import Tensor
 
 from . import _ops
 from ._lib import torch_op
+from .paged_cache import PagedCache
 from .relative_position import _int32, distance_buckets
 
 
@@ -98,3 +99,9 @@ class SequenceAttention(nn.Module):
         return attention(q, k, v, scale=self.scale, cap=self.cap, bias_table=self.bias, bias_buckets=self.buckets,
                          segments=segments, key_segments=key_segments, causal=self.causal, prefix=prefix,
                          cache_lengths=cache_lengths)
+
+    def paged(self, q: Tensor, cache: PagedCache, page_table: Tensor, lengths: Tensor,
+              counts: Tensor | None = None) -> Tensor:
+        """The same of new tokens over a cache in pages (``paged_attention``; no gradients)."""
+        return cache.attend(q, page_table, lengths, counts=counts, scale=self.scale, cap=self.cap,
+                            bias_table=self.bias.detach(), bias_buckets=self.buckets, causal=self.causal)

@@ -15,9 +15,9 @@
 // then rounded once.
 //
 // Reading the keys and values bounds it; a stream of 2 GB is read at 6.2 TB/s.  Measured, join included, in bf16: 8 tokens
-// over 8200 to 32768 keys, 32/8 heads of 128, 117 us (6.1 TB/s); 64 over up to 4000, 28/4 heads of 128, 65 us (4.9).
-// Short caches take the latency of a walk: one token over 773 keys of 16 heads of 64, 11 us.  In fp32 the 16 x 16 x 4
-// product works as long as the reading: 4 x 5 queries over up to 5000 keys, 8/2 heads of 32, 16 us and a join of 4.
+// over 8200 to 32768 keys, 32/8 heads of 128, 117 us (6.1 TB/s); 64 over up to 4000, 32/4 heads of 128, 65 us (4.9).
+// Short caches take the latency of a walk, memory read after memory read (lengths, page table, keys): one token over 773
+// keys of 16 heads of 64, 11 us; in fp32 4 x 5 tokens over up to 5000, 16/4 heads of 64, 16 us and a join of 4.
 #include <algorithm>
 
 #include "attn.h"

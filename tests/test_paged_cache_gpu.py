@@ -19,7 +19,7 @@ import pytest
 import torch
 
 from bioemu2_amd._lib import torch_op
-from bioemu2_amd.attention import attention
+from bioemu2_amd.attention import SequenceAttention, attention
 from bioemu2_amd.paged_cache import PagedCache, paged_append, paged_attention
 from bioemu2_amd.relative_position import distance_buckets
 from bioemu2_amd.rotary import RotaryPosition, rotary, rotary_frequencies
@@ -518,6 +518,22 @@ def test_prompt_then_tokens_as_one_pass(gpu_device, dtype):
     step([3, 3])
     while done[0] < 90:
         step([1, 1] if done[1] < 61 else [1, 0])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_sequence_attention_over_pages(gpu_device, dtype):
+    """A trained module over a cache: its bias wants gradients, the call has none; a query that does is refused."""
+    c = Case([70, 5, 33], dtype, Nq=3, counts=[3, 1, 2], cap=20.0, radius=8, num_buckets=8, tdtype=F32, scale=0.2)
+    att = SequenceAttention(4, radius=8, num_buckets=8, scale=0.2, cap=20.0, causal=True).cuda()
+    with torch.no_grad():
+        att.bias.copy_(c.bias)
+    cache = PagedCache(1, c.page, c.Hk, c.D, dtype=dtype, device="cuda")
+    cache.keys, cache.values = c.keys, c.values
+    out = att.paged(c.q, cache, c.table, c.lengths, c.counts)
+    assert not out.requires_grad
+    c.check(out)
+    with pytest.raises(NotImplementedError, match="no backward pass"):
+        att.paged(c.q.clone().requires_grad_(), cache, c.table, c.lengths, c.counts)
 
 
 @pytest.mark.parametrize("width", [8, 100])
