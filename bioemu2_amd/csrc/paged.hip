@@ -174,6 +174,7 @@ struct Walk {
   static constexpr int VL = VC * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : VC;   // values a load of V
   static constexpr int KL = sizeof(T) == 2 ? 8 : 4, KS = DP / (4 * KL), KU = KEYS / 16;
   static constexpr int VK = KEYS / 4;   // keys whose values a lane loads
+  static constexpr int STEP = 64 * W / (16 * RB);   // threads to a row of the block
   // Four lanes' pieces of a key are 64 bytes, half a cache line, and a second load of the line would wait for the first
   // one's in the cache.  So the lanes of two keys read a line of one key, then that line of the other: of the first load an
   // even lane has its key's first half and an odd lane the other key's second half, and of the second load the reverse.
@@ -378,28 +379,48 @@ struct Walk {
     for (int u = 0; u < KU; ++u)
 #pragma unroll
       for (int s = 0; s < KS; ++s) kf[u][s] = kvec{};   // without a tile: else the last item's are kept for this
+    // the bias by bucket and row, and the buckets by distance, where the waves' parts go later, requested beside the page and
+    // many at once (one by one, 46 x 7 tokens of 32/4 heads and 65 buckets took 18 us, so 16).  Past the last one it again, to
+    // the same place.
+    float* bias = reinterpret_cast<float*>(lds);                         // [buckets][16 RB]
+    uint8_t* buckets = reinterpret_cast<uint8_t*>(bias + 256 * 16 * RB);   // [2 radius + 1]
+    if (a.table) {
+      int self = threadIdx.x;
+      asm volatile("" : "+v"(self));
+      const int r = self % (16 * RB), head = hk * a.G + (row0 + r) % a.G;
+#pragma unroll 1
+      for (int n = 0; n * 8 * STEP < a.nb || n * 4 * 64 * W <= 2 * a.radius; ++n) {
+        int e[8], d[4];
+        uint8_t y[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          d[k] = min((4 * n + k) * 64 * W + self, 2 * a.radius);
+          y[k] = a.buckets[d[k]];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) e[k] = min((8 * n + k) * STEP + self / (16 * RB), a.nb - 1);
+        const auto fill = [&](auto* table) {
+          std::decay_t<decltype(*table)> x[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x[k] = table[e[k] * a.H + head];
+          __builtin_amdgcn_sched_barrier(0);   // all requested before the first is waited for
+#pragma unroll
+          for (int k = 0; k < 8; ++k) bias[e[k] * 16 * RB + r] = bias_log2((float)x[k]);
+        };
+        if (a.table_bf16)
+          fill(static_cast<const bf16*>(a.table));
+        else
+          fill(static_cast<const float*>(a.table));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) buckets[d[k]] = min(y[k], (uint8_t)(a.nb - 1));
+      }
+    }
     if (t < t1) {
       there = locate(t, page, length);
       load_k();
       page = page_of(table, after(t));
     }
-    // the bias by bucket and row, and the buckets by distance, where the waves' parts go later
-    float* bias = reinterpret_cast<float*>(lds);                         // [buckets][n_rows]
-    uint8_t* buckets = reinterpret_cast<uint8_t*>(bias + 256 * 16 * RB);   // [2 radius + 1]
-    if (a.table) {
-      int self = threadIdx.x;
-      asm volatile("" : "+v"(self));
-#pragma unroll 1
-      for (int e = self; e < a.nb * n_rows; e += 64 * W) {
-        const int bucket = e / n_rows, head = hk * a.G + (row0 + e - bucket * n_rows) % a.G;
-        const int64_t at = (int64_t)bucket * a.H + head;
-        bias[e] = bias_log2(a.table_bf16 ? (float)static_cast<const bf16*>(a.table)[at]
-                                         : static_cast<const float*>(a.table)[at]);
-      }
-#pragma unroll 1
-      for (int e = self; e <= 2 * a.radius; e += 64 * W) buckets[e] = (uint8_t)min((int)a.buckets[e], a.nb - 1);
-      __syncthreads();
-    }
+    if (a.table) __syncthreads();
 
     f32x4 acc[RB][VC];
     float top[RB], ref[RB], l[RB];
@@ -456,17 +477,31 @@ struct Walk {
       }
       if (a.table) {
         const int rel0 = j0 - first;   // the first key from the first query
-        const bool far = rel0 - (a.Nq - 1) >= a.radius || rel0 + KEYS - 1 <= -a.radius;
+        const auto bucket_of = [&](int rel) { return (int)buckets[min(max(rel, -a.radius), a.radius) + a.radius]; };
+        if (rel0 - (a.Nq - 1) >= a.radius || rel0 + KEYS - 1 <= -a.radius) {   // all of one bucket
+          const float* one = bias + bucket_of(rel0) * (16 * RB) + m;
 #pragma unroll
-        for (int q = 0; q < RB; ++q)
+          for (int q = 0; q < RB; ++q)
 #pragma unroll
-          for (int u = 0; u < KU; ++u)
+            for (int u = 0; u < KU; ++u)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int rel = far ? rel0 : j0 + 16 * u + 4 * h + r - pos[q];
-              const int bucket = buckets[min(max(rel, -a.radius), a.radius) + a.radius];
-              x[q][u][r] += bias[bucket * n_rows + min(16 * q + m, n_rows - 1)];
-            }
+              for (int r = 0; r < 4; ++r) x[q][u][r] += one[16 * q];
+        } else {
+          int bucket[RB][KU][4];
+#pragma unroll
+          for (int q = 0; q < RB; ++q)
+#pragma unroll
+            for (int u = 0; u < KU; ++u)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) bucket[q][u][r] = bucket_of(j0 + 16 * u + 4 * h + r - pos[q]);
+          __builtin_amdgcn_sched_barrier(0);   // all of them requested before the first is waited for
+#pragma unroll
+          for (int q = 0; q < RB; ++q)
+#pragma unroll
+            for (int u = 0; u < KU; ++u)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) x[q][u][r] += bias[bucket[q][u][r] * (16 * RB) + 16 * q + m];
+        }
       }
 #pragma unroll
       for (int q = 0; q < RB; ++q) {
@@ -783,13 +818,18 @@ Plan plan(const AttnArgs& a, const bioemu_paged_cache& c, bool f32) {
   // what a walk of one workgroup takes no longer than parts and the join: up to 1024 keys of 64 values in bf16 (in a graph
   // 8.4 us for 512 and 11.0 for 1024; in parts 9.8 and 10.0, and a second launch)
   if (most * std::max(a.D, 64) * (f32 ? 4 : 2) <= 1024 * 64 * 2 || p.items >= 16 * attn_units()) {
-    // with workgroups to spare eight waves share a walk (sixteen, where registers allow it, start 1.5 us later: 12.9 us for
-    // one token over 773 keys of 16 heads of 64, 11.3 with eight, 17 with four)
-    if ((p.once || p.rb == 1) && p.items <= 2 * attn_units() && (f32 || a.cap <= kFastCap)) p.waves = 8;
+    // With a CU for each, eight waves share a walk (sixteen, where registers allow it, start 1.5 us later: 12.9 us for one
+    // token over 773 keys of 16 heads of 64, 11.3 with eight, 17 with four).  Two of eight do not fit a CU, two of four do:
+    // 273 items of 64 values, 13 keys 6.1 us by four and 10.2 by eight, 1000 keys 18.4 and 23.8.
+    if ((p.once || p.rb == 1) && p.items <= attn_units() && (f32 || a.cap <= kFastCap)) p.waves = 8;
     return p;
   }
-  // two a CU: with three or four, where registers allow them, 64 sequences of 4096 keys took 206 us, with these 184
-  p.groups = 2 * attn_units();
+  // Two a CU: with three or four, where registers allow them, 64 sequences of 4096 keys took 206 us, with these 184.  Four
+  // where heads are narrow, so that enough is requested at once, and shares of some length: 64 sequences of 2000 keys of 16
+  // heads of 24 37 us (with two 42), in fp32 75 to 82 (87), but 8 of 8000 keys of 4 heads of 32, eight tiles a share, 15.3
+  // (14.6).
+  const bool four = a.D <= 32 && p.rb == 1 && p.items * most >= 4 * attn_units() * 16 * (f32 ? 16 : 32);
+  p.groups = (four ? 4 : 2) * attn_units();
   p.least = p.waves;
   p.slots = p.groups + p.items;
   return p;

@@ -177,6 +177,26 @@ def test_many_sequences(gpu_device):
     Case(lengths * 4, H=8, Hk=8, D=16, width=90).check()   # so many that none is split
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B,H,keys", [(43, 6, 20), (73, 7, 90), (37, 7, 9)])
+def test_more_walks_than_units(gpu_device, dtype, B, H, keys):
+    Case([1 + i * keys % 97 % keys for i in range(B)], dtype, H=H, Hk=H, D=64, radius=8).check()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("slots_first", [False, True])
+def test_long_walks_of_narrow_heads(gpu_device, dtype, slots_first):
+    Case([17011, 40], dtype, H=16, Hk=16, D=24, slots_first=slots_first).check()
+    Case([17011, 0, 9000, 15], dtype, H=16, Hk=8, D=32, page=20, radius=100, slots_first=slots_first).check()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("H,Hk,Nq", [(1, 1, 1), (40, 1, 1), (12, 2, 3), (9, 3, 11)])
+@pytest.mark.parametrize("radius,num_buckets", [(0, None), (127, None), (512, 256), (300, 8)])
+def test_bias_tables(gpu_device, dtype, H, Hk, Nq, radius, num_buckets):
+    Case([1100, 3, 300], dtype, H=H, Hk=Hk, Nq=Nq, radius=radius, num_buckets=num_buckets, tdtype=F32).check()
+
+
 def test_one_long_sequence(gpu_device):
     for dtype in (BF16, F32):
         Case([70001], dtype, H=2, Hk=1, D=64, page=64).check()
