@@ -15,9 +15,9 @@
 // then rounded once.
 //
 // Reading the keys and values bounds it; a stream of 2 GB is read at 6.2 TB/s.  Measured, join included, in bf16: 8 tokens
-// over 8200 to 32768 keys, 32/8 heads of 128, 117 us (6.1 TB/s); 64 over up to 4000, 32/4 heads of 128, 65 us (4.9).
+// over 8200 to 32768 keys, 32/8 heads of 128, 116 us (6.2 TB/s); 64 over up to 4000, 32/4 heads of 128, 65 us (4.8).
 // Short caches take the latency of a walk, memory read after memory read (lengths, page table, keys): one token over 773
-// keys of 16 heads of 64, 11 us; in fp32 4 x 5 tokens over up to 5000, 16/4 heads of 64, 16 us and a join of 4.
+// keys of 16 heads of 64, 10 us; in fp32 4 x 5 tokens over up to 5000, 16/4 heads of 64, 15 us and a join of 5.
 #include <algorithm>
 
 #include "attn.h"
@@ -36,12 +36,12 @@ struct PagedArgs {
   int pages, page_size, table_width, blocks;   // blocks of rows a key head
   unsigned div_mul, div_shift;                  // key / page_size = key * div_mul >> div_shift, for keys below 2^28
   bool even;                                    // pages are whole blocks of 16 keys
-  int groups, least;                            // workgroups that share the keys, of `least` tiles at least; 0: one an item
+  int groups, least;                            // workgroups at a time, parts of `least` tiles at least; 0: one an item
 };
 
 struct Parts {
   float *o, *ml;   // [slots][rows][D], [slots][rows][2]
-  int* range;      // [items][2]: the first and last workgroup of an item
+  int* range;      // [items][2]: the first and last part of an item
 };
 
 template <class T>
@@ -100,25 +100,25 @@ __device__ __forceinline__ int scan(int x) {
   return x;
 }
 
-// A workgroup's share of the tiles of all items (their number is below 2^31): `left` of them, the first being tile t0 of
-// item `item` of sequence b.  Every wave by itself.  Two ways of dealing them:
-// long walks: all tiles, one item behind the other, in equal shares, whatever the sequences' lengths;
-// short ones: every item in equal parts of its own, at most `part` tiles, so that no share has two items' ends: what an
-// item's start and end cost, some kItemCost tiles' time, is then more than what the shares are longer.  (In a graph, one
-// token over 773 keys of 16 heads of 64: 13.4 us by the first way, 9.9 by the second; 64 over up to 4000 keys, four key
-// heads of 128: 73 and 86.)
-struct Share {
-  int b, item, t0, left, w;   // w: the share's number
+// A workgroup's part of an item (a block of rows of a key head of a sequence): tiles t0 .. t0 + n - 1 of item `item` of
+// sequence b; n = 0: none.  Every wave by itself, from the sequences' lengths.  Every item is cut into equal parts, the
+// shortest with which all parts run at once, unless they would be kMost tiles longer than an equal share of all the work (or
+// have to be looked for in more lengths than a wave has lanes): then kLonger longer, and the last parts start late.  Parts of
+// equal length that begin in one item and end in the next cost more.  (In a graph, with such parts, and with parts 16, 24 and
+// 48 tiles longer: 48 sequences of up to 2000 keys, 8 key heads of 128, 61 us, 51, 47 and 54; 32 of up to 2048, 46, 34, 36
+// and 36; 100 of up to 3000, 4 key heads, 74, 68, 65 and 65; 56 of up to 2000, 8 key heads of 80, 61, 42, 42 and 38.)
+struct Part {
+  int b, item, t0, n, w;   // w: the part's number
 };
-constexpr int kItemCost = 16;
-// Shares in order over the XCDs (workgroup i runs on XCD i % 8): neighbours, which may read parts of the same cache lines
+constexpr int kLonger = 24, kMost = 48;
+// Parts in order over the XCDs (workgroup i runs on XCD i % 8): neighbours, which may read parts of the same cache lines
 // or the same keys for other rows, get one L2.  -1: none.
 __device__ __forceinline__ int xcd_order(int n) {
   const int per = (n + kAttnXcds - 1) / kAttnXcds, i = blockIdx.x / kAttnXcds, w = blockIdx.x % kAttnXcds * per + i;
   return i < per && w < n ? w : -1;
 }
 template <int KEYS>
-__device__ __forceinline__ Share share_of(const PagedArgs& p, int B, int items) {
+__device__ __forceinline__ Part part_of(const PagedArgs& p, int B, int items) {
   const int lane = threadIdx.x & 63, groups = p.groups;
   int total = 0, live = 0, sums = 0, own = 0;
   for (int b0 = 0; b0 < B; b0 += 64) {
@@ -129,39 +129,45 @@ __device__ __forceinline__ Share share_of(const PagedArgs& p, int B, int items) 
   }
   total *= items;
   live *= items;
-  const Share none{0, 0, 0, 0, 0};
-  const unsigned spare = max(groups - live, 1), part = max(((unsigned)total + spare - 1) / spare, (unsigned)p.least);
-  const unsigned each = (unsigned)total / (unsigned)groups;
-  const bool parts = live < groups && part < each + kItemCost;
-  int n = groups;
-  if (parts) {
-    n = 0;
+  const unsigned spare = max(groups - live, 1), even = ((unsigned)total + spare - 1) / spare, each = (unsigned)total / groups;
+  unsigned part = max(min(even, each + kLonger), (unsigned)p.least);
+  const auto count = [&]() {   // parts: at most `groups` and one an item
+    int n = 0;
     for (int b0 = 0; b0 < B; b0 += 64) {
       if (B > 64) own = b0 + lane < B ? tiles_of<KEYS>(p, b0 + lane) : 0;
       sums = scan(((unsigned)own + part - 1) / part);
       n += __builtin_amdgcn_readlane(sums, 63);
     }
-    n *= items;
+    return n;
+  };
+  if (B <= 64 && even > each + each / 6 + 4 && part > (unsigned)p.least) {   // else the search gains nothing
+    unsigned fits = 0;
+    for (int step = kMost / 2, longer = kMost; step > 1; step /= 2) {
+      part = max(each + longer, (unsigned)p.least);
+      const bool ok = count() * items <= groups;
+      if (ok) fits = part;
+      else if (longer == kMost) break;
+      longer += ok ? -step : step;
+    }
+    part = fits ? fits : each + kLonger;
   }
+  int n = count();
+  n *= items;
   const int w = xcd_order(n);
+  const Part none{0, 0, 0, 0, 0};
   if (w < 0) return none;
-  // where the share starts, in tiles, or the number of the part
-  const int more = total - (int)each * groups, at = parts ? w : w * (int)each + min(w, more);
   int before = 0, b = 0;
   for (;; b += 64) {
     if (B > 64) own = b + lane < B ? tiles_of<KEYS>(p, b + lane) : 0;
-    int mine = own;
-    if (parts) mine = ((unsigned)own + part - 1) / part;
+    const int mine = ((unsigned)own + part - 1) / part;
     if (B > 64) sums = scan(mine);
-    const uint64_t past = __ballot(before + sums * items > at);
+    const uint64_t past = __ballot(before + sums * items > w);
     if (past) {
       const int l = __ffsll((unsigned long long)past) - 1;
-      b += l;
       before += __builtin_amdgcn_readlane(sums - mine, l) * items;
-      const unsigned in = at - before, n = __builtin_amdgcn_readlane(mine, l), item = in / n;
-      if (!parts) return {b, (int)item, (int)(in - item * n), (int)each + (w < more), w};
-      const unsigned tiles = __builtin_amdgcn_readlane(own, l), i = in - item * n, size = tiles / n, rest = tiles - size * n;
-      return {b, (int)item, (int)(i * size + min(i, rest)), (int)(size + (i < rest)), w};
+      const unsigned in = w - before, of = __builtin_amdgcn_readlane(mine, l), item = in / of, i = in - item * of;
+      const unsigned tiles = __builtin_amdgcn_readlane(own, l), size = tiles / of, rest = tiles - size * of;
+      return {b + l, (int)item, (int)(i * size + min(i, rest)), (int)(size + (i < rest)), w};
     }
     before += __builtin_amdgcn_readlane(sums, 63) * items;
     if (b + 64 >= B) return none;   // not with lengths that stay
@@ -375,10 +381,6 @@ struct Walk {
     // keys, values and the page after next are requested as soon as there is room; behind the last tile it once more (a
     // load that may not be made would have to be waited for at once)
     const auto after = [&](int t) { return t + W < t1 ? t + W : t; };
-#pragma unroll
-    for (int u = 0; u < KU; ++u)
-#pragma unroll
-      for (int s = 0; s < KS; ++s) kf[u][s] = kvec{};   // without a tile: else the last item's are kept for this
     // the bias by bucket and row, and the buckets by distance, where the waves' parts go later, requested beside the page and
     // many at once (one by one, 46 x 7 tokens of 32/4 heads and 65 buckets took 18 us, so 16).  Past the last one it again, to
     // the same place.
@@ -630,7 +632,6 @@ struct Walk {
         }
       }
     }
-    __syncthreads();
   }
 };
 
@@ -641,16 +642,15 @@ constexpr int lds_bytes() {
   return parts > bias ? parts : bias;
 }
 
-// An item is a block of rows of a key head of a sequence.  Without groups a workgroup takes an item; with them the tiles
-// of all items, one behind the other, are dealt evenly to the workgroups, whatever the sequences' lengths: a workgroup's
-// share of an item is its part (workgroup + item) of the join, or the whole, which is written at once.
+// Without groups a workgroup takes an item; with them a part of one, for the join, or the whole, which is written at once.
 template <class T, int DP, int RB, int CAP, int W, bool EVEN, bool ONCE>
 __global__ __launch_bounds__(64 * W, 2) void paged_kernel(const AttnArgs a, const PagedArgs p, T* __restrict__ out,
                                                           Parts parts) {
   constexpr int KEYS = Cache<T>::KEYS;
   __shared__ __attribute__((aligned(16))) char lds[lds_bytes<DP, RB, W>()];
   const int items = a.Hk * p.blocks;   // of a sequence
-  Share s;
+  Part s;
+  int64_t slot = -1;
   if (p.groups == 0) {
     const int w = xcd_order(a.B * items);
     if (w < 0) return;
@@ -665,31 +665,21 @@ __global__ __launch_bounds__(64 * W, 2) void paged_kernel(const AttnArgs a, cons
       return;
     }
   } else {
-    s = share_of<KEYS>(p, a.B, items);
-  }
-  while (s.left > 0) {
-    const int tiles = __builtin_amdgcn_readfirstlane(tiles_of<KEYS>(p, s.b));
-    if (s.item == items || tiles == 0) {
-      s.item = 0;
-      if (++s.b >= a.B) return;
-      continue;
-    }
-    const int t1 = min(tiles, s.t0 + s.left);
-    const int64_t item = (int64_t)s.b * items + s.item, slot = s.t0 == 0 && t1 == tiles ? -1 : s.w + item;
-    if (p.groups && threadIdx.x == 0) {
+    s = part_of<KEYS>(p, a.B, items);
+    if (s.n == 0) return;
+    const int tiles = tiles_of<KEYS>(p, s.b);
+    const int64_t item = (int64_t)s.b * items + s.item;
+    if (s.n < tiles) slot = s.w;
+    if (threadIdx.x == 0) {
       if (s.t0 == 0) parts.range[2 * item] = s.w;
-      if (t1 == tiles) parts.range[2 * item + 1] = s.w;
+      if (s.t0 + s.n == tiles) parts.range[2 * item + 1] = s.w;
     }
-    Walk<T, DP, RB, CAP, W, EVEN, ONCE>(a, p).run(s.b, s.item / p.blocks, s.item % p.blocks * 16 * RB, s.t0, t1, out,
-                                                  parts, slot, lds);
-    s.left -= t1 - s.t0;
-    s.t0 = 0;
-    ++s.item;
   }
+  Walk<T, DP, RB, CAP, W, EVEN, ONCE>(a, p).run(s.b, s.item / p.blocks, s.item % p.blocks * 16 * RB, s.t0, s.t0 + s.n, out,
+                                                parts, slot, lds);
 }
 
-// The parts of a row: those of workgroups first .. last of its item, slot workgroup + item; none where the sequence is
-// empty, one where the result is there already.
+// The parts of a row: first .. last of its item; none where the sequence is empty, one where the result is there already.
 struct RowParts {
   int64_t row0;   // of the first part
   int n, stride;
@@ -703,7 +693,7 @@ __device__ __forceinline__ RowParts row_parts(const AttnArgs& a, const PagedArgs
   const int stride = min(a.Nq * a.G, block_rows);
   const int first = parts.range[2 * item], last = parts.range[2 * item + 1];   // not set where the sequence is empty
   if (tiles_of<KEYS>(p, b) == 0) return {0, 0, stride};
-  return {(first + item) * stride + r - blk * block_rows, last - first + 1, stride};
+  return {(int64_t)first * stride + r - blk * block_rows, last - first + 1, stride};
 }
 
 // Parts w, w + step, ... of a row added in order, four at a time and in one pass; N values of each.
@@ -825,13 +815,13 @@ Plan plan(const AttnArgs& a, const bioemu_paged_cache& c, bool f32) {
     return p;
   }
   // Two a CU: with three or four, where registers allow them, 64 sequences of 4096 keys took 206 us, with these 184.  Four
-  // where heads are narrow, so that enough is requested at once, and shares of some length: 64 sequences of 2000 keys of 16
-  // heads of 24 37 us (with two 42), in fp32 75 to 82 (87), but 8 of 8000 keys of 4 heads of 32, eight tiles a share, 15.3
-  // (14.6).
+  // where heads are narrow, so that enough is requested at once, and parts are of some length: 64 sequences of 2000 keys of 16
+  // heads of 24 37 us (with two 42), in fp32 75 to 82 (87), but 8 of 8000 keys of 4 heads of 32, eight tiles a part,
+  // 15.3 (14.6).
   const bool four = a.D <= 32 && p.rb == 1 && p.items * most >= 4 * attn_units() * 16 * (f32 ? 16 : 32);
   p.groups = (four ? 4 : 2) * attn_units();
   p.least = p.waves;
-  p.slots = p.groups + p.items;
+  p.slots = p.groups + p.items;   // parts at most (see part_of)
   return p;
 }
 
@@ -864,7 +854,7 @@ int launch(const AttnArgs& a, const PagedArgs& p, const Plan& pl, T* out, void* 
   }
   {
     KernelTimerScope timer("paged_attention", stream);
-    const dim3 grid((unsigned)round_up(pl.groups ? pl.groups : pl.items, kAttnXcds));
+    const dim3 grid((unsigned)round_up(pl.groups ? pl.slots : pl.items, kAttnXcds));
     const auto go = [&](auto kernel) { kernel<<<grid, 64 * pl.waves, 0, stream>>>(a, p, out, parts); };
     const bool wide = !fast_cap<T>(a);
     // few calls have a wide cap: one form for them

@@ -61,7 +61,8 @@ def paged_attention(q: Tensor, keys: Tensor, values: Tensor, page_table: Tensor,
     q: [B, Nq, H, D] in the cache's type (or fp32 under bf16 autocast over a bf16 cache), H a multiple of the cache's Hk,
     D a multiple of 8 up to 128; row i of sequence b is at position ``lengths[b] - counts[b] + i`` (counts: Nq by
     default) and sees the keys up to its own (all of the sequence's, not causal); padding rows and rows that see nothing
-    give zeros.  Made for a few rows a sequence: keys are read once for every 32 rows of queries times H / Hk.
+    give zeros.  Made for a few rows a sequence: keys are read once for every 32 rows of queries times H / Hk (past some 256
+    rows ``attention`` over keys laid side by side is faster, the copy included).
     Keys whose table entry names no page are not seen; what unused slots hold does not matter.
     Values that are not finite reach the rows that see them, and no others.
     scale, cap, bias_table, bias_buckets: as in ``attention``.  The table's width times the page size is at most 2^27, and

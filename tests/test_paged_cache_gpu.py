@@ -197,6 +197,15 @@ def test_bias_tables(gpu_device, dtype, H, Hk, Nq, radius, num_buckets):
     Case([1100, 3, 300], dtype, H=H, Hk=Hk, Nq=Nq, radius=radius, num_buckets=num_buckets, tdtype=F32).check()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B,D,most", [(24, 64, 3000), (48, 24, 2500), (64, 32, 1500), (65, 64, 1500), (33, 128, 1100)])
+def test_parts_of_unequal_lengths(gpu_device, dtype, B, D, most):
+    g = torch.Generator().manual_seed(B)
+    lengths = torch.randint(0, most, (B,), generator=g).tolist()
+    lengths[B // 2], lengths[1] = most, 0
+    Case(lengths, dtype, H=8, Hk=8, D=D).check()
+
+
 def test_one_long_sequence(gpu_device):
     for dtype in (BF16, F32):
         Case([70001], dtype, H=2, Hk=1, D=64, page=64).check()
