@@ -101,12 +101,13 @@ __device__ __forceinline__ int scan(int x) {
 }
 
 // A workgroup's part of an item (a block of rows of a key head of a sequence): tiles t0 .. t0 + n - 1 of item `item` of
-// sequence b; n = 0: none.  Every wave by itself, from the sequences' lengths.  Every item is cut into equal parts, the
-// shortest with which all parts run at once, unless they would be kMost tiles longer than an equal share of all the work (or
-// have to be looked for in more lengths than a wave has lanes): then kLonger longer, and the last parts start late.  Parts of
-// equal length that begin in one item and end in the next cost more.  (In a graph, with such parts, and with parts 16, 24 and
-// 48 tiles longer: 48 sequences of up to 2000 keys, 8 key heads of 128, 61 us, 51, 47 and 54; 32 of up to 2048, 46, 34, 36
-// and 36; 100 of up to 3000, 4 key heads, 74, 68, 65 and 65; 56 of up to 2000, 8 key heads of 80, 61, 42, 42 and 38.)
+// sequence b; n = 0: none. Every wave by itself, from the sequences' lengths. Every item is cut into equal parts, the
+// shortest with which all parts run at once, unless they would be kMost tiles longer than an equal share of all the
+// work (or have to be looked for in more lengths than a wave has lanes): then kLonger longer, and the last parts start
+// late. Parts of equal length that begin in one item and end in the next cost more. (In a graph, with such parts, and
+// with parts 16, 24 and 48 tiles longer: 48 sequences of up to 2000 keys, 8 key heads of 128, 61 us, 51, 47 and 54; 32
+// of up to 2048, 46, 34, 36 and 36; 100 of up to 3000, 4 key heads, 74, 68, 65 and 65; 56 of up to 2000, 8 key heads of
+// 80, 61, 42, 42 and 38.)
 struct Part {
   int b, item, t0, n, w;   // w: the part's number
 };
@@ -182,10 +183,11 @@ struct Walk {
   static constexpr int VK = KEYS / 4;   // keys whose values a lane loads
   static constexpr int STEP = 64 * W / (16 * RB);   // threads to a row of the block
   // Four lanes' pieces of a key are 64 bytes, half a cache line, and a second load of the line would wait for the first
-  // one's in the cache.  So the lanes of two keys read a line of one key, then that line of the other: of the first load an
-  // even lane has its key's first half and an odd lane the other key's second half, and of the second load the reverse.
-  // The first halves make one product, the second halves another, whose rows (keys) are then swapped in pairs.  (One token
-  // over 773 keys of 16 heads of 64: 11.4 us, 11.9 by halves; 64 over up to 4000, 72 and 73.  In fp32 it gains nothing.)
+  // one's in the cache. So the lanes of two keys read a line of one key, then that line of the other: of the first
+  // load an even lane has its key's first half and an odd lane the other key's second half, and of the second load the
+  // reverse. The first halves make one product, the second halves another, whose rows (keys) are then swapped in
+  // pairs. (One token over 773 keys of 16 heads of 64: 11.4 us, 11.9 by halves; 64 over up to 4000, 72 and 73. In
+  // fp32 it gains nothing.)
   static constexpr bool LINES = sizeof(T) == 2 && KS % 2 == 0;
   static constexpr unsigned kAll = KEYS == 32 ? 0xffffffffu : 0xffffu;
   typedef T kvec __attribute__((ext_vector_type(KL)));
@@ -225,8 +227,8 @@ struct Walk {
     const int at = page_index(t * KEYS + (lane & (KEYS - 1)));
     return at < p.table_width ? table[at] : -1;
   }
-  // Which of a tile's keys are there, and where they lie.  Sixteen keys of one page: where their rows begin, for all lanes;
-  // else each lane's own key, shared as it is loaded.  Keys of no page are read as the first page's.
+  // Which of a tile's keys are there, and where they lie. Sixteen keys of one page: where their rows begin, for all
+  // lanes; else each lane's own key, shared as it is loaded. Keys of no page are read as the first page's.
   __device__ __forceinline__ unsigned locate(int t, int page, int length) {
     const int j = t * KEYS + (lane & (KEYS - 1));
     const bool ok = j < length && (unsigned)page < (unsigned)p.pages;
@@ -381,9 +383,9 @@ struct Walk {
     // keys, values and the page after next are requested as soon as there is room; behind the last tile it once more (a
     // load that may not be made would have to be waited for at once)
     const auto after = [&](int t) { return t + W < t1 ? t + W : t; };
-    // the bias by bucket and row, and the buckets by distance, where the waves' parts go later, requested beside the page and
-    // many at once (one by one, 46 x 7 tokens of 32/4 heads and 65 buckets took 18 us, so 16).  Past the last one it again, to
-    // the same place.
+    // the bias by bucket and row, and the buckets by distance, where the waves' parts go later, requested beside the
+    // page and many at once (one by one, 46 x 7 tokens of 32/4 heads and 65 buckets took 18 us, so 16). Past the last
+    // one it again, to the same place.
     float* bias = reinterpret_cast<float*>(lds);                         // [buckets][16 RB]
     uint8_t* buckets = reinterpret_cast<uint8_t*>(bias + 256 * 16 * RB);   // [2 radius + 1]
     if (a.table) {
@@ -642,7 +644,8 @@ constexpr int lds_bytes() {
   return parts > bias ? parts : bias;
 }
 
-// Without groups a workgroup takes an item; with them a part of one, for the join, or the whole, which is written at once.
+// Without groups a workgroup takes an item; with them a part of one, for the join, or the whole, which is written at
+// once.
 template <class T, int DP, int RB, int CAP, int W, bool EVEN, bool ONCE>
 __global__ __launch_bounds__(64 * W, 2) void paged_kernel(const AttnArgs a, const PagedArgs p, T* __restrict__ out,
                                                           Parts parts) {
@@ -729,8 +732,8 @@ struct Sum {
   }
 };
 
-// paged_join: few rows of many parts, a workgroup a row: wave w takes parts w, w + waves, ..., then the waves are added in
-// order.  Lane d holds values d and 64 + d.
+// paged_join: few rows of many parts, a workgroup a row: wave w takes parts w, w + waves, ..., then the waves are added
+// in order. Lane d holds values d and 64 + d.
 constexpr int kJoinWaves = 8;
 template <class T, int KEYS>
 __global__ __launch_bounds__(64 * kJoinWaves) void paged_join_kernel(const AttnArgs a, const PagedArgs p,
@@ -805,19 +808,19 @@ Plan plan(const AttnArgs& a, const bioemu_paged_cache& c, bool f32) {
   p.items = (int64_t)a.B * a.Hk * p.blocks;
   p.once = p.blocks == 1 && a.D * (f32 ? 4 : 2) % 128 == 0;
   const int64_t most = c.pages > 0 ? c.table_width * c.page_size : 0;
-  // what a walk of one workgroup takes no longer than parts and the join: up to 1024 keys of 64 values in bf16 (in a graph
-  // 8.4 us for 512 and 11.0 for 1024; in parts 9.8 and 10.0, and a second launch)
+  // what a walk of one workgroup takes no longer than parts and the join: up to 1024 keys of 64 values in bf16 (in a
+  // graph 8.4 us for 512 and 11.0 for 1024; in parts 9.8 and 10.0, and a second launch)
   if (most * std::max(a.D, 64) * (f32 ? 4 : 2) <= 1024 * 64 * 2 || p.items >= 16 * attn_units()) {
-    // With a CU for each, eight waves share a walk (sixteen, where registers allow it, start 1.5 us later: 12.9 us for one
-    // token over 773 keys of 16 heads of 64, 11.3 with eight, 17 with four).  Two of eight do not fit a CU, two of four do:
-    // 273 items of 64 values, 13 keys 6.1 us by four and 10.2 by eight, 1000 keys 18.4 and 23.8.
+    // With a CU for each, eight waves share a walk (sixteen, where registers allow it, start 1.5 us later: 12.9 us for
+    // one token over 773 keys of 16 heads of 64, 11.3 with eight, 17 with four). Two of eight do not fit a CU, two of
+    // four do: 273 items of 64 values, 13 keys 6.1 us by four and 10.2 by eight, 1000 keys 18.4 and 23.8.
     if ((p.once || p.rb == 1) && p.items <= attn_units() && (f32 || a.cap <= kFastCap)) p.waves = 8;
     return p;
   }
-  // Two a CU: with three or four, where registers allow them, 64 sequences of 4096 keys took 206 us, with these 184.  Four
-  // where heads are narrow, so that enough is requested at once, and parts are of some length: 64 sequences of 2000 keys of 16
-  // heads of 24 37 us (with two 42), in fp32 75 to 82 (87), but 8 of 8000 keys of 4 heads of 32, eight tiles a part,
-  // 15.3 (14.6).
+  // Two a CU: with three or four, where registers allow them, 64 sequences of 4096 keys took 206 us, with these 184.
+  // Four where heads are narrow, so that enough is requested at once, and parts are of some length: 64 sequences of
+  // 2000 keys of 16 heads of 24 37 us (with two 42), in fp32 75 to 82 (87), but 8 of 8000 keys of 4 heads of 32, eight
+  // tiles a part, 15.3 (14.6).
   const bool four = a.D <= 32 && p.rb == 1 && p.items * most >= 4 * attn_units() * 16 * (f32 ? 16 : 32);
   p.groups = (four ? 4 : 2) * attn_units();
   p.least = p.waves;
@@ -920,7 +923,8 @@ extern "C" int bioemu_paged_attention(const bioemu_paged_cache* cache, const bio
     return set_error(BIOEMU_ERR_WORKSPACE, "paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   const int item = args->f32 ? 4 : 2;
   const int64_t *ks = cache->keys_stride, *vs = cache->values_stride;
-  // key / page_size: 2^(28 + l) / page_size rounded up, l = log2 of page_size rounded up, is off by less than 2^l / page_size
+  // key / page_size: 2^(28 + l) / page_size rounded up, l = log2 of page_size rounded up, is off by less than 2^l /
+  // page_size
   unsigned l = 0;
   while ((int64_t(1) << l) < cache->page_size) ++l;
   const unsigned mul = (unsigned)(((int64_t(1) << (28 + l)) + cache->page_size - 1) / cache->page_size);
