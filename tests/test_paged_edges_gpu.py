@@ -1,0 +1,68 @@
+"""Edges of rotary positions and the paged cache against float64: the table's end, numbers of 64 bits, caches that share
+memory, workgroups of several sequences or of more values than their threads hold at once.  Bounds as derived in the
+files of the operators' other tests."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+from test_paged_cache_gpu import Case, _close, _turned
+from test_rotary_gpu import check, exact, rand
+
+from bioemu2_amd.paged_cache import paged_append
+from bioemu2_amd.rotary import rotary, rotary_frequencies
+
+pytestmark = pytest.mark.gpu
+BF16, F32, I32 = torch.bfloat16, torch.float32, torch.int32
+
+
+# ----------------------------------------------------------------------------
+# More than the threads of a workgroup hold at once, and several sequences in one
+# ----------------------------------------------------------------------------
+MANY = [  # B, N, H, Hk, D, rot
+    (1, 3, 64, 2, 128, 6),        # an odd number of pairs: pieces of one pair, 4224 of them a token
+    (2, 1, 48, 8, 512, 512), (1, 2, 40, 24, 512, 20),
+    (3, 1001, 3, 1, 24, 24),      # two tokens a workgroup: the sequences' borders inside one, the last of one token
+    (3, 6667, 1, 1, 8, 4)]        # sixteen
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("B,N,H,Hk,D,rot", MANY)
+def test_rotary_by_workgroups(gpu_device, dtype, interleaved, B, N, H, Hk, D, rot):
+    q, k = rand(B, N, H, D, dtype=dtype), rand(B, N, Hk, D, dtype=dtype, seed=1)
+    pos = torch.randint(-5000, 5000, (B, N), generator=torch.Generator().manual_seed(N), dtype=I32).cuda()
+    f = rotary_frequencies(rot, device="cuda")
+    for at in (pos, None):
+        y = rotary(q, k, at, f, interleaved=interleaved, magnitude=1.25)
+        check(y[0], exact(q, at, f, interleaved, 1.25))
+        check(y[1], exact(k, at, f, interleaved, 1.25))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("B,N,H,Hk,D,rot", MANY)
+def test_append_by_workgroups(gpu_device, dtype, interleaved, B, N, H, Hk, D, rot):
+    page = 20
+    counts = [N, N // 2, max(N - 3, 0)][:B]
+    lengths = [N + 45, N // 2 + 7, N][:B]
+    q, k, v = (rand(B, N, h, D, dtype=dtype, seed=s) for s, h in enumerate((H, Hk, Hk)))
+    used = [-(-n // page) for n in lengths]
+    order = torch.randperm(sum(used) + 1, generator=torch.Generator().manual_seed(N))
+    table = torch.full((B, max(used)), -1, dtype=I32)
+    for b in range(B):
+        table[b, :used[b]] = order[sum(used[:b]):sum(used[:b + 1])].to(I32)
+    keys, values = (rand(sum(used) + 1, page, Hk, D, dtype=dtype, seed=s) for s in (3, 4))
+    k0, v0 = keys.clone(), values.clone()
+    f = rotary_frequencies(rot, device="cuda")
+    got = paged_append(keys, values, k, v, table.cuda(), torch.tensor(lengths, dtype=I32, device="cuda"),
+                       counts=torch.tensor(counts, dtype=I32, device="cuda"), q=q, frequencies=f, interleaved=interleaved,
+                       magnitude=1.5)
+    for b, n in enumerate(counts):
+        pos = torch.arange(lengths[b] - n, lengths[b])
+        at = (table[b][pos // page].long().cuda(), (pos % page).cuda())
+        _close(got[b, :n], _turned(q[b, :n], pos.cuda(), f, interleaved, 1.5))
+        _close(keys[at], _turned(k[b, :n], pos.cuda(), f, interleaved, 1.5))
+        assert torch.equal(values[at], v[b, :n]) and bool((got[b, n:] == 0).all())
+        keys[at], values[at] = k0[at], v0[at]
+    assert torch.equal(keys, k0) and torch.equal(values, v0)     # nothing else was written
