@@ -2,6 +2,7 @@
 //
 //   s(i, j) = cap tanh(scale q_i . k_j / cap) + bias[clamp(j - p_i, -R, R)],   o_i = sum_j softmax_j(s) v_j
 //   p_i = length - count + i, keys j <= p_i (causal) or j < length; key j is slot j % page_size of page table[j / page_size]
+// (none where the table ends)
 //
 // The queries of a group of heads that share a key head are the rows of one operand, up to 32 of them, so every key and
 // value is read once.  A wave takes tiles of 32 keys (bf16) or 16 (fp32), straight from memory into the operands'
@@ -356,7 +357,8 @@ struct Walk {
     const int wave = wave_id(), length = __builtin_amdgcn_readfirstlane(length_of(p, b));
     const int rows = a.Nq * a.G, n_rows = min(rows - row0, 16 * RB);
     const int count = __builtin_amdgcn_readfirstlane(p.counts ? min(max(p.counts[b], 0), a.Nq) : a.Nq);
-    const int first = length - count;   // position of the first query
+    // position of the first query: by the length as given, also where it is past the table (2^30 stands for all beyond it)
+    const int first = __builtin_amdgcn_readfirstlane(min(max(p.lengths[b], 0), 1 << 30)) - count;
     const int* table = p.page_table + b * p.table_stride;
     kbase = (const char*)p.keys + hk * p.khead;
     vbase = (const char*)p.values + hk * p.vhead;

@@ -63,7 +63,8 @@ def paged_attention(q: Tensor, keys: Tensor, values: Tensor, page_table: Tensor,
     default) and sees the keys up to its own (all of the sequence's, not causal); padding rows and rows that see nothing
     give zeros.  Made for a few rows a sequence: keys are read once for every 32 rows of queries times H / Hk (past some 256
     rows ``attention`` over keys laid side by side is faster, the copy included).
-    Keys whose table entry names no page are not seen; what unused slots hold does not matter.
+    Keys whose table entry names no page, or that the table does not reach, are not seen (positions count on past its
+    end); what unused slots hold does not matter.
     Values that are not finite reach the rows that see them, and no others.
     scale, cap, bias_table, bias_buckets: as in ``attention``.  The table's width times the page size is at most 2^27, and
     times B Hk (and, past 32 rows, their blocks) below 2^35."""

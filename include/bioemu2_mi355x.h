@@ -565,7 +565,8 @@ int bioemu_rotary(const bioemu_rotary_args* args, void* q_out, void* k_out, hipS
  * page_table[b * table_stride + p / page_size].  lengths [B]: positions in use,
  * the last counts[b] of them new (counts NULL: as many as the call has rows).
  * A table entry that names no page is not read or written: its keys are not
- * seen.  Lengths past table_width pages are taken as that many; counts into
+ * seen; nor are positions that the table does not reach.  A length past it
+ * counts for the positions of the new rows all the same.  counts are taken into
  * 0 .. rows.
  */
 typedef struct bioemu_paged_cache {

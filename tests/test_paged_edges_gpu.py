@@ -66,3 +66,48 @@ def test_append_by_workgroups(gpu_device, dtype, interleaved, B, N, H, Hk, D, ro
         assert torch.equal(values[at], v[b, :n]) and bool((got[b, n:] == 0).all())
         keys[at], values[at] = k0[at], v0[at]
     assert torch.equal(keys, k0) and torch.equal(values, v0)     # nothing else was written
+
+
+# ----------------------------------------------------------------------------
+# Sequences longer than their table
+# ----------------------------------------------------------------------------
+def _past_the_table(c, width):
+    return [torch.arange(k.shape[0], device="cuda") >= width * c.page for k, _ in c.dense]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("Nq", [1, 4, 40])
+@pytest.mark.parametrize("width", [6, 80])
+def test_positions_past_the_table(gpu_device, dtype, causal, Nq, width):
+    """Queries keep the positions that the lengths give them; only the keys end with the table."""
+    room = 16 * width
+    lengths = [room + 4, room, room + 30, 20, room + 1000]
+    c = Case(lengths, dtype, Nq=Nq, width=width, radius=8, causal=causal, counts=[min(Nq, 8), Nq, Nq, min(Nq, 20), Nq])
+    c.check(hidden=_past_the_table(c, width))
+
+
+def test_lengths_at_the_end_of_32_bits(gpu_device):
+    c = Case([64, 64], Nq=3, page=16, radius=8, counts=[3, 1])
+    c.lengths.fill_(2 ** 31 - 1)
+    far = c.call()
+    c.lengths.fill_(2 ** 20)
+    assert torch.equal(far, c.call())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_append_then_attend_across_the_tables_end(gpu_device, dtype):
+    """Eight new rows of which four have a slot: each row sees what was written up to its own position."""
+    c = Case([100, 60], dtype, Nq=8, width=6, radius=8)
+    keys, values = c.keys.clone(), c.values.clone()
+    k, v = (torch.stack([s[n][-8:] for s in c.dense]) for n in (0, 1))
+    for b, n in enumerate((100, 60)):
+        at = torch.arange(n - 8, min(n, 96), device="cuda")
+        c.keys[c.table[b, at // 16].long(), at % 16] = c.values[c.table[b, at // 16].long(), at % 16] = 0
+    paged_append(c.keys, c.values, k, v, c.table, c.lengths)
+    for got, want in ((c.keys, keys), (c.values, values)):
+        for b, n in enumerate((96, 60)):
+            at = torch.arange(n, device="cuda")
+            where = c.table[b, at // 16].long(), at % 16
+            assert torch.equal(got[where], want[where])
+    c.check(hidden=_past_the_table(c, 6))
