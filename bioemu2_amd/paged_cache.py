@@ -13,7 +13,8 @@ Both take ``lengths`` (positions in use with the new ones) and, for batches of
 unequal rows, ``counts`` (how many of them are new: row i of sequence b is position
 ``lengths[b] - counts[b] + i``, and rows from ``counts[b]`` on are padding).  Table,
 lengths and counts are read on the GPU only, so a captured graph can be replayed
-with other values in them.  No gradients.
+with other values in them.  They are of 32 bits; of 64 they are taken to the nearest
+number of 32, two small kernels for each.  No gradients.
 """
 
 from __future__ import annotations
@@ -26,9 +27,18 @@ from ._lib import torch_op
 from .relative_position import _int32
 
 
+def _nearest_int32(t: Tensor, what: str) -> Tensor:
+    """Whole numbers as the nearest of 32 bits: an entry of 2^32 is past any pool, not the first page."""
+    if t.dtype in (torch.uint32, torch.uint64):
+        t = t.to(torch.int64)
+    if t.dtype != torch.int64:
+        return _int32(t, what)
+    return t.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
+
+
 def _ints(what: str, page_table: Tensor, lengths: Tensor, counts: Tensor | None):
-    return (_int32(page_table, f"{what} page_table"), _int32(lengths, f"{what} lengths"),
-            None if counts is None else _int32(counts, f"{what} counts"))
+    return (_nearest_int32(page_table, f"{what} page_table"), _nearest_int32(lengths, f"{what} lengths"),
+            None if counts is None else _nearest_int32(counts, f"{what} counts"))
 
 
 def paged_append(keys: Tensor, values: Tensor, k: Tensor, v: Tensor, page_table: Tensor, lengths: Tensor, *,
@@ -39,9 +49,9 @@ def paged_append(keys: Tensor, values: Tensor, k: Tensor, v: Tensor, page_table:
     keys, values: [pages, page_size, Hk, D] of k's type (bf16 or fp32; bf16 also for fp32 under bf16 autocast), values of
     a head adjacent, rows at 16-byte addresses, the other dimensions in any order in memory.  page_table: whole numbers of
     32 bits [B, width]; lengths, counts: [B].  With ``frequencies`` k and q are turned as ``rotary`` does, to their
-    positions in the sequence or to ``positions`` ([B, N]).  Padding rows write nothing, and are zeros in the result; nor
-    does a position whose table entry names no page (below 0, past the pool, or past the table).  A slot that a call names
-    twice gets values of both, in any order."""
+    positions in the sequence or to ``positions`` ([B, N], whole numbers that 32 bits hold).  Padding rows write nothing,
+    and are zeros in the result; nor does a position whose table entry names no page (below 0, past the pool, or past the
+    table).  A slot that a call names twice gets values of both, in any order."""
     _ops.require_gpu(k, "paged_append")
     page_table, lengths, counts = _ints("paged_append", page_table, lengths, counts)
     dtype = None if q is None else q.dtype

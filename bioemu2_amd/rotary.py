@@ -60,7 +60,7 @@ def rotary(q: Tensor | None, k: Tensor | None, positions: Tensor | None, frequen
     The first ``2 * len(frequencies)`` values of a head are taken as pairs (a, b): values i and i + len(frequencies), or
     2 i and 2 i + 1 (``interleaved``).  With t = position * frequency: a' = magnitude (a cos t - b sin t), b' =
     magnitude (a sin t + b cos t).  The rest of the head is left alone.
-    positions: whole numbers of 32 bits [B, N] (None: 0, 1, ...); frequencies: 64 bits (``rotary_frequencies``).
+    positions: whole numbers that 32 bits hold [B, N] (None: 0, 1, ...); frequencies: 64 bits (``rotary_frequencies``).
     Either of q and k may be None, and is then None in the result.  D is a multiple of 8 up to 512.  Angles are computed
     in 64 bits: no position is too far.  Gradients: q and k."""
     like = k if q is None else q

@@ -111,3 +111,31 @@ def test_append_then_attend_across_the_tables_end(gpu_device, dtype):
             where = c.table[b, at // 16].long(), at % 16
             assert torch.equal(got[where], want[where])
     c.check(hidden=_past_the_table(c, 6))
+
+
+# ----------------------------------------------------------------------------
+# Numbers of 64 bits
+# ----------------------------------------------------------------------------
+def test_tables_and_lengths_of_64_bits(gpu_device):
+    """What 32 bits do not hold names no page, is past any table, or below every length."""
+    c = Case([64, 100, 32], page=16)
+    table, lengths = c.table.long(), c.lengths.long()
+    table[0, 1], table[1, 0], table[2, 0] = 2 ** 32, 2 ** 33 + 1, -2 ** 32
+    c.table[0, 1] = c.table[1, 0] = c.table[2, 0] = -1
+    lengths[1] += 2 ** 32
+    c.lengths[1] = 2 ** 31 - 1
+    counts = torch.tensor([1, 2 ** 32 + 1, -2 ** 40], device="cuda")
+    c.counts = torch.tensor([1, 1, 0], dtype=I32, device="cuda")
+    want = c.call()
+    c.table, c.lengths, c.counts, want_of = table, lengths, counts, (c.table, c.lengths, c.counts)
+    # as bits: with its length past the table, sequence 1 sees slots that hold NaN
+    assert torch.equal(c.call().view(torch.int16), want.view(torch.int16)) and want[0].isfinite().all()
+    k = torch.ones(3, 1, 2, 32, dtype=BF16, device="cuda")
+    stores = [(c.keys.clone(), c.values.clone()) for _ in range(2)]
+    for (keys, values), (t, n, m) in zip(stores, ((table, lengths, counts), want_of)):
+        t = t.clone()
+        t[0, 3] = t[0, 1]      # the new token's page: none
+        paged_append(keys, values, k, k, t, n, counts=m)
+    for got, want in zip(*stores):
+        assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+    assert torch.equal(stores[0][0].view(torch.int16), c.keys.view(torch.int16))     # nothing was written

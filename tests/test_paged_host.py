@@ -173,3 +173,22 @@ def test_forward_derivatives_are_refused():
         dual = fw.make_dual(x, torch.zeros_like(x))
         with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
             op(dual, None, None, f, False, 1.0, False)
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.uint64, torch.uint32, torch.int32, torch.int16, torch.uint8])
+def test_numbers_that_32_bits_do_not_hold(dtype):
+    """Tables and lengths of 64 bits are taken to the nearest number of 32 bits: 2^32 names no page, not the first."""
+    from bioemu2_amd.paged_cache import _ints
+
+    info = torch.iinfo(dtype)
+    want = [0, 3, 100, max(info.min, -2 ** 31), min(info.max, 2 ** 31 - 1)]
+    have = [0, 3, 100, info.min, info.max if dtype != torch.uint64 else 2 ** 63 - 1]
+    if info.bits == 64:
+        have += [2 ** 32, 2 ** 32 + 3, 2 ** 31]
+        want += [2 ** 31 - 1] * 3
+    for t in _ints("here", *[torch.tensor(have, dtype=dtype)] * 3):
+        assert t.dtype == torch.int32 and t.tolist() == want
+    table = torch.tensor([have, have], dtype=dtype).T
+    assert _ints("here", table, table[:, 0], None)[0].tolist() == [[w, w] for w in want]
+    with pytest.raises(ValueError, match="whole numbers"):
+        _ints("here", table.float(), table[:, 0], None)
