@@ -718,10 +718,51 @@ void check_no_gradients(const char* what, const T&... inputs) {
       const optional<Tensor>&frequencies, const optional<Tensor>&positions, bool interleaved, double magnitude
 #define APPEND_ARGS keys, values, k, v, page_table, lengths, counts, q, frequencies, positions, interleaved, magnitude
 
-// Two slots of one tensor in the same place (a dimension of stride 0) cannot both be written.
-void check_writable(const Tensor& t, const char* what) {
-  for (int d = 0; d < 3; ++d)
-    TORCH_CHECK_VALUE(t.size(d) <= 1 || t.stride(d) > 0, what, ": expanded tensors cannot be appended to");
+// Where the values of a cache lie, in bytes from its first: dimensions of more than one entry, the widest step first.
+struct Places {
+  const char* first;
+  int64_t item, extent, step[4], count[4];   // extent: bytes from the first value to the end of the last
+  int dims = 0;
+
+  // Refuses slots that share memory, which could not both be written (a dimension of step 0 among them): each dimension
+  // has to step over all that lies within it.
+  Places(const Tensor& t, const char* what)
+      : first(static_cast<const char*>(t.data_ptr())), item(t.element_size()), extent(t.numel() ? item : 0) {
+    if (t.numel() == 0) return;
+    for (int d = 0; d < 4; ++d) {
+      if (t.size(d) == 1) continue;
+      int at = dims++;
+      for (; at > 0 && step[at - 1] < t.stride(d) * item; --at) step[at] = step[at - 1], count[at] = count[at - 1];
+      step[at] = t.stride(d) * item;
+      count[at] = t.size(d);
+    }
+    for (int d = dims - 1; d >= 0; --d) {
+      TORCH_CHECK_VALUE(step[d] >= extent, what, ": slots that share memory cannot be appended to (sizes ", t.sizes(),
+                        ", strides ", t.strides(), ")");
+      extent += (count[d] - 1) * step[d];
+    }
+  }
+  // Whether two values lie `off` bytes apart, the difference of their places in dimensions d and on: what is left of off
+  // after a dimension has to be less than its step, which leaves two numbers of steps to try.
+  bool apart_by(int64_t off, int d = 0) const {
+    if (d == dims) return off > -item && off < item;
+    const int64_t n = off / step[d] - (off % step[d] < 0);
+    for (const int64_t k : {n, n + 1})
+      if (k > -count[d] && k < count[d] && apart_by(off - k * step[d], d + 1)) return true;
+    return false;
+  }
+  bool same_steps(const Places& other) const {
+    return dims == other.dims && std::equal(step, step + dims, other.step) && std::equal(count, count + dims, other.count);
+  }
+};
+
+// Keys and values of one allocation may lie between each other, in steps alike, but not in each other's place.
+void check_writable(const Tensor& keys, const Tensor& values) {
+  const Places k(keys, "paged_append keys"), v(values, "paged_append values");
+  if (k.first + k.extent <= v.first || v.first + v.extent <= k.first) return;
+  TORCH_CHECK_VALUE(k.same_steps(v) && !k.apart_by(v.first - k.first),
+                    "paged_append: keys and values share memory, or lie between each other with strides ", keys.strides(),
+                    " and ", values.strides());
 }
 
 Tensor paged_append_cuda(APPEND_PARAMS) {
@@ -738,10 +779,9 @@ Tensor paged_append_cuda(APPEND_PARAMS) {
                       k.scalar_type(), " on ", k.device());
   }
   TORCH_CHECK_VALUE(!positions || frequencies, "paged_append: positions come with frequencies");
-  check_writable(keys, "paged_append keys");
-  check_writable(values, "paged_append values");
   const c10::OptionalDeviceGuard guard(k.device());
   const CacheCall c("paged_append", keys, values, page_table, lengths, counts, k, k.size(2));
+  check_writable(keys, values);
   const int64_t bn[2] = {k.size(0), k.size(1)};
   const optional<Tensor> pos = whole_numbers(positions, "paged_append positions", bn, k);
   Tensor f, qs, out;

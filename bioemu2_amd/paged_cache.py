@@ -47,8 +47,9 @@ def paged_append(keys: Tensor, values: Tensor, k: Tensor, v: Tensor, page_table:
     """Writes k and v ([B, N, Hk, D]) into the pages, in place, and returns q ([B, N, H, D]) turned like k (None without).
 
     keys, values: [pages, page_size, Hk, D] of k's type (bf16 or fp32; bf16 also for fp32 under bf16 autocast), values of
-    a head adjacent, rows at 16-byte addresses, the other dimensions in any order in memory.  page_table: whole numbers of
-    32 bits [B, width]; lengths, counts: [B].  With ``frequencies`` k and q are turned as ``rotary`` does, to their
+    a head adjacent, rows at 16-byte addresses, the other dimensions in any order in memory, no two slots in the same place
+    (parts of one tensor may lie between each other if their strides are alike).  page_table: whole numbers of 32 bits
+    [B, width]; lengths, counts: [B].  With ``frequencies`` k and q are turned as ``rotary`` does, to their
     positions in the sequence or to ``positions`` ([B, N], whole numbers that 32 bits hold).  Padding rows write nothing,
     and are zeros in the result; nor does a position whose table entry names no page (below 0, past the pool, or past the
     table).  A slot that a call names twice gets values of both, in any order."""

@@ -584,7 +584,9 @@ typedef struct bioemu_paged_cache {
  * position, or positions[b, i] where given; pairs = 0: not at all), and q_out =
  * q turned the same (zeros in rows counts[b] and on; q and q_out may be NULL).
  * inverse is not taken.  v: [B, N, Hk, D].  Positions that the table does not
- * hold are left out.  No slot may be named twice in one call.
+ * hold are left out.  No slot may be named twice in one call, no two slots of
+ * keys and values may share memory, and q, k, v and q_out may not overlap the
+ * cache.
  */
 int bioemu_paged_append(const bioemu_paged_cache* cache, const bioemu_rotary_args* args, const void* v,
                         const int64_t* v_stride, void* q_out, hipStream_t stream);

@@ -139,3 +139,90 @@ def test_tables_and_lengths_of_64_bits(gpu_device):
     for got, want in zip(*stores):
         assert torch.equal(got.view(torch.int16), want.view(torch.int16))
     assert torch.equal(stores[0][0].view(torch.int16), c.keys.view(torch.int16))     # nothing was written
+
+
+# ----------------------------------------------------------------------------
+# Caches that share memory
+# ----------------------------------------------------------------------------
+def _append_ones(keys, values):
+    """Every slot of every page gets keys 1 and values 2."""
+    pages, page = keys.shape[:2]
+    k = torch.ones(1, pages * page, *keys.shape[2:], dtype=keys.dtype, device="cuda")
+    paged_append(keys, values, k, 2 * k, torch.arange(pages, dtype=I32, device="cuda")[None],
+                 torch.tensor([pages * page], dtype=I32, device="cuda"))
+
+
+def test_parts_of_one_allocation(gpu_device):
+    P, S, H, D = 3, 4, 2, 16
+    for whole, dim in [((2, P, S, H, D), 0), ((P, 2, S, H, D), 1), ((P, S, 2, H, D), 2), ((P, S, H, 2, D), 3),
+                       ((P, H, 2, S, D), 2)]:
+        both = torch.zeros(whole, dtype=BF16, device="cuda")
+        keys, values = both.select(dim, 0), both.select(dim, 1)
+        if whole[1] == H:
+            keys, values = keys.transpose(1, 2), values.transpose(1, 2)
+        _append_ones(keys, values)
+        assert bool((keys == 1).all()) and bool((values == 2).all())
+        _append_ones(values, keys)
+        assert bool((keys == 2).all()) and bool((values == 1).all())
+
+
+def test_slots_in_the_same_place_are_refused(gpu_device):
+    both = torch.zeros(6, 4, 2, 16, dtype=F32, device="cuda")
+    flat = both.flatten()
+    same = lambda *st, at=0: flat.as_strided((2, 4, 2, 16), (*st, 1), at)  # noqa: E731
+    for keys, values in [(both, both), (both[:4], both[2:]), (both[:, :3], both[:, 1:]), (both[..., :8], both[..., 4:12]),
+                         (both[:3], both[2:5]),
+                         (same(128, 32, 16), same(128, 16, 64, at=64)), (same(64, 32, 16), both[4:]),
+                         (same(16, 32, 16), both[2:4]), (same(128, 0, 16), both[2:4]), (both[4:], same(128, 8, 64))]:
+        with pytest.raises(ValueError):
+            _append_ones(keys, values)
+    assert both.abs().max() == 0
+
+
+def test_any_layout_within_one_allocation(gpu_device):
+    """Against the sets of places: what overlaps is refused; what does not is taken where steps are alike and each
+    dimension steps over what lies within it."""
+    import random
+
+    r = random.Random(2)
+    flat = torch.zeros(4096, dtype=BF16, device="cuda")
+    size = []
+
+    def layout():
+        within, steps = 8, [0, 0, 0, 1]
+        for d in r.sample(range(3), 3):
+            steps[d] = within + 8 * r.choice([0, 0, 1, 3, 9]) - (8 if r.random() < 0.1 and within > 8 else 0)
+            within += (size[d] - 1) * steps[d]
+        return steps
+
+    def steps_over(steps):
+        within = 8
+        for s, n in sorted((s, n) for s, n in zip(steps[:3], size[:3]) if n > 1):
+            if s < within:
+                return False
+            within += (n - 1) * s
+        return True
+
+    taken = refused = 0
+    while taken < 60 or refused < 60:
+        size[:] = [r.randint(1, 3) for _ in range(3)] + [8]
+        steps = [layout(), layout()]
+        if r.random() < 0.8:
+            steps[1] = steps[0]
+        at = [8 * r.randint(0, 40) for _ in "kv"]
+        places = [[a + i * st[0] + j * st[1] + k * st[2] + e for i in range(size[0]) for j in range(size[1])
+                   for k in range(size[2]) for e in range(8)] for st, a in zip(steps, at)]
+        clear = all(len(set(p)) == len(p) for p in places) and not set(places[0]) & set(places[1])
+        keys, values = (flat.as_strided(size, st, a) for st, a in zip(steps, at))
+        flat.zero_()
+        try:
+            _append_ones(keys, values)
+        except ValueError as e:
+            assert "share memory" in str(e), e
+            refused += 1
+            apart = max(places[0]) < min(places[1]) or max(places[1]) < min(places[0])
+            # without need only where steps differ, or where a dimension steps into another
+            assert not clear or not all(map(steps_over, steps)) or (steps[0] != steps[1] and not apart)
+        else:
+            taken += 1
+            assert clear and bool((keys == 1).all()) and bool((values == 2).all())
