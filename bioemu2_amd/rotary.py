@@ -42,15 +42,15 @@ def rotary_frequencies(dim: int, base: float = 10000.0, *, scaling: str | None =
         raise ValueError("rotary_frequencies: a factor comes with its scaling")
     if scaling == "base" and dim > 2:
         base = base * factor ** (dim / (dim - 2))
-    f = torch.tensor([base ** (-2.0 * i / dim) for i in range(dim // 2)], dtype=torch.float64)
+    f = [base ** (-2.0 * i / dim) for i in range(dim // 2)]
     if scaling == "linear":
-        f = f / factor
+        f = [x / factor for x in f]
     elif scaling == "parts":
         if length is None or length < 1 or not turns[1] > turns[0]:
             raise ValueError(f"rotary_frequencies: scaling 'parts' takes a length and growing turns, got {length}, {turns}")
-        kept = ((length * f / (2 * math.pi) - turns[0]) / (turns[1] - turns[0])).clamp(0.0, 1.0)
-        f = f * (kept + (1.0 - kept) / factor)
-    return f.to(device)
+        kept = [min(max((length * x / (2 * math.pi) - turns[0]) / (turns[1] - turns[0]), 0.0), 1.0) for x in f]
+        f = [x * (k + (1.0 - k) / factor) for x, k in zip(f, kept)]
+    return torch.tensor(f, dtype=torch.float64, device=device)
 
 
 def rotary(q: Tensor | None, k: Tensor | None, positions: Tensor | None, frequencies: Tensor, *,
@@ -85,11 +85,18 @@ class RotaryPosition(nn.Module):
             magnitude = 0.1 * math.log(factor) + 1.0 if scaling == "parts" and factor > 1.0 else 1.0
         self.magnitude = magnitude
         # not a buffer: module.to(dtype) and half() would round it
-        self.frequencies = rotary_frequencies(dim, base, scaling=scaling, factor=factor, length=length, turns=turns)
+        self._args = (dim, base, scaling, factor, length, turns)
+        self.frequencies = self._make(None)
+
+    def _make(self, device) -> Tensor:
+        dim, base, scaling, factor, length, turns = self._args
+        return rotary_frequencies(dim, base, scaling=scaling, factor=factor, length=length, turns=turns, device=device)
 
     def _apply(self, fn, recurse=True):
         super()._apply(fn, recurse)
-        self.frequencies = self.frequencies.to(fn(torch.empty(0, device=self.frequencies.device)).device)
+        device = fn(torch.empty(0, device=self.frequencies.device)).device
+        # those of the meta device have no values to move (``to_empty``)
+        self.frequencies = self._make(device) if self.frequencies.is_meta else self.frequencies.to(device)
         return self
 
     def forward(self, q: Tensor | None, k: Tensor | None = None,

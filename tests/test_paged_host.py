@@ -192,3 +192,20 @@ def test_numbers_that_32_bits_do_not_hold(dtype):
     assert _ints("here", table, table[:, 0], None)[0].tolist() == [[w, w] for w in want]
     with pytest.raises(ValueError, match="whole numbers"):
         _ints("here", table.float(), table[:, 0], None)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(scaling="linear", factor=3.0), dict(scaling="base", factor=3.0),
+                                dict(scaling="parts", factor=8.0, length=2000, turns=(2.0, 20.0))], ids=str)
+def test_module_made_without_values(kw):
+    """Built on the meta device, the module has its frequencies once it is brought to another."""
+    want = RotaryPosition(32, base=5000.0, **kw).frequencies
+    assert torch.equal(want, rotary_frequencies(32, 5000.0, **kw)) and want.device.type == "cpu"
+    with torch.device("meta"):
+        m = RotaryPosition(32, base=5000.0, **kw)
+    assert m.frequencies.is_meta and m.frequencies.shape == (16,)
+    got = m.to_empty(device="cpu").frequencies
+    assert got.dtype == F64 and torch.equal(got, want)
+    m = RotaryPosition(32, base=5000.0, **kw).to("meta")
+    assert m.frequencies.is_meta and torch.equal(m.to_empty(device="cpu").half().frequencies, want)
+    both = torch.nn.ModuleList([torch.nn.Linear(2, 2, device="meta"), m.to("meta")]).to_empty(device="cpu")
+    assert torch.equal(both[1].frequencies, want)
