@@ -236,6 +236,9 @@ int run(const char* what, RotaryArgs& a, bool f32, hipStream_t stream) {
   const int64_t held = kThreads * (a.interleaved ? kUnits<true> : kUnits<false>);
   a.per = (int)std::min(std::max(held / ((int64_t)a.heads * a.pieces), (int64_t)1), (int64_t)16);
   while (a.per > 1 && a.tokens / a.per < 1024) a.per /= 2;
+  // a launch has fewer than 2^32 threads.  So many tokens fit a GPU only with narrow heads: 128 of them at most, and
+  // 40 KB of LDS
+  while ((a.tokens + a.per - 1) / a.per >= 1 << 24) a.per *= 2;
   a.by_n = Divisor(a.N);
   a.by_heads = Divisor(a.heads);
   a.by_pieces = Divisor(a.pieces);

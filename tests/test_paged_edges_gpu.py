@@ -226,3 +226,19 @@ def test_any_layout_within_one_allocation(gpu_device):
         else:
             taken += 1
             assert clear and bool((keys == 1).all()) and bool((values == 2).all())
+
+
+# ----------------------------------------------------------------------------
+# Long calls
+# ----------------------------------------------------------------------------
+def test_more_tokens_than_a_launch_has_threads_for(gpu_device):
+    """2^28 tokens and some, sixteen a workgroup of 256 threads, would be 2^32 threads."""
+    n = 2 ** 28 + 5
+    q = torch.empty(1, n, 1, 8, dtype=BF16, device="cuda").normal_()
+    f = rotary_frequencies(4, device="cuda")
+    got = rotary(q, None, None, f)[0]
+    g = torch.Generator(device="cuda").manual_seed(0)
+    some = torch.cat((torch.arange(2000, device="cuda"), torch.arange(n - 2000, n, device="cuda"),
+                      torch.randint(0, n, (1000000,), generator=g, device="cuda")))
+    check(got[:, some], exact(q[:, some], some.to(I32)[None], f))
+    assert bool((got[0, :, 0, 4:] == q[0, :, 0, 4:]).all())     # all rows: what does not turn
