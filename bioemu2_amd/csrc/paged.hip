@@ -842,7 +842,8 @@ int paged_args(const bioemu_paged_cache* c, const bioemu_attention_args* in, Att
   if (const int rc = paged_cache_args("paged_attention", c, a->B, a->Hk, in->f32 != 0)) return rc;
   *pl = plan(*a, *c, in->f32 != 0);
   const int64_t tiles = (c->table_width * c->page_size + 15) / 16;
-  if (pl->items * std::max(tiles, (int64_t)1) >= (int64_t(1) << 31) || (int64_t)a->B * a->Nq * a->H >= (int64_t(1) << 31))
+  // tiles are counted in 32 bits; a launch of a workgroup an item has fewer than 2^32 threads
+  if (pl->items * std::max(tiles, (int64_t)1) >= (int64_t(1) << 31) || round_up(pl->items, kAttnXcds) >= 1 << 24)
     return set_error(BIOEMU_ERR_UNSUPPORTED, "paged_attention: B=%d, Nq=%d, H=%d over %ld keys are too many", a->B,
                      a->Nq, a->H, (long)(c->table_width * c->page_size));
   return BIOEMU_OK;

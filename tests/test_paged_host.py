@@ -209,3 +209,13 @@ def test_module_made_without_values(kw):
     assert m.frequencies.is_meta and torch.equal(m.to_empty(device="cpu").half().frequencies, want)
     both = torch.nn.ModuleList([torch.nn.Linear(2, 2, device="meta"), m.to("meta")]).to_empty(device="cpu")
     assert torch.equal(both[1].frequencies, want)
+
+
+def test_as_many_rows_as_a_launch_has_threads_for():
+    """2^24 - 4 blocks of 32 rows, a workgroup of 256 threads each and rounded up to 8, would be 2^32 threads."""
+    lib = _lib.lib()
+    many = dict(B=69, Nq=89 * 683 * 128, H=1, Hk=1, D=8, q_batch=8 * 89 * 683 * 128, q_row=8, q_head=8)
+    assert 69 * many["Nq"] // 32 == (1 << 24) - 4
+    assert lib.bioemu_paged_attention(_cache(), _attention(**many), 16, None, 0, None) == -2
+    assert b"too many" in lib.bioemu_last_error()
+    assert lib.bioemu_paged_attention_workspace_bytes(_cache(), _attention(**many)) == 0
