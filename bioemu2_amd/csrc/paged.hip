@@ -22,6 +22,7 @@
 #include <algorithm>
 
 #include "attn.h"
+#include "paged_parts.h"
 
 namespace bioemu {
 namespace {
@@ -102,17 +103,13 @@ __device__ __forceinline__ int scan(int x) {
 }
 
 // A workgroup's part of an item (a block of rows of a key head of a sequence): tiles t0 .. t0 + n - 1 of item `item` of
-// sequence b; n = 0: none. Every wave by itself, from the sequences' lengths. Every item is cut into equal parts, the
-// shortest with which all parts run at once, unless they would be kMost tiles longer than an equal share of all the
-// work (or have to be looked for in more lengths than a wave has lanes): then kLonger longer, and the last parts start
-// late. Parts of equal length that begin in one item and end in the next cost more. (In a graph, with such parts, and
-// with parts 16, 24 and 48 tiles longer: 48 sequences of up to 2000 keys, 8 key heads of 128, 61 us, 51, 47 and 54; 32
-// of up to 2048, 46, 34, 36 and 36; 100 of up to 3000, 4 key heads, 74, 68, 65 and 65; 56 of up to 2000, 8 key heads of
-// 80, 61, 42, 42 and 38.)
+// sequence b; n = 0: none. Every wave by itself, from the sequences' lengths. Every item is cut into equal parts of at most
+// part_length's tiles, which may be looked for where a wave has a lane for every sequence. Parts of equal length that begin
+// in one item and end in the next cost more (48 sequences of up to 2000 keys, 8 key heads of 128, 61 us; 32 of up to 2048,
+// 46; 100 of up to 3000, 4 key heads, 74; 56 of up to 2000, 8 key heads of 80, 61: part_length has the others' times).
 struct Part {
   int b, item, t0, n, w;   // w: the part's number
 };
-constexpr int kLonger = 24, kMost = 48;
 // Parts in order over the XCDs (workgroup i runs on XCD i % 8): neighbours, which may read parts of the same cache lines
 // or the same keys for other rows, get one L2.  -1: none.
 __device__ __forceinline__ int xcd_order(int n) {
@@ -131,30 +128,17 @@ __device__ __forceinline__ Part part_of(const PagedArgs& p, int B, int items) {
   }
   total *= items;
   live *= items;
-  const unsigned spare = max(groups - live, 1), even = ((unsigned)total + spare - 1) / spare, each = (unsigned)total / groups;
-  unsigned part = max(min(even, each + kLonger), (unsigned)p.least);
-  const auto count = [&]() {   // parts: at most `groups` and one an item
+  const auto count = [&](unsigned part) {
     int n = 0;
     for (int b0 = 0; b0 < B; b0 += 64) {
       if (B > 64) own = b0 + lane < B ? tiles_of<KEYS>(p, b0 + lane) : 0;
       sums = scan(((unsigned)own + part - 1) / part);
       n += __builtin_amdgcn_readlane(sums, 63);
     }
-    return n;
+    return (unsigned)(n * items);
   };
-  if (B <= 64 && even > each + each / 6 + 4 && part > (unsigned)p.least) {   // else the search gains nothing
-    unsigned fits = 0;
-    for (int step = kMost / 2, longer = kMost; step > 1; step /= 2) {
-      part = max(each + longer, (unsigned)p.least);
-      const bool ok = count() * items <= groups;
-      if (ok) fits = part;
-      else if (longer == kMost) break;
-      longer += ok ? -step : step;
-    }
-    part = fits ? fits : each + kLonger;
-  }
-  int n = count();
-  n *= items;
+  const unsigned part = part_length(total, live, groups, p.least, B <= 64, count);
+  const int n = (int)count(part);   // at most `groups` and one an item
   const int w = xcd_order(n);
   const Part none{0, 0, 0, 0, 0};
   if (w < 0) return none;

@@ -242,3 +242,9 @@ def test_more_tokens_than_a_launch_has_threads_for(gpu_device):
                       torch.randint(0, n, (1000000,), generator=g, device="cuda")))
     check(got[:, some], exact(q[:, some], some.to(I32)[None], f))
     assert bool((got[0, :, 0, 4:] == q[0, :, 0, 4:]).all())     # all rows: what does not turn
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("lengths,heads", [([131072, 118528], 32), ([131072, 115680, 47936, 50784], 16)])
+def test_parts_of_long_contexts(gpu_device, dtype, lengths, heads):
+    Case(lengths, dtype, H=heads, Hk=heads, D=8, page=64).check()
