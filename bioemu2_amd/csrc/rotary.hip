@@ -207,7 +207,7 @@ int piece(const RotaryArgs& a, bool f32) {
 
 template <class T, int V, bool APPEND, bool STREAM>
 void launch(const RotaryArgs& a, hipStream_t stream) {
-  const dim3 grid((unsigned)((a.tokens + a.per - 1) / a.per));
+  const dim3 grid((unsigned)((a.tokens - 1) / a.per + 1));
   const size_t lds = a.per * (sizeof(Token) + a.pairs * sizeof(f32x2));
   if (a.interleaved) {
     if constexpr (V > 1) rotary_kernel<T, V, true, APPEND, STREAM><<<grid, kThreads, lds, stream>>>(a);
@@ -238,7 +238,7 @@ int run(const char* what, RotaryArgs& a, bool f32, hipStream_t stream) {
   while (a.per > 1 && a.tokens / a.per < 1024) a.per /= 2;
   // a launch has fewer than 2^32 threads.  So many tokens fit a GPU only with narrow heads: 128 of them at most, and
   // 40 KB of LDS
-  while ((a.tokens + a.per - 1) / a.per >= 1 << 24) a.per *= 2;
+  while ((a.tokens - 1) / a.per + 1 >= 1 << 24) a.per *= 2;
   a.by_n = Divisor(a.N);
   a.by_heads = Divisor(a.heads);
   a.by_pieces = Divisor(a.pieces);
