@@ -728,17 +728,18 @@ struct Places {
   // has to step over all that lies within it.
   Places(const Tensor& t, const char* what)
       : first(static_cast<const char*>(t.data_ptr())), item(t.element_size()), extent(t.numel() ? item : 0) {
-    if (t.numel() == 0) return;
+    if (extent == 0) return;
+    const at::IntArrayRef sizes = t.sizes(), strides = t.strides();
     for (int d = 0; d < 4; ++d) {
-      if (t.size(d) == 1) continue;
+      if (sizes[d] == 1) continue;
       int at = dims++;
-      for (; at > 0 && step[at - 1] < t.stride(d) * item; --at) step[at] = step[at - 1], count[at] = count[at - 1];
-      step[at] = t.stride(d) * item;
-      count[at] = t.size(d);
+      for (; at > 0 && step[at - 1] < strides[d] * item; --at) step[at] = step[at - 1], count[at] = count[at - 1];
+      step[at] = strides[d] * item;
+      count[at] = sizes[d];
     }
     for (int d = dims - 1; d >= 0; --d) {
-      TORCH_CHECK_VALUE(step[d] >= extent, what, ": slots that share memory cannot be appended to (sizes ", t.sizes(),
-                        ", strides ", t.strides(), ")");
+      TORCH_CHECK_VALUE(step[d] >= extent, what, ": slots that share memory cannot be appended to (sizes ", sizes,
+                        ", strides ", strides, ")");
       extent += (count[d] - 1) * step[d];
     }
   }

@@ -29,6 +29,8 @@ from .relative_position import _int32
 
 def _nearest_int32(t: Tensor, what: str) -> Tensor:
     """Whole numbers as the nearest of 32 bits: an entry of 2^32 is past any pool, not the first page."""
+    if t.dtype == torch.int32:
+        return t
     if t.dtype in (torch.uint32, torch.uint64):
         t = t.to(torch.int64)
     if t.dtype != torch.int64:
