@@ -796,6 +796,8 @@ Plan plan(const AttnArgs& a, const bioemu_paged_cache& c, bool f32) {
   const int64_t most = c.pages > 0 ? c.table_width * c.page_size : 0;
   // what a walk of one workgroup takes no longer than parts and the join: up to 1024 keys of 64 values in bf16 (in a
   // graph 8.4 us for 512 and 11.0 for 1024; in parts 9.8 and 10.0, and a second launch)
+  // and items enough for 16 a CU, whose lengths the host does not know. Where one is far longer, its walk is what the call
+  // takes: 511 sequences of 50 to 400 keys of 8 heads of 128 and one of 400, 100 us; one of 8192, 164; one of 32768, 380.
   if (most * std::max(a.D, 64) * (f32 ? 4 : 2) <= 1024 * 64 * 2 || p.items >= 16 * attn_units()) {
     // With a CU for each, eight waves share a walk (sixteen, where registers allow it, start 1.5 us later: 12.9 us for
     // one token over 773 keys of 16 heads of 64, 11.3 with eight, 17 with four). Two of eight do not fit a CU, two of
@@ -847,7 +849,8 @@ int launch(const AttnArgs& a, const PagedArgs& p, const Plan& pl, T* out, void* 
     const dim3 grid((unsigned)round_up(pl.groups ? pl.slots : pl.items, kAttnXcds));
     const auto go = [&](auto kernel) { kernel<<<grid, 64 * pl.waves, 0, stream>>>(a, p, out, parts); };
     const bool wide = !fast_cap<T>(a);
-    // few calls have a wide cap: one form for them
+    // few calls have a wide cap: one form for them (64 tokens over up to 4000 keys, 32/4 heads of 128: 72 us, 64 with a cap
+    // of 50)
 #define BIOEMU_GO(RB, W, EVEN, ONCE)                                                                 \
   if (pl.rb == RB && !wide && pl.waves == W && p.even == EVEN && pl.once == ONCE)                     \
     go(paged_kernel<T, DP, RB, kCapped, W, EVEN, ONCE>);

@@ -54,7 +54,9 @@ def paged_append(keys: Tensor, values: Tensor, k: Tensor, v: Tensor, page_table:
     [B, width]; lengths, counts: [B].  With ``frequencies`` k and q are turned as ``rotary`` does, to their
     positions in the sequence or to ``positions`` ([B, N], whole numbers that 32 bits hold).  Padding rows write nothing,
     and are zeros in the result; nor does a position whose table entry names no page (below 0, past the pool, or past the
-    table).  A slot that a call names twice gets values of both, in any order."""
+    table).  A slot that a call names twice gets values of both, in any order.
+    fp32 under bf16 autocast is rounded before it is turned, and again after: turn with ``rotary`` and append what it
+    returns for one rounding."""
     _ops.require_gpu(k, "paged_append")
     page_table, lengths, counts = _ints("paged_append", page_table, lengths, counts)
     dtype = None if q is None else q.dtype
